@@ -277,6 +277,78 @@ int mambo_gemm_check_config(int64_t m, int64_t n, int64_t blocks, const mambo_ge
 int64_t mambo_gemm_config_enumerate(int64_t m, int64_t n, int64_t blocks, mambo_gemm_config *out,
                                     int64_t capacity);
 
+/* ------------------------------------------------------------- experts and 8-bit block weights
+ * No reference counterpart. The layer that these make up: mambo_route_experts turns router
+ * logits into a plan, the products read each token's row with the weight of the experts it goes
+ * to, mambo_combine_experts adds the experts' rows up. All of it stays on the device: no call
+ * reads a size back.
+ *
+ * The plan of `experts` experts over r = m * top_k rows:
+ *   offsets i32[experts + 1]: expert e has the rows [offsets[e], offsets[e+1]); offsets[0] == 0
+ *   rows    i32[r]: the token of each row, ascending within an expert; -1 past offsets[experts]
+ *   slots   i32[m, top_k]: the row of each choice; -1 where a token had none
+ * A product holds what it reads of offsets and rows within [0, r] and [0, m), so that a plan with
+ * other values gives wrong sums and no stray access. Rows past offsets[experts] come out as zeros. */
+
+/* Block quantizer: x [m, k] f32 or bf16 (row stride ldx), k % 16 == 0, in groups of 128 along K (the
+ * last may be shorter): scales[m, lds] f32 = max(amax / 448, 2^-100) and values [m, ldv] = E4M3 of
+ * x / scale, computed as one division by amax and rounded once to nearest even. A group that holds
+ * a NaN or an infinity gets the scale NaN and E4M3 NaN codes. m == 0: nothing to do. */
+int mambo_quantize_fp8_block(const void *x, int x_dtype, int64_t m, int64_t k, int64_t ldx, uint8_t *values,
+                             int64_t ldv, float *scales, int64_t lds, mambo_stream_t stream);
+
+/* Bytes of the private layout of `experts` weights [n, k] of E4M3 codes. */
+int64_t mambo_fp8_block_packed_bytes(int64_t experts, int64_t n, int64_t k);
+
+/* E4M3 codes w [experts, n, k] (strides in elements, K contiguous; any alignment) to the private
+ * layout that the products read: once per weight. */
+int mambo_fp8_block_pack(const uint8_t *w, int64_t experts, int64_t n, int64_t k, int64_t stride_e,
+                         int64_t stride_n, uint8_t *packed, mambo_stream_t stream);
+
+/* out[m, n] (f32 or bf16: out_dtype; row stride ldo) = sum over K groups g of 128 of
+ * xs[m, g] * ws[n / 128, g] * sum over the group of xv[m, k] * w[n, k], in f32, groups in a fixed
+ * order. xv u8 [m, ldxv] E4M3, 16-byte aligned rows; xs f32 [m, ldxs]; packed from
+ * mambo_fp8_block_pack with one expert; ws f32 [ceil(n/128), ceil(k/128)] contiguous;
+ * k % 16 == 0. m == 0: nothing to do. */
+int mambo_fp8_block_matmul(const uint8_t *xv, int64_t ldxv, const float *xs, int64_t ldxs, int64_t m,
+                           const uint8_t *packed, const float *ws, int64_t n, int64_t k, void *out,
+                           int out_dtype, int64_t ldo, mambo_stream_t stream);
+
+/* The same grouped by expert: out [r, n], row i of expert e (offsets) with weight e of packed
+ * [experts] and ws [experts, ceil(n/128), ceil(k/128)]. rows: row i reads xv/xs row rows[i] of m
+ * (NULL: row i, and m == r). experts <= MAMBO_MAX_EXPERTS; r == 0: nothing to do. */
+#define MAMBO_MAX_EXPERTS 1024
+int mambo_fp8_block_matmul_experts(const uint8_t *xv, int64_t ldxv, const float *xs, int64_t ldxs, int64_t m,
+                                   const int32_t *rows, int64_t r, const int32_t *offsets, int64_t experts,
+                                   const uint8_t *packed, const float *ws, int64_t n, int64_t k, void *out,
+                                   int out_dtype, int64_t ldo, mambo_stream_t stream);
+
+/* mambo_iq3s_fp8_matmul grouped by expert: rows and offsets as above, weight e in the tile layout
+ * (mambo_iq3s_prepare) at packed + e * expert_stride bytes, a multiple of 16 and at least
+ * mambo_iq3s_packed_bytes(n, blocks). xv/xs as for mambo_iq3s_fp8_matmul, with xs and ldxs 8-byte
+ * aligned. */
+int mambo_iq3s_fp8_matmul_experts(const uint8_t *xv, int64_t ldxv, const uint8_t *xs, int64_t ldxs, int64_t m,
+                                  const int32_t *rows, int64_t r, const int32_t *offsets, int64_t experts,
+                                  const uint8_t *packed, int64_t expert_stride, int64_t n, int64_t blocks,
+                                  void *out, int out_dtype, int64_t ldo, mambo_stream_t stream);
+
+/* The router's plan: logits [m, ld] f32 or bf16 over `experts` <= MAMBO_MAX_EXPERTS; each token
+ * takes its top_k (<= MAMBO_MAX_TOP_K) largest, ties to the lowest index, never one that is -inf or
+ * NaN. ids i32 [m, top_k] in falling order, -1 where none was left; weights f32 [m, top_k]: the
+ * softmax over all its experts, or over the chosen ones (renormalize != 0), 0 beside an id of -1.
+ * The plan as above. m == 0: offsets are zeroed. */
+#define MAMBO_MAX_TOP_K 64
+int mambo_route_experts(const void *logits, int dtype, int64_t ld, int64_t m, int64_t experts, int64_t top_k,
+                        int renormalize, int32_t *ids, float *weights, int32_t *offsets, int32_t *rows,
+                        int32_t *slots, mambo_stream_t stream);
+
+/* out[t] = sum over j of weights[t, j] * y[slots[t, j]], in f32 and in order of j; choices whose slot is
+ * outside [0, r) add nothing. y [r, ldy] and out [m, ldo] f32 or bf16, n columns; slots and weights
+ * [m, top_k] contiguous. */
+int mambo_combine_experts(const void *y, int y_dtype, int64_t ldy, int64_t r, const int32_t *slots,
+                          const float *weights, int64_t m, int64_t top_k, int64_t n, void *out, int out_dtype,
+                          int64_t ldo, mambo_stream_t stream);
+
 /* Synthetic inputs for benchmarks and full-size checks (no reference counterpart; the
  * reference draws them with numpy/cupy RNGs, test_iq3_s_fp8.py:41-51). Counter-based:
  *   rnd(seed, stream, i) = splitmix64(splitmix64(seed*0xD1B54A32D192ED03 + stream) + i);

@@ -120,6 +120,16 @@ SIGNATURES = {
                                ctypes.POINTER(GemmConfig)]),
     "mambo_gemm_check_config": (_i32, [_i64, _i64, _i64, ctypes.POINTER(GemmConfig)]),
     "mambo_gemm_config_enumerate": (_i64, [_i64, _i64, _i64, ctypes.POINTER(GemmConfig), _i64]),
+    "mambo_quantize_fp8_block": (_i32, [_vp, _i32, _i64, _i64, _i64, _vp, _i64, _vp, _i64, _vp]),
+    "mambo_fp8_block_packed_bytes": (_i64, [_i64, _i64, _i64]),
+    "mambo_fp8_block_pack": (_i32, [_vp, _i64, _i64, _i64, _i64, _i64, _vp, _vp]),
+    "mambo_fp8_block_matmul": (_i32, [_vp, _i64, _vp, _i64, _i64, _vp, _vp, _i64, _i64, _vp, _i32, _i64, _vp]),
+    "mambo_fp8_block_matmul_experts": (_i32, [_vp, _i64, _vp, _i64, _i64, _vp, _i64, _vp, _i64, _vp, _vp, _i64, _i64,
+                                              _vp, _i32, _i64, _vp]),
+    "mambo_iq3s_fp8_matmul_experts": (_i32, [_vp, _i64, _vp, _i64, _i64, _vp, _i64, _vp, _i64, _vp, _i64, _i64, _i64,
+                                             _vp, _i32, _i64, _vp]),
+    "mambo_route_experts": (_i32, [_vp, _i32, _i64, _i64, _i64, _i64, _i32, _vp, _vp, _vp, _vp, _vp, _vp]),
+    "mambo_combine_experts": (_i32, [_vp, _i32, _i64, _i64, _vp, _vp, _i64, _i64, _i64, _vp, _i32, _i64, _vp]),
     "mambo_synth_iq3s": (_i32, [_u64, _i64, _i64, _i64, _vp, _vp]),
     "mambo_synth_bf16": (_i32, [_u64, _u64, ctypes.c_double, _i64, _i64, _vp, _vp]),
     "mambo_e4m3_convert": (_i32, [_vp, _i64, _vp, _vp, _vp]),
@@ -198,6 +208,21 @@ def device_arch(device=None) -> str:
 
 
 _here = nullcontext()
+
+
+def on_stream(stream, device):
+    """Context in which torch's memory of `device` belongs to `stream` (None, an int handle or a
+    torch.cuda.Stream): what a launcher allocates or copies for work on that stream must not be
+    handed out again, or written, in the order of another."""
+    import torch
+    if stream is None:
+        return _here
+    handle = stream_handle(stream)
+    if handle == torch._C._cuda_getCurrentRawStream(device.index):
+        return _here
+    if not isinstance(stream, torch.cuda.Stream):
+        stream = torch.cuda.ExternalStream(handle, device=device) if handle else torch.cuda.default_stream(device)
+    return torch.cuda.stream(stream)
 
 
 def on_device(device):

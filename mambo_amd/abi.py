@@ -177,6 +177,54 @@ CONSTRAINTS: dict[str, list[dict]] = {
     "mambo_gemm_check_config": [_arr("cfg", "mambo_gemm_config", ["1"], align=4, memory="host")],
     "mambo_gemm_config_enumerate": [
         _arr("out", "mambo_gemm_config", ["capacity"], align=4, memory="host", nullable=True, access="write")],
+    "mambo_quantize_fp8_block": [
+        _arr("x", "float32|bfloat16", ["m", "k"], ["ldx", "1"], align=2),
+        _arr("values", "uint8", ["m", "k"], ["ldv", "1"], access="write"),
+        _arr("scales", "float32", ["m", "(k+127)/128"], ["lds", "1"], align=4, access="write"),
+    ],
+    "mambo_fp8_block_packed_bytes": [],
+    "mambo_fp8_block_pack": [
+        _arr("w", "uint8", ["experts", "n", "k"], ["stride_e", "stride_n", "1"]),
+        _arr("packed", "uint8", ["experts*((n+31)/32)*((k+127)/128)*4096"], align=16, access="write"),
+    ],
+    "mambo_fp8_block_matmul": [
+        _arr("xv", "uint8", ["m", "k"], ["ldxv", "1"], align=16),
+        _arr("xs", "float32", ["m", "(k+127)/128"], ["ldxs", "1"], align=4),
+        _arr("packed", "uint8", ["((n+31)/32)*((k+127)/128)*4096"], align=16),
+        _arr("ws", "float32", ["(n+127)/128", "(k+127)/128"], align=4),
+        _arr("out", "float32|bfloat16", ["m", "n"], ["ldo", "1"], align=2, access="write"),
+    ],
+    "mambo_fp8_block_matmul_experts": [
+        _arr("xv", "uint8", ["m", "k"], ["ldxv", "1"], align=16),
+        _arr("xs", "float32", ["m", "(k+127)/128"], ["ldxs", "1"], align=4),
+        _arr("rows", "int32", ["r"], align=4, nullable=True),
+        _arr("offsets", "int32", ["experts+1"], align=4),
+        _arr("packed", "uint8", ["experts*((n+31)/32)*((k+127)/128)*4096"], align=16),
+        _arr("ws", "float32", ["experts", "(n+127)/128", "(k+127)/128"], align=4),
+        _arr("out", "float32|bfloat16", ["r", "n"], ["ldo", "1"], align=2, access="write"),
+    ],
+    "mambo_iq3s_fp8_matmul_experts": [
+        _arr("xv", "uint8", ["m", "blocks*256"], ["ldxv", "1"], align=16),
+        _arr("xs", "uint8", ["m", "blocks*8"], ["ldxs", "1"], align=8),
+        _arr("rows", "int32", ["r"], align=4, nullable=True),
+        _arr("offsets", "int32", ["experts+1"], align=4),
+        _arr("packed", "uint8", ["experts", _PACKED], ["expert_stride", "1"], align=16),
+        _arr("out", "float32|bfloat16", ["r", "n"], ["ldo", "1"], align=2, access="write"),
+    ],
+    "mambo_route_experts": [
+        _arr("logits", "float32|bfloat16", ["m", "experts"], ["ld", "1"], align=2),
+        _arr("ids", "int32", ["m", "top_k"], align=4, access="write"),
+        _arr("weights", "float32", ["m", "top_k"], align=4, access="write"),
+        _arr("offsets", "int32", ["experts+1"], align=4, access="write"),
+        _arr("rows", "int32", ["m*top_k"], align=4, access="write"),
+        _arr("slots", "int32", ["m", "top_k"], align=4, access="write"),
+    ],
+    "mambo_combine_experts": [
+        _arr("y", "float32|bfloat16", ["r", "n"], ["ldy", "1"], align=2),
+        _arr("slots", "int32", ["m", "top_k"], align=4),
+        _arr("weights", "float32", ["m", "top_k"], align=4),
+        _arr("out", "float32|bfloat16", ["m", "n"], ["ldo", "1"], align=2, access="write"),
+    ],
     "mambo_synth_iq3s": [_arr("raw", "uint8", ["nrows", "blocks", "110"], access="write")],
     "mambo_synth_bf16": [_arr("out", "uint16", ["count"], align=2, access="write")],
     "mambo_e4m3_convert": [

@@ -26,7 +26,7 @@ BUILD_DIR = CSRC / "_build"
 ARCH = "gfx950"
 
 SOURCES = ["api.hip", "quantize_mxfp8.hip", "iq3s_layout.hip", "iq3s_gemm.hip", "iq3s_wide.hip", "iq3s_chain.hip",
-           "synth.hip"]
+           "iq3s_experts.hip", "fp8_block.hip", "experts.hip", "synth.hip"]
 
 HIPCC_FLAGS = [
     f"--offload-arch={ARCH}",

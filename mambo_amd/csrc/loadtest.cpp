@@ -349,6 +349,20 @@ const std::vector<EntryDecl> &compiled_entries()
         MAMBO_ENTRY(mambo_gemm_plan, "m", "proj", "count", "blocks", "ldxv", "ldxs", "cfg", "out"),
         MAMBO_ENTRY(mambo_gemm_check_config, "m", "n", "blocks", "cfg"),
         MAMBO_ENTRY(mambo_gemm_config_enumerate, "m", "n", "blocks", "out", "capacity"),
+        MAMBO_ENTRY(mambo_quantize_fp8_block, "x", "x_dtype", "m", "k", "ldx", "values", "ldv", "scales", "lds",
+                    "stream"),
+        MAMBO_ENTRY(mambo_fp8_block_packed_bytes, "experts", "n", "k"),
+        MAMBO_ENTRY(mambo_fp8_block_pack, "w", "experts", "n", "k", "stride_e", "stride_n", "packed", "stream"),
+        MAMBO_ENTRY(mambo_fp8_block_matmul, "xv", "ldxv", "xs", "ldxs", "m", "packed", "ws", "n", "k", "out",
+                    "out_dtype", "ldo", "stream"),
+        MAMBO_ENTRY(mambo_fp8_block_matmul_experts, "xv", "ldxv", "xs", "ldxs", "m", "rows", "r", "offsets", "experts",
+                    "packed", "ws", "n", "k", "out", "out_dtype", "ldo", "stream"),
+        MAMBO_ENTRY(mambo_iq3s_fp8_matmul_experts, "xv", "ldxv", "xs", "ldxs", "m", "rows", "r", "offsets", "experts",
+                    "packed", "expert_stride", "n", "blocks", "out", "out_dtype", "ldo", "stream"),
+        MAMBO_ENTRY(mambo_route_experts, "logits", "dtype", "ld", "m", "experts", "top_k", "renormalize", "ids",
+                    "weights", "offsets", "rows", "slots", "stream"),
+        MAMBO_ENTRY(mambo_combine_experts, "y", "y_dtype", "ldy", "r", "slots", "weights", "m", "top_k", "n", "out",
+                    "out_dtype", "ldo", "stream"),
         MAMBO_ENTRY(mambo_synth_iq3s, "seed", "blocks", "row0", "nrows", "raw", "stream"),
         MAMBO_ENTRY(mambo_synth_bf16, "seed", "outlier_seed", "outlier_frac", "i0", "count", "out", "stream"),
         MAMBO_ENTRY(mambo_e4m3_convert, "in", "n", "out_sw", "out_hw", "stream"),

@@ -1,0 +1,115 @@
+"""E4M3 products with an f32 scale for each block of 128 on gfx950: the quantizer of the rows
+and the product with a prepared weight (mambo_amd.utils.fp8_block_weight). The kernels are
+hand-written HIP (mambo_amd/csrc/fp8_block.hip) behind the C ABI. The reference has no counterpart.
+
+    out[m, n] = sum_g xs[m, g] * ws[n // 128, g] * sum_{k in group g} xv[m, k] * w[n, k]
+
+over the groups g of 128 along K, summed in float32 in a fixed order.
+"""
+
+from __future__ import annotations
+
+import torch
+
+from mambo_amd import _native
+from mambo_amd.utils.fp8_block_weight import FP8_BLOCK, Fp8BlockWeight
+
+ROW_DTYPES = {torch.float32: _native.DTYPE_F32, torch.bfloat16: _native.DTYPE_BF16}
+
+
+def launch_quantize_fp8_block(x: torch.Tensor, *, stream=None, out: tuple[torch.Tensor, torch.Tensor] | None = None
+                              ) -> tuple[torch.Tensor, torch.Tensor]:
+    """Return uint8 [M,K] E4M3 codes and float32 [M,ceil(K/128)] scales of ``x``.
+
+    ``x`` is float32 or bfloat16 [M,K] on the GPU, K a multiple of 16, M >= 0. A group of 128 along K
+    (the last may be shorter) has the scale max(amax / 448, 2^-100) and the codes of x / scale,
+    rounded once to nearest even; a group that holds a NaN or an infinity becomes NaN. Row-strided
+    inputs are read in place. ``out`` optionally supplies (codes, scales) with unit column stride.
+    """
+    if not isinstance(x, torch.Tensor) or x.ndim != 2 or x.dtype not in ROW_DTYPES or x.shape[1] % 16 or x.shape[1] < 16:
+        raise ValueError("activation must be float32 or bfloat16 [M,K] with K a multiple of 16")
+    if not x.is_cuda:
+        raise ValueError("activation must be a GPU tensor")
+    (m, k), dev = x.shape, x.device
+    groups = -(-k // FP8_BLOCK)
+    with _native.on_device(dev), _native.on_stream(stream, dev):
+        if not _plain_rows(x):
+            x = x.contiguous()
+        if out is None:
+            values = torch.empty((m, k), dtype=torch.uint8, device=dev)
+            scales = torch.empty((m, groups), dtype=torch.float32, device=dev)
+        else:
+            values, scales = out
+            if values.shape != (m, k) or values.dtype != torch.uint8 or scales.shape != (m, groups) \
+                    or scales.dtype != torch.float32 or values.device != dev or scales.device != dev \
+                    or not _plain_rows(values) or not _plain_rows(scales):
+                raise ValueError("out must be (uint8 [M,K], float32 [M,ceil(K/128)]) with unit column stride on the "
+                                 "activation's device")
+        _native.check(_native.lib().mambo_quantize_fp8_block(
+            x.data_ptr(), ROW_DTYPES[x.dtype], m, k, _row_stride(x), values.data_ptr(), _row_stride(values),
+            scales.data_ptr(), _row_stride(scales), _native.stream_handle(stream)), "launch_quantize_fp8_block")
+    return values, scales
+
+
+def _row_stride(t: torch.Tensor) -> int:
+    """Stride of the rows; of a single row, whose stride torch leaves open, its length."""
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+
+
+def _plain_rows(t: torch.Tensor) -> bool:
+    """Whether rows do not overlap and their elements are next to each other."""
+    return (t.shape[1] <= 1 or t.stride(1) == 1) and (t.shape[0] <= 1 or t.stride(0) >= t.shape[1])
+
+
+def block_activations(x_values, x_scales, k: int):
+    """Validate E4M3 rows [M,K] and scales [M,ceil(K/128)]; return them in a form that the kernels
+    read in place (16-byte aligned rows), copied only if needed."""
+    if not isinstance(x_values, torch.Tensor) or x_values.ndim != 2 or x_values.dtype != torch.uint8 \
+            or x_values.shape[1] != k:
+        raise ValueError(f"x_values must be uint8 [M,{k}]")
+    m = x_values.shape[0]
+    if not isinstance(x_scales, torch.Tensor) or tuple(x_scales.shape) != (m, -(-k // FP8_BLOCK)) \
+            or x_scales.dtype != torch.float32:
+        raise ValueError("x_scales must be float32 [M,ceil(K/128)]")
+    if not x_values.is_cuda or x_scales.device != x_values.device:
+        raise ValueError("x_values and x_scales must be on the same GPU")
+    if not _plain_rows(x_values) or x_values.data_ptr() % 16 or _row_stride(x_values) % 16:
+        x_values = torch.empty(x_values.shape, dtype=torch.uint8, device=x_values.device).copy_(x_values)
+    if not _plain_rows(x_scales):
+        x_scales = x_scales.contiguous()
+    return x_values, x_scales, m
+
+
+def product_output(out, rows: int, n: int, dtype, dev) -> torch.Tensor:
+    """The given output, checked, or a new one."""
+    if dtype not in ROW_DTYPES:
+        raise ValueError("out_dtype must be float32 or bfloat16")
+    if out is None:
+        return torch.empty((rows, n), dtype=dtype, device=dev)
+    if not isinstance(out, torch.Tensor) or tuple(out.shape) != (rows, n) or out.dtype != dtype or out.device != dev \
+            or not _plain_rows(out):
+        raise ValueError(f"out must be {dtype} [{rows},{n}] with unit column stride on the rows' device")
+    return out
+
+
+def launch_fp8_block_matmul(x_values: torch.Tensor, x_scales: torch.Tensor, weight: Fp8BlockWeight, *,
+                            out_dtype: torch.dtype = torch.float32, stream=None,
+                            out: torch.Tensor | None = None) -> torch.Tensor:
+    """Multiply rows from launch_quantize_fp8_block by a prepared weight: [M,N] of ``out_dtype``
+    (float32 or bfloat16, rounded once from the float32 sums). M may be 0. Rows that are not 16-byte
+    aligned are copied first; ``out`` optionally supplies the output."""
+    if not isinstance(weight, Fp8BlockWeight):
+        raise TypeError("prepare FP8 weights with prepare_fp8_block_weight before launch")
+    if weight.experts != 1:
+        raise ValueError("a weight of several experts takes launch_fp8_block_matmul_experts")
+    dev = weight.packed.device
+    with _native.on_device(dev), _native.on_stream(stream, dev):
+        x_values, x_scales, m = block_activations(x_values, x_scales, weight.k)
+        if x_values.device != dev:
+            raise ValueError("the rows and the weight must be on the same device")
+        out = product_output(out, m, weight.n, out_dtype, dev)
+        _native.check(_native.lib().mambo_fp8_block_matmul(
+            x_values.data_ptr(), _row_stride(x_values), x_scales.data_ptr(), _row_stride(x_scales), m,
+            weight.packed.data_ptr(), weight.scales.data_ptr(), weight.n, weight.k, out.data_ptr(),
+            ROW_DTYPES[out_dtype], _row_stride(out), _native.stream_handle(stream)), "launch_fp8_block_matmul")
+    return out

@@ -195,3 +195,31 @@ def ensure_packed(iq3_weight: IQ3SFields, stream=None) -> torch.Tensor:
     object.__setattr__(iq3_weight, "packed", packed)
     object.__setattr__(iq3_weight, "packed_from", fields_signature(iq3_weight))
     return packed
+
+
+@dataclass(frozen=True)
+class IQ3SExperts:
+    """IQ3_S weights of one shape, one per expert, in the tile layout: ``packed`` uint8
+    [experts, bytes of a weight] (launch_iq3_s_fp8_matmul_experts)."""
+
+    packed: torch.Tensor
+    experts: int
+    n: int
+    blocks: int
+
+
+def prepare_iq3_s_experts(iq3_weights: torch.Tensor, *, stream=None) -> IQ3SExperts:
+    """Bring GGUF uint8 [E,N,B,110] blocks, a weight [N,B,110] for each of E experts, into the tile
+    layout once. Any strides and any byte alignment of the source are accepted."""
+    if not isinstance(iq3_weights, torch.Tensor) or iq3_weights.ndim != 4 or not 1 <= iq3_weights.shape[0] <= 1024:
+        raise ValueError("IQ3_S experts must be uint8 [E,N,K/256,110] with E in [1, 1024]")
+    n, blocks = _check_raw(iq3_weights[0])
+    dev, experts = iq3_weights.device, int(iq3_weights.shape[0])
+    with _native.on_device(dev), _native.on_stream(stream, dev):
+        packed = torch.empty((experts, packed_bytes(n, blocks)), dtype=torch.uint8, device=dev)
+        se, sn, sb, sbyte = iq3_weights.stride()
+        for e in range(experts):
+            _native.check(_native.lib().mambo_iq3s_prepare(
+                iq3_weights.data_ptr() + e * se, n, blocks, sn, sb, sbyte, None, None, None, None, None,
+                packed.data_ptr() + e * packed.stride(0), _native.stream_handle(stream)), "prepare_iq3_s_experts")
+    return IQ3SExperts(packed, experts, n, blocks)
