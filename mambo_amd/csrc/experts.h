@@ -108,9 +108,28 @@ __device__ __forceinline__ void store_row4(void *out, int64_t at, v4f v, int64_t
     }
 }
 
-// Whether a row of f32 or bf16 outputs takes store_row4's one store at multiples of four.
+// 16 bytes of a row, those past its end (`left` elements on) left out.
+template <bool kBf16>
+__device__ __forceinline__ void store_chunk(void *out, int64_t at, uint4 v, int64_t left, bool vec)
+{
+    constexpr int n = kBf16 ? 8 : 4;
+    row_t<kBf16> *o = reinterpret_cast<row_t<kBf16> *>(out) + at;
+    if (vec && left >= n) {
+        *reinterpret_cast<uint4 *>(o) = v;
+    } else {
+        struct Values {
+            row_t<kBf16> v[n];
+        };
+        const Values e = __builtin_bit_cast(Values, v);
+#pragma unroll
+        for (int i = 0; i < n; ++i)
+            if (i < left)
+                o[i] = e.v[i];
+    }
+}
+
+// Whether a row of f32 or bf16 outputs takes 16 bytes in one store.
 inline bool rows_take_vectors(const void *out, int64_t ldo, int dtype)
 {
-    const uintptr_t size = dtype == MAMBO_DTYPE_BF16 ? 8 : 16;
-    return (uintptr_t)out % size == 0 && ldo % 4 == 0;
+    return (uintptr_t)out % 16 == 0 && ldo % (dtype == MAMBO_DTYPE_BF16 ? 8 : 4) == 0;
 }

@@ -23,6 +23,7 @@
 // operand: lane (i, h) of the 32 x 32 MFMA of K step s takes chunks 4s + h and 4s + 2 + h, of the 16 x
 // 16 MFMA chunks h and 4 + h. Rows past n and K past k are zeros, so nothing else looks after the
 // ends of a weight. (Any order of K serves that both operands share.)
+#include <cmath>
 #include <type_traits>
 
 #include "experts.h"
@@ -223,122 +224,95 @@ __device__ __forceinline__ v16f multiply(const uint4 (&w)[2], const uint4 (&x)[2
     }
 }
 
-// Few rows: bound by the weights' bytes. A workgroup computes T tokens x 32 weight rows; its W waves
-// take the K groups in turn and every wave streams its own, a ring of D groups of weights and rows in
-// registers and no barrier before the end, where the waves' sums meet in LDS and are added in order.
-template <int T, int W, int D, bool kExperts, bool kBf16>
+// Few rows: bound by the weights' bytes. A workgroup computes 16 tokens x 16 H weight rows; its W waves take the K groups in
+// turn and every wave streams its own, the next group's weights and rows in flight while one is multiplied and no barrier
+// before the end, where the waves' sums meet in LDS and are added in order. The weights pass the caches by (each byte is read
+// once by one workgroup in a launch of few rows; 58 MB 13.1 -> 12.2 us, 117 MB 22.7 -> 20.4; weights that a cache still
+// holds from before lose by it, 4 MB 4.6 -> 5.1). Three and four groups in flight were slower (58 MB 15.8 us).
+typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
+
+template <int H, int W, bool kExperts, bool kBf16>
 __global__ __launch_bounds__(W * 64) void fp8_stream_kernel(Fp8Args a)
 {
-    constexpr int S = T < 32 ? 16 : 32;  // tokens of an MFMA
-    constexpr int U = T / S;             // MFMAs side by side
-    constexpr int kRegs = S == 16 ? 4 : 16; // sums per lane of an MFMA
-    constexpr int kHalves = S == 16 ? 2 : 1; // MFMAs that 32 weight rows take
-    constexpr int kPad = 36;             // floats of a token's 32 sums in LDS
+    constexpr int T = 16, kCols = 16 * H;
+    constexpr int kPad = kCols + 4; // floats of a token's sums in LDS
     __shared__ __align__(16) float s_red[W * T * kPad];
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int nt = blockIdx.x % a.ntiles;
+    const int tiles_n = (a.n + kCols - 1) / kCols;
+    const int nt = blockIdx.x % tiles_n;
     RowTile rt;
-    if (!row_tile<kExperts>(a, T, blockIdx.x / a.ntiles, &rt))
+    if (!row_tile<kExperts>(a, T, blockIdx.x / tiles_n, &rt))
         return;
     const bool none = kExperts && rt.expert == a.er.experts;
 
     if (!none) {
-        const int col = lane & (S - 1), h = lane / S;
-        const uint8_t *xp[U];
-        const float *sp[U];
-#pragma unroll
-        for (int u = 0; u < U; ++u) { // lanes past the last row read it again: they feed sums that are not stored
-            const int64_t src = source_row(a.er, rt.row0 + min(S * u + col, rt.count - 1));
-            xp[u] = a.xv + src * a.ldxv;
-            sp[u] = a.xs + src * a.ldxs;
-        }
-        const int64_t wtile = (int64_t)rt.expert * a.ntiles + nt;
-        const uint8_t *wp = a.packed + wtile * a.groups * kFp8Tile + (S == 16 ? 512 * h + 16 * col : 16 * lane);
-        const float *ws = a.ws + ((int64_t)rt.expert * ((a.n + kGroup - 1) / kGroup) + nt * kTileN / kGroup) * a.groups;
+        // lanes past the last row read it again: they feed sums that are not stored
+        const int col = lane & 15, q = lane >> 4;
+        const int64_t src = source_row(a.er, rt.row0 + min(col, rt.count - 1));
+        const uint8_t *xp = a.xv + src * a.ldxv;
+        const float *sp = a.xs + src * a.ldxs;
+        // chunk q + 4 j of weight row 16 t + col: halves t of a tile of 32 rows, H 4: of this one and the next (the last
+        // tile stands in for one past it)
+        const int tile = nt * kCols / kTileN;
+        const uint8_t *wp = a.packed + ((int64_t)rt.expert * a.ntiles + tile) * a.groups * kFp8Tile + 512 * q + 16 * col +
+                            (H == 1 ? 256 * (nt & 1) : 0);
+        const int64_t next = tile + 1 < a.ntiles ? (int64_t)a.groups * kFp8Tile : 0;
+        const float *ws = a.ws + ((int64_t)rt.expert * ((a.n + kGroup - 1) / kGroup) + nt * kCols / kGroup) * a.groups;
 
-        float acc[U][kHalves][kRegs];
-#pragma unroll
-        for (int u = 0; u < U; ++u)
-#pragma unroll
-            for (int t = 0; t < kHalves; ++t)
-#pragma unroll
-                for (int i = 0; i < kRegs; ++i)
-                    acc[u][t][i] = 0.0f;
-
-        // operands of one K group: weights [half or step][32 bytes], rows [step][32 bytes]
-        constexpr int kSteps = S == 16 ? 1 : 2;
+        float acc[H][4] = {};
         struct Ring {
-            uint4 w[2][2], x[U][kSteps][2];
-            float xs[U], ws;
-        } ring[D];
+            uint4 w[H][2], x[2];
+            float xs, ws;
+        } ring[2];
         const int count = wave < a.groups ? (a.groups - wave + W - 1) / W : 0;
         auto load = [&](Ring &r, int i) {
-            const int g = min(wave + min(i, count - 1) * W, a.groups - 1); // count 0: any group, scaled by 0
-            const int gc = max(g, 0);
-            const uint8_t *p = wp + (int64_t)gc * kFp8Tile;
+            const int g = max(min(wave + min(i, count - 1) * W, a.groups - 1), 0); // past the last: any, scaled by 0
+            const uint8_t *p = wp + (int64_t)g * kFp8Tile;
 #pragma unroll
-            for (int j = 0; j < 4; ++j) { // S 16: (half j >> 1, chunk h + 4 (j & 1)); else (step j >> 1, chunk 4s + 2 (j & 1) + h)
-                const int off = S == 16 ? 2048 * (j & 1) + 256 * (j >> 1) : 1024 * j;
-                r.w[j >> 1][j & 1] = *reinterpret_cast<const uint4 *>(p + off);
-            }
-            const int k0 = gc * kGroup;
+            for (int t = 0; t < H; ++t)
 #pragma unroll
-            for (int u = 0; u < U; ++u) {
-#pragma unroll
-                for (int j = 0; j < 2 * kSteps; ++j) {
-                    // a chunk past the row's end meets zero weights: any chunk of the row does
-                    const int at = k0 + 16 * (S == 16 ? h + 4 * j : 2 * j + h);
-                    r.x[u][j >> 1][j & 1] = *reinterpret_cast<const uint4 *>(xp[u] + (at < a.k ? at : k0));
+                for (int j = 0; j < 2; ++j) {
+                    const u32x4 v = __builtin_nontemporal_load(
+                        reinterpret_cast<const u32x4 *>(p + 2048 * j + 256 * (t & 1) + (t >> 1) * next));
+                    r.w[t][j] = uint4{v[0], v[1], v[2], v[3]};
                 }
-                r.xs[u] = sp[u][gc];
+            const int k0 = g * kGroup;
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                const int at = k0 + 16 * (q + 4 * j); // a chunk past the row's end meets zero weights: any of the row does
+                r.x[j] = *reinterpret_cast<const uint4 *>(xp + (at < a.k ? at : k0));
             }
-            r.ws = i < count ? ws[gc] : 0.0f;
+            r.xs = sp[g];
+            r.ws = i < count ? ws[g] : 0.0f;
         };
+        load(ring[0], 0);
+        for (int i0 = 0; i0 < count; i0 += 2) {
 #pragma unroll
-        for (int j = 0; j < D - 1; ++j)
-            load(ring[j], j);
-        for (int i0 = 0; i0 < count; i0 += D) {
-#pragma unroll
-            for (int j = 0; j < D; ++j) {
-                load(ring[(j + D - 1) % D], i0 + j + D - 1);
+            for (int j = 0; j < 2; ++j) {
+                load(ring[j ^ 1], i0 + j + 1);
                 __builtin_amdgcn_sched_barrier(0);
                 const Ring &r = ring[j];
+                const float f = r.xs * r.ws;
 #pragma unroll
-                for (int u = 0; u < U; ++u) {
-                    const float f = r.xs[u] * r.ws;
-                    if constexpr (S == 16) {
+                for (int t = 0; t < H; ++t) {
+                    const v4f c = multiply<!kBf16>(r.w[t], r.x, v4f{});
 #pragma unroll
-                        for (int t = 0; t < 2; ++t) {
-                            const v4f c = multiply<!kBf16>(r.w[t], r.x[u][0], v4f{});
-#pragma unroll
-                            for (int q = 0; q < 4; ++q)
-                                acc[u][t][q] = __builtin_fmaf(c[q], f, acc[u][t][q]);
-                        }
-                    } else {
-                        const v16f c = multiply<!kBf16>(r.w[1], r.x[u][1], multiply<!kBf16>(r.w[0], r.x[u][0], v16f{}));
-#pragma unroll
-                        for (int q = 0; q < 16; ++q)
-                            acc[u][0][q] = __builtin_fmaf(c[q], f, acc[u][0][q]);
-                    }
+                    for (int i = 0; i < 4; ++i)
+                        acc[t][i] = __builtin_fmaf(c[i], f, acc[t][i]);
                 }
                 __builtin_amdgcn_sched_barrier(0);
             }
         }
-        // the sums of a lane: token col, weight rows 4 h + .. (S 16, half t: 16 t more), 8 j + 4 h + .. (S 32)
-        float *red = s_red + wave * T * kPad;
+        // the sums of a lane: token col, weight rows 16 t + 4 q .. 4 q + 3
+        float *red = s_red + (wave * T + col) * kPad + 4 * q;
 #pragma unroll
-        for (int u = 0; u < U; ++u)
-#pragma unroll
-            for (int t = 0; t < kHalves; ++t)
-#pragma unroll
-                for (int j = 0; j < kRegs; j += 4)
-                    *reinterpret_cast<v4f *>(red + (S * u + col) * kPad + 16 * t + 2 * j + 4 * h) =
-                        v4f{acc[u][t][j], acc[u][t][j + 1], acc[u][t][j + 2], acc[u][t][j + 3]};
+        for (int t = 0; t < H; ++t)
+            *reinterpret_cast<v4f *>(red + 16 * t) = v4f{acc[t][0], acc[t][1], acc[t][2], acc[t][3]};
     }
     __syncthreads();
-    for (int i = tid; i < T * 8; i += W * 64) {
-        const int token = i >> 3, n4 = 4 * (i & 7);
+    for (int i = tid; i < T * 4 * H; i += W * 64) {
+        const int token = i / (4 * H), n4 = 4 * (i % (4 * H)), at = nt * kCols + n4;
         if (token >= rt.count)
             break;
         v4f v = {0.0f, 0.0f, 0.0f, 0.0f};
@@ -346,24 +320,349 @@ __global__ __launch_bounds__(W * 64) void fp8_stream_kernel(Fp8Args a)
 #pragma unroll
             for (int w = 0; w < W; ++w)
                 v += *reinterpret_cast<const v4f *>(s_red + (w * T + token) * kPad + n4);
-        const int at = nt * kTileN + n4;
         if (at < a.n)
             store_row4<kBf16>(a.out, (rt.row0 + token) * a.ldo + at, v, a.n - at, a.vec);
     }
 }
 
-template <bool kExperts, bool kBf16>
-int launch_products(const Fp8Args &a, hipStream_t stream)
+// LDS destination of the direct global-to-LDS copies.
+typedef __attribute__((address_space(3))) void *lds_ptr;
+typedef const __attribute__((address_space(4))) float *constant_floats; // read by scalar loads
+
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t open_rsrc(const void *base)
 {
-    const int64_t per = kExperts ? cdiv(a.er.r, a.er.experts) : a.er.r; // rows of an expert on average
-    const int tile = per <= 16 ? 16 : 32;
-    const int64_t tiles = kExperts ? expert_row_tiles(a.er.r, a.er.experts, tile) : cdiv(a.er.r, tile);
-    const int64_t wgs = tiles * a.ntiles;
-    MAMBO_REQUIRE(wgs <= 0x7FFFFFFF, MAMBO_ERR_VALUE, "too many rows and columns for one launch");
-    if (tile == 16)
-        MAMBO_LAUNCH((fp8_stream_kernel<16, 8, 3, kExperts, kBf16>), dim3((unsigned)wgs), dim3(512), 0, stream, a);
-    else
-        MAMBO_LAUNCH((fp8_stream_kernel<32, 8, 3, kExperts, kBf16>), dim3((unsigned)wgs), dim3(512), 0, stream, a);
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<void *>(base), 0, (int)0xFFFFFFFFu, 0x00020000);
+}
+
+// Row i's 16-byte chunk c lies at slot c ^ slot_of(i) of its 128 bytes in LDS: the chunks c of 16 consecutive rows lie in
+// different banks.
+__device__ __forceinline__ int slot_of(int row) { return (row ^ ((row >> 3) & 3)) & 7; }
+
+// More rows: bound by the matrix units where the launch fills the chip, else by the latency of a K group. A workgroup
+// computes 32 MT tokens x 32 NB WN weight rows with KG groups of WN waves, each group taking a KG-th of K; a wave owns 32 NB
+// weight rows and all the tokens. A K group's token rows are copied straight into LDS, double buffered, their scales beside
+// them; the weights go to registers as they lie. Within a wave the MFMAs of one 32 x 32 tile and the f32 scalings of
+// the one before alternate, and the LDS reads of the next 32 tokens go between.
+template <int MT, int NB, int WN, int KG, bool kExperts, bool kBf16>
+__global__ __launch_bounds__(WN * KG * 64) __attribute__((amdgpu_waves_per_eu(2))) void fp8_tile_kernel(Fp8Args a)
+{
+    constexpr int kRows = 32 * MT;
+    constexpr int kCopies = kRows / 8 / WN;            // of a wave, 1 KiB each: 8 rows
+    constexpr int kScaleCopies = (kRows + 63) / 64;    // of a K group, 64 rows each
+    constexpr int kRowBytes = kRows * kGroup;
+    static_assert(kRows % (8 * WN) == 0 && kScaleCopies <= WN, "copies spread evenly over the waves");
+    static_assert(WN == 2 || WN % 4 == 0, "a wave's copies lie 8 WN rows apart: slots of one kind, or of two in turn");
+    __shared__ __align__(1024) uint8_t s_rows0[KG * kRowBytes];
+    __shared__ __align__(1024) uint8_t s_rows1[KG * kRowBytes];
+    __shared__ __align__(256) float s_scale0[KG * 64 * kScaleCopies];
+    __shared__ __align__(256) float s_scale1[KG * 64 * kScaleCopies];
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int wgwave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int wave = wgwave % WN, kg = wgwave / WN; // wave within its K group
+    const int col = lane & 31, h = lane >> 5;
+    const int tiles_n = (a.ntiles + NB * WN - 1) / (NB * WN);
+    RowTile rt;
+    if (!row_tile<kExperts>(a, kRows, blockIdx.x / tiles_n, &rt))
+        return;
+    const int nt = (blockIdx.x % tiles_n) * (NB * WN) + wave * NB; // this wave's first tile of 32 weight rows
+    float acc[MT][NB][16];
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+                acc[mt][nb][i] = 0.0f;
+
+    if (!(kExperts && rt.expert == a.er.experts)) {
+        const int G = a.groups, per = (G + KG - 1) / KG, g0 = kg * per, end = g0 + per; // G and more: scaled by 0
+        // Copy j of a wave moves 8 rows, lane l chunk (l & 7) ^ slot_of(row) of row 8 (wave + WN j) + l / 8. Rows are told
+        // by 32-bit offsets: from the first row of the tile, or of all input rows where they are gathered (the host
+        // sees to it that these reach). Rows past the last one are the last one again.
+        const int chunk = (lane & 7) ^ slot_of((8 * wave + (lane >> 3)) & 31); // of even copies; odd ones with WN == 2: ^ 2
+        const __amdgpu_buffer_rsrc_t xr = open_rsrc(a.er.rows ? a.xv : a.xv + rt.row0 * a.ldxv);
+        uint32_t xo[kCopies];
+#pragma unroll
+        for (int j = 0; j < kCopies; ++j) {
+            const int row = min(8 * (wave + WN * j) + (lane >> 3), rt.count - 1);
+            xo[j] = (uint32_t)(a.er.rows ? source_row(a.er, rt.row0 + row) : row) * (uint32_t)a.ldxv;
+        }
+        const __amdgpu_buffer_rsrc_t sr = open_rsrc(a.er.rows ? a.xs : a.xs + rt.row0 * a.ldxs);
+        const int srow = min(64 * (wave % kScaleCopies) + lane, rt.count - 1);
+        const uint32_t so = 4u * (uint32_t)(a.er.rows ? source_row(a.er, rt.row0 + srow) : srow) * (uint32_t)a.ldxs;
+        // tiles past the weight's last read it again: their sums are not stored
+        __amdgpu_buffer_rsrc_t wp[NB];
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb)
+            wp[nb] = open_rsrc(a.packed + ((int64_t)rt.expert * a.ntiles + min(nt + nb, a.ntiles - 1)) * G * kFp8Tile);
+        const constant_floats ws = (constant_floats)(uintptr_t)(a.ws + ((int64_t)rt.expert * ((a.n + kGroup - 1) / kGroup) +
+                                                                        min(nt, a.ntiles - 1) * kTileN / kGroup) * G);
+        // a chunk past the row's end meets zero weights: any of the row does
+        const uint32_t whole = 16u * chunk, last = (G - 1) * kGroup + 16 * chunk < a.k ? whole : 0u;
+        const uint32_t whole1 = whole ^ 32u, last1 = (G - 1) * kGroup + (int)whole1 < a.k ? whole1 : 0u;
+
+        auto stage = [&](uint8_t *rows, float *scale, int g) {
+            const uint32_t off[2] = {g >= G - 1 ? last : whole, g >= G - 1 ? last1 : whole1};
+            const int gc = min(g, G - 1);
+#pragma unroll
+            for (int j = 0; j < kCopies; ++j) {
+                const uint32_t vo = xo[j] + off[WN == 2 ? j & 1 : 0]; // (the host pass drops the kernel with the element as an argument)
+                __builtin_amdgcn_raw_ptr_buffer_load_lds(xr, (lds_ptr)(rows + kg * kRowBytes + 1024 * (wave + WN * j)), 16,
+                                                         vo, gc * kGroup, 0, 0);
+            }
+            if (wave < kScaleCopies)
+                __builtin_amdgcn_raw_ptr_buffer_load_lds(sr, (lds_ptr)(scale + 64 * (kg * kScaleCopies + wave)), 4, so,
+                                                         4 * gc, 0, 0);
+        };
+        uint4 w[NB][2][2]; // [tile][K step of 64][half]
+        float wscale;
+        uint32_t lane16 = 16 * lane;
+        asm volatile("" : "+v"(lane16)); // or the compiler keeps a register for each of the four offsets below
+        auto load_w = [&](int g) {
+            const int gc = min(g, G - 1);
+#pragma unroll
+            for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const auto v = __builtin_amdgcn_raw_buffer_load_b128(wp[nb], lane16 + 1024 * j, gc * kFp8Tile, 0);
+                    w[nb][j >> 1][j & 1] = uint4{v[0], v[1], v[2], v[3]};
+                }
+            wscale = KG == 1 || g < G ? ws[gc] : 0.0f;
+        };
+        // chunk 4s + 2j + h of row r
+        uint32_t slot[2][2];
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            slot[j >> 1][j & 1] = kg * kRowBytes + 128u * col + 16u * ((2 * j + h) ^ slot_of(col));
+
+        auto multiply_group = [&](const uint8_t *rows, const float *scale) {
+            v16f c[2];
+            float f[2];
+            uint4 x[2][2][2];
+            auto load_x = [&](int mt) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    x[mt & 1][j >> 1][j & 1] = *reinterpret_cast<const uint4 *>(rows + 4096 * mt + slot[j >> 1][j & 1]);
+                f[mt & 1] = scale[64 * kg * kScaleCopies + 32 * mt + col] * wscale;
+            };
+            load_x(0);
+#pragma unroll
+            for (int p = 0; p <= MT * NB; ++p) {
+                const int mt = p / NB, nb = p % NB, q = p > 0 ? p - 1 : 0;
+                const float fq = f[(q / NB) & 1];
+                auto scale_sums = [&](int i0) {
+                    if (p > 0)
+#pragma unroll
+                        for (int i = i0; i < i0 + 8; ++i)
+                            acc[q / NB][q % NB][i] = __builtin_fmaf(c[q & 1][i], fq, acc[q / NB][q % NB][i]);
+                    __builtin_amdgcn_sched_barrier(0);
+                };
+                if (p < MT * NB) {
+                    c[p & 1] = multiply<!kBf16>(w[nb][0], x[mt & 1][0], v16f{});
+                    __builtin_amdgcn_sched_barrier(0);
+                    if (nb == 0 && NB > 1 && mt + 1 < MT)
+                        load_x(mt + 1);
+                }
+                scale_sums(0);
+                if (p < MT * NB) {
+                    c[p & 1] = multiply<!kBf16>(w[nb][1], x[mt & 1][1], c[p & 1]);
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+                scale_sums(8);
+                if (NB == 1 && p < MT * NB && mt + 1 < MT)
+                    load_x(mt + 1);
+            }
+        };
+        constexpr int kVm = 0x0F70 | (4 * NB); // the copies are done, the weights behind them need not be
+        stage(s_rows0, s_scale0, g0);
+        __builtin_amdgcn_sched_barrier(0);
+        load_w(g0);
+        __builtin_amdgcn_sched_barrier(0);
+        __builtin_amdgcn_s_waitcnt(kVm);
+        __syncthreads();
+        __builtin_amdgcn_sched_barrier(0);
+        for (int g = g0; g < end; g += 2) {
+            stage(s_rows1, s_scale1, g + 1);
+            __builtin_amdgcn_sched_barrier(0);
+            multiply_group(s_rows0, s_scale0);
+            __builtin_amdgcn_sched_barrier(0);
+            load_w(g + 1);
+            __builtin_amdgcn_sched_barrier(0);
+            __builtin_amdgcn_s_waitcnt(kVm);
+            __syncthreads();
+            __builtin_amdgcn_sched_barrier(0);
+            if (g + 1 >= end)
+                break;
+            stage(s_rows0, s_scale0, g + 2);
+            __builtin_amdgcn_sched_barrier(0);
+            multiply_group(s_rows1, s_scale1);
+            __builtin_amdgcn_sched_barrier(0);
+            load_w(g + 2);
+            __builtin_amdgcn_sched_barrier(0);
+            __builtin_amdgcn_s_waitcnt(kVm);
+            __syncthreads();
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        __builtin_amdgcn_s_waitcnt(0x0F70);
+        // the K groups' sums, the upper half's added to the lower half's until one is left
+        if constexpr (KG > 1) {
+            static_assert(WN * 4096 * (KG / 2) <= KG * kRowBytes, "half the groups' sums of a tile fit a buffer");
+#pragma unroll
+            for (int half = KG / 2; half > 0; half /= 2)
+#pragma unroll
+                for (int t = 0; t < MT * NB; ++t) {
+                    __syncthreads();
+                    float *red = reinterpret_cast<float *>(t & 1 ? s_rows1 : s_rows0) + 1024 * (wave + WN * (kg % half));
+                    float(&sum)[16] = acc[t / NB][t % NB];
+                    if (kg >= half && kg < 2 * half)
+#pragma unroll
+                        for (int i = 0; i < 16; ++i)
+                            red[64 * i + lane] = sum[i];
+                    __syncthreads();
+                    if (kg < half)
+#pragma unroll
+                        for (int i = 0; i < 16; ++i)
+                            sum[i] += red[64 * i + lane];
+                }
+        }
+    }
+    __syncthreads(); // every wave has read its last rows
+    if (kg)
+        return;
+    // A lane's sums are those of token col and weight rows 8 j + 4 h + 0 .. 3 of each 32: stored as they are, every store
+    // would touch 32 lines with 16 bytes each. They go through LDS, 128 bytes a token at a time (chunk c of token t at slot
+    // c ^ (t & 7), in a region of the wave's own), and out in whole lines.
+    constexpr int kSpan = kBf16 && NB > 1 ? 64 : 32; // columns
+    constexpr int kTiles = kSpan / kTileN;
+    constexpr int kBytes = kSpan * (kBf16 ? 2 : 4), kChunks = kBytes / 16; // of a token
+    static_assert(NB % kTiles == 0 && KG * kRowBytes >= kBytes * 32 * (WN / 2), "a region per wave");
+    uint8_t *region = (wave & 1 ? s_rows1 : s_rows0) + 32 * kBytes * (wave >> 1);
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+        for (int nb = 0; nb < NB; nb += kTiles) {
+#pragma unroll
+            for (int t = 0; t < kTiles; ++t)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const v4f v = {acc[mt][nb + t][4 * j], acc[mt][nb + t][4 * j + 1], acc[mt][nb + t][4 * j + 2],
+                                   acc[mt][nb + t][4 * j + 3]};
+                    const int c = kBf16 ? 4 * t + j : 2 * j + h;
+                    uint8_t *to = region + kBytes * col + 16 * (c ^ (col & (kChunks - 1)));
+                    if constexpr (kBf16)
+                        *reinterpret_cast<bf16x4 *>(to + 8 * h) = __builtin_convertvector(v, bf16x4);
+                    else
+                        *reinterpret_cast<v4f *>(to) = v;
+                }
+            const int c = lane & (kChunks - 1), at = (nt + nb) * kTileN + c * (kSpan / kChunks);
+#pragma unroll
+            for (int p = 0; p < kChunks / 2; ++p) {
+                const int t = 64 / kChunks * p + lane / kChunks, token = 32 * mt + t;
+                const uint4 v = *reinterpret_cast<const uint4 *>(region + kBytes * t + 16 * (c ^ (t & (kChunks - 1))));
+                if (token < rt.count)
+                    store_chunk<kBf16>(a.out, (rt.row0 + token) * a.ldo + at, v, a.n - at, a.vec);
+            }
+        }
+}
+
+// The kernels of a product: tokens and weight rows of a workgroup, K groups of waves in it, workgroups that a CU holds, and
+// microseconds: of a launch, of a round of workgroups on the busiest CU, of a step of a K group with 1, 2, .. of them on
+// the CU, per million outputs and per million weights.
+struct Fp8Kernel {
+    int tokens, rows, kg, resident;
+    double launch, round, step[4], outputs, weights;
+};
+// Fitted to 302 products (1 to 8192 tokens, 300 to 57344 rows, K 272 to 28672, weights rotated past the caches): 7 to
+// 15% rms each, and the kernel that they pick takes 2% (f32 1%) more than the fastest of the nine on average. None of the
+// nine is spare: without it the fastest of the others takes 0.4 to 3.6% more on average, up to 1.14 to 1.75 times.
+constexpr Fp8Kernel kFp8Kernels[2][9] = {
+    {{16, 16, 8, 2, 2.363, 0.561, {0.756, 1.488}, 15.108, 0.0},
+     {16, 32, 4, 4, 1.977, 1.064, {0.525, 1.1, 1.762, 2.27}, 4.977, 0.02},
+     {16, 64, 4, 4, 0.323, 2.951, {0.791, 1.711, 2.976, 3.97}, 2.418, 0.051},
+     {32, 64, 8, 1, 1.562, 2.093, {1.181}, 2.463, 0.104},
+     {64, 64, 4, 2, 1.93, 2.3, {0.976, 2.471}, 1.501, 0.062},
+     {64, 128, 2, 2, 3.063, 0.57, {0.953, 2.182}, 1.036, 0.068},
+     {64, 256, 2, 1, 2.137, 2.716, {1.588}, 1.186, 0.047},
+     {64, 256, 1, 2, 2.8, 1.188, {1.041, 1.632}, 0.78, 0.048},
+     {0, 0, 0, 0, 0.0, 0.0, {}, 0.0, 0.0}}, // 128 x 256 tiles through bf16 spill
+    {{16, 16, 8, 2, 2.539, 0.088, {0.793, 1.516}, 19.206, 0.0},
+     {16, 32, 4, 4, 2.301, 0.446, {0.532, 1.116, 1.787, 2.217}, 6.001, 0.017},
+     {16, 64, 4, 4, 1.381, 1.564, {0.812, 1.758, 3.018, 4.113}, 3.182, 0.039},
+     {32, 64, 8, 1, 1.854, 1.6, {1.242}, 1.817, 0.106},
+     {64, 64, 4, 2, 2.907, 0.841, {0.727, 1.744}, 0.867, 0.083},
+     {64, 128, 2, 2, 3.059, 0.173, {0.606, 1.316}, 0.48, 0.098},
+     {64, 256, 2, 1, 1.547, 2.554, {1.033}, 0.415, 0.099},
+     {64, 256, 1, 2, 1.666, 1.661, {0.666, 1.032}, 0.29, 0.076},
+     {128, 256, 1, 2, 1.438, 2.763, {1.001, 1.619}, 0.307, 0.062}}};
+constexpr int kFirstTile = 3; // those from here on address rows by 32-bit offsets
+constexpr int64_t kCUs = 256;
+
+double fp8_time(const Fp8Kernel &t, int64_t wgs, int64_t groups, double outputs, double weights)
+{
+    const int64_t per = cdiv(wgs, kCUs), full = per / t.resident, rem = per % t.resident;
+    return t.launch + t.round * (double)(full + (rem ? 1 : 0)) +
+           (double)cdiv(groups, t.kg) * ((double)full * t.step[t.resident - 1] + (rem ? t.step[rem - 1] : 0.0)) +
+           1e-6 * (t.outputs * outputs + t.weights * weights);
+}
+
+// The kernel of a product and its grid. How the rows fall to the experts is not known here: the tiles that they take
+// are counted for rows that fall to them at random, and the grid holds the most that they can take.
+int fp8_plan(const Fp8Args &a, bool bf16, int64_t *wgs)
+{
+    const ExpertRows &er = a.er;
+    const bool far = a.ldxv * (er.rows ? er.m : 128) + a.k >= ((int64_t)1 << 32) ||
+                     4 * (a.ldxs * (er.rows ? er.m : 128) + a.groups) >= ((int64_t)1 << 32);
+    const double r = (double)er.r, taken = er.offsets ? er.experts * -std::expm1(-r / er.experts) : 1.0;
+    int best = -1;
+    double least = 0.0;
+    for (int i = 0; i < (far ? kFirstTile : 9); ++i) {
+        const Fp8Kernel &t = kFp8Kernels[bf16][i];
+        if (!t.tokens)
+            continue;
+        const int64_t columns = cdiv(a.n, t.rows), most = er.offsets ? expert_row_tiles(er.r, er.experts, t.tokens) : cdiv(er.r, t.tokens);
+        if (most * columns > 0x7FFFFFFF)
+            continue;
+        const double tiles = er.offsets ? std::fmax(taken, r / t.tokens + 0.5 * taken) : (double)most;
+        const double us = fp8_time(t, (int64_t)std::ceil(tiles) * columns, a.groups, r * a.n, taken * a.n * a.k);
+        if (best < 0 || us < least) {
+            best = i;
+            least = us;
+            *wgs = most * columns;
+        }
+    }
+    return best;
+}
+
+template <bool kExperts, bool kBf16>
+int launch_products(const Fp8Args &a, int which, int64_t wgs, hipStream_t stream)
+{
+#define MAMBO_STREAM(I, H, W)                                                                                      \
+    case I:                                                                                                        \
+        MAMBO_LAUNCH((fp8_stream_kernel<H, W, kExperts, kBf16>), dim3((unsigned)wgs), dim3(W * 64), 0, stream, a); \
+        break
+#define MAMBO_TILE(I, MT, NB, WN, KG)                                                                              \
+    case I:                                                                                                        \
+        MAMBO_LAUNCH((fp8_tile_kernel<MT, NB, WN, KG, kExperts, kBf16>), dim3((unsigned)wgs), dim3(WN * KG * 64), 0,     \
+                     stream, a);                                                                                   \
+        break
+    switch (which) {
+        MAMBO_STREAM(0, 1, 8);
+        MAMBO_STREAM(1, 2, 4);
+        MAMBO_STREAM(2, 4, 4);
+        MAMBO_TILE(3, 1, 1, 2, 8);
+        MAMBO_TILE(4, 2, 1, 2, 4);
+        MAMBO_TILE(5, 2, 1, 4, 2);
+        MAMBO_TILE(6, 2, 2, 4, 2);
+        MAMBO_TILE(7, 2, 2, 4, 1);
+    default:
+        if constexpr (kBf16) {
+            switch (which) {
+                MAMBO_TILE(8, 4, 2, 4, 1);
+            }
+        }
+    }
+#undef MAMBO_STREAM
+#undef MAMBO_TILE
     return mambo_check_launch("fp8_block_matmul");
 }
 
@@ -387,9 +686,12 @@ int run_products(const uint8_t *xv, int64_t ldxv, const float *xs, int64_t ldxs,
     Fp8Args a = {xv, xs, ldxv, ldxs, er, packed, ws, out, ldo, (int)n, (int)k, (int)cdiv(k, kGroup), (int)cdiv(n, kTileN),
                  rows_take_vectors(out, ldo, out_dtype)};
     const bool bf16 = out_dtype == MAMBO_DTYPE_BF16;
+    int64_t wgs = 0;
+    const int which = fp8_plan(a, bf16, &wgs);
+    MAMBO_REQUIRE(which >= 0, MAMBO_ERR_VALUE, "too many rows and columns for one launch");
     if (er.offsets)
-        return bf16 ? launch_products<true, true>(a, stream) : launch_products<true, false>(a, stream);
-    return bf16 ? launch_products<false, true>(a, stream) : launch_products<false, false>(a, stream);
+        return bf16 ? launch_products<true, true>(a, which, wgs, stream) : launch_products<true, false>(a, which, wgs, stream);
+    return bf16 ? launch_products<false, true>(a, which, wgs, stream) : launch_products<false, false>(a, which, wgs, stream);
 }
 
 } // namespace
