@@ -1,6 +1,8 @@
 // Rows grouped by expert: what the grouped products are told of them, the search of a workgroup's
 // rows, and the stores of f32 sums as f32 or bf16.
 #pragma once
+#include <type_traits>
+
 #include "mambo_common.h"
 
 // r output rows, expert e's at [offsets[e], offsets[e+1]); row i reads row rows[i] (NULL: i) of the m

@@ -5,10 +5,10 @@
 // registers, decoded as the dense kernel's (iq3s_dense.h): exact two-term E4M3 operands in the order of
 // the dense MFMA, four MFMAs a block and 16 rows, the block's fp16 d in f32. The waves' sums meet in
 // LDS at the end and are added in order.
-#include <type_traits>
+#include <cmath>
 
-#include "experts.h"
 #include "iq3s_dense.h"
+#include "iq3s_wide.h"
 
 namespace {
 
@@ -154,13 +154,27 @@ extern "C" int mambo_iq3s_fp8_matmul_experts(const uint8_t *xv, int64_t ldxv, co
                   MAMBO_ERR_VALUE, "rows and packed weights must be 16-byte aligned, scales 8-byte aligned");
     MAMBO_REQUIRE((uintptr_t)out % (out_dtype == MAMBO_DTYPE_BF16 ? 2 : 4) == 0, MAMBO_ERR_VALUE,
                   "outputs must be aligned to their type");
-    const Iq3sArgs a = {xv, xs, ldxv, ldxs, {offsets, rows, r, m, (int)experts}, packed, expert_stride, out, ldo, (int)n,
+    const ExpertRows er = {offsets, rows, r, m, (int)experts};
+    const bool bf16 = out_dtype == MAMBO_DTYPE_BF16;
+    hipStream_t s = (hipStream_t)stream;
+    // the 32 x 32 MFMA kernel from 17 rows of an expert on; it tells rows by 32-bit offsets
+    const double taken = (double)experts * -std::expm1(-(double)r / (double)experts);
+    if ((double)r > 16.0 * taken && (rows ? m : 256) * ldxv + 256 * blocks < ((int64_t)1 << 32) &&
+        (rows ? m : 256) * ldxs + 8 * blocks < ((int64_t)1 << 32) && expert_row_tiles(r, experts, 64) <= 65535) {
+        double tiles_of[2];
+        for (int i = 0; i < 2; ++i)
+            tiles_of[i] = std::fmax(taken, (double)r / (64 << i) + 0.5 * taken);
+        WidePlan plan;
+        mambo_wide_experts_plan(er, n, blocks, tiles_of, &plan);
+        return mambo_wide_experts_launch(plan, xv, ldxv, xs, ldxs, er, packed, expert_stride, n, blocks, out, bf16, ldo, s);
+    }
+    const Iq3sArgs a = {xv, xs, ldxv, ldxs, er, packed, expert_stride, out, ldo, (int)n,
                         (int)blocks, (int)((n + 31) / 32), rows_take_vectors(out, ldo, out_dtype)};
     const int64_t wgs = expert_row_tiles(r, experts, 16) * a.ntiles;
     MAMBO_REQUIRE(wgs <= 0x7FFFFFFF, MAMBO_ERR_VALUE, "too many rows and columns for one launch");
-    if (out_dtype == MAMBO_DTYPE_BF16)
-        MAMBO_LAUNCH((iq3s_expert_stream_kernel<4, true>), dim3((unsigned)wgs), dim3(256), 0, (hipStream_t)stream, a);
+    if (bf16)
+        MAMBO_LAUNCH((iq3s_expert_stream_kernel<4, true>), dim3((unsigned)wgs), dim3(256), 0, s, a);
     else
-        MAMBO_LAUNCH((iq3s_expert_stream_kernel<4, false>), dim3((unsigned)wgs), dim3(256), 0, (hipStream_t)stream, a);
+        MAMBO_LAUNCH((iq3s_expert_stream_kernel<4, false>), dim3((unsigned)wgs), dim3(256), 0, s, a);
     return mambo_check_launch("iq3s_fp8_matmul_experts");
 }

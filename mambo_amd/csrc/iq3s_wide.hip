@@ -48,6 +48,7 @@
 #include "iq3s_wide.h"
 #include "iq3s_wide_copies.h"
 
+#include "experts.h"
 #include "iq3s_dense.h"
 
 namespace {
@@ -131,10 +132,22 @@ __device__ __forceinline__ void finish_words(uint32_t p, const uint32_t (&lw)[8]
 
 // kPolicy: cache policy of the weight loads, non-temporal where one token tile reads each
 // weight once (57344 x 8192 at 128 tokens 0-2%), the default where several do.
-template <int MT, int W, int KG, int kPolicy>
+// Experts: WideExperts for rows grouped by expert (ga names one projection, the first expert's, and its
+// outputs), whose row tiles blockIdx.y counts; WideDense for rows of one weight.
+struct WideDense {
+    static constexpr bool kExperts = false, kBf16 = false;
+};
+template <bool kBf16Out>
+struct WideExperts {
+    static constexpr bool kExperts = true, kBf16 = kBf16Out;
+    ExpertRows er;
+    int64_t expert_stride; // bytes between the experts' packed weights
+};
+
+template <int MT, int W, int KG, int kPolicy, class Rows>
 __global__ __launch_bounds__(W * KG * 64) __attribute__((amdgpu_waves_per_eu(2))) void gemm_wide_kernel(
     const uint8_t *__restrict__ xv, int64_t ldxv, const uint8_t *__restrict__ xs, int64_t ldxs, int64_t M, GroupArgs ga,
-    int B, int bps, int atomic)
+    int B, int bps, int atomic, Rows rows)
 {
     constexpr int kRows = 32 * MT;
     constexpr int kVCopies = kRows / 4 / W;
@@ -167,8 +180,23 @@ __global__ __launch_bounds__(W * KG * 64) __attribute__((amdgpu_waves_per_eu(2))
             wg = blockIdx.x - ga.tile_begin[i];
         }
     const int64_t tiles = (N + kTileRows - 1) / kTileRows;
-    const int64_t m0 = (int64_t)blockIdx.y * kRows;
+    int64_t m0 = (int64_t)blockIdx.y * kRows;
     const int64_t tile = 2 * (wg * W + wave); // first of this wave's two 16-row tiles
+    if constexpr (Rows::kExperts) {
+        RowTile rt;
+        if (!find_row_tile(rows.er, kRows, (int)blockIdx.y, &rt))
+            return;
+        m0 = rt.row0;
+        M = m0 + rt.count;
+        if (rt.expert == rows.er.experts) { // rows of no expert
+            const int64_t n = tile * kTileRows + r32;
+            if (kg == 0 && n < N)
+                for (int64_t m = m0 + g; m < M; m += 2)
+                    reinterpret_cast<row_t<Rows::kBf16> *>(out)[m * ldo + n] = (row_t<Rows::kBf16>)0.0f;
+            return;
+        }
+        packed += rt.expert * rows.expert_stride;
+    }
     const __amdgpu_buffer_rsrc_t wt = byte_rsrc(packed + min(tile, tiles - 1) * (int64_t)B * kTileBytes);
     const uint32_t second = (lane & 16) && tile + 1 < tiles ? (uint32_t)B * kTileBytes : 0u;
     const uint32_t rl = (uint32_t)(col + 16 * g);
@@ -185,14 +213,30 @@ __global__ __launch_bounds__(W * KG * 64) __attribute__((amdgpu_waves_per_eu(2))
         return __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t *>(base + m0 * ld), 0,
                                                  __builtin_amdgcn_readfirstlane((int)n), 0x00020000);
     };
-    const __amdgpu_buffer_rsrc_t xrows = rows_rsrc(xv, ldxv, B * 256), srows = rows_rsrc(xs, ldxs, B * 8);
+    bool gather = false; // the tokens' rows, by offsets from the first of all of them
+    if constexpr (Rows::kExperts)
+        gather = rows.er.rows != nullptr;
+    const __amdgpu_buffer_rsrc_t xrows = gather ? byte_rsrc(xv) : rows_rsrc(xv, ldxv, B * 256),
+                                 srows = gather ? byte_rsrc(xs) : rows_rsrc(xs, ldxs, B * 8);
     const int last_row = (int)min<int64_t>(M - 1 - m0, kRows - 1);
     const int srow = wave & (MT - 1); // waves past MT repeat a scale copy (the same bytes): no branch
     uint32_t voff[kVCopies];
 #pragma unroll
     for (int j = 0; j < kVCopies; ++j)
         voff[j] = wide_value_offset(wave, lane, W, j, last_row, (uint32_t)ldxv);
-    const uint32_t soff_stage = wide_scale_offset(srow, lane, last_row, (uint32_t)ldxs);
+    uint32_t soff_stage = wide_scale_offset(srow, lane, last_row, (uint32_t)ldxs);
+    if constexpr (Rows::kExperts) {
+        if (gather) {
+#pragma unroll
+            for (int j = 0; j < kVCopies; ++j) {
+                const int row = 4 * (wave + W * j) + (lane >> 4);
+                voff[j] = (uint32_t)source_row(rows.er, m0 + min(row, last_row)) * (uint32_t)ldxv +
+                          16u * (uint32_t)((lane & 15) ^ (row & 15));
+            }
+            soff_stage = (uint32_t)source_row(rows.er, m0 + min(32 * srow + (lane >> 1), last_row)) * (uint32_t)ldxs +
+                         4u * (uint32_t)(lane & 1);
+        }
+    }
 
     const uint32_t a0 = (uint32_t)(kg * kRows * 256) + 256u * r32 + 16u * (uint32_t)(g ^ col);
     const uint32_t soff = (uint32_t)(kg * kRows * 8) + 8u * r32 + 2u * g;
@@ -429,7 +473,9 @@ __global__ __launch_bounds__(W * KG * 64) __attribute__((amdgpu_waves_per_eu(2))
             for (int i = 0; i < 16; ++i) {
                 const int64_t m = m0 + 32 * mt + 8 * (i >> 2) + 4 * g + (i & 3);
                 if (m < M) {
-                    if (atomic)
+                    if constexpr (Rows::kBf16)
+                        reinterpret_cast<__bf16 *>(out)[m * ldo + n] = (__bf16)acc[mt][i];
+                    else if (atomic)
                         atomicAdd(out + m * ldo + n, acc[mt][i]);
                     else
                         __builtin_nontemporal_store(acc[mt][i], out + m * ldo + n);
@@ -488,11 +534,11 @@ void launch_wide(const WidePlan &p, dim3 grid, hipStream_t stream, const uint8_t
                  int64_t ldxs, int64_t m, const GroupArgs &ga, int blocks)
 {
     if (grid.y > 1)
-        MAMBO_LAUNCH((gemm_wide_kernel<MT, W, KG, 0>), grid, dim3(W * KG * 64), 0, stream, xv, ldxv, xs, ldxs, m,
-                     ga, blocks, p.bps, p.splits > 1);
+        MAMBO_LAUNCH((gemm_wide_kernel<MT, W, KG, 0, WideDense>), grid, dim3(W * KG * 64), 0, stream, xv, ldxv, xs, ldxs, m,
+                     ga, blocks, p.bps, p.splits > 1, WideDense{});
     else
-        MAMBO_LAUNCH((gemm_wide_kernel<MT, W, KG, kStreamPolicy>), grid, dim3(W * KG * 64), 0, stream, xv, ldxv, xs,
-                     ldxs, m, ga, blocks, p.bps, p.splits > 1);
+        MAMBO_LAUNCH((gemm_wide_kernel<MT, W, KG, kStreamPolicy, WideDense>), grid, dim3(W * KG * 64), 0, stream, xv, ldxv, xs,
+                     ldxs, m, ga, blocks, p.bps, p.splits > 1, WideDense{});
 }
 
 } // namespace
@@ -592,4 +638,55 @@ int mambo_wide_launch(const WidePlan &p, const uint8_t *xv, int64_t ldxv, const 
     MAMBO_WIDE_SHAPE(4, 8, 1);
 #undef MAMBO_WIDE_SHAPE
     return mambo_check_launch("iq3s_fp8_matmul (wide)");
+}
+
+// Rows grouped by expert: one round of the weights per tile of rows, K unsplit (no atomics), the shapes of one K group,
+// by the same times with the tiles that rows falling to the experts at random take (fp8_plan counts them alike).
+double mambo_wide_experts_plan(const ExpertRows &er, int64_t n, int64_t blocks, double tiles_of[2], WidePlan *plan)
+{
+    const double mb = 4e-6 * (double)er.r * (double)n;
+    double best = 0.0;
+    for (const WideShape &w : kWideShapes) {
+        if (w.kg > 1)
+            continue;
+        const int64_t wgs = cdiv(cdiv(n, 32), w.waves) * (int64_t)(tiles_of[w.mt == 4] + 0.5);
+        const double t = wide_time(w, wgs, blocks, 1, mb);
+        if (best == 0.0 || t < best) {
+            best = t;
+            *plan = {w.mt, w.waves, w.kg, 1, (int)blocks, t};
+        }
+    }
+    return best;
+}
+
+template <int MT, int W>
+static void launch_wide_experts(dim3 grid, hipStream_t stream, const uint8_t *xv, int64_t ldxv, const uint8_t *xs, int64_t ldxs,
+                                const GroupArgs &ga, int blocks, bool bf16, const ExpertRows &er, int64_t expert_stride)
+{
+    if (bf16)
+        MAMBO_LAUNCH((gemm_wide_kernel<MT, W, 1, 0, WideExperts<true>>), grid, dim3(W * 64), 0, stream, xv, ldxv, xs, ldxs,
+                     (int64_t)0, ga, blocks, blocks, 0, (WideExperts<true>{er, expert_stride}));
+    else
+        MAMBO_LAUNCH((gemm_wide_kernel<MT, W, 1, 0, WideExperts<false>>), grid, dim3(W * 64), 0, stream, xv, ldxv, xs, ldxs,
+                     (int64_t)0, ga, blocks, blocks, 0, (WideExperts<false>{er, expert_stride}));
+}
+
+int mambo_wide_experts_launch(const WidePlan &p, const uint8_t *xv, int64_t ldxv, const uint8_t *xs, int64_t ldxs,
+                              const ExpertRows &er, const uint8_t *packed, int64_t expert_stride, int64_t n, int64_t blocks,
+                              void *out, bool bf16, int64_t ldo, hipStream_t stream)
+{
+    GroupArgs ga = {};
+    ga.count = 1;
+    ga.packed[0] = packed;
+    ga.out[0] = (float *)out;
+    ga.n[0] = n;
+    ga.ldo[0] = ldo;
+    const dim3 grid((unsigned)cdiv(cdiv(n, 32), p.waves), (unsigned)expert_row_tiles(er.r, er.experts, 32 * p.mt));
+    if (p.mt == 2)
+        launch_wide_experts<2, 4>(grid, stream, xv, ldxv, xs, ldxs, ga, (int)blocks, bf16, er, expert_stride);
+    else if (p.waves == 4)
+        launch_wide_experts<4, 4>(grid, stream, xv, ldxv, xs, ldxs, ga, (int)blocks, bf16, er, expert_stride);
+    else
+        launch_wide_experts<4, 8>(grid, stream, xv, ldxv, xs, ldxs, ga, (int)blocks, bf16, er, expert_stride);
+    return mambo_check_launch("iq3s_fp8_matmul_experts");
 }
