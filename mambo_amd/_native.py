@@ -210,21 +210,6 @@ def device_arch(device=None) -> str:
 _here = nullcontext()
 
 
-def on_stream(stream, device):
-    """Context in which torch's memory of `device` belongs to `stream` (None, an int handle or a
-    torch.cuda.Stream): what a launcher allocates or copies for work on that stream must not be
-    handed out again, or written, in the order of another."""
-    import torch
-    if stream is None:
-        return _here
-    handle = stream_handle(stream)
-    if handle == torch._C._cuda_getCurrentRawStream(device.index):
-        return _here
-    if not isinstance(stream, torch.cuda.Stream):
-        stream = torch.cuda.ExternalStream(handle, device=device) if handle else torch.cuda.default_stream(device)
-    return torch.cuda.stream(stream)
-
-
 def on_device(device):
     """Context with `device` (a tensor's) current; nothing to do where it is already, as in most
     calls: entering and leaving torch.cuda.device costs an eager call about 2 us. An exchange with
@@ -237,6 +222,22 @@ def on_device(device):
             return _here
         torch.cuda._maybe_exchange_device(before)
     return torch.cuda.device(device)
+
+
+def launch_on(device, stream):
+    """Context of a launch on `stream` of `device`: the device current, as on_device, and torch's memory
+    belonging to the stream where that is not the current one - what a launcher allocates or copies for
+    work on a stream must not be handed out again, or written, in the order of another."""
+    here = on_device(device)
+    if stream is None:
+        return here
+    import torch
+    handle = stream_handle(stream)
+    if here is _here and handle == torch._C._cuda_getCurrentRawStream(device.index):
+        return here
+    if not isinstance(stream, torch.cuda.Stream):
+        stream = torch.cuda.ExternalStream(handle, device=device) if handle else torch.cuda.default_stream(device)
+    return torch.cuda.stream(stream)  # makes the stream's device current too
 
 
 def ptr(t) -> int:

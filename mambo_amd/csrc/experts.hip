@@ -8,10 +8,11 @@ namespace {
 int64_t cdiv(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 // ============================================================================ router
-// One wave per token, V logits a lane (expert 64 v + lane). A logit's key orders as the logit does
-// (sign-folded bits, -0 as 0; 0: not to be chosen), so a choice is the largest key and, of equal ones,
-// the lowest expert: a maximum over the lanes, a ballot of those that hold it and the lowest index of
-// these. Each choice takes its key out. Bound by the lane swaps: six a choice.
+// One wave per token, V logits a lane (experts V * lane .. + V - 1). A logit's key orders as the logit
+// does (sign-folded bits, -0 as 0; 0: not to be chosen), so a choice is the largest key and, of equal
+// ones, the lowest expert: a maximum over the lanes, the lowest lane that holds it and that lane's first.
+// Each choice takes its key out; the softmax is taken of the choices at the end, one a lane. Bound by the
+// vector instructions of a choice (about 20 + 5 V).
 __device__ __forceinline__ uint32_t logit_key(float l)
 {
     if (!(l > -__builtin_inff())) // -inf and NaN
@@ -28,23 +29,46 @@ __device__ __forceinline__ float key_logit(uint32_t key)
 // exp(l - max), with 1 where both are infinite
 __device__ __forceinline__ float softmax_term(float l, float max) { return l == max ? 1.0f : expf(l - max); }
 
-template <int V, bool kBf16>
-__global__ __launch_bounds__(256) void route_choose_kernel(const void *__restrict__ logits, int64_t ld, int64_t m,
-                                                           int experts, int top_k, bool renormalize,
-                                                           int32_t *__restrict__ ids, float *__restrict__ weights)
+// Maximum over the wave's lanes by DPP moves: pairs, fours, halves and whole rows of 16, then across rows.
+template <int kCtrl>
+__device__ __forceinline__ uint32_t max_dpp(uint32_t v)
 {
-    const int lane = threadIdx.x & 63;
-    const int64_t token = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (token >= m)
-        return;
+    return ::max(v, (uint32_t)__builtin_amdgcn_update_dpp((int)v, (int)v, kCtrl, 0xF, 0xF, false));
+}
+__device__ __forceinline__ uint32_t wave_max(uint32_t v)
+{
+    v = max_dpp<0xB1>(v);  // quad_perm 1 0 3 2
+    v = max_dpp<0x4E>(v);  // quad_perm 2 3 0 1
+    v = max_dpp<0x141>(v); // row_half_mirror
+    v = max_dpp<0x140>(v); // row_mirror
+    const uint32_t a = ::max((uint32_t)__builtin_amdgcn_readlane((int)v, 0), (uint32_t)__builtin_amdgcn_readlane((int)v, 16));
+    const uint32_t b = ::max((uint32_t)__builtin_amdgcn_readlane((int)v, 32), (uint32_t)__builtin_amdgcn_readlane((int)v, 48));
+    return ::max(a, b);
+}
+
+// Sum over the wave's lanes.
+__device__ __forceinline__ float wave_sum(float v)
+{
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1)
+        v += __shfl_xor(v, d);
+    return v;
+}
+
+// The choices of one token by one wave: lane j < top_k gets choice j.
+template <int V, bool kBf16>
+__device__ __forceinline__ void choose(const void *logits, int64_t ld, int64_t token, int experts, int top_k,
+                                       bool renormalize, int lane, int *id_out, float *weight_out)
+{
     const row_t<kBf16> *row = reinterpret_cast<const row_t<kBf16> *>(logits) + token * ld;
     uint32_t key[V];
 #pragma unroll
     for (int v = 0; v < V; ++v) {
-        const int e = 64 * v + lane;
+        const int e = V * lane + v;
         key[v] = e < experts ? logit_key((float)row[e]) : 0u;
     }
-    float max = 0.0f, sum = 0.0f, mine = 0.0f; // lane j keeps choice j
+    float all = 0.0f; // softmax terms of all experts
+    uint32_t mine = 0u, first = 0u;
     int id = -1;
     for (int j = 0; j < top_k; ++j) {
         uint32_t best = key[0];
@@ -55,167 +79,283 @@ __global__ __launch_bounds__(256) void route_choose_kernel(const void *__restric
                 best = key[v];
                 at = v;
             }
-        uint32_t top = best;
-#pragma unroll
-        for (int d = 1; d < 64; d <<= 1)
-            top = ::max(top, (uint32_t)__shfl_xor((int)top, d));
+        const uint32_t top = wave_max(best);
         if (top == 0u)
             break;
-        int e = best == top ? 64 * at + lane : 0x7FFFFFFF; // a lane's lowest of equal keys
-        const uint64_t holders = __ballot(best == top);
-        if (holders & (holders - 1)) { // several lanes hold it
-#pragma unroll
-            for (int d = 1; d < 64; d <<= 1)
-                e = min(e, __shfl_xor(e, d));
-        } else {
-            e = __builtin_amdgcn_readlane(e, __builtin_ctzll(holders));
-        }
-        if ((e & 63) == lane) {
-#pragma unroll
-            for (int v = 0; v < V; ++v)
-                if (v == e >> 6) {
-                    key[v] = 0u;
-                }
-        }
-        const float l = key_logit(top);
         if (j == 0) {
-            max = l;
+            first = top;
             if (!renormalize) {
-                float s = 0.0f;
+                float t = 0.0f;
 #pragma unroll
-                for (int v = 0; v < V; ++v) // the first choice's key is out already
-                    s += key[v] ? softmax_term(key_logit(key[v]), max) : 0.0f;
-#pragma unroll
-                for (int d = 1; d < 64; d <<= 1)
-                    s += __shfl_xor(s, d);
-                sum = s + 1.0f;
+                for (int v = 0; v < V; ++v)
+                    t += key[v] ? softmax_term(key_logit(key[v]), key_logit(top)) : 0.0f;
+                all = wave_sum(t);
             }
         }
-        const float p = softmax_term(l, max);
-        if (renormalize)
-            sum += p;
+        const int holder = __builtin_ctzll(__ballot(best == top));
+        const int slot = V == 1 ? 0 : __builtin_amdgcn_readlane(at, holder);
+        if (lane == holder)
+#pragma unroll
+            for (int v = 0; v < V; ++v)
+                if (v == slot)
+                    key[v] = 0u;
         if (lane == j) {
-            mine = p;
-            id = e;
+            mine = top;
+            id = V * holder + slot;
         }
     }
+    const float term = id < 0 ? 0.0f : softmax_term(key_logit(mine), key_logit(first));
+    if (renormalize)
+        all = wave_sum(term);
+    *id_out = id;
+    *weight_out = id < 0 ? 0.0f : term / all;
+}
+
+template <int V, bool kBf16>
+__global__ __launch_bounds__(256) void route_choose_kernel(const void *__restrict__ logits, int64_t ld, int64_t m,
+                                                           int experts, int top_k, bool renormalize,
+                                                           int32_t *__restrict__ ids, float *__restrict__ weights)
+{
+    const int lane = threadIdx.x & 63;
+    const int64_t token = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (token >= m)
+        return;
+    int id;
+    float weight;
+    choose<V, kBf16>(logits, ld, token, experts, top_k, renormalize, lane, &id, &weight);
     if (lane < top_k) {
         ids[token * top_k + lane] = id;
-        weights[token * top_k + lane] = id < 0 ? 0.0f : mine / sum;
+        weights[token * top_k + lane] = weight;
     }
 }
 
-// Workgroup e counts the choices of lower experts and its own, a stretch of the choices a thread, and
-// puts its own down in their order: a sort that keeps the order of tokens, with no counter that
-// workgroups share and the same result every time. e == experts: the choices of none. The choices
-// are read by every workgroup, out of the caches.
-constexpr int kSortThreads = 256;
+// Workgroup e counts the choices of lower experts and its own, a stretch of the choices a wave, and puts
+// its own down in their order: a sort that keeps the order of tokens, with no counter that workgroups share
+// and the same result every time. e == experts: the choices of none, -1, which is after them all as an
+// unsigned number. Every workgroup reads all choices, out of the caches, two vector instructions for 64 of
+// them (65536 choices of 256 experts, 67 MB: 12.4 us; as 256 lanes with a stretch each 118).
+constexpr int kSortWaves = 16;
+constexpr int kSortLoads = 8; // of 64 choices each, in flight
 
-__global__ __launch_bounds__(kSortThreads) void route_sort_kernel(const int32_t *__restrict__ ids, int count, int top_k,
-                                                                  int experts, int32_t *__restrict__ offsets,
-                                                                  int32_t *__restrict__ rows, int32_t *__restrict__ slots)
+__global__ __launch_bounds__(kSortWaves * 64) void route_sort_kernel(const uint32_t *__restrict__ ids, int count, int top_k,
+                                                                     int experts, int32_t *__restrict__ offsets,
+                                                                     int32_t *__restrict__ rows,
+                                                                     int32_t *__restrict__ slots)
 {
-    __shared__ int s_less[kSortThreads / 64], s_equal[kSortThreads / 64];
-    const int e = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const int per = (count + kSortThreads - 1) / kSortThreads;
-    const int lo = (int)min<int64_t>((int64_t)tid * per, count), hi = min(lo + per, count);
-    int less = 0, equal = 0;
-    for (int i = lo; i < hi; ++i) {
-        const int id = ids[i] < 0 ? experts : ids[i];
-        less += id < e;
-        equal += id == e;
-    }
-    int before = equal; // own choices of the lanes up to this one
+    __shared__ int s_less[kSortWaves], s_equal[kSortWaves];
+    const int e = blockIdx.x, tid = threadIdx.x, lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const uint32_t own = e < experts ? (uint32_t)e : 0xFFFFFFFFu;
+    const int per = (int)(((int64_t)count + 64 * kSortWaves - 1) / (64 * kSortWaves)) * 64;
+    const int lo = (int)min<int64_t>((int64_t)wave * per, count), hi = (int)min<int64_t>((int64_t)lo + per, count);
+    // eight times 64 choices from i on; `last`: those past the stretch are of no expert, and not -1
+    auto load = [&](uint32_t(&id)[kSortLoads], int i, bool last) {
 #pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-        const int up = __shfl_up(before, d);
-        before += lane >= d ? up : 0;
-        less += __shfl_xor(less, d);
-    }
-    if (lane == 63) {
-        s_equal[wave] = before;
+        for (int j = 0; j < kSortLoads; ++j)
+            id[j] = !last || i + 64 * j + lane < hi ? ids[i + 64 * j + lane] : 0xFFFFFFFEu;
+    };
+    constexpr int kStep = 64 * kSortLoads;
+    int less = 0, equal = 0;
+    auto tally = [&](int i, bool last) {
+        uint32_t id[kSortLoads];
+        load(id, i, last);
+#pragma unroll
+        for (int j = 0; j < kSortLoads; ++j) {
+            less += __popcll(__ballot(id[j] < (uint32_t)e));
+            equal += __popcll(__ballot(id[j] == own));
+        }
+    };
+    int i = lo;
+    for (; i + kStep <= hi; i += kStep)
+        tally(i, false);
+    if (i < hi)
+        tally(i, true);
+    if (lane == 0) {
         s_less[wave] = less;
+        s_equal[wave] = equal;
     }
     __syncthreads();
-    int at = before - equal, begin = 0;
+    int at = 0, begin = 0;
 #pragma unroll
-    for (int w = 0; w < kSortThreads / 64; ++w) {
+    for (int w = 0; w < kSortWaves; ++w) {
         begin += s_less[w];
         at += w < wave ? s_equal[w] : 0;
     }
     if (tid == 0)
         offsets[e] = begin;
+    if (equal == 0)
+        return;
     at += begin;
-    for (int i = lo; i < hi; ++i) {
-        const int id = ids[i] < 0 ? experts : ids[i];
-        if (id == e) {
-            rows[at] = e < experts ? i / top_k : -1;
-            slots[i] = e < experts ? at : -1;
-            ++at;
+    const uint64_t lower = ((uint64_t)1 << lane) - 1;
+    auto place = [&](int i, bool last) {
+        uint32_t id[kSortLoads];
+        load(id, i, last);
+#pragma unroll
+        for (int j = 0; j < kSortLoads; ++j) {
+            const uint64_t here = __ballot(id[j] == own);
+            if (here == 0)
+                continue;
+            if (id[j] == own) {
+                const int slot = at + __popcll(here & lower), c = i + 64 * j + lane;
+                rows[slot] = e < experts ? c / top_k : -1;
+                slots[c] = e < experts ? slot : -1;
+            }
+            at += __popcll(here);
         }
+    };
+    for (i = lo; i + kStep <= hi; i += kStep)
+        place(i, false);
+    if (i < hi)
+        place(i, true);
+}
+
+// Few choices: both steps by one workgroup. A choice sets its bit among those of its expert, 64 choices a word, in
+// LDS (whatever order the bits come in, the words are the same); an expert's count is the bits set, a scan of
+// the counts the offsets, and a choice's row the offset and the lower bits set. One launch instead of two, the
+// second of which costs more than this (16 tokens x 8 of 64 experts: 5.4 us, against 3.1 and 6.7).
+constexpr int kFewChoices = 1024, kFewTokens = 64, kFewWords = 4096;
+
+template <int V, bool kBf16>
+__global__ __launch_bounds__(1024) void route_few_kernel(const void *__restrict__ logits, int64_t ld, int m, int experts,
+                                                         int top_k, bool renormalize, int32_t *__restrict__ ids,
+                                                         float *__restrict__ weights, int32_t *__restrict__ offsets,
+                                                         int32_t *__restrict__ rows, int32_t *__restrict__ slots)
+{
+    __shared__ unsigned long long s_bits[kFewWords]; // [expert, the last one none][words]
+    __shared__ int s_ids[kFewChoices], s_wave[16], s_begin[1025];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, count = m * top_k, words = (count + 63) / 64;
+    for (int i = tid; i < (experts + 1) * words; i += 1024)
+        s_bits[i] = 0;
+    __syncthreads();
+    for (int token = wave; token < m; token += 16) {
+        int id;
+        float weight;
+        choose<V, kBf16>(logits, ld, token, experts, top_k, renormalize, lane, &id, &weight);
+        if (lane < top_k) {
+            const int c = token * top_k + lane, e = id < 0 ? experts : id;
+            ids[c] = id;
+            weights[c] = weight;
+            s_ids[c] = e;
+            atomicOr(&s_bits[e * words + (c >> 6)], 1ull << (c & 63));
+        }
+    }
+    __syncthreads();
+    int mine = 0;
+    if (tid < experts)
+        for (int w = 0; w < words; ++w)
+            mine += __popcll(s_bits[tid * words + w]);
+    int upto = mine; // of the wave's experts up to this one
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+        const int up = __shfl_up(upto, d);
+        upto += lane >= d ? up : 0;
+    }
+    if (lane == 63)
+        s_wave[wave] = upto;
+    __syncthreads();
+    int begin = upto - mine;
+    for (int w = 0; w < wave; ++w)
+        begin += s_wave[w];
+    if (tid < experts) {
+        offsets[tid] = begin;
+        s_begin[tid] = begin;
+        if (tid == experts - 1) {
+            offsets[experts] = begin + mine;
+            s_begin[experts] = begin + mine;
+        }
+    }
+    __syncthreads();
+    if (tid < count) {
+        const int e = s_ids[tid];
+        int row = s_begin[e] + __popcll(s_bits[e * words + (tid >> 6)] & ((1ull << (tid & 63)) - 1));
+        for (int w = 0; w < tid >> 6; ++w)
+            row += __popcll(s_bits[e * words + w]);
+        rows[row] = e < experts ? tid / top_k : -1;
+        slots[tid] = e < experts ? row : -1;
     }
 }
 
 // ============================================================================ join
-// A thread adds four columns of a token, choice by choice. Bound by HBM: top_k rows read, one written.
-template <bool kYBf16, bool kVec>
-__device__ __forceinline__ v4f load_row4(const void *y, int64_t at, int64_t left)
+// A thread adds 16 bytes' worth of columns of a token, the rows of four choices in flight, in the order of the choices.
+// Bound by HBM: top_k rows read, one written (8192 tokens x 8 rows of 4096 bf16, 605 MB: 98 us).
+template <bool kBf16, int N>
+__device__ __forceinline__ void load_columns(const void *y, int64_t at, int64_t left, bool vec, float (&v)[N])
 {
-    const row_t<kYBf16> *p = reinterpret_cast<const row_t<kYBf16> *>(y) + at;
-    if constexpr (kVec) {
-        if (left >= 4) {
-            if constexpr (kYBf16)
-                return __builtin_convertvector(__builtin_nontemporal_load(reinterpret_cast<const bf16x4 *>(p)), v4f);
-            else
-                return __builtin_nontemporal_load(reinterpret_cast<const v4f *>(p));
-        }
-    }
-    v4f v = {0.0f, 0.0f, 0.0f, 0.0f};
+    const row_t<kBf16> *p = reinterpret_cast<const row_t<kBf16> *>(y) + at;
+    if (vec && left >= N) {
+        typedef row_t<kBf16> row16 __attribute__((ext_vector_type(kBf16 ? 8 : 4)));
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-        if (i < left)
-            v[i] = (float)p[i];
-    return v;
+        for (int i = 0; i < N; i += kBf16 ? 8 : 4) {
+            const row16 r = __builtin_nontemporal_load(reinterpret_cast<const row16 *>(p + i));
+#pragma unroll
+            for (int j = 0; j < (kBf16 ? 8 : 4); ++j)
+                v[i + j] = (float)r[j];
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+            v[i] = i < left ? (float)p[i] : 0.0f;
+    }
 }
 
-template <bool kYBf16, bool kBf16, bool kVec>
+template <bool kYBf16, bool kBf16>
 __global__ __launch_bounds__(256) void combine_kernel(const void *__restrict__ y, int64_t ldy, int64_t r,
                                                       const int32_t *__restrict__ slots,
                                                       const float *__restrict__ weights, int64_t m, int top_k, int64_t n,
-                                                      void *__restrict__ out, int64_t ldo, bool vec)
+                                                      void *__restrict__ out, int64_t ldo, bool in_vec, bool out_vec)
 {
-    const int64_t at = 4 * ((int64_t)blockIdx.x * 256 + threadIdx.x);
+    constexpr int N = kYBf16 ? 8 : 4;
+    const int64_t at = N * ((int64_t)blockIdx.x * blockDim.x + threadIdx.x);
     if (at >= n)
         return;
     for (int64_t token = blockIdx.y; token < m; token += gridDim.y) {
-        v4f sum = {0.0f, 0.0f, 0.0f, 0.0f};
-        for (int j = 0; j < top_k; ++j) {
-            const int64_t slot = slots[token * top_k + j];
-            if (slot < 0 || slot >= r)
-                continue;
-            const float w = weights[token * top_k + j];
-            const v4f v = load_row4<kYBf16, kVec>(y, slot * ldy + at, n - at);
+        float sum[N] = {};
+        for (int j0 = 0; j0 < top_k; j0 += 4) {
+            float v[4][N], w[4];
+            bool some[4];
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
-                sum[i] = __builtin_fmaf(w, v[i], sum[i]);
+            for (int j = 0; j < 4; ++j) {
+                const int64_t c = token * top_k + min(j0 + j, top_k - 1);
+                const int64_t slot = slots[c];
+                some[j] = j0 + j < top_k && slot >= 0 && slot < r;
+                w[j] = weights[c];
+                if (some[j])
+                    load_columns<kYBf16, N>(y, slot * ldy + at, n - at, in_vec, v[j]);
+            }
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                if (some[j])
+#pragma unroll
+                    for (int i = 0; i < N; ++i)
+                        sum[i] = __builtin_fmaf(w[j], v[j][i], sum[i]);
         }
-        store_row4<kBf16>(out, token * ldo + at, sum, n - at, vec);
+#pragma unroll
+        for (int i = 0; i < N; i += 4)
+            store_row4<kBf16>(out, token * ldo + at + i, v4f{sum[i], sum[i + 1], sum[i + 2], sum[i + 3]}, n - at - i, out_vec);
     }
 }
 
 bool float_rows(int dtype) { return dtype == MAMBO_DTYPE_F32 || dtype == MAMBO_DTYPE_BF16; }
 
-template <int V>
-void launch_choose(bool bf16, hipStream_t s, const void *logits, int64_t ld, int64_t m, int experts, int top_k,
-                   bool renormalize, int32_t *ids, float *weights)
+struct Route {
+    const void *logits;
+    int64_t ld, m;
+    int experts, top_k;
+    bool renormalize;
+    int32_t *ids;
+    float *weights;
+    int32_t *offsets, *rows, *slots;
+};
+
+template <int V, bool kBf16>
+void launch_choose(const Route &a, bool few, hipStream_t s)
 {
-    const dim3 grid((unsigned)cdiv(m, 4));
-    if (bf16)
-        MAMBO_LAUNCH((route_choose_kernel<V, true>), grid, dim3(256), 0, s, logits, ld, m, experts, top_k, renormalize,
-                     ids, weights);
+    if (few)
+        MAMBO_LAUNCH((route_few_kernel<V, kBf16>), dim3(1), dim3(1024), 0, s, a.logits, a.ld, (int)a.m, a.experts, a.top_k,
+                     a.renormalize, a.ids, a.weights, a.offsets, a.rows, a.slots);
     else
-        MAMBO_LAUNCH((route_choose_kernel<V, false>), grid, dim3(256), 0, s, logits, ld, m, experts, top_k,
-                     renormalize, ids, weights);
+        MAMBO_LAUNCH((route_choose_kernel<V, kBf16>), dim3((unsigned)cdiv(a.m, 4)), dim3(256), 0, s, a.logits, a.ld, a.m,
+                     a.experts, a.top_k, a.renormalize, a.ids, a.weights);
 }
 
 } // namespace
@@ -234,9 +374,12 @@ extern "C" int mambo_route_experts(const void *logits, int dtype, int64_t ld, in
     MAMBO_REQUIRE(ld >= experts, MAMBO_ERR_VALUE, "row strides must cover the experts");
     MAMBO_REQUIRE(offsets && (m == 0 || (logits && ids && weights && rows && slots)), MAMBO_ERR_VALUE, "null pointer");
     hipStream_t s = (hipStream_t)stream;
+    // one workgroup for both steps while every wave of it has at most four tokens and the bits fit its LDS
+    const bool few = m > 0 && m <= kFewTokens && m * top_k <= kFewChoices && (experts + 1) * cdiv(m * top_k, 64) <= kFewWords;
     if (m > 0) {
+        const Route a = {logits, ld, m, (int)experts, (int)top_k, renormalize != 0, ids, weights, offsets, rows, slots};
         const bool bf16 = dtype == MAMBO_DTYPE_BF16;
-#define MAMBO_CHOOSE(V) launch_choose<V>(bf16, s, logits, ld, m, (int)experts, (int)top_k, renormalize != 0, ids, weights)
+#define MAMBO_CHOOSE(V) (bf16 ? launch_choose<V, true>(a, few, s) : launch_choose<V, false>(a, few, s))
         if (experts <= 64)
             MAMBO_CHOOSE(1);
         else if (experts <= 128)
@@ -249,10 +392,10 @@ extern "C" int mambo_route_experts(const void *logits, int dtype, int64_t ld, in
             MAMBO_CHOOSE(16);
 #undef MAMBO_CHOOSE
         const int rc = mambo_check_launch("route_experts");
-        if (rc != MAMBO_OK)
+        if (rc != MAMBO_OK || few)
             return rc;
     }
-    MAMBO_LAUNCH(route_sort_kernel, dim3((unsigned)(experts + 1)), dim3(kSortThreads), 0, s, ids, (int)(m * top_k),
+    MAMBO_LAUNCH(route_sort_kernel, dim3((unsigned)(experts + 1)), dim3(kSortWaves * 64), 0, s, (const uint32_t *)ids, (int)(m * top_k),
                  (int)top_k, (int)experts, offsets, rows, slots);
     return mambo_check_launch("route_experts");
 }
@@ -272,23 +415,20 @@ extern "C" int mambo_combine_experts(const void *y, int y_dtype, int64_t ldy, in
     const bool yb = y_dtype == MAMBO_DTYPE_BF16, ob = out_dtype == MAMBO_DTYPE_BF16;
     MAMBO_REQUIRE((uintptr_t)y % (yb ? 2 : 4) == 0 && (uintptr_t)out % (ob ? 2 : 4) == 0, MAMBO_ERR_VALUE,
                   "rows must be aligned to their type");
-    const int64_t columns = cdiv(n, 4 * 256);
+    const int threads = n <= (yb ? 512 : 256) ? 64 : 256;
+    const int64_t columns = cdiv(n, (yb ? 8 : 4) * threads);
     MAMBO_REQUIRE(columns <= 0x7FFFFFFF, MAMBO_ERR_VALUE, "rows too long");
     const dim3 grid((unsigned)columns, (unsigned)(m < 65535 ? m : 65535));
     const bool in_vec = rows_take_vectors(y, ldy, y_dtype), out_vec = rows_take_vectors(out, ldo, out_dtype);
     hipStream_t s = (hipStream_t)stream;
-#define MAMBO_COMBINE(YB, OB, V)                                                                                   \
-    if (yb == YB && ob == OB && in_vec == V)                                                                       \
-    MAMBO_LAUNCH((combine_kernel<YB, OB, V>), grid, dim3(256), 0, s, y, ldy, r, slots, weights, m, (int)top_k, n, out, \
-                 ldo, out_vec)
-    MAMBO_COMBINE(true, true, true);
-    MAMBO_COMBINE(true, true, false);
-    MAMBO_COMBINE(true, false, true);
-    MAMBO_COMBINE(true, false, false);
-    MAMBO_COMBINE(false, true, true);
-    MAMBO_COMBINE(false, true, false);
-    MAMBO_COMBINE(false, false, true);
-    MAMBO_COMBINE(false, false, false);
+#define MAMBO_COMBINE(YB, OB)                                                                                      \
+    if (yb == YB && ob == OB)                                                                                      \
+    MAMBO_LAUNCH((combine_kernel<YB, OB>), grid, dim3(threads), 0, s, y, ldy, r, slots, weights, m, (int)top_k, n, out,  \
+                 ldo, in_vec, out_vec)
+    MAMBO_COMBINE(true, true);
+    MAMBO_COMBINE(true, false);
+    MAMBO_COMBINE(false, true);
+    MAMBO_COMBINE(false, false);
 #undef MAMBO_COMBINE
     return mambo_check_launch("combine_experts");
 }

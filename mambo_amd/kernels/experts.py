@@ -11,12 +11,12 @@ no counterpart.
 
 from __future__ import annotations
 
-from dataclasses import dataclass
+from typing import NamedTuple
 
 import torch
 
 from mambo_amd import _native
-from mambo_amd.kernels.fp8_block import ROW_DTYPES, _plain_rows, _row_stride, block_activations, product_output
+from mambo_amd.kernels.fp8_block import ROW_DTYPES, block_activations, plain_rows, product_output, row_stride, rows_in_place
 from mambo_amd.utils.fp8_block_weight import Fp8BlockWeight
 from mambo_amd.utils.iq3_s_weight import IQ3SExperts, IQ3_S_BLOCK_VALUES
 
@@ -24,8 +24,7 @@ MAX_EXPERTS = 1024  # MAMBO_MAX_EXPERTS
 MAX_TOP_K = 64  # MAMBO_MAX_TOP_K
 
 
-@dataclass(frozen=True)
-class ExpertPlan:
+class ExpertPlan(NamedTuple):
     """What launch_route_experts decides for M tokens of ``top_k`` choices, R = M * top_k rows.
 
     ids: int32 [M, top_k], the chosen experts in falling order (-1: none was left)
@@ -59,25 +58,23 @@ def launch_route_experts(logits: torch.Tensor, top_k: int, *, renormalize: bool 
         raise ValueError(f"between 1 and {MAX_EXPERTS} experts, got {experts}")
     if not 1 <= top_k <= min(experts, MAX_TOP_K):
         raise ValueError(f"top_k must be in [1, min(E, {MAX_TOP_K})], got {top_k}")
-    with _native.on_device(dev), _native.on_stream(stream, dev):
-        if not _plain_rows(logits):
+    with _native.launch_on(dev, stream):
+        if not logits.is_contiguous() and not plain_rows(logits):
             logits = logits.contiguous()
-        r = m * top_k
-        buf = torch.empty(4 * r + experts + 1, dtype=torch.int32, device=dev)  # one allocation for the plan
-        ids, slots = buf[:r].view(m, top_k), buf[r:2 * r].view(m, top_k)
-        rows, weights = buf[2 * r:3 * r], buf[3 * r:4 * r].view(torch.float32).view(m, top_k)
-        plan = ExpertPlan(ids, weights, buf[4 * r:], rows, slots)
-        base = buf.data_ptr()
+        # int32 planes of one buffer: allocated and taken apart in few calls
+        ids, slots, rows, weights = torch.empty((4, m, top_k), dtype=torch.int32, device=dev).unbind(0)
+        rows, weights = rows.view(-1), weights.view(torch.float32)
+        offsets = torch.empty(experts + 1, dtype=torch.int32, device=dev)
         _native.check(_native.lib().mambo_route_experts(
-            logits.data_ptr(), ROW_DTYPES[logits.dtype], _row_stride(logits), m, experts, top_k, bool(renormalize),
-            base, base + 12 * r, base + 16 * r, base + 8 * r, base + 4 * r, _native.stream_handle(stream)),
-            "launch_route_experts")
-    return plan
+            logits.data_ptr(), ROW_DTYPES[logits.dtype], row_stride(logits), m, experts, top_k, bool(renormalize),
+            ids.data_ptr(), weights.data_ptr(), offsets.data_ptr(), rows.data_ptr(), slots.data_ptr(),
+            _native.stream_handle(stream)), "launch_route_experts")
+    return ExpertPlan(ids, weights, offsets, rows, slots)
 
 
 def _plan_tensors(offsets, rows, m: int, experts: int, dev) -> int:
     """Validate the plan of a grouped product; return its number of output rows."""
-    if not isinstance(offsets, torch.Tensor) or tuple(offsets.shape) != (experts + 1,) or offsets.dtype != torch.int32 \
+    if not isinstance(offsets, torch.Tensor) or offsets.shape != (experts + 1,) or offsets.dtype != torch.int32 \
             or not offsets.is_contiguous() or offsets.device != dev:
         raise ValueError(f"offsets must be contiguous int32 [{experts + 1}] on the rows' device")
     if rows is None:
@@ -103,16 +100,14 @@ def launch_fp8_block_matmul_experts(x_values: torch.Tensor, x_scales: torch.Tens
     if not isinstance(weight, Fp8BlockWeight):
         raise TypeError("prepare FP8 weights with prepare_fp8_block_weight before launch")
     dev = weight.packed.device
-    with _native.on_device(dev), _native.on_stream(stream, dev):
-        x_values, x_scales, m = block_activations(x_values, x_scales, weight.k)
-        if x_values.device != dev:
-            raise ValueError("the rows and the weight must be on the same device")
+    with _native.launch_on(dev, stream):
+        x_values, x_scales, m = block_activations(x_values, x_scales, weight.k, dev)
         r = _plan_tensors(offsets, rows, m, weight.experts, dev)
         out = product_output(out, r, weight.n, out_dtype, dev)
         _native.check(_native.lib().mambo_fp8_block_matmul_experts(
-            x_values.data_ptr(), _row_stride(x_values), x_scales.data_ptr(), _row_stride(x_scales), m,
+            x_values.data_ptr(), row_stride(x_values), x_scales.data_ptr(), row_stride(x_scales), m,
             None if rows is None else rows.data_ptr(), r, offsets.data_ptr(), weight.experts, weight.packed.data_ptr(),
-            weight.scales.data_ptr(), weight.n, weight.k, out.data_ptr(), ROW_DTYPES[out_dtype], _row_stride(out),
+            weight.scales.data_ptr(), weight.n, weight.k, out.data_ptr(), ROW_DTYPES[out_dtype], row_stride(out),
             _native.stream_handle(stream)), "launch_fp8_block_matmul_experts")
     return out
 
@@ -127,7 +122,7 @@ def launch_iq3_s_fp8_matmul_experts(x_values: torch.Tensor, x_scales: torch.Tens
     if not isinstance(weight, IQ3SExperts):
         raise TypeError("prepare IQ3_S experts with prepare_iq3_s_experts before launch")
     k, dev = weight.blocks * IQ3_S_BLOCK_VALUES, weight.packed.device
-    with _native.on_device(dev), _native.on_stream(stream, dev):
+    with _native.launch_on(dev, stream):
         if not isinstance(x_values, torch.Tensor) or x_values.ndim != 2 or x_values.dtype != torch.uint8 \
                 or x_values.shape[1] != k:
             raise ValueError(f"x_values must be uint8 [M,{k}]")
@@ -137,16 +132,13 @@ def launch_iq3_s_fp8_matmul_experts(x_values: torch.Tensor, x_scales: torch.Tens
             raise ValueError("x_scales must be uint8 [M,K/32]")
         if x_values.device != dev or x_scales.device != dev:
             raise ValueError("the rows, their scales and the weight must be on the same device")
-        x_values, x_scales = (
-            t if _plain_rows(t) and t.data_ptr() % align == 0 and _row_stride(t) % align == 0
-            else torch.empty(t.shape, dtype=t.dtype, device=dev).copy_(t)
-            for t, align in ((x_values, 16), (x_scales, 8)))
+        x_values, x_scales = rows_in_place(x_values, 16), rows_in_place(x_scales, 8)
         r = _plan_tensors(offsets, rows, m, weight.experts, dev)
         out = product_output(out, r, weight.n, out_dtype, dev)
         _native.check(_native.lib().mambo_iq3s_fp8_matmul_experts(
-            x_values.data_ptr(), _row_stride(x_values), x_scales.data_ptr(), _row_stride(x_scales), m,
+            x_values.data_ptr(), row_stride(x_values), x_scales.data_ptr(), row_stride(x_scales), m,
             None if rows is None else rows.data_ptr(), r, offsets.data_ptr(), weight.experts, weight.packed.data_ptr(),
-            weight.packed.stride(0), weight.n, weight.blocks, out.data_ptr(), ROW_DTYPES[out_dtype], _row_stride(out),
+            weight.packed.stride(0), weight.n, weight.blocks, out.data_ptr(), ROW_DTYPES[out_dtype], row_stride(out),
             _native.stream_handle(stream)), "launch_iq3_s_fp8_matmul_experts")
     return out
 
@@ -172,12 +164,12 @@ def launch_combine_experts(y: torch.Tensor, slots: torch.Tensor, weights: torch.
         raise ValueError("weights must be float32 of the shape of slots on y's device")
     m, top_k = slots.shape
     out_dtype = y.dtype if out_dtype is None else out_dtype
-    with _native.on_device(dev), _native.on_stream(stream, dev):
-        y = y if _plain_rows(y) else y.contiguous()
+    with _native.launch_on(dev, stream):
+        y = y if y.is_contiguous() or plain_rows(y) else y.contiguous()
         slots, weights = slots.contiguous(), weights.contiguous()
         out = product_output(out, m, y.shape[1], out_dtype, dev)
         _native.check(_native.lib().mambo_combine_experts(
-            y.data_ptr(), ROW_DTYPES[y.dtype], _row_stride(y), y.shape[0], slots.data_ptr(), weights.data_ptr(), m,
-            top_k, y.shape[1], out.data_ptr(), ROW_DTYPES[out_dtype], _row_stride(out),
+            y.data_ptr(), ROW_DTYPES[y.dtype], row_stride(y), y.shape[0], slots.data_ptr(), weights.data_ptr(), m,
+            top_k, y.shape[1], out.data_ptr(), ROW_DTYPES[out_dtype], row_stride(out),
             _native.stream_handle(stream)), "launch_combine_experts")
     return out

@@ -32,52 +32,61 @@ def launch_quantize_fp8_block(x: torch.Tensor, *, stream=None, out: tuple[torch.
         raise ValueError("activation must be a GPU tensor")
     (m, k), dev = x.shape, x.device
     groups = -(-k // FP8_BLOCK)
-    with _native.on_device(dev), _native.on_stream(stream, dev):
-        if not _plain_rows(x):
+    with _native.launch_on(dev, stream):
+        if not x.is_contiguous() and not plain_rows(x):
             x = x.contiguous()
         if out is None:
             values = torch.empty((m, k), dtype=torch.uint8, device=dev)
             scales = torch.empty((m, groups), dtype=torch.float32, device=dev)
+            ldv, lds = k, groups
         else:
             values, scales = out
             if values.shape != (m, k) or values.dtype != torch.uint8 or scales.shape != (m, groups) \
                     or scales.dtype != torch.float32 or values.device != dev or scales.device != dev \
-                    or not _plain_rows(values) or not _plain_rows(scales):
+                    or not plain_rows(values) or not plain_rows(scales):
                 raise ValueError("out must be (uint8 [M,K], float32 [M,ceil(K/128)]) with unit column stride on the "
                                  "activation's device")
+            ldv, lds = row_stride(values), row_stride(scales)
         _native.check(_native.lib().mambo_quantize_fp8_block(
-            x.data_ptr(), ROW_DTYPES[x.dtype], m, k, _row_stride(x), values.data_ptr(), _row_stride(values),
-            scales.data_ptr(), _row_stride(scales), _native.stream_handle(stream)), "launch_quantize_fp8_block")
+            x.data_ptr(), ROW_DTYPES[x.dtype], m, k, row_stride(x), values.data_ptr(), ldv, scales.data_ptr(), lds,
+            _native.stream_handle(stream)), "launch_quantize_fp8_block")
     return values, scales
 
 
-def _row_stride(t: torch.Tensor) -> int:
+def row_stride(t: torch.Tensor) -> int:
     """Stride of the rows; of a single row, whose stride torch leaves open, its length."""
     return t.stride(0) if t.shape[0] > 1 else t.shape[1]
 
 
-def _plain_rows(t: torch.Tensor) -> bool:
+def plain_rows(t: torch.Tensor) -> bool:
     """Whether rows do not overlap and their elements are next to each other."""
     return (t.shape[1] <= 1 or t.stride(1) == 1) and (t.shape[0] <= 1 or t.stride(0) >= t.shape[1])
 
 
-def block_activations(x_values, x_scales, k: int):
-    """Validate E4M3 rows [M,K] and scales [M,ceil(K/128)]; return them in a form that the kernels
-    read in place (16-byte aligned rows), copied only if needed."""
+def rows_in_place(t: torch.Tensor, align: int) -> torch.Tensor:
+    """`t` itself where the kernels can read its rows as they lie (elements next to each other, rows
+    apart and `align` bytes aligned), else a contiguous copy."""
+    if t.is_contiguous():
+        if t.data_ptr() % align == 0 and t.shape[1] * t.element_size() % align == 0:
+            return t
+    elif plain_rows(t) and t.data_ptr() % align == 0 and row_stride(t) * t.element_size() % align == 0:
+        return t
+    return torch.empty(t.shape, dtype=t.dtype, device=t.device).copy_(t)
+
+
+def block_activations(x_values, x_scales, k: int, dev) -> tuple[torch.Tensor, torch.Tensor, int]:
+    """Validate E4M3 rows [M,K] and scales [M,ceil(K/128)] on `dev`; return them in a form that the
+    kernels read in place, and M."""
     if not isinstance(x_values, torch.Tensor) or x_values.ndim != 2 or x_values.dtype != torch.uint8 \
             or x_values.shape[1] != k:
         raise ValueError(f"x_values must be uint8 [M,{k}]")
     m = x_values.shape[0]
-    if not isinstance(x_scales, torch.Tensor) or tuple(x_scales.shape) != (m, -(-k // FP8_BLOCK)) \
+    if not isinstance(x_scales, torch.Tensor) or x_scales.shape != (m, -(-k // FP8_BLOCK)) \
             or x_scales.dtype != torch.float32:
         raise ValueError("x_scales must be float32 [M,ceil(K/128)]")
-    if not x_values.is_cuda or x_scales.device != x_values.device:
-        raise ValueError("x_values and x_scales must be on the same GPU")
-    if not _plain_rows(x_values) or x_values.data_ptr() % 16 or _row_stride(x_values) % 16:
-        x_values = torch.empty(x_values.shape, dtype=torch.uint8, device=x_values.device).copy_(x_values)
-    if not _plain_rows(x_scales):
-        x_scales = x_scales.contiguous()
-    return x_values, x_scales, m
+    if x_values.device != dev or x_scales.device != dev:
+        raise ValueError("x_values and x_scales must be on the weight's device")
+    return rows_in_place(x_values, 16), rows_in_place(x_scales, 4), m
 
 
 def product_output(out, rows: int, n: int, dtype, dev) -> torch.Tensor:
@@ -87,7 +96,7 @@ def product_output(out, rows: int, n: int, dtype, dev) -> torch.Tensor:
     if out is None:
         return torch.empty((rows, n), dtype=dtype, device=dev)
     if not isinstance(out, torch.Tensor) or tuple(out.shape) != (rows, n) or out.dtype != dtype or out.device != dev \
-            or not _plain_rows(out):
+            or not plain_rows(out):
         raise ValueError(f"out must be {dtype} [{rows},{n}] with unit column stride on the rows' device")
     return out
 
@@ -96,20 +105,21 @@ def launch_fp8_block_matmul(x_values: torch.Tensor, x_scales: torch.Tensor, weig
                             out_dtype: torch.dtype = torch.float32, stream=None,
                             out: torch.Tensor | None = None) -> torch.Tensor:
     """Multiply rows from launch_quantize_fp8_block by a prepared weight: [M,N] of ``out_dtype``
-    (float32 or bfloat16, rounded once from the float32 sums). M may be 0. Rows that are not 16-byte
-    aligned are copied first; ``out`` optionally supplies the output."""
+    (float32 or bfloat16, rounded once from the float32 sums). bfloat16 outputs are computed by the
+    FP8 matrix instructions, float32 ones by the bfloat16 instructions, which add more exactly and at
+    half the rate. M may be 0. Rows that are not 16-byte aligned are copied first; ``out`` optionally
+    supplies the output."""
     if not isinstance(weight, Fp8BlockWeight):
         raise TypeError("prepare FP8 weights with prepare_fp8_block_weight before launch")
     if weight.experts != 1:
         raise ValueError("a weight of several experts takes launch_fp8_block_matmul_experts")
-    dev = weight.packed.device
-    with _native.on_device(dev), _native.on_stream(stream, dev):
-        x_values, x_scales, m = block_activations(x_values, x_scales, weight.k)
-        if x_values.device != dev:
-            raise ValueError("the rows and the weight must be on the same device")
-        out = product_output(out, m, weight.n, out_dtype, dev)
+    packed, n, k = weight.packed, weight.n, weight.k
+    dev = packed.device
+    with _native.launch_on(dev, stream):
+        x_values, x_scales, m = block_activations(x_values, x_scales, k, dev)
+        out = product_output(out, m, n, out_dtype, dev)
         _native.check(_native.lib().mambo_fp8_block_matmul(
-            x_values.data_ptr(), _row_stride(x_values), x_scales.data_ptr(), _row_stride(x_scales), m,
-            weight.packed.data_ptr(), weight.scales.data_ptr(), weight.n, weight.k, out.data_ptr(),
-            ROW_DTYPES[out_dtype], _row_stride(out), _native.stream_handle(stream)), "launch_fp8_block_matmul")
+            x_values.data_ptr(), row_stride(x_values), x_scales.data_ptr(), row_stride(x_scales), m, packed.data_ptr(),
+            weight.scales.data_ptr(), n, k, out.data_ptr(), ROW_DTYPES[out_dtype], row_stride(out),
+            _native.stream_handle(stream)), "launch_fp8_block_matmul")
     return out

@@ -49,7 +49,7 @@ def prepare_fp8_block_weight(codes: torch.Tensor, scales: torch.Tensor, *, strea
     if scales.device != codes.device:
         raise ValueError("codes and scales must be on the same device")
     dev = codes.device
-    with _native.on_device(dev), _native.on_stream(stream, dev):
+    with _native.launch_on(dev, stream):
         codes = codes.view(torch.uint8) if codes.dtype != torch.uint8 else codes
         if codes.ndim == 2:
             codes, scales = codes[None], scales[None]

@@ -215,7 +215,7 @@ def prepare_iq3_s_experts(iq3_weights: torch.Tensor, *, stream=None) -> IQ3SExpe
         raise ValueError("IQ3_S experts must be uint8 [E,N,K/256,110] with E in [1, 1024]")
     n, blocks = _check_raw(iq3_weights[0])
     dev, experts = iq3_weights.device, int(iq3_weights.shape[0])
-    with _native.on_device(dev), _native.on_stream(stream, dev):
+    with _native.launch_on(dev, stream):
         packed = torch.empty((experts, packed_bytes(n, blocks)), dtype=torch.uint8, device=dev)
         se, sn, sb, sbyte = iq3_weights.stride()
         for e in range(experts):
