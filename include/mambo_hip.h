@@ -291,11 +291,13 @@ int64_t mambo_gemm_config_enumerate(int64_t m, int64_t n, int64_t blocks, mambo_
  * other values gives wrong sums and no stray access. Rows past offsets[experts] come out as zeros. */
 
 /* Block quantizer: x [m, k] f32 or bf16 (row stride ldx), k % 16 == 0, in groups of 128 along K (the
- * last may be shorter): scales[m, lds] f32 = max(amax / 448, 2^-100) and values [m, ldv] = E4M3 of
- * x / scale, computed as one division by amax and rounded once to nearest even. A group that holds
- * a NaN or an infinity gets the scale NaN and E4M3 NaN codes. m == 0: nothing to do. */
+ * last may be shorter): f32 scales = max(amax / 448, 2^-100), row i's of group g at scales + i * lds +
+ * g * gss, and values [m, ldv] = E4M3 of x / scale, computed as one division by amax and rounded
+ * once to nearest even. A group that holds a NaN or an infinity gets the scale NaN and E4M3 NaN codes.
+ * The products read scales of groups of rows (lds 1, gss >= m) faster than rows of groups (gss 1,
+ * lds >= ceil(k/128)). m == 0: nothing to do. */
 int mambo_quantize_fp8_block(const void *x, int x_dtype, int64_t m, int64_t k, int64_t ldx, uint8_t *values,
-                             int64_t ldv, float *scales, int64_t lds, mambo_stream_t stream);
+                             int64_t ldv, float *scales, int64_t lds, int64_t gss, mambo_stream_t stream);
 
 /* Bytes of the private layout of `experts` weights [n, k] of E4M3 codes. */
 int64_t mambo_fp8_block_packed_bytes(int64_t experts, int64_t n, int64_t k);
@@ -307,19 +309,20 @@ int mambo_fp8_block_pack(const uint8_t *w, int64_t experts, int64_t n, int64_t k
 
 /* out[m, n] (f32 or bf16: out_dtype; row stride ldo) = sum over K groups g of 128 of
  * xs[m, g] * ws[n / 128, g] * sum over the group of xv[m, k] * w[n, k], in f32, groups in a fixed
- * order. xv u8 [m, ldxv] E4M3, 16-byte aligned rows; xs f32 [m, ldxs]; packed from
+ * order. xv u8 [m, ldxv] E4M3, 16-byte aligned rows; xs f32, row i's of group g at xs + i * ldxs + g *
+ * gsxs (rows or groups apart); packed from
  * mambo_fp8_block_pack with one expert; ws f32 [ceil(n/128), ceil(k/128)] contiguous;
  * k % 16 == 0. m == 0: nothing to do. */
-int mambo_fp8_block_matmul(const uint8_t *xv, int64_t ldxv, const float *xs, int64_t ldxs, int64_t m,
-                           const uint8_t *packed, const float *ws, int64_t n, int64_t k, void *out,
+int mambo_fp8_block_matmul(const uint8_t *xv, int64_t ldxv, const float *xs, int64_t ldxs, int64_t gsxs,
+                           int64_t m, const uint8_t *packed, const float *ws, int64_t n, int64_t k, void *out,
                            int out_dtype, int64_t ldo, mambo_stream_t stream);
 
 /* The same grouped by expert: out [r, n], row i of expert e (offsets) with weight e of packed
  * [experts] and ws [experts, ceil(n/128), ceil(k/128)]. rows: row i reads xv/xs row rows[i] of m
  * (NULL: row i, and m == r). experts <= MAMBO_MAX_EXPERTS; r == 0: nothing to do. */
 #define MAMBO_MAX_EXPERTS 1024
-int mambo_fp8_block_matmul_experts(const uint8_t *xv, int64_t ldxv, const float *xs, int64_t ldxs, int64_t m,
-                                   const int32_t *rows, int64_t r, const int32_t *offsets, int64_t experts,
+int mambo_fp8_block_matmul_experts(const uint8_t *xv, int64_t ldxv, const float *xs, int64_t ldxs, int64_t gsxs,
+                                   int64_t m, const int32_t *rows, int64_t r, const int32_t *offsets, int64_t experts,
                                    const uint8_t *packed, const float *ws, int64_t n, int64_t k, void *out,
                                    int out_dtype, int64_t ldo, mambo_stream_t stream);
 

@@ -120,11 +120,11 @@ SIGNATURES = {
                                ctypes.POINTER(GemmConfig)]),
     "mambo_gemm_check_config": (_i32, [_i64, _i64, _i64, ctypes.POINTER(GemmConfig)]),
     "mambo_gemm_config_enumerate": (_i64, [_i64, _i64, _i64, ctypes.POINTER(GemmConfig), _i64]),
-    "mambo_quantize_fp8_block": (_i32, [_vp, _i32, _i64, _i64, _i64, _vp, _i64, _vp, _i64, _vp]),
+    "mambo_quantize_fp8_block": (_i32, [_vp, _i32, _i64, _i64, _i64, _vp, _i64, _vp, _i64, _i64, _vp]),
     "mambo_fp8_block_packed_bytes": (_i64, [_i64, _i64, _i64]),
     "mambo_fp8_block_pack": (_i32, [_vp, _i64, _i64, _i64, _i64, _i64, _vp, _vp]),
-    "mambo_fp8_block_matmul": (_i32, [_vp, _i64, _vp, _i64, _i64, _vp, _vp, _i64, _i64, _vp, _i32, _i64, _vp]),
-    "mambo_fp8_block_matmul_experts": (_i32, [_vp, _i64, _vp, _i64, _i64, _vp, _i64, _vp, _i64, _vp, _vp, _i64, _i64,
+    "mambo_fp8_block_matmul": (_i32, [_vp, _i64, _vp, _i64, _i64, _i64, _vp, _vp, _i64, _i64, _vp, _i32, _i64, _vp]),
+    "mambo_fp8_block_matmul_experts": (_i32, [_vp, _i64, _vp, _i64, _i64, _i64, _vp, _i64, _vp, _i64, _vp, _vp, _i64, _i64,
                                               _vp, _i32, _i64, _vp]),
     "mambo_iq3s_fp8_matmul_experts": (_i32, [_vp, _i64, _vp, _i64, _i64, _vp, _i64, _vp, _i64, _vp, _i64, _i64, _i64,
                                              _vp, _i32, _i64, _vp]),

@@ -180,7 +180,7 @@ CONSTRAINTS: dict[str, list[dict]] = {
     "mambo_quantize_fp8_block": [
         _arr("x", "float32|bfloat16", ["m", "k"], ["ldx", "1"], align=2),
         _arr("values", "uint8", ["m", "k"], ["ldv", "1"], access="write"),
-        _arr("scales", "float32", ["m", "(k+127)/128"], ["lds", "1"], align=4, access="write"),
+        _arr("scales", "float32", ["m", "(k+127)/128"], ["lds", "gss"], align=4, access="write"),
     ],
     "mambo_fp8_block_packed_bytes": [],
     "mambo_fp8_block_pack": [
@@ -189,14 +189,14 @@ CONSTRAINTS: dict[str, list[dict]] = {
     ],
     "mambo_fp8_block_matmul": [
         _arr("xv", "uint8", ["m", "k"], ["ldxv", "1"], align=16),
-        _arr("xs", "float32", ["m", "(k+127)/128"], ["ldxs", "1"], align=4),
+        _arr("xs", "float32", ["m", "(k+127)/128"], ["ldxs", "gsxs"], align=4),
         _arr("packed", "uint8", ["((n+31)/32)*((k+127)/128)*4096"], align=16),
         _arr("ws", "float32", ["(n+127)/128", "(k+127)/128"], align=4),
         _arr("out", "float32|bfloat16", ["m", "n"], ["ldo", "1"], align=2, access="write"),
     ],
     "mambo_fp8_block_matmul_experts": [
         _arr("xv", "uint8", ["m", "k"], ["ldxv", "1"], align=16),
-        _arr("xs", "float32", ["m", "(k+127)/128"], ["ldxs", "1"], align=4),
+        _arr("xs", "float32", ["m", "(k+127)/128"], ["ldxs", "gsxs"], align=4),
         _arr("rows", "int32", ["r"], align=4, nullable=True),
         _arr("offsets", "int32", ["experts+1"], align=4),
         _arr("packed", "uint8", ["experts*((n+31)/32)*((k+127)/128)*4096"], align=16),

@@ -68,55 +68,63 @@ __device__ __forceinline__ void load8(const void *x, int64_t at, float (&v)[8])
     }
 }
 
-template <bool kBf16, bool kVec>
+// R rows at a time, their loads issued before either is converted: 8192 x 4096 bf16 takes 26.9 us with one row, 22.2 (4.5
+// TB/s of reads and writes) with two, 23.9 with four and 28.0 with eight; 512 x 4096 with one 4.3, with two 4.9.
+template <bool kBf16, bool kVec, int R>
 __global__ __launch_bounds__(256) void quantize_fp8_block_kernel(const void *__restrict__ x, int64_t ldx, int64_t m,
                                                                  int k, uint8_t *__restrict__ values, int64_t ldv,
-                                                                 float *__restrict__ scales, int64_t lds)
+                                                                 float *__restrict__ scales, int64_t lds, int64_t gss)
 {
     const int at = (int)(blockIdx.x * 16 + (threadIdx.x >> 4)) * kGroup + 8 * (threadIdx.x & 15); // in the row
     const bool in = at < k; // k is a multiple of 16, so all eight or none
-    for (int64_t row = blockIdx.y; row < m; row += gridDim.y) {
-        float v[8] = {};
-        if (in)
-            load8<kBf16, kVec>(x, row * ldx + at, v);
-        uint32_t amax = 0u; // over the magnitude bits: a NaN beats an infinity, that every number
+    for (int64_t row0 = (int64_t)blockIdx.y * R; row0 < m; row0 += (int64_t)gridDim.y * R) {
+        float v[R][8] = {};
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
-            amax = max(amax, abs_bits(v[i]));
+        for (int r = 0; r < R; ++r)
+            if (in && row0 + r < m)
+                load8<kBf16, kVec>(x, (row0 + r) * ldx + at, v[r]);
 #pragma unroll
-        for (int d = 1; d < 16; d <<= 1)
-            amax = max(amax, (uint32_t)__shfl_xor((int)amax, d));
-        if (!in)
-            continue;
-        const bool finite = amax < kNonFiniteBits;
-        const float top = fmaxf(__uint_as_float(amax), 448.0f * kSmallestScale);
-        const float b = top * 0x1p-9f, inv = 1.0f / b;
-        float q[8];
+        for (int r = 0; r < R; ++r) {
+            const int64_t row = row0 + r;
+            uint32_t amax = 0u; // over the magnitude bits: a NaN beats an infinity, that every number
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const float a = 0.875f * v[i], y = a * inv;
-            q[i] = __builtin_copysignf(__builtin_fmaf(__builtin_fmaf(-y, b, a), inv, y), a); // -0 stays -0
-        }
-        uint2 codes;
-        if (finite) {
-            codes.x = pack4<kQuantHwCvt>(q[0], q[1], q[2], q[3]);
-            codes.y = pack4<kQuantHwCvt>(q[4], q[5], q[6], q[7]);
-        } else {
-            codes.x = nan4(v[0], v[1], v[2], v[3]);
-            codes.y = nan4(v[4], v[5], v[6], v[7]);
-        }
-        uint8_t *o = values + row * ldv + at;
-        if constexpr (kVec) {
-            *reinterpret_cast<uint2 *>(o) = codes; // read again by the product that follows
-        } else {
+            for (int i = 0; i < 8; ++i)
+                amax = max(amax, abs_bits(v[r][i]));
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                o[i] = (uint8_t)(codes.x >> (8 * i));
-                o[4 + i] = (uint8_t)(codes.y >> (8 * i));
+            for (int d = 1; d < 16; d <<= 1)
+                amax = max(amax, (uint32_t)__shfl_xor((int)amax, d));
+            if (!in || row >= m)
+                continue;
+            const bool finite = amax < kNonFiniteBits;
+            const float top = fmaxf(__uint_as_float(amax), 448.0f * kSmallestScale);
+            const float b = top * 0x1p-9f, inv = 1.0f / b;
+            float q[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const float a = 0.875f * v[r][i], y = a * inv;
+                q[i] = __builtin_copysignf(__builtin_fmaf(__builtin_fmaf(-y, b, a), inv, y), a); // -0 stays -0
             }
+            uint2 codes;
+            if (finite) {
+                codes.x = pack4<kQuantHwCvt>(q[0], q[1], q[2], q[3]);
+                codes.y = pack4<kQuantHwCvt>(q[4], q[5], q[6], q[7]);
+            } else {
+                codes.x = nan4(v[r][0], v[r][1], v[r][2], v[r][3]);
+                codes.y = nan4(v[r][4], v[r][5], v[r][6], v[r][7]);
+            }
+            uint8_t *o = values + row * ldv + at;
+            if constexpr (kVec) {
+                *reinterpret_cast<uint2 *>(o) = codes; // read again by the product that follows
+            } else {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    o[i] = (uint8_t)(codes.x >> (8 * i));
+                    o[4 + i] = (uint8_t)(codes.y >> (8 * i));
+                }
+            }
+            if ((threadIdx.x & 15) == 0)
+                scales[row * lds + at / kGroup * gss] = finite ? top / 448.0f : __builtin_nanf("");
         }
-        if ((threadIdx.x & 15) == 0)
-            scales[row * lds + at / kGroup] = finite ? top / 448.0f : __builtin_nanf("");
     }
 }
 
@@ -150,7 +158,7 @@ __global__ __launch_bounds__(256) void fp8_block_pack_kernel(const uint8_t *__re
 struct Fp8Args {
     const uint8_t *xv;
     const float *xs;
-    int64_t ldxv, ldxs;
+    int64_t ldxv, ldxs, gsxs; // xs: strides of rows and of groups
     ExpertRows er;
     const uint8_t *packed;
     const float *ws;
@@ -283,7 +291,7 @@ __global__ __launch_bounds__(W * 64) void fp8_stream_kernel(Fp8Args a)
                 const int at = k0 + 16 * (q + 4 * j); // a chunk past the row's end meets zero weights: any of the row does
                 r.x[j] = *reinterpret_cast<const uint4 *>(xp + (at < a.k ? at : k0));
             }
-            r.xs = sp[g];
+            r.xs = sp[g * a.gsxs];
             r.ws = i < count ? ws[g] : 0.0f;
         };
         load(ring[0], 0);
@@ -388,6 +396,7 @@ __global__ __launch_bounds__(WN * KG * 64) __attribute__((amdgpu_waves_per_eu(2)
             xo[j] = (uint32_t)(a.er.rows ? source_row(a.er, rt.row0 + row) : row) * (uint32_t)a.ldxv;
         }
         const __amdgpu_buffer_rsrc_t sr = open_rsrc(a.er.rows ? a.xs : a.xs + rt.row0 * a.ldxs);
+        const uint32_t gs4 = 4u * (uint32_t)a.gsxs;
         const int srow = min(64 * (wave % kScaleCopies) + lane, rt.count - 1);
         const uint32_t so = 4u * (uint32_t)(a.er.rows ? source_row(a.er, rt.row0 + srow) : srow) * (uint32_t)a.ldxs;
         // tiles past the weight's last read it again: their sums are not stored
@@ -410,9 +419,10 @@ __global__ __launch_bounds__(WN * KG * 64) __attribute__((amdgpu_waves_per_eu(2)
                 __builtin_amdgcn_raw_ptr_buffer_load_lds(xr, (lds_ptr)(rows + kg * kRowBytes + 1024 * (wave + WN * j)), 16,
                                                          vo, gc * kGroup, 0, 0);
             }
-            if (wave < kScaleCopies)
-                __builtin_amdgcn_raw_ptr_buffer_load_lds(sr, (lds_ptr)(scale + 64 * (kg * kScaleCopies + wave)), 4, so,
-                                                         4 * gc, 0, 0);
+            // waves past the last 64 rows repeat a copy (the same bytes): behind a branch the compiler could not count the
+            // copies in flight
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(sr, (lds_ptr)(scale + 64 * (kg * kScaleCopies + wave % kScaleCopies)), 4,
+                                                     so, gc * gs4, 0, 0);
         };
         uint4 w[NB][2][2]; // [tile][K step of 64][half]
         float wscale;
@@ -572,28 +582,30 @@ struct Fp8Kernel {
     int tokens, rows, kg, resident;
     double launch, round, step[4], outputs, weights;
 };
-// Fitted to 302 products (1 to 8192 tokens, 300 to 57344 rows, K 272 to 28672, weights rotated past the caches): 7 to
-// 15% rms each, and the kernel that they pick takes 2% (f32 1%) more than the fastest of the nine on average. None of the
-// nine is spare: without it the fastest of the others takes 0.4 to 3.6% more on average, up to 1.14 to 1.75 times.
+// Fitted to 355 products (1 to 8192 tokens, 300 to 57344 rows, K 272 to 28672, weights rotated past the caches) and, with
+// less weight, 174 grouped ones: the kernel that they pick takes 1.8% more than the fastest of the nine on average (f32 1.4%,
+// grouped, where they do not know how the rows fall, 6%). None of the nine is spare: without it the fastest of the
+// others takes 0.1 to 1.7% more on average and up to 1.15 to 1.6 times. 128 x 128 tiles, 64 x 128 tiles of one K group and
+// a second buffer for the weights were measured too, and either gained less than 0.6% or lost (the buffer 1 to 10%).
 constexpr Fp8Kernel kFp8Kernels[2][9] = {
-    {{16, 16, 8, 2, 2.363, 0.561, {0.756, 1.488}, 15.108, 0.0},
-     {16, 32, 4, 4, 1.977, 1.064, {0.525, 1.1, 1.762, 2.27}, 4.977, 0.02},
-     {16, 64, 4, 4, 0.323, 2.951, {0.791, 1.711, 2.976, 3.97}, 2.418, 0.051},
-     {32, 64, 8, 1, 1.562, 2.093, {1.181}, 2.463, 0.104},
-     {64, 64, 4, 2, 1.93, 2.3, {0.976, 2.471}, 1.501, 0.062},
-     {64, 128, 2, 2, 3.063, 0.57, {0.953, 2.182}, 1.036, 0.068},
-     {64, 256, 2, 1, 2.137, 2.716, {1.588}, 1.186, 0.047},
-     {64, 256, 1, 2, 2.8, 1.188, {1.041, 1.632}, 0.78, 0.048},
+    {{16, 16, 8, 2, 2.750, 0.270, {0.676, 1.423}, 9.980, 0.000},
+     {16, 32, 4, 4, 1.577, 1.555, {0.490, 1.020, 1.624, 2.157}, 3.334, 0.024},
+     {16, 64, 4, 4, 0.000, 3.336, {0.741, 1.586, 2.586, 3.719}, 1.911, 0.061},
+     {32, 64, 8, 1, 1.579, 2.274, {1.102}, 2.152, 0.106},
+     {64, 64, 4, 2, 1.791, 2.547, {0.961, 2.330}, 1.579, 0.058},
+     {64, 128, 2, 2, 3.181, 0.583, {0.932, 2.123}, 1.198, 0.062},
+     {64, 256, 2, 1, 2.667, 2.028, {1.623}, 1.397, 0.046},
+     {64, 256, 1, 2, 3.695, 0.240, {1.081, 1.661}, 0.875, 0.048},
      {0, 0, 0, 0, 0.0, 0.0, {}, 0.0, 0.0}}, // 128 x 256 tiles through bf16 spill
-    {{16, 16, 8, 2, 2.539, 0.088, {0.793, 1.516}, 19.206, 0.0},
-     {16, 32, 4, 4, 2.301, 0.446, {0.532, 1.116, 1.787, 2.217}, 6.001, 0.017},
-     {16, 64, 4, 4, 1.381, 1.564, {0.812, 1.758, 3.018, 4.113}, 3.182, 0.039},
-     {32, 64, 8, 1, 1.854, 1.6, {1.242}, 1.817, 0.106},
-     {64, 64, 4, 2, 2.907, 0.841, {0.727, 1.744}, 0.867, 0.083},
-     {64, 128, 2, 2, 3.059, 0.173, {0.606, 1.316}, 0.48, 0.098},
-     {64, 256, 2, 1, 1.547, 2.554, {1.033}, 0.415, 0.099},
-     {64, 256, 1, 2, 1.666, 1.661, {0.666, 1.032}, 0.29, 0.076},
-     {128, 256, 1, 2, 1.438, 2.763, {1.001, 1.619}, 0.307, 0.062}}};
+    {{16, 16, 8, 2, 2.806, 0.000, {0.696, 1.401}, 13.114, 0.000},
+     {16, 32, 4, 4, 2.833, 0.000, {0.495, 1.020, 1.560, 1.852}, 5.448, 0.021},
+     {16, 64, 4, 4, 3.088, 0.000, {0.719, 1.564, 1.888, 2.495}, 3.400, 0.051},
+     {32, 64, 8, 1, 2.162, 1.477, {1.072}, 1.853, 0.108},
+     {64, 64, 4, 2, 3.640, 0.155, {0.679, 1.404}, 1.226, 0.081},
+     {64, 128, 2, 2, 3.457, 0.000, {0.548, 1.125}, 0.665, 0.083},
+     {64, 256, 2, 1, 2.765, 1.462, {0.998}, 0.669, 0.074},
+     {64, 256, 1, 2, 2.406, 1.225, {0.690, 0.964}, 0.423, 0.058},
+     {128, 256, 1, 2, 3.855, 0.000, {1.034, 1.546}, 0.498, 0.038}}};
 constexpr int kFirstTile = 3; // those from here on address rows by 32-bit offsets
 constexpr int64_t kCUs = 256;
 
@@ -611,8 +623,9 @@ int fp8_plan(const Fp8Args &a, bool bf16, int64_t *wgs)
 {
     const ExpertRows &er = a.er;
     const bool far = a.ldxv * (er.rows ? er.m : 128) + a.k >= ((int64_t)1 << 32) ||
-                     4 * (a.ldxs * (er.rows ? er.m : 128) + a.groups) >= ((int64_t)1 << 32);
-    const double r = (double)er.r, taken = er.offsets ? er.experts * -std::expm1(-r / er.experts) : 1.0;
+                     4 * (a.ldxs * (er.rows ? er.m : 128) + a.gsxs * a.groups) >= ((int64_t)1 << 32);
+    const bool grouped = er.offsets && er.experts > 1; // one expert's rows take the kernel that they would take without
+    const double r = (double)er.r, taken = grouped ? er.experts * -std::expm1(-r / er.experts) : 1.0;
     int best = -1;
     double least = 0.0;
     for (int i = 0; i < (far ? kFirstTile : 9); ++i) {
@@ -622,7 +635,7 @@ int fp8_plan(const Fp8Args &a, bool bf16, int64_t *wgs)
         const int64_t columns = cdiv(a.n, t.rows), most = er.offsets ? expert_row_tiles(er.r, er.experts, t.tokens) : cdiv(er.r, t.tokens);
         if (most * columns > 0x7FFFFFFF)
             continue;
-        const double tiles = er.offsets ? std::fmax(taken, r / t.tokens + 0.5 * taken) : (double)most;
+        const double tiles = grouped ? std::fmax(taken, r / t.tokens + 0.5 * taken) : (double)cdiv(er.r, t.tokens);
         const double us = fp8_time(t, (int64_t)std::ceil(tiles) * columns, a.groups, r * a.n, taken * a.n * a.k);
         if (best < 0 || us < least) {
             best = i;
@@ -631,6 +644,12 @@ int fp8_plan(const Fp8Args &a, bool bf16, int64_t *wgs)
         }
     }
     return best;
+}
+
+// Whether scales of m rows and `groups` groups at these strides lie apart: rows of groups, or groups of rows.
+bool scales_apart(int64_t ld, int64_t gs, int64_t m, int64_t groups)
+{
+    return m == 0 || (ld >= 1 && gs >= 1 && (ld >= gs * groups || gs >= ld * m));
 }
 
 template <bool kExperts, bool kBf16>
@@ -666,7 +685,7 @@ int launch_products(const Fp8Args &a, int which, int64_t wgs, hipStream_t stream
     return mambo_check_launch("fp8_block_matmul");
 }
 
-int run_products(const uint8_t *xv, int64_t ldxv, const float *xs, int64_t ldxs, const ExpertRows &er,
+int run_products(const uint8_t *xv, int64_t ldxv, const float *xs, int64_t ldxs, int64_t gsxs, const ExpertRows &er,
                  const uint8_t *packed, const float *ws, int64_t n, int64_t k, void *out, int out_dtype, int64_t ldo,
                  hipStream_t stream)
 {
@@ -674,7 +693,8 @@ int run_products(const uint8_t *xv, int64_t ldxv, const float *xs, int64_t ldxs,
                   "outputs must be float32 or bfloat16");
     MAMBO_REQUIRE(n >= 1 && n <= 0x7FFFFF00 && k >= 16 && k <= 0x7FFFFF00 && k % 16 == 0, MAMBO_ERR_VALUE,
                   "weights must be [N,K] with N >= 1 and K a multiple of 16 (got N=%lld K=%lld)", (long long)n, (long long)k);
-    MAMBO_REQUIRE(ldxv >= k && ldxs >= cdiv(k, kGroup) && ldo >= n, MAMBO_ERR_VALUE, "row strides must cover the rows");
+    MAMBO_REQUIRE(ldxv >= k && ldo >= n && scales_apart(ldxs, gsxs, er.m, cdiv(k, kGroup)), MAMBO_ERR_VALUE,
+                  "strides must cover the rows");
     if (er.r == 0)
         return MAMBO_OK;
     MAMBO_REQUIRE(xv && xs && packed && ws && out, MAMBO_ERR_VALUE, "null pointer");
@@ -683,7 +703,7 @@ int run_products(const uint8_t *xv, int64_t ldxv, const float *xs, int64_t ldxs,
     MAMBO_REQUIRE((uintptr_t)xs % 4 == 0 && (uintptr_t)ws % 4 == 0 &&
                       (uintptr_t)out % (out_dtype == MAMBO_DTYPE_BF16 ? 2 : 4) == 0,
                   MAMBO_ERR_VALUE, "scales and outputs must be aligned to their type");
-    Fp8Args a = {xv, xs, ldxv, ldxs, er, packed, ws, out, ldo, (int)n, (int)k, (int)cdiv(k, kGroup), (int)cdiv(n, kTileN),
+    Fp8Args a = {xv, xs, ldxv, ldxs, gsxs, er, packed, ws, out, ldo, (int)n, (int)k, (int)cdiv(k, kGroup), (int)cdiv(n, kTileN),
                  rows_take_vectors(out, ldo, out_dtype)};
     const bool bf16 = out_dtype == MAMBO_DTYPE_BF16;
     int64_t wgs = 0;
@@ -697,14 +717,14 @@ int run_products(const uint8_t *xv, int64_t ldxv, const float *xs, int64_t ldxs,
 } // namespace
 
 extern "C" int mambo_quantize_fp8_block(const void *x, int x_dtype, int64_t m, int64_t k, int64_t ldx, uint8_t *values,
-                                        int64_t ldv, float *scales, int64_t lds, mambo_stream_t stream)
+                                        int64_t ldv, float *scales, int64_t lds, int64_t gss, mambo_stream_t stream)
 {
     MAMBO_REQUIRE(x_dtype == MAMBO_DTYPE_F32 || x_dtype == MAMBO_DTYPE_BF16, MAMBO_ERR_VALUE,
                   "activation dtype must be float32 or bfloat16");
     MAMBO_REQUIRE(m >= 0 && k >= 16 && k <= 0x7FFFFF00 && k % 16 == 0, MAMBO_ERR_VALUE,
                   "activation must be [M,K] with K a multiple of 16 (got M=%lld K=%lld)", (long long)m, (long long)k);
     const int64_t groups = cdiv(k, kGroup);
-    MAMBO_REQUIRE(ldx >= k && ldv >= k && lds >= groups, MAMBO_ERR_VALUE, "row strides must cover K");
+    MAMBO_REQUIRE(ldx >= k && ldv >= k && scales_apart(lds, gss, m, groups), MAMBO_ERR_VALUE, "strides must cover K");
     if (m == 0)
         return MAMBO_OK;
     MAMBO_REQUIRE(x && values && scales, MAMBO_ERR_VALUE, "null pointer");
@@ -712,15 +732,22 @@ extern "C" int mambo_quantize_fp8_block(const void *x, int x_dtype, int64_t m, i
     MAMBO_REQUIRE((uintptr_t)x % (bf16 ? 2 : 4) == 0 && (uintptr_t)scales % 4 == 0, MAMBO_ERR_VALUE,
                   "rows and scales must be aligned to their type");
     const bool vec = (uintptr_t)x % 16 == 0 && ldx % (bf16 ? 8 : 4) == 0 && (uintptr_t)values % 8 == 0 && ldv % 8 == 0;
-    const dim3 grid((unsigned)cdiv(groups, 16), (unsigned)(m < 65535 ? m : 65535));
+    const int at_once = m * cdiv(groups, 16) >= 4096 ? 2 : 1; // fewer do not fill the card twice
+    const int64_t ry = cdiv(m, at_once);
+    const dim3 grid((unsigned)cdiv(groups, 16), (unsigned)(ry < 65535 ? ry : 65535));
     hipStream_t s = (hipStream_t)stream;
-#define MAMBO_QUANT(B, V)                                                                                          \
-    if (bf16 == B && vec == V)                                                                                     \
-    MAMBO_LAUNCH((quantize_fp8_block_kernel<B, V>), grid, dim3(256), 0, s, x, ldx, m, (int)k, values, ldv, scales, lds)
-    MAMBO_QUANT(true, true);
-    MAMBO_QUANT(true, false);
-    MAMBO_QUANT(false, true);
-    MAMBO_QUANT(false, false);
+#define MAMBO_QUANT(B, V, R)                                                                                       \
+    if (bf16 == B && vec == V && at_once == R)                                                                     \
+    MAMBO_LAUNCH((quantize_fp8_block_kernel<B, V, R>), grid, dim3(256), 0, s, x, ldx, m, (int)k, values, ldv, scales, lds, \
+                 gss)
+    MAMBO_QUANT(true, true, 1);
+    MAMBO_QUANT(true, true, 2);
+    MAMBO_QUANT(true, false, 1);
+    MAMBO_QUANT(true, false, 2);
+    MAMBO_QUANT(false, true, 1);
+    MAMBO_QUANT(false, true, 2);
+    MAMBO_QUANT(false, false, 1);
+    MAMBO_QUANT(false, false, 2);
 #undef MAMBO_QUANT
     return mambo_check_launch("quantize_fp8_block");
 }
@@ -750,17 +777,17 @@ extern "C" int mambo_fp8_block_pack(const uint8_t *w, int64_t experts, int64_t n
     return mambo_check_launch("fp8_block_pack");
 }
 
-extern "C" int mambo_fp8_block_matmul(const uint8_t *xv, int64_t ldxv, const float *xs, int64_t ldxs, int64_t m,
-                                      const uint8_t *packed, const float *ws, int64_t n, int64_t k, void *out,
+extern "C" int mambo_fp8_block_matmul(const uint8_t *xv, int64_t ldxv, const float *xs, int64_t ldxs, int64_t gsxs,
+                                      int64_t m, const uint8_t *packed, const float *ws, int64_t n, int64_t k, void *out,
                                       int out_dtype, int64_t ldo, mambo_stream_t stream)
 {
     MAMBO_REQUIRE(m >= 0, MAMBO_ERR_VALUE, "rows must not be negative");
     const ExpertRows er = {nullptr, nullptr, m, m, 1};
-    return run_products(xv, ldxv, xs, ldxs, er, packed, ws, n, k, out, out_dtype, ldo, (hipStream_t)stream);
+    return run_products(xv, ldxv, xs, ldxs, gsxs, er, packed, ws, n, k, out, out_dtype, ldo, (hipStream_t)stream);
 }
 
-extern "C" int mambo_fp8_block_matmul_experts(const uint8_t *xv, int64_t ldxv, const float *xs, int64_t ldxs, int64_t m,
-                                              const int32_t *rows, int64_t r, const int32_t *offsets, int64_t experts,
+extern "C" int mambo_fp8_block_matmul_experts(const uint8_t *xv, int64_t ldxv, const float *xs, int64_t ldxs, int64_t gsxs,
+                                              int64_t m, const int32_t *rows, int64_t r, const int32_t *offsets, int64_t experts,
                                               const uint8_t *packed, const float *ws, int64_t n, int64_t k, void *out,
                                               int out_dtype, int64_t ldo, mambo_stream_t stream)
 {
@@ -768,5 +795,5 @@ extern "C" int mambo_fp8_block_matmul_experts(const uint8_t *xv, int64_t ldxv, c
     if (rc != MAMBO_OK)
         return rc;
     const ExpertRows er = {offsets, rows, r, m, (int)experts};
-    return run_products(xv, ldxv, xs, ldxs, er, packed, ws, n, k, out, out_dtype, ldo, (hipStream_t)stream);
+    return run_products(xv, ldxv, xs, ldxs, gsxs, er, packed, ws, n, k, out, out_dtype, ldo, (hipStream_t)stream);
 }

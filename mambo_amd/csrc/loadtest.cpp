@@ -350,12 +350,12 @@ const std::vector<EntryDecl> &compiled_entries()
         MAMBO_ENTRY(mambo_gemm_check_config, "m", "n", "blocks", "cfg"),
         MAMBO_ENTRY(mambo_gemm_config_enumerate, "m", "n", "blocks", "out", "capacity"),
         MAMBO_ENTRY(mambo_quantize_fp8_block, "x", "x_dtype", "m", "k", "ldx", "values", "ldv", "scales", "lds",
-                    "stream"),
+                    "gss", "stream"),
         MAMBO_ENTRY(mambo_fp8_block_packed_bytes, "experts", "n", "k"),
         MAMBO_ENTRY(mambo_fp8_block_pack, "w", "experts", "n", "k", "stride_e", "stride_n", "packed", "stream"),
-        MAMBO_ENTRY(mambo_fp8_block_matmul, "xv", "ldxv", "xs", "ldxs", "m", "packed", "ws", "n", "k", "out",
+        MAMBO_ENTRY(mambo_fp8_block_matmul, "xv", "ldxv", "xs", "ldxs", "gsxs", "m", "packed", "ws", "n", "k", "out",
                     "out_dtype", "ldo", "stream"),
-        MAMBO_ENTRY(mambo_fp8_block_matmul_experts, "xv", "ldxv", "xs", "ldxs", "m", "rows", "r", "offsets", "experts",
+        MAMBO_ENTRY(mambo_fp8_block_matmul_experts, "xv", "ldxv", "xs", "ldxs", "gsxs", "m", "rows", "r", "offsets", "experts",
                     "packed", "ws", "n", "k", "out", "out_dtype", "ldo", "stream"),
         MAMBO_ENTRY(mambo_iq3s_fp8_matmul_experts, "xv", "ldxv", "xs", "ldxs", "m", "rows", "r", "offsets", "experts",
                     "packed", "expert_stride", "n", "blocks", "out", "out_dtype", "ldo", "stream"),

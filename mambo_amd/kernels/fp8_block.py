@@ -24,7 +24,8 @@ def launch_quantize_fp8_block(x: torch.Tensor, *, stream=None, out: tuple[torch.
     ``x`` is float32 or bfloat16 [M,K] on the GPU, K a multiple of 16, M >= 0. A group of 128 along K
     (the last may be shorter) has the scale max(amax / 448, 2^-100) and the codes of x / scale,
     rounded once to nearest even; a group that holds a NaN or an infinity becomes NaN. Row-strided
-    inputs are read in place. ``out`` optionally supplies (codes, scales) with unit column stride.
+    inputs are read in place. The scales are laid out group by group (strides (1, M)); ``out``
+    optionally supplies codes with unit column stride and scales of either order.
     """
     if not isinstance(x, torch.Tensor) or x.ndim != 2 or x.dtype not in ROW_DTYPES or x.shape[1] % 16 or x.shape[1] < 16:
         raise ValueError("activation must be float32 or bfloat16 [M,K] with K a multiple of 16")
@@ -37,18 +38,19 @@ def launch_quantize_fp8_block(x: torch.Tensor, *, stream=None, out: tuple[torch.
             x = x.contiguous()
         if out is None:
             values = torch.empty((m, k), dtype=torch.uint8, device=dev)
-            scales = torch.empty((m, groups), dtype=torch.float32, device=dev)
-            ldv, lds = k, groups
+            # a group's scales next to each other: the products copy those of 64 rows in one piece
+            scales = torch.empty((groups, m), dtype=torch.float32, device=dev).t()
+            ldv, (lds, gss) = k, (1, m)
         else:
             values, scales = out
             if values.shape != (m, k) or values.dtype != torch.uint8 or scales.shape != (m, groups) \
                     or scales.dtype != torch.float32 or values.device != dev or scales.device != dev \
-                    or not plain_rows(values) or not plain_rows(scales):
-                raise ValueError("out must be (uint8 [M,K], float32 [M,ceil(K/128)]) with unit column stride on the "
-                                 "activation's device")
-            ldv, lds = row_stride(values), row_stride(scales)
+                    or not plain_rows(values) or not (plain_rows(scales) or plain_rows(scales.t())):
+                raise ValueError("out must be (uint8 [M,K] with unit column stride, float32 [M,ceil(K/128)] with unit "
+                                 "row or column stride) on the activation's device")
+            ldv, (lds, gss) = row_stride(values), scale_strides(scales)
         _native.check(_native.lib().mambo_quantize_fp8_block(
-            x.data_ptr(), ROW_DTYPES[x.dtype], m, k, row_stride(x), values.data_ptr(), ldv, scales.data_ptr(), lds,
+            x.data_ptr(), ROW_DTYPES[x.dtype], m, k, row_stride(x), values.data_ptr(), ldv, scales.data_ptr(), lds, gss,
             _native.stream_handle(stream)), "launch_quantize_fp8_block")
     return values, scales
 
@@ -61,6 +63,13 @@ def row_stride(t: torch.Tensor) -> int:
 def plain_rows(t: torch.Tensor) -> bool:
     """Whether rows do not overlap and their elements are next to each other."""
     return (t.shape[1] <= 1 or t.stride(1) == 1) and (t.shape[0] <= 1 or t.stride(0) >= t.shape[1])
+
+
+def scale_strides(t: torch.Tensor) -> tuple[int, int]:
+    """Strides of the rows and the groups of scales [M,G] that are plain rows of groups or of rows."""
+    if t.shape[1] <= 1 or t.stride(1) == 1:
+        return row_stride(t), 1
+    return 1, t.stride(1)
 
 
 def rows_in_place(t: torch.Tensor, align: int) -> torch.Tensor:
@@ -86,7 +95,9 @@ def block_activations(x_values, x_scales, k: int, dev) -> tuple[torch.Tensor, to
         raise ValueError("x_scales must be float32 [M,ceil(K/128)]")
     if x_values.device != dev or x_scales.device != dev:
         raise ValueError("x_values and x_scales must be on the weight's device")
-    return rows_in_place(x_values, 16), rows_in_place(x_scales, 4), m
+    if not plain_rows(x_scales) and not plain_rows(x_scales.t()):
+        x_scales = x_scales.contiguous()
+    return rows_in_place(x_values, 16), x_scales, m
 
 
 def product_output(out, rows: int, n: int, dtype, dev) -> torch.Tensor:
@@ -119,7 +130,7 @@ def launch_fp8_block_matmul(x_values: torch.Tensor, x_scales: torch.Tensor, weig
         x_values, x_scales, m = block_activations(x_values, x_scales, k, dev)
         out = product_output(out, m, n, out_dtype, dev)
         _native.check(_native.lib().mambo_fp8_block_matmul(
-            x_values.data_ptr(), row_stride(x_values), x_scales.data_ptr(), row_stride(x_scales), m, packed.data_ptr(),
+            x_values.data_ptr(), row_stride(x_values), x_scales.data_ptr(), *scale_strides(x_scales), m, packed.data_ptr(),
             weight.scales.data_ptr(), n, k, out.data_ptr(), ROW_DTYPES[out_dtype], row_stride(out),
             _native.stream_handle(stream)), "launch_fp8_block_matmul")
     return out

@@ -29,14 +29,14 @@ def test_packed_bytes(lib):
 
 def test_quantizer_refusals(lib):
     f = lib.mambo_quantize_fp8_block
-    refused(lib, f(16, 2, 1, 128, 128, 16, 128, 16, 1, None), "float32 or bfloat16")
-    refused(lib, f(16, 0, 1, 24, 24, 16, 24, 16, 1, None), "multiple of 16")
-    refused(lib, f(16, 0, -1, 32, 32, 16, 32, 16, 1, None), "multiple of 16")
-    refused(lib, f(16, 0, 1, 144, 144, 16, 144, 16, 1, None), "strides must cover K")
-    refused(lib, f(16, 0, 2, 144, 128, 16, 144, 16, 2, None), "strides must cover K")
-    refused(lib, f(None, 0, 1, 32, 32, 16, 32, 16, 1, None), "null pointer")
-    refused(lib, f(18, 0, 1, 32, 32, 16, 32, 16, 1, None), "aligned to their type")
-    assert f(None, 0, 0, 32, 32, None, 32, None, 1, None) == 0
+    refused(lib, f(16, 2, 1, 128, 128, 16, 128, 16, 1, 1, None), "float32 or bfloat16")
+    refused(lib, f(16, 0, 1, 24, 24, 16, 24, 16, 1, 1, None), "multiple of 16")
+    refused(lib, f(16, 0, -1, 32, 32, 16, 32, 16, 1, 1, None), "multiple of 16")
+    refused(lib, f(16, 0, 2, 144, 144, 16, 144, 16, 1, 1, None), "strides must cover K")
+    refused(lib, f(16, 0, 2, 144, 128, 16, 144, 16, 2, 1, None), "strides must cover K")
+    refused(lib, f(None, 0, 1, 32, 32, 16, 32, 16, 1, 1, None), "null pointer")
+    refused(lib, f(18, 0, 1, 32, 32, 16, 32, 16, 1, 1, None), "aligned to their type")
+    assert f(None, 0, 0, 32, 32, None, 32, None, 1, 1, None) == 0
 
 
 def test_pack_refusals(lib):
@@ -48,18 +48,18 @@ def test_pack_refusals(lib):
 
 
 def test_product_refusals(lib):
-    #      xv  ldxv xs ldxs m packed ws n k out dtype ldo stream
-    good = [16, 32, 16, 1, 2, 16, 16, 8, 32, 16, 0, 8, None]
+    #      xv  ldxv xs ldxs gsxs m packed ws n k out dtype ldo stream
+    good = [16, 32, 16, 1, 1, 2, 16, 16, 8, 32, 16, 0, 8, None]
 
     def call(**change):
-        names = ["xv", "ldxv", "xs", "ldxs", "m", "packed", "ws", "n", "k", "out", "dtype", "ldo", "stream"]
+        names = ["xv", "ldxv", "xs", "ldxs", "gsxs", "m", "packed", "ws", "n", "k", "out", "dtype", "ldo", "stream"]
         args = list(good)
         for name, value in change.items():
             args[names.index(name)] = value
         return lib.mambo_fp8_block_matmul(*args)
 
     for change, text in (({"dtype": 2}, "float32 or bfloat16"), ({"m": -1}, "negative"), ({"k": 40, "ldxv": 48}, "multiple of 16"),
-                         ({"n": 0}, "multiple of 16"), ({"ldxv": 16}, "must cover"), ({"ldxs": 0}, "must cover"),
+                         ({"n": 0}, "multiple of 16"), ({"ldxv": 16}, "must cover"), ({"ldxs": 0}, "must cover"), ({"gsxs": 0}, "must cover"),
                          ({"ldo": 7}, "must cover"), ({"xv": None}, "null pointer"), ({"out": None}, "null pointer"),
                          ({"xv": 8}, "16-byte aligned"), ({"ldxv": 40}, "16-byte aligned"), ({"packed": 24}, "16-byte aligned"),
                          ({"xs": 18}, "aligned to their type"), ({"out": 18}, "aligned to their type")):
@@ -74,9 +74,9 @@ def test_expert_product_refusals(lib):
                                                (16, 2, 16, 1025, 2, "experts must be"), (16, 2, None, 2, 2, "null pointer"),
                                                (16, 2, 16, 2, 0, "a row of its own")):
         text = text.replace("a row of its own", "an input row of its own")
-        refused(lib, f(16, 32, 16, 1, m, rows, r, offsets, experts, 16, 16, 8, 32, 16, 0, 8, None), text)
+        refused(lib, f(16, 32, 16, 1, 1, m, rows, r, offsets, experts, 16, 16, 8, 32, 16, 0, 8, None), text)
         refused(lib, q(16, 256, 16, 8, m, rows, r, offsets, experts, 16, 1760, 8, 1, 16, 0, 8, None), text)
-    assert f(None, 32, None, 1, 0, None, 0, None, 2, None, None, 8, 32, None, 0, 8, None) == 0
+    assert f(None, 32, None, 1, 1, 0, None, 0, None, 2, None, None, 8, 32, None, 0, 8, None) == 0
     assert q(None, 256, None, 8, 0, None, 0, None, 2, None, 1760, 8, 1, None, 0, 8, None) == 0
     for stride, xs, ldxs, text in ((1744, 16, 8, "expert_stride"), (1768, 16, 8, "expert_stride"), (1760, 12, 8, "aligned"),
                                    (1760, 16, 12, "aligned"), (1760, 16, 7, "must cover")):
