@@ -308,11 +308,11 @@ int mambo_fp8_block_pack(const uint8_t *w, int64_t experts, int64_t n, int64_t k
                          int64_t stride_n, uint8_t *packed, mambo_stream_t stream);
 
 /* out[m, n] (f32 or bf16: out_dtype; row stride ldo) = sum over K groups g of 128 of
- * xs[m, g] * ws[n / 128, g] * sum over the group of xv[m, k] * w[n, k], in f32, groups in a fixed
- * order. xv u8 [m, ldxv] E4M3, 16-byte aligned rows; xs f32, row i's of group g at xs + i * ldxs + g *
- * gsxs (rows or groups apart); packed from
- * mambo_fp8_block_pack with one expert; ws f32 [ceil(n/128), ceil(k/128)] contiguous;
- * k % 16 == 0. m == 0: nothing to do. */
+ * xs[m, g] * ws[n / 128, g] * sum over the group of xv[m, k] * w[n, k], in f32, in an order that the
+ * shape fixes (bf16 outputs by the FP8 MFMAs, f32 ones by the bf16 MFMAs, which add more exactly at half
+ * the rate). xv u8 [m, ldxv] E4M3, 16-byte aligned rows; xs f32, row i's of group g at xs + i * ldxs + g *
+ * gsxs (rows or groups apart); packed from mambo_fp8_block_pack with one expert; ws f32 [ceil(n/128),
+ * ceil(k/128)] contiguous; k % 16 == 0. m == 0: nothing to do. */
 int mambo_fp8_block_matmul(const uint8_t *xv, int64_t ldxv, const float *xs, int64_t ldxs, int64_t gsxs,
                            int64_t m, const uint8_t *packed, const float *ws, int64_t n, int64_t k, void *out,
                            int out_dtype, int64_t ldo, mambo_stream_t stream);
@@ -325,6 +325,12 @@ int mambo_fp8_block_matmul_experts(const uint8_t *xv, int64_t ldxv, const float 
                                    int64_t m, const int32_t *rows, int64_t r, const int32_t *offsets, int64_t experts,
                                    const uint8_t *packed, const float *ws, int64_t n, int64_t k, void *out,
                                    int out_dtype, int64_t ldo, mambo_stream_t stream);
+
+/* The workgroup that such a product takes, on the host alone: tile[3] = tokens, weight rows and parts of
+ * K that it works on at once. experts 0: mambo_fp8_block_matmul of m rows; else r rows of m (m != r: by
+ * rows). Scales as mambo_quantize_fp8_block lays them out best. */
+int mambo_fp8_block_plan(int64_t m, int64_t r, int64_t experts, int64_t n, int64_t k, int64_t ldxv, int out_dtype,
+                         int32_t *tile);
 
 /* mambo_iq3s_fp8_matmul grouped by expert: rows and offsets as above, weight e in the tile layout
  * (mambo_iq3s_prepare) at packed + e * expert_stride bytes, a multiple of 16 and at least

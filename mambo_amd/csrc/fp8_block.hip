@@ -685,14 +685,22 @@ int launch_products(const Fp8Args &a, int which, int64_t wgs, hipStream_t stream
     return mambo_check_launch("fp8_block_matmul");
 }
 
-int run_products(const uint8_t *xv, int64_t ldxv, const float *xs, int64_t ldxs, int64_t gsxs, const ExpertRows &er,
-                 const uint8_t *packed, const float *ws, int64_t n, int64_t k, void *out, int out_dtype, int64_t ldo,
-                 hipStream_t stream)
+int check_product(int64_t n, int64_t k, int out_dtype)
 {
     MAMBO_REQUIRE(out_dtype == MAMBO_DTYPE_F32 || out_dtype == MAMBO_DTYPE_BF16, MAMBO_ERR_VALUE,
                   "outputs must be float32 or bfloat16");
     MAMBO_REQUIRE(n >= 1 && n <= 0x7FFFFF00 && k >= 16 && k <= 0x7FFFFF00 && k % 16 == 0, MAMBO_ERR_VALUE,
                   "weights must be [N,K] with N >= 1 and K a multiple of 16 (got N=%lld K=%lld)", (long long)n, (long long)k);
+    return MAMBO_OK;
+}
+
+int run_products(const uint8_t *xv, int64_t ldxv, const float *xs, int64_t ldxs, int64_t gsxs, const ExpertRows &er,
+                 const uint8_t *packed, const float *ws, int64_t n, int64_t k, void *out, int out_dtype, int64_t ldo,
+                 hipStream_t stream)
+{
+    const int rc = check_product(n, k, out_dtype);
+    if (rc != MAMBO_OK)
+        return rc;
     MAMBO_REQUIRE(ldxv >= k && ldo >= n && scales_apart(ldxs, gsxs, er.m, cdiv(k, kGroup)), MAMBO_ERR_VALUE,
                   "strides must cover the rows");
     if (er.r == 0)
@@ -784,6 +792,29 @@ extern "C" int mambo_fp8_block_matmul(const uint8_t *xv, int64_t ldxv, const flo
     MAMBO_REQUIRE(m >= 0, MAMBO_ERR_VALUE, "rows must not be negative");
     const ExpertRows er = {nullptr, nullptr, m, m, 1};
     return run_products(xv, ldxv, xs, ldxs, gsxs, er, packed, ws, n, k, out, out_dtype, ldo, (hipStream_t)stream);
+}
+
+extern "C" int mambo_fp8_block_plan(int64_t m, int64_t r, int64_t experts, int64_t n, int64_t k, int64_t ldxv,
+                                    int out_dtype, int32_t *tile)
+{
+    static const int32_t one = 0; // never read: that the plan is of rows by expert, or gathered
+    const int32_t *rows = experts && m != r ? &one : nullptr, *offsets = experts ? &one : nullptr;
+    int rc = check_product(n, k, out_dtype);
+    if (rc == MAMBO_OK)
+        rc = check_expert_rows(m, rows, experts ? r : m, experts ? offsets : &one, experts ? experts : 1);
+    if (rc != MAMBO_OK)
+        return rc;
+    MAMBO_REQUIRE(ldxv >= k && tile && (experts ? r : m) >= 1, MAMBO_ERR_VALUE, "a plan is of one row or more");
+    Fp8Args a = {};
+    a.er = {offsets, rows, experts ? r : m, m, (int)(experts ? experts : 1)};
+    a.ldxv = ldxv, a.ldxs = 1, a.gsxs = m;
+    a.n = (int)n, a.k = (int)k, a.groups = (int)cdiv(k, kGroup);
+    int64_t wgs = 0;
+    const int which = fp8_plan(a, out_dtype == MAMBO_DTYPE_BF16, &wgs);
+    MAMBO_REQUIRE(which >= 0, MAMBO_ERR_VALUE, "too many rows and columns for one launch");
+    const Fp8Kernel &t = kFp8Kernels[out_dtype == MAMBO_DTYPE_BF16][which];
+    tile[0] = t.tokens, tile[1] = t.rows, tile[2] = t.kg;
+    return MAMBO_OK;
 }
 
 extern "C" int mambo_fp8_block_matmul_experts(const uint8_t *xv, int64_t ldxv, const float *xs, int64_t ldxs, int64_t gsxs,
