@@ -1,10 +1,8 @@
 // IQ3_S x MXFP8 products grouped by expert.
 //
-// Few rows an expert: the weights' bytes bound it. A workgroup computes 16 tokens x 32 weight rows;
-// its W waves take the K blocks in turn and each streams its own through a ring of two blocks in
-// registers, decoded as the dense kernel's (iq3s_dense.h): exact two-term E4M3 operands in the order of
-// the dense MFMA, four MFMAs a block and 16 rows, the block's fp16 d in f32. The waves' sums meet in
-// LDS at the end and are added in order.
+// Few rows an expert: a workgroup computes 16 tokens, or 4, x 32 weight rows; its W waves take the K blocks
+// in turn and each streams its own through a ring of two blocks in registers. The waves' sums meet in
+// LDS at the end and are added in order. More rows: the 32 x 32 MFMA kernel (iq3s_wide.h).
 #include <cmath>
 
 #include "iq3s_dense.h"
@@ -24,56 +22,74 @@ struct Iq3sArgs {
     bool vec;
 };
 
-template <int W, bool kBf16>
+// kDiag false: 16 tokens, every weight as an exact pair of E4M3 terms (iq3s_dense.h), four MFMAs a block and 16 rows.
+// kDiag true: 4 tokens, whose rows fill the MFMA's 16 by its four blocks of K (ALane), so that a weight is its codebook
+// word alone and its scale multiplies the sums: two MFMAs and 88 vector instructions a block and 16 rows against 120.
+// Both are bound by those instructions (16 lookups, signs, addresses), not by the weights' bytes: 8 experts of 14336 x 4096,
+// of which 6 have rows, 151 MB: 4 tokens each at most 33.9 us (4.5 TB/s), 16 36.3 (with four waves a workgroup 34.4 and
+// 41.4). More copies of the codebook in LDS, against bank conflicts, gained nothing; a workgroup of several
+// columns (which share the codebook) neither; 16 weight rows a wave instead of 32 lost 20%, 64 lost 5%.
+template <bool kDiag, int W, bool kBf16>
 __global__ __launch_bounds__(W * 64) __attribute__((amdgpu_waves_per_eu(2))) void iq3s_expert_stream_kernel(Iq3sArgs a)
 {
-    constexpr int T = 16, NT = 2, kPad = 36;
-    __shared__ uint32_t s_lvl[512];
+    constexpr int T = kDiag ? 4 : 16, NT = 2, kPad = 16 * NT + 4, kQuads = 4 * NT;
+    __shared__ __align__(16) uint32_t s_lut[512];
     __shared__ uint4 s_split[16];
     __shared__ __align__(16) float s_red[W * T * kPad];
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int nt = blockIdx.x % a.ntiles;
+    const int tiles = (a.n + kTileRows - 1) / kTileRows, nt = blockIdx.x % a.ntiles;
     RowTile rt;
     if (!find_row_tile(a.er, T, blockIdx.x / a.ntiles, &rt))
         return;
     const bool none = rt.expert == a.er.experts;
     if (!none) {
-        for (int i = tid; i < 512; i += W * 64)
-            s_lvl[i] = c_grid.level[i];
-        if (tid < 16)
-            s_split[tid] = uint4{c_split.w[tid][0], c_split.w[tid][1], c_split.w[tid][2], c_split.w[tid][3]};
-        const int col = lane & 15, q = lane >> 4;
-        const int B = a.blocks, tiles = (a.n + kTileRows - 1) / kTileRows;
+        const int col = lane & 15, q = lane >> 4, B = a.blocks;
         const uint8_t *weight = a.packed + (int64_t)rt.expert * a.expert_stride;
         __amdgpu_buffer_rsrc_t wt[NT];
 #pragma unroll
         for (int t = 0; t < NT; ++t)
             wt[t] = byte_rsrc(weight + (int64_t)min(NT * nt + t, tiles - 1) * B * kTileBytes);
-        // the bytes and the scale of this lane's token (compute_dense, load_a_dense)
-        const int64_t src = source_row(a.er, rt.row0 + min(col, rt.count - 1));
-        const uint8_t *xp = a.xv + src * a.ldxv + 32 * (4 * (q >> 1)) + 16 * (q & 1);
-        const uint8_t *sp = a.xs + src * a.ldxs + 4 * (q & 1) + 2 * (q >> 1);
-        const uint8_t *lvl = reinterpret_cast<const uint8_t *>(s_lvl);
         const int count = wave < B ? (B - wave + W - 1) / W : 0;
+        const int token = kDiag ? lane & 3 : col;
+        const int64_t src = source_row(a.er, rt.row0 + min(token, rt.count - 1));
+        const uint8_t *xrow = a.xv + src * a.ldxv, *srow = a.xs + src * a.ldxs;
+        const ALane al[1] = {a_lane<false>(lane, token < rt.count, xrow, srow, g_zero_chunk, g_unit_scales)};
+        // the bytes and the scale of this lane's token (compute_dense, load_a_dense)
+        const uint8_t *xp = xrow + 32 * (4 * (q >> 1)) + 16 * (q & 1), *sp = srow + 4 * (q & 1) + 2 * (q >> 1);
         struct Ring {
             WTile w[NT];
-            uint4 x[4];
-            uint16_t s;
+            ATile<1> x;
         } ring[2];
         auto load = [&](Ring &r, int i) {
             const int b = min(wave + max(min(i, count - 1), 0) * W, B - 1);
 #pragma unroll
             for (int t = 0; t < NT; ++t)
                 r.w[t] = load_w_rsrc(wt[t], (uint32_t)b * kTileBytes, lane, col);
-            const uint8_t *p = xp + 256 * (int64_t)b;
+            if constexpr (kDiag) {
+                load_a<1>(r.x, al, b, g_zero_chunk);
+            } else {
+                const uint8_t *p = xp + 256 * (int64_t)b;
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
-                r.x[j] = *reinterpret_cast<const uint4 *>(p + 32 * (j >> 1) + 64 * (j & 1));
-            r.s = *reinterpret_cast<const uint16_t *>(sp + 8 * (int64_t)b);
+                for (int h = 0; h < 2; ++h) {
+                    const uint4 l = *reinterpret_cast<const uint4 *>(p + 32 * h), u = *reinterpret_cast<const uint4 *>(p + 32 * h + 64);
+                    r.x.a[0][h] = v8i{(int)l.x, (int)l.y, (int)l.z, (int)l.w, (int)u.x, (int)u.y, (int)u.z, (int)u.w};
+                }
+                r.x.s[0] = *reinterpret_cast<const uint16_t *>(sp + 8 * (int64_t)b);
+            }
         };
-        float acc[NT][4] = {};
         load(ring[0], 0);
+        if constexpr (kDiag) {
+            for (int i = tid; i < 128; i += W * 64)
+                reinterpret_cast<uint4 *>(s_lut)[i] = reinterpret_cast<const uint4 *>(rep_grid<0>())[i];
+        } else {
+            for (int i = tid; i < 512; i += W * 64)
+                s_lut[i] = c_grid.level[i];
+            if (tid < 16)
+                s_split[tid] = uint4{c_split.w[tid][0], c_split.w[tid][1], c_split.w[tid][2], c_split.w[tid][3]};
+        }
+        const uint8_t *lut = reinterpret_cast<const uint8_t *>(s_lut);
+        float acc[NT][1][4] = {};
         __syncthreads();
         for (int i0 = 0; i0 < count; i0 += 2) {
 #pragma unroll
@@ -81,50 +97,53 @@ __global__ __launch_bounds__(W * 64) __attribute__((amdgpu_waves_per_eu(2))) voi
                 load(ring[j ^ 1], i0 + j + 1);
                 __builtin_amdgcn_sched_barrier(0);
                 const Ring &r = ring[j];
-                v8i x[2];
-#pragma unroll
-                for (int h = 0; h < 2; ++h)
-                    x[h] = v8i{(int)r.x[2 * h].x,     (int)r.x[2 * h].y,     (int)r.x[2 * h].z,     (int)r.x[2 * h].w,
-                               (int)r.x[2 * h + 1].x, (int)r.x[2 * h + 1].y, (int)r.x[2 * h + 1].z, (int)r.x[2 * h + 1].w};
 #pragma unroll
                 for (int t = 0; t < NT; ++t) {
-                    v8i bh[2], bl[2];
-                    decode_block(r.w[t], lvl, s_split, bh, bl);
-                    const float d = i0 + j < count ? half_bits_to_float(r.w[t].dh) : 0.0f;
-                    v4f c = {0.0f, 0.0f, 0.0f, 0.0f};
-                    const int s0 = r.s & 255, s1 = r.s >> 8;
-                    c = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(x[0], bh[0], c, 0, 0, 0, s0, 0, 128);
-                    c = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(x[0], bl[0], c, 0, 0, 0, s0, 0, 128);
-                    c = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(x[1], bh[1], c, 0, 0, 0, s1, 0, 128);
-                    c = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(x[1], bl[1], c, 0, 0, 0, s1, 0, 128);
+                    if constexpr (kDiag) {
+                        compute_block<1, 0>(r.w[t], r.x, lut, 0, acc[t], i0 + j < count);
+                    } else {
+                        v8i bh[2], bl[2];
+                        decode_block(r.w[t], lut, s_split, bh, bl);
+                        const float d = i0 + j < count ? half_bits_to_float(r.w[t].dh) : 0.0f;
+                        v4f c = {0.0f, 0.0f, 0.0f, 0.0f};
+                        const int s0 = r.x.s[0] & 255, s1 = r.x.s[0] >> 8;
+                        c = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(r.x.a[0][0], bh[0], c, 0, 0, 0, s0, 0, 128);
+                        c = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(r.x.a[0][0], bl[0], c, 0, 0, 0, s0, 0, 128);
+                        c = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(r.x.a[0][1], bh[1], c, 0, 0, 0, s1, 0, 128);
+                        c = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(r.x.a[0][1], bl[1], c, 0, 0, 0, s1, 0, 128);
 #pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        acc[t][i] = __builtin_fmaf(c[i], d, acc[t][i]);
+                        for (int i = 0; i < 4; ++i)
+                            acc[t][0][i] = __builtin_fmaf(c[i], d, acc[t][0][i]);
+                    }
                 }
                 __builtin_amdgcn_sched_barrier(0);
             }
         }
-        // the sums of a lane: tokens 4q .. 4q + 3, weight row col of each tile
-        float *red = s_red + (wave * T + 4 * q) * kPad + col;
+        float *red = s_red + wave * T * kPad + col;
 #pragma unroll
         for (int t = 0; t < NT; ++t)
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
-                red[i * kPad + 16 * t] = acc[t][i];
+            for (int i = 0; i < 4; ++i) {
+                if constexpr (kDiag) {
+                    const float v = lane_group_sum(acc[t][0][i]);
+                    if (lane < 16)
+                        red[i * kPad + 16 * t] = v;
+                } else {
+                    red[(4 * q + i) * kPad + 16 * t] = acc[t][0][i];
+                }
+            }
     }
     __syncthreads();
-    for (int i = tid; i < T * 8; i += W * 64) {
-        const int token = i >> 3, n4 = 4 * (i & 7);
-        if (token >= rt.count)
-            break;
+    for (int i = tid; i < T * kQuads; i += W * 64) {
+        const int token = i / kQuads, n4 = 4 * (i % kQuads), at = nt * 16 * NT + n4;
+        if (token >= rt.count || at >= a.n)
+            continue;
         v4f v = {0.0f, 0.0f, 0.0f, 0.0f};
         if (!none)
 #pragma unroll
             for (int w = 0; w < W; ++w)
                 v += *reinterpret_cast<const v4f *>(s_red + (w * T + token) * kPad + n4);
-        const int at = nt * 32 + n4;
-        if (at < a.n)
-            store_row4<kBf16>(a.out, (rt.row0 + token) * a.ldo + at, v, a.n - at, a.vec);
+        store_row4<kBf16>(a.out, (rt.row0 + token) * a.ldo + at, v, a.n - at, a.vec);
     }
 }
 
@@ -157,24 +176,43 @@ extern "C" int mambo_iq3s_fp8_matmul_experts(const uint8_t *xv, int64_t ldxv, co
     const ExpertRows er = {offsets, rows, r, m, (int)experts};
     const bool bf16 = out_dtype == MAMBO_DTYPE_BF16;
     hipStream_t s = (hipStream_t)stream;
-    // the 32 x 32 MFMA kernel from 17 rows of an expert on; it tells rows by 32-bit offsets
+    const Iq3sArgs a = {xv, xs, ldxv, ldxs, er, packed, expert_stride, out, ldo, (int)n,
+                        (int)blocks, (int)((n + 31) / 32), rows_take_vectors(out, ldo, out_dtype)};
+    // How the rows fall is not known here: experts with rows and tiles are counted for rows that fall at random.
     const double taken = (double)experts * -std::expm1(-(double)r / (double)experts);
-    if ((double)r > 16.0 * taken && (rows ? m : 256) * ldxv + 256 * blocks < ((int64_t)1 << 32) &&
+    auto tiles = [&](int t) { return std::fmax(taken, (double)r / t + 0.5 * taken); };
+    // The 32 x 32 MFMA kernel from 14 rows of an expert on, where 16 tokens a tile fill the card four times: 64 experts of
+    // 2048 x 4096 with 12 rows each take it 75.4 us (the 16-token kernel 72.5), with 16 76.1 (94.6), 4 experts of 1024 x
+    // 4096 with 64 rows 24.8 (16.1). It tells rows by 32-bit offsets.
+    if ((double)r > 14.0 * taken && tiles(16) * a.ntiles >= 1024.0 && (rows ? m : 256) * ldxv + 256 * blocks < ((int64_t)1 << 32) &&
         (rows ? m : 256) * ldxs + 8 * blocks < ((int64_t)1 << 32) && expert_row_tiles(r, experts, 64) <= 65535) {
-        double tiles_of[2];
-        for (int i = 0; i < 2; ++i)
-            tiles_of[i] = std::fmax(taken, (double)r / (64 << i) + 0.5 * taken);
+        double tiles_of[2] = {tiles(64), tiles(128)};
         WidePlan plan;
         mambo_wide_experts_plan(er, n, blocks, tiles_of, &plan);
         return mambo_wide_experts_launch(plan, xv, ldxv, xs, ldxs, er, packed, expert_stride, n, blocks, out, bf16, ldo, s);
     }
-    const Iq3sArgs a = {xv, xs, ldxv, ldxs, er, packed, expert_stride, out, ldo, (int)n,
-                        (int)blocks, (int)((n + 31) / 32), rows_take_vectors(out, ldo, out_dtype)};
-    const int64_t wgs = expert_row_tiles(r, experts, 16) * a.ntiles;
+    // 4 tokens a tile up to 2.5 rows of an expert: 64 experts of 2048 x 4096 with 2.3 rows take 43.4 us (16 tokens a tile
+    // 47.6), with 4 62.5 (50.8).
+    const bool diag = (double)r <= 2.5 * taken;
+    // Waves that share a workgroup's K, two blocks each at least: one where workgroups fill the card, more where they do
+    // not (8 x 14336 x 4096, 4 tokens a tile, 3136 workgroups: 40.0 us with one, 42.1 with two, 43.6 with four; 2 experts,
+    // 896: 16.1, 14.5, 14.9; 2 of 4096 x 14336, 256: 34.8, 21.1, 14.7).
+    const double expected = tiles(diag ? 4 : 16) * a.ntiles;
+    const int waves = expected >= 2560.0 || blocks < 4 ? 1 : expected >= 640.0 || blocks < 8 ? 2 : 4;
+    const int64_t wgs = expert_row_tiles(r, experts, diag ? 4 : 16) * a.ntiles;
     MAMBO_REQUIRE(wgs <= 0x7FFFFFFF, MAMBO_ERR_VALUE, "too many rows and columns for one launch");
-    if (bf16)
-        MAMBO_LAUNCH((iq3s_expert_stream_kernel<4, true>), dim3((unsigned)wgs), dim3(256), 0, s, a);
-    else
-        MAMBO_LAUNCH((iq3s_expert_stream_kernel<4, false>), dim3((unsigned)wgs), dim3(256), 0, s, a);
+#define MAMBO_IQ3S(D, W, B)                                                                                            \
+    if (diag == D && waves == W && bf16 == B)                                                                          \
+    MAMBO_LAUNCH((iq3s_expert_stream_kernel<D, W, B>), dim3((unsigned)wgs), dim3(W * 64), 0, s, a)
+#define MAMBO_IQ3S_WAVES(D, B) \
+    MAMBO_IQ3S(D, 1, B);       \
+    MAMBO_IQ3S(D, 2, B);       \
+    MAMBO_IQ3S(D, 4, B)
+    MAMBO_IQ3S_WAVES(false, false);
+    MAMBO_IQ3S_WAVES(false, true);
+    MAMBO_IQ3S_WAVES(true, false);
+    MAMBO_IQ3S_WAVES(true, true);
+#undef MAMBO_IQ3S_WAVES
+#undef MAMBO_IQ3S
     return mambo_check_launch("iq3s_fp8_matmul_experts");
 }

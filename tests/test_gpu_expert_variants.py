@@ -241,3 +241,43 @@ def test_join_and_router_far_apart(gpu):
     logits.copy_(torch.from_numpy(rng.standard_normal((40, 70)).astype(np.float32)))
     for a, b in zip(launch_route_experts(logits, 3), launch_route_experts(logits.contiguous(), 3)):
         assert torch.equal(a, b)
+
+
+# ------------------------------------------------------------------------------ IQ3_S by expert
+@pytest.mark.gpu
+@pytest.mark.parametrize("gather", [True, False])
+@pytest.mark.parametrize("r,experts,n,k", [
+    (3, 4, 70, 2304), (6, 4, 9000, 2304), (150, 120, 1000, 2304),  # 4 tokens a tile: four waves, two, one
+    (20, 4, 70, 2304), (60, 6, 6000, 2304), (200, 20, 4000, 2048),  # 16 tokens a tile: four, two, one
+    (300, 4, 2211, 1024),  # the 32 x 32 MFMAs
+])
+def test_iq3s_kernels(gpu, r, experts, n, k, gather):
+    """As test_gpu_experts.test_iq3s_experts, at sizes that each of the kernels takes; an expert may have
+    more rows than the tile of the kernel that the average chose."""
+    from mambo_amd.kernels.experts import launch_iq3_s_fp8_matmul_experts
+    from mambo_amd.kernels.quantize_fp8 import launch_quantize_fp8
+    from mambo_amd.utils.iq3_s_weight import prepare_iq3_s_experts
+    from oracle import oracle
+    rng = np.random.default_rng(r + experts + n + k)
+    m = max(1, r // 3) if gather else r
+    raws = rng.integers(0, 256, size=(experts, n, k // 256, 110), dtype=np.uint8)
+    raws[..., :2] = (0.01 + 0.02 * rng.random((experts, n, k // 256, 1))).astype(np.float16).view(np.uint8)
+    x = rng.standard_normal((m, k)).astype(np.float32)
+    offsets = ref.some_offsets(rng, r, experts, 1)
+    rows = rng.integers(0, m, size=r).astype(np.int32) if gather else np.arange(r, dtype=np.int32)
+    eq, es = oracle.quantize_mxfp8(x)
+    expected = np.zeros((r, n))
+    for e in range(experts):
+        at = rows[offsets[e]:offsets[e + 1]]
+        if at.size:
+            expected[offsets[e]:offsets[e + 1]] = oracle.iq3s_fp8_matmul(eq[at], es[at], raws[e])
+    x, raws, offsets, rows = (torch.from_numpy(a).to(gpu) for a in (x, raws, offsets, rows))
+    w = prepare_iq3_s_experts(raws)
+    values, scales = launch_quantize_fp8(x)
+    taken = int(offsets[-1])
+    for dtype, tolerance in ((F32, 1e-4), (BF16, 2.0**-8)):
+        out = launch_iq3_s_fp8_matmul_experts(values, scales, w, offsets, rows=rows if gather else None,
+                                              out_dtype=dtype).double().cpu().numpy()
+        assert not out[taken:].any()
+        for i in range(taken):  # row by row, so that one wrong row shows
+            assert np.linalg.norm(out[i] - expected[i]) <= tolerance * np.linalg.norm(expected[i]), i
