@@ -326,11 +326,12 @@ int mambo_fp8_block_matmul_experts(const uint8_t *xv, int64_t ldxv, const float 
                                    const uint8_t *packed, const float *ws, int64_t n, int64_t k, void *out,
                                    int out_dtype, int64_t ldo, mambo_stream_t stream);
 
-/* The workgroup that such a product takes, on the host alone: tile[3] = tokens, weight rows and parts of
- * K that it works on at once. experts 0: mambo_fp8_block_matmul of m rows; else r rows of m (m != r: by
+/* How such a product is launched, on the host alone: plan[5] = tokens, weight rows and parts of K that a
+ * workgroup works on at once, and the order of workgroups: columns of a group, and how many go to an XCD
+ * at a time. experts 0: mambo_fp8_block_matmul of m rows; else r rows of m (m != r: by
  * rows). Scales as mambo_quantize_fp8_block lays them out best. */
 int mambo_fp8_block_plan(int64_t m, int64_t r, int64_t experts, int64_t n, int64_t k, int64_t ldxv, int out_dtype,
-                         int32_t *tile);
+                         int32_t *plan);
 
 /* mambo_iq3s_fp8_matmul grouped by expert: rows and offsets as above, weight e in the tile layout
  * (mambo_iq3s_prepare) at packed + e * expert_stride bytes, a multiple of 16 and at least

@@ -194,7 +194,7 @@ CONSTRAINTS: dict[str, list[dict]] = {
         _arr("ws", "float32", ["(n+127)/128", "(k+127)/128"], align=4),
         _arr("out", "float32|bfloat16", ["m", "n"], ["ldo", "1"], align=2, access="write"),
     ],
-    "mambo_fp8_block_plan": [_arr("tile", "int32", ["3"], align=4, memory="host", access="write")],
+    "mambo_fp8_block_plan": [_arr("plan", "int32", ["5"], align=4, memory="host", access="write")],
     "mambo_fp8_block_matmul_experts": [
         _arr("xv", "uint8", ["m", "k"], ["ldxv", "1"], align=16),
         _arr("xs", "float32", ["m", "(k+127)/128"], ["ldxs", "gsxs"], align=4),

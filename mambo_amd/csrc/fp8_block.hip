@@ -23,6 +23,7 @@
 // operand: lane (i, h) of the 32 x 32 MFMA of K step s takes chunks 4s + h and 4s + 2 + h, of the 16 x
 // 16 MFMA chunks h and 4 + h. Rows past n and K past k are zeros, so nothing else looks after the
 // ends of a weight. (Any order of K serves that both operands share.)
+#include <algorithm>
 #include <cmath>
 #include <type_traits>
 
@@ -166,7 +167,24 @@ struct Fp8Args {
     int64_t ldo;
     int n, k, groups, ntiles; // groups of K, tiles of 32 weight rows
     bool vec;                 // the outputs take one store of four
+    uint32_t tiles, group, deal; // Order
 };
+
+// The row tile and the column tile of this workgroup. Workgroups go to the eight XCDs in turn, and each XCD has an L2 of its
+// own: they are dealt to it `deal` at a time from an order of column groups (`group` columns wide), in a group row tile by row
+// tile, in a row tile column by column. False: a workgroup past the last.
+__device__ __forceinline__ bool place(const Fp8Args &a, int columns, int *tile, int *column)
+{
+    const uint32_t xcd = blockIdx.x & 7, i = blockIdx.x >> 3, round = i / a.deal;
+    const uint32_t at = (round * 8 + xcd) * a.deal + (i - round * a.deal);
+    if (at >= a.tiles * (uint32_t)columns)
+        return false;
+    const uint32_t span = a.group * a.tiles, group = at / span, rest = at - group * span;
+    const uint32_t width = min(a.group, (uint32_t)columns - group * a.group);
+    *tile = (int)(rest / width);
+    *column = (int)(group * a.group + (rest - (uint32_t)*tile * width));
+    return true;
+}
 
 template <bool kExperts>
 __device__ __forceinline__ bool row_tile(const Fp8Args &a, int tile, int t, RowTile *rt)
@@ -248,9 +266,9 @@ __global__ __launch_bounds__(W * 64) void fp8_stream_kernel(Fp8Args a)
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int tiles_n = (a.n + kCols - 1) / kCols;
-    const int nt = blockIdx.x % tiles_n;
     RowTile rt;
-    if (!row_tile<kExperts>(a, T, blockIdx.x / tiles_n, &rt))
+    int tile_m, nt;
+    if (!place(a, tiles_n, &tile_m, &nt) || !row_tile<kExperts>(a, T, tile_m, &rt))
         return;
     const bool none = kExperts && rt.expert == a.er.experts;
 
@@ -370,9 +388,10 @@ __global__ __launch_bounds__(WN * KG * 64) __attribute__((amdgpu_waves_per_eu(2)
     const int col = lane & 31, h = lane >> 5;
     const int tiles_n = (a.ntiles + NB * WN - 1) / (NB * WN);
     RowTile rt;
-    if (!row_tile<kExperts>(a, kRows, blockIdx.x / tiles_n, &rt))
+    int tile_m, column;
+    if (!place(a, tiles_n, &tile_m, &column) || !row_tile<kExperts>(a, kRows, tile_m, &rt))
         return;
-    const int nt = (blockIdx.x % tiles_n) * (NB * WN) + wave * NB; // this wave's first tile of 32 weight rows
+    const int nt = column * (NB * WN) + wave * NB; // this wave's first tile of 32 weight rows
     float acc[MT][NB][16];
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt)
@@ -577,70 +596,111 @@ __global__ __launch_bounds__(WN * KG * 64) __attribute__((amdgpu_waves_per_eu(2)
 
 // The kernels of a product: tokens and weight rows of a workgroup, K groups of waves in it, workgroups that a CU holds, and
 // microseconds: of a launch, of a round of workgroups on the busiest CU, of a step of a K group with 1, 2, .. of them on
-// the CU, per million outputs and per million weights.
+// the CU, per million outputs and, beside these (the longer of the two hides most of the other: their squares add up), per
+// million weights.
 struct Fp8Kernel {
     int tokens, rows, kg, resident;
     double launch, round, step[4], outputs, weights;
 };
-// Fitted to 355 products (1 to 8192 tokens, 300 to 57344 rows, K 272 to 28672, weights rotated past the caches) and, with
-// less weight, 174 grouped ones: the kernel that they pick takes 1.8% more than the fastest of the nine on average (f32 1.4%,
-// grouped, where they do not know how the rows fall, 6%). None of the nine is spare: without it the fastest of the
-// others takes 0.1 to 1.7% more on average and up to 1.15 to 1.6 times. 128 x 128 tiles, 64 x 128 tiles of one K group and
-// a second buffer for the weights were measured too, and either gained less than 0.6% or lost (the buffer 1 to 10%).
-constexpr Fp8Kernel kFp8Kernels[2][9] = {
-    {{16, 16, 8, 2, 2.750, 0.270, {0.676, 1.423}, 9.980, 0.000},
-     {16, 32, 4, 4, 1.577, 1.555, {0.490, 1.020, 1.624, 2.157}, 3.334, 0.024},
-     {16, 64, 4, 4, 0.000, 3.336, {0.741, 1.586, 2.586, 3.719}, 1.911, 0.061},
-     {32, 64, 8, 1, 1.579, 2.274, {1.102}, 2.152, 0.106},
-     {64, 64, 4, 2, 1.791, 2.547, {0.961, 2.330}, 1.579, 0.058},
-     {64, 128, 2, 2, 3.181, 0.583, {0.932, 2.123}, 1.198, 0.062},
-     {64, 256, 2, 1, 2.667, 2.028, {1.623}, 1.397, 0.046},
-     {64, 256, 1, 2, 3.695, 0.240, {1.081, 1.661}, 0.875, 0.048},
+// Fitted to 355 products a dense table (1 to 8192 tokens, 300 to 57344 rows, K 272 to 28672, weights rotated past the caches)
+// and 174 by expert. The kernel that they pick takes 0.8% more than the fastest of the nine on average (f32 0.9%, by
+// expert, where they do not know how the rows fall, 3.3%). None of the nine is spare: without it the fastest of the others
+// takes 0.2 to 3% more on average and up to 1.11 to 1.63 times. Measured beside them: 128 x 128 tiles, 64 x 64 of eight K
+// groups, 64 x 128 and 64 x 64 of one and two (no gain of 0.5%); a second and a third buffer for the weights and the rows
+// (0 to 25% slower: a step is not bound by the latency of its loads).
+constexpr Fp8Kernel kFp8Kernels[3][9] = {
+    // float32 outputs
+    {{16, 16, 8, 2, 2.601, 0.338, {0.707, 1.432}, 9.221, 0.000},
+     {16, 32, 4, 4, 2.726, 0.394, {0.474, 0.952, 1.534, 1.873}, 2.753, 0.110},
+     {16, 64, 4, 4, 2.533, 0.749, {0.750, 1.498, 2.334, 3.287}, 1.519, 0.144},
+     {32, 64, 4, 3, 3.442, 0.230, {0.638, 1.208, 1.874}, 1.844, 0.166},
+     {64, 64, 4, 2, 3.421, 1.014, {1.004, 2.267}, 2.027, 0.145},
+     {64, 128, 2, 2, 4.146, 0.000, {0.965, 2.095}, 1.180, 0.136},
+     {64, 256, 2, 1, 3.914, 0.791, {1.676}, 1.215, 0.137},
+     {64, 256, 1, 2, 4.216, 0.000, {1.101, 1.726}, 0.644, 0.149},
      {0, 0, 0, 0, 0.0, 0.0, {}, 0.0, 0.0}}, // 128 x 256 tiles through bf16 spill
-    {{16, 16, 8, 2, 2.806, 0.000, {0.696, 1.401}, 13.114, 0.000},
-     {16, 32, 4, 4, 2.833, 0.000, {0.495, 1.020, 1.560, 1.852}, 5.448, 0.021},
-     {16, 64, 4, 4, 3.088, 0.000, {0.719, 1.564, 1.888, 2.495}, 3.400, 0.051},
-     {32, 64, 8, 1, 2.162, 1.477, {1.072}, 1.853, 0.108},
-     {64, 64, 4, 2, 3.640, 0.155, {0.679, 1.404}, 1.226, 0.081},
-     {64, 128, 2, 2, 3.457, 0.000, {0.548, 1.125}, 0.665, 0.083},
-     {64, 256, 2, 1, 2.765, 1.462, {0.998}, 0.669, 0.074},
-     {64, 256, 1, 2, 2.406, 1.225, {0.690, 0.964}, 0.423, 0.058},
-     {128, 256, 1, 2, 3.855, 0.000, {1.034, 1.546}, 0.498, 0.038}}};
+    // bfloat16 outputs
+    {{16, 16, 8, 2, 2.617, 0.179, {0.729, 1.417}, 12.342, 0.000},
+     {16, 32, 4, 4, 2.904, 0.000, {0.472, 0.943, 1.505, 1.882}, 3.222, 0.108},
+     {16, 64, 4, 4, 3.040, 0.000, {0.726, 1.432, 2.188, 3.133}, 1.687, 0.134},
+     {32, 64, 4, 3, 3.307, 0.320, {0.500, 1.100, 1.610}, 0.913, 0.180},
+     {64, 64, 4, 2, 3.453, 0.669, {0.695, 1.476}, 0.996, 0.184},
+     {64, 128, 2, 2, 3.595, 0.120, {0.595, 1.183}, 0.514, 0.179},
+     {64, 256, 2, 1, 3.285, 1.096, {1.075}, 0.570, 0.182},
+     {64, 256, 1, 2, 3.324, 0.000, {0.754, 1.005}, 0.381, 0.160},
+     {128, 256, 1, 2, 3.501, 1.251, {1.049, 1.706}, 0.240, 0.150}},
+    // bfloat16 outputs by expert
+    {{16, 16, 8, 2, 4.761, 0.359, {0.334, 1.006}, 31.116, 0.066},
+     {16, 32, 4, 4, 4.101, 0.000, {0.572, 0.893, 1.395, 1.797}, 9.507, 0.068},
+     {16, 64, 4, 4, 3.539, 0.000, {1.028, 1.887, 2.402, 2.838}, 10.820, 0.086},
+     {32, 64, 4, 3, 4.257, 0.000, {0.548, 1.371, 1.921}, 2.891, 0.138},
+     {64, 64, 4, 2, 5.214, 0.000, {0.645, 1.406}, 3.692, 0.139},
+     {64, 128, 2, 2, 4.246, 0.000, {0.560, 1.346}, 1.068, 0.155},
+     {64, 256, 2, 1, 4.125, 0.000, {0.898}, 2.742, 0.162},
+     {64, 256, 1, 2, 2.893, 0.000, {0.697, 1.118}, 0.775, 0.154},
+     {128, 256, 1, 2, 4.436, 0.000, {1.007, 1.513}, 0.833, 0.139}}};
 constexpr int kFirstTile = 3; // those from here on address rows by 32-bit offsets
 constexpr int64_t kCUs = 256;
 
 double fp8_time(const Fp8Kernel &t, int64_t wgs, int64_t groups, double outputs, double weights)
 {
     const int64_t per = cdiv(wgs, kCUs), full = per / t.resident, rem = per % t.resident;
-    return t.launch + t.round * (double)(full + (rem ? 1 : 0)) +
-           (double)cdiv(groups, t.kg) * ((double)full * t.step[t.resident - 1] + (rem ? t.step[rem - 1] : 0.0)) +
-           1e-6 * (t.outputs * outputs + t.weights * weights);
+    const double work = t.round * (double)(full + (rem ? 1 : 0)) + 1e-6 * t.outputs * outputs +
+                        (double)cdiv(groups, t.kg) * ((double)full * t.step[t.resident - 1] + (rem ? t.step[rem - 1] : 0.0));
+    return t.launch + std::hypot(work, 1e-6 * t.weights * weights);
 }
 
-// The kernel of a product and its grid. How the rows fall to the experts is not known here: the tiles that they take
-// are counted for rows that fall to them at random, and the grid holds the most that they can take.
-int fp8_plan(const Fp8Args &a, bool bf16, int64_t *wgs)
+// The order in which workgroups of `tokens` tokens, `tiles` x `columns` of them, go to the XCDs, and their number.
+int64_t order_tiles(Fp8Args *a, int tokens, int64_t tiles, int64_t columns, double rows_of_expert)
 {
-    const ExpertRows &er = a.er;
-    const bool far = a.ldxv * (er.rows ? er.m : 128) + a.k >= ((int64_t)1 << 32) ||
-                     4 * (a.ldxs * (er.rows ? er.m : 128) + a.gsxs * a.groups) >= ((int64_t)1 << 32);
+    const int64_t total = tiles * columns;
+    const bool grouped = a->er.offsets && a->er.experts > 1, reused = rows_of_expert > tokens;
+    int64_t group = columns, deal = 1; // row tile by row tile, to the XCDs in turn
+    if (!grouped) {
+        // An eighth of all to each XCD, so that the row tiles that read a weight do it in one L2: 256 x 2880 x 5120 16.5 ->
+        // 12.3 us, 768 x 7000 x 6144 81 -> 49, the more the less the columns are a multiple of eight by themselves. Of many
+        // row tiles a few columns at a time, which share the rows (8192 x 14336 x 4096 468 -> 444).
+        group = tiles >= 8 ? 4 : 1;
+        deal = cdiv(total, 8);
+    } else if (reused && total >= 768) {
+        // 32 neighbours at a time, for which row tiles there are is not known: an eighth at a time, the last XCD would have
+        // the tiles of no rows (65536 rows of 64 experts, 2048 x 4096: 601 us in turn, 553; 8192 of 32, 600 x 5120: 89, 62)
+        group = 8;
+        deal = 32;
+    } else if (reused && columns >= 8 && columns % 8) {
+        group = 1; // every XCD has columns of its own
+        deal = cdiv(total, 8);
+    }
+    a->tiles = (uint32_t)tiles;
+    a->group = (uint32_t)std::min(group, columns);
+    a->deal = (uint32_t)deal;
+    return cdiv(total, 8 * deal) * 8 * deal;
+}
+
+// The kernel of a product, the order of its workgroups and their number. How the rows fall to the experts is not known here:
+// the tiles that they take are counted for rows that fall to them at random, and the grid holds the most that they can take.
+int fp8_plan(Fp8Args *a, bool bf16, int64_t *wgs)
+{
+    const ExpertRows &er = a->er;
+    const bool far = a->ldxv * (er.rows ? er.m : 128) + a->k >= ((int64_t)1 << 32) ||
+                     4 * (a->ldxs * (er.rows ? er.m : 128) + a->gsxs * a->groups) >= ((int64_t)1 << 32);
     const bool grouped = er.offsets && er.experts > 1; // one expert's rows take the kernel that they would take without
     const double r = (double)er.r, taken = grouped ? er.experts * -std::expm1(-r / er.experts) : 1.0;
     int best = -1;
     double least = 0.0;
     for (int i = 0; i < (far ? kFirstTile : 9); ++i) {
-        const Fp8Kernel &t = kFp8Kernels[bf16][i];
+        const Fp8Kernel &t = kFp8Kernels[bf16 ? grouped ? 2 : 1 : 0][i];
         if (!t.tokens)
             continue;
-        const int64_t columns = cdiv(a.n, t.rows), most = er.offsets ? expert_row_tiles(er.r, er.experts, t.tokens) : cdiv(er.r, t.tokens);
-        if (most * columns > 0x7FFFFFFF)
+        const int64_t columns = cdiv(a->n, t.rows), most = er.offsets ? expert_row_tiles(er.r, er.experts, t.tokens) : cdiv(er.r, t.tokens);
+        if (most * columns > 0x3FFFFFFF) // with the order's rest, and the sums in place()
             continue;
         const double tiles = grouped ? std::fmax(taken, r / t.tokens + 0.5 * taken) : (double)cdiv(er.r, t.tokens);
-        const double us = fp8_time(t, (int64_t)std::ceil(tiles) * columns, a.groups, r * a.n, taken * a.n * a.k);
+        const double us = fp8_time(t, (int64_t)std::ceil(tiles) * columns, a->groups, r * a->n, taken * a->n * a->k);
         if (best < 0 || us < least) {
             best = i;
             least = us;
-            *wgs = most * columns;
+            *wgs = order_tiles(a, t.tokens, most, columns, r / taken);
         }
     }
     return best;
@@ -668,7 +728,7 @@ int launch_products(const Fp8Args &a, int which, int64_t wgs, hipStream_t stream
         MAMBO_STREAM(0, 1, 8);
         MAMBO_STREAM(1, 2, 4);
         MAMBO_STREAM(2, 4, 4);
-        MAMBO_TILE(3, 1, 1, 2, 8);
+        MAMBO_TILE(3, 1, 1, 2, 4);
         MAMBO_TILE(4, 2, 1, 2, 4);
         MAMBO_TILE(5, 2, 1, 4, 2);
         MAMBO_TILE(6, 2, 2, 4, 2);
@@ -712,10 +772,10 @@ int run_products(const uint8_t *xv, int64_t ldxv, const float *xs, int64_t ldxs,
                       (uintptr_t)out % (out_dtype == MAMBO_DTYPE_BF16 ? 2 : 4) == 0,
                   MAMBO_ERR_VALUE, "scales and outputs must be aligned to their type");
     Fp8Args a = {xv, xs, ldxv, ldxs, gsxs, er, packed, ws, out, ldo, (int)n, (int)k, (int)cdiv(k, kGroup), (int)cdiv(n, kTileN),
-                 rows_take_vectors(out, ldo, out_dtype)};
+                 rows_take_vectors(out, ldo, out_dtype), 0, 0, 0};
     const bool bf16 = out_dtype == MAMBO_DTYPE_BF16;
     int64_t wgs = 0;
-    const int which = fp8_plan(a, bf16, &wgs);
+    const int which = fp8_plan(&a, bf16, &wgs);
     MAMBO_REQUIRE(which >= 0, MAMBO_ERR_VALUE, "too many rows and columns for one launch");
     if (er.offsets)
         return bf16 ? launch_products<true, true>(a, which, wgs, stream) : launch_products<true, false>(a, which, wgs, stream);
@@ -795,7 +855,7 @@ extern "C" int mambo_fp8_block_matmul(const uint8_t *xv, int64_t ldxv, const flo
 }
 
 extern "C" int mambo_fp8_block_plan(int64_t m, int64_t r, int64_t experts, int64_t n, int64_t k, int64_t ldxv,
-                                    int out_dtype, int32_t *tile)
+                                    int out_dtype, int32_t *plan)
 {
     static const int32_t one = 0; // never read: that the plan is of rows by expert, or gathered
     const int32_t *rows = experts && m != r ? &one : nullptr, *offsets = experts ? &one : nullptr;
@@ -804,16 +864,17 @@ extern "C" int mambo_fp8_block_plan(int64_t m, int64_t r, int64_t experts, int64
         rc = check_expert_rows(m, rows, experts ? r : m, experts ? offsets : &one, experts ? experts : 1);
     if (rc != MAMBO_OK)
         return rc;
-    MAMBO_REQUIRE(ldxv >= k && tile && (experts ? r : m) >= 1, MAMBO_ERR_VALUE, "a plan is of one row or more");
+    MAMBO_REQUIRE(ldxv >= k && plan && (experts ? r : m) >= 1, MAMBO_ERR_VALUE, "a plan is of one row or more");
     Fp8Args a = {};
     a.er = {offsets, rows, experts ? r : m, m, (int)(experts ? experts : 1)};
     a.ldxv = ldxv, a.ldxs = 1, a.gsxs = m;
     a.n = (int)n, a.k = (int)k, a.groups = (int)cdiv(k, kGroup);
     int64_t wgs = 0;
-    const int which = fp8_plan(a, out_dtype == MAMBO_DTYPE_BF16, &wgs);
+    const int which = fp8_plan(&a, out_dtype == MAMBO_DTYPE_BF16, &wgs);
     MAMBO_REQUIRE(which >= 0, MAMBO_ERR_VALUE, "too many rows and columns for one launch");
-    const Fp8Kernel &t = kFp8Kernels[out_dtype == MAMBO_DTYPE_BF16][which];
-    tile[0] = t.tokens, tile[1] = t.rows, tile[2] = t.kg;
+    const Fp8Kernel &t = kFp8Kernels[out_dtype == MAMBO_DTYPE_BF16][which]; // the sizes are the same by expert
+    plan[0] = t.tokens, plan[1] = t.rows, plan[2] = t.kg;
+    plan[3] = (int32_t)a.group, plan[4] = (int32_t)a.deal;
     return MAMBO_OK;
 }
 

@@ -357,7 +357,7 @@ const std::vector<EntryDecl> &compiled_entries()
                     "out_dtype", "ldo", "stream"),
         MAMBO_ENTRY(mambo_fp8_block_matmul_experts, "xv", "ldxv", "xs", "ldxs", "gsxs", "m", "rows", "r", "offsets", "experts",
                     "packed", "ws", "n", "k", "out", "out_dtype", "ldo", "stream"),
-        MAMBO_ENTRY(mambo_fp8_block_plan, "m", "r", "experts", "n", "k", "ldxv", "out_dtype", "tile"),
+        MAMBO_ENTRY(mambo_fp8_block_plan, "m", "r", "experts", "n", "k", "ldxv", "out_dtype", "plan"),
         MAMBO_ENTRY(mambo_iq3s_fp8_matmul_experts, "xv", "ldxv", "xs", "ldxs", "m", "rows", "r", "offsets", "experts",
                     "packed", "expert_stride", "n", "blocks", "out", "out_dtype", "ldo", "stream"),
         MAMBO_ENTRY(mambo_route_experts, "logits", "dtype", "ld", "m", "experts", "top_k", "renormalize", "ids",

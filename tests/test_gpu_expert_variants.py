@@ -14,54 +14,58 @@ from conftest import make_synthetic_iq3_s
 
 F32, BF16 = torch.float32, torch.bfloat16
 
-# (dtype, tokens, experts (0: dense), N, K, the workgroup that takes it: tokens, weight rows, parts of K)
+# (dtype, tokens, experts (0: dense), N, K)
 VARIANTS = [
-    (F32, 1, 0, 33, 4112, (16, 16, 8)), (F32, 1500, 0, 33, 2064, (16, 32, 4)), (F32, 2050, 0, 33, 2064, (16, 64, 4)),
-    (F32, 2050, 0, 33, 4112, (32, 64, 8)), (F32, 3001, 0, 130, 2064, (64, 64, 4)),
-    (F32, 67, 0, 8200, 1040, (64, 128, 2)), (F32, 203, 0, 8200, 528, (64, 256, 1)),
-    (F32, 203, 0, 8200, 1040, (64, 256, 2)),
-    (F32, 1, 2, 33, 4112, (16, 16, 8)), (F32, 1500, 2, 33, 2064, (16, 32, 4)), (F32, 2050, 2, 33, 2064, (16, 64, 4)),
-    (F32, 2050, 2, 33, 4112, (32, 64, 8)), (F32, 3001, 2, 130, 2064, (64, 64, 4)),
-    (F32, 33, 2, 8200, 1040, (64, 128, 2)), (F32, 67, 4, 8200, 528, (64, 256, 1)),
-    (F32, 67, 4, 8200, 1040, (64, 256, 2)),
-    (BF16, 1, 0, 33, 4112, (16, 16, 8)), (BF16, 1500, 0, 33, 2064, (16, 32, 4)),
-    (BF16, 2050, 0, 33, 2064, (16, 64, 4)), (BF16, 2050, 0, 33, 4112, (32, 64, 8)),
-    (BF16, 17, 0, 8200, 2064, (64, 64, 4)), (BF16, 1030, 0, 650, 1040, (64, 128, 2)),
-    (BF16, 203, 0, 8200, 528, (64, 256, 1)), (BF16, 203, 0, 8200, 1552, (64, 256, 2)),
-    (BF16, 523, 0, 15000, 528, (128, 256, 1)),
-    (BF16, 1, 2, 33, 4112, (16, 16, 8)), (BF16, 1500, 2, 33, 2064, (16, 32, 4)),
-    (BF16, 2050, 2, 33, 2064, (16, 64, 4)), (BF16, 2050, 2, 33, 4112, (32, 64, 8)),
-    (BF16, 1500, 40, 130, 2064, (64, 64, 4)), (BF16, 5, 2, 8200, 1040, (64, 128, 2)),
-    (BF16, 17, 4, 8200, 528, (64, 256, 1)), (BF16, 131, 2, 8200, 1040, (64, 256, 2)),
-    (BF16, 131, 4, 15000, 1040, (128, 256, 1)),
+    (F32, 1, 0, 33, 4112), (F32, 1500, 0, 33, 2064), (F32, 2050, 0, 33, 2064), (F32, 2050, 0, 33, 4112),
+    (F32, 3001, 0, 130, 2064), (F32, 67, 0, 8200, 1040), (F32, 203, 0, 8200, 528), (F32, 203, 0, 8200, 1040),
+    (F32, 1, 2, 33, 4112), (F32, 1500, 2, 33, 2064), (F32, 2050, 2, 33, 2064), (F32, 2050, 2, 33, 4112),
+    (F32, 3001, 2, 130, 2064), (F32, 33, 2, 8200, 1040), (F32, 67, 4, 8200, 528), (F32, 67, 4, 8200, 1040),
+    (BF16, 1, 0, 33, 4112), (BF16, 1500, 0, 33, 2064), (BF16, 2050, 0, 33, 2064), (BF16, 2050, 0, 33, 4112),
+    (BF16, 17, 0, 8200, 2064), (BF16, 1030, 0, 650, 1040), (BF16, 203, 0, 8200, 528),
+    (BF16, 203, 0, 8200, 1552), (BF16, 523, 0, 15000, 528), (BF16, 1, 2, 33, 4112), (BF16, 1500, 2, 33, 2064),
+    (BF16, 2050, 2, 33, 2064), (BF16, 2050, 2, 33, 4112), (BF16, 1500, 40, 130, 2064), (BF16, 5, 2, 8200, 1040),
+    (BF16, 17, 4, 8200, 528), (BF16, 131, 2, 8200, 1040), (BF16, 131, 4, 15000, 1040), (F32, 1, 0, 8200, 2064),
+    (F32, 1500, 0, 650, 1040), (F32, 3001, 0, 650, 1552), (F32, 523, 40, 130, 2064), (F32, 131, 2, 8200, 528),
+    (F32, 67, 2, 8200, 1040), (F32, 17, 4, 15000, 1040), (BF16, 1, 0, 8200, 2064), (BF16, 1030, 0, 33, 2064),
+    (BF16, 3001, 0, 130, 2064), (BF16, 67, 0, 8200, 1040), (BF16, 203, 0, 8200, 2064),
+    (BF16, 1030, 0, 8200, 528), (BF16, 17, 4, 1100, 2064), (BF16, 96, 40, 1100, 2064),
+    (BF16, 1030, 2, 33, 2064), (BF16, 1030, 40, 300, 2064), (BF16, 5, 2, 15000, 528), (BF16, 17, 4, 8200, 1552),
+    (BF16, 401, 4, 15000, 656), (BF16, 6000, 2, 4100, 272), (BF16, 801, 2, 1100, 2064),
+    (F32, 801, 2, 1100, 2064), (F32, 8200, 2, 1300, 272),
 ]
-IDS = [f"{str(d)[6:]}-{m}x{e}x{n}x{k}" for d, m, e, n, k, _ in VARIANTS]
+IDS = [f"{str(d)[6:]}-{m}x{e}x{n}x{k}" for d, m, e, n, k in VARIANTS]
 
 
 def plan(m, r, experts, n, k, dtype, ldxv=None):
     from mambo_amd import _native
-    tile = (ctypes.c_int32 * 3)()
+    out = (ctypes.c_int32 * 5)()
     _native.check(_native.lib().mambo_fp8_block_plan(m, r, experts, n, k, ldxv or k,
-                                                     _native.DTYPE_BF16 if dtype == BF16 else _native.DTYPE_F32, tile))
-    return tuple(tile)
+                                                     _native.DTYPE_BF16 if dtype == BF16 else _native.DTYPE_F32, out))
+    return tuple(out)
 
 
 def test_each_kernel_is_tested():
-    for dtype, m, experts, n, k, tile in VARIANTS:
-        assert plan(m, m, experts, n, k, dtype) == tile, (m, experts, n, k)
+    """Every kernel of a dtype, dense and by expert, and every order of the workgroups: in turn, an eighth
+    to each XCD (one column at a time, or four), 32 at a time."""
     for dtype, kernels in ((F32, 8), (BF16, 9)):
         for grouped in (False, True):
-            assert len({v[5] for v in VARIANTS if v[0] == dtype and (v[2] > 0) == grouped}) == kernels
+            plans = {plan(m, m, e, n, k, d) for d, m, e, n, k in VARIANTS if d == dtype and (e > 0) == grouped}
+            assert len({p[:3] for p in plans}) == kernels, (dtype, grouped)
+            assert any(p[4] not in (1, 32) and p[3] == 1 for p in plans)
+            if grouped:
+                assert {1, 32} <= {p[4] for p in plans}
+            else:
+                assert any(p[3] == 4 for p in plans)
 
 
 def test_far_rows_take_the_streaming_kernels():
     for m, experts, ld in ((3, 0, 1 << 25), (300, 0, 1 << 25), (1 << 20, 4, 4096), (600, 4, 1 << 25)):
-        assert plan(m, 500 if experts else m, experts, 8200, 1040, BF16, ld) in ((16, 16, 8), (16, 32, 4), (16, 64, 4))
+        assert plan(m, 500 if experts else m, experts, 8200, 1040, BF16, ld)[:3] in ((16, 16, 8), (16, 32, 4), (16, 64, 4))
 
 
 def test_plan_refuses_what_the_call_refuses():
     from mambo_amd import _native
-    lib, tile = _native.lib(), (ctypes.c_int32 * 3)()
+    lib, tile = _native.lib(), (ctypes.c_int32 * 5)()
     good = dict(m=5, r=5, experts=2, n=64, k=128, ldxv=128, out_dtype=_native.DTYPE_F32)
     assert lib.mambo_fp8_block_plan(*good.values(), tile) == 0
     for bad in (dict(k=120), dict(n=0), dict(out_dtype=7), dict(experts=1025), dict(experts=-1), dict(r=0), dict(r=-1),
@@ -89,8 +93,8 @@ def grouped(xv, xs, wv, ws, offsets):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("dtype,m,experts,n,k,tile", VARIANTS, ids=IDS)
-def test_integers_add_up_exactly(gpu, dtype, m, experts, n, k, tile):
+@pytest.mark.parametrize("dtype,m,experts,n,k", VARIANTS, ids=IDS)
+def test_integers_add_up_exactly(gpu, dtype, m, experts, n, k):
     """Codes of small integers and scales of powers of two: every order of the sum gives the same
     float32. Scales group by group and row by row give the same."""
     from mambo_amd.kernels.experts import launch_fp8_block_matmul_experts
@@ -128,8 +132,8 @@ def test_integers_add_up_exactly(gpu, dtype, m, experts, n, k, tile):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("dtype,m,experts,n,k,tile", [v for v in VARIANTS if v[0] == F32 and not v[2]])
-def test_real_values_within_the_bound_of_float32_sums(gpu, dtype, m, experts, n, k, tile):
+@pytest.mark.parametrize("dtype,m,experts,n,k", [v for v in VARIANTS if v[0] == F32 and not v[2]])
+def test_real_values_within_the_bound_of_float32_sums(gpu, dtype, m, experts, n, k):
     from mambo_amd.kernels.fp8_block import launch_fp8_block_matmul
     from mambo_amd.utils.fp8_block_weight import prepare_fp8_block_weight
     gen = torch.Generator(device=gpu).manual_seed(m + n + k)
