@@ -178,11 +178,12 @@ def check(rc: int, what: str = "") -> None:
     raise RuntimeError(text)
 
 
-def stream_handle(stream) -> int:
-    """HIP stream handle of `stream` (None = torch's current stream on the current device)."""
+def stream_handle(stream, device=None) -> int:
+    """HIP stream handle of `stream` (None = torch's current stream on the current device, which a
+    caller that has it names)."""
     if stream is None:
         import torch
-        return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device())
+        return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device() if device is None else device.index)
     if isinstance(stream, int):
         return stream
     handle = getattr(stream, "cuda_stream", None)

@@ -68,7 +68,7 @@ def launch_route_experts(logits: torch.Tensor, top_k: int, *, renormalize: bool 
         _native.check(_native.lib().mambo_route_experts(
             logits.data_ptr(), ROW_DTYPES[logits.dtype], row_stride(logits), m, experts, top_k, bool(renormalize),
             ids.data_ptr(), weights.data_ptr(), offsets.data_ptr(), rows.data_ptr(), slots.data_ptr(),
-            _native.stream_handle(stream)), "launch_route_experts")
+            _native.stream_handle(stream, dev)), "launch_route_experts")
     return ExpertPlan(ids, weights, offsets, rows, slots)
 
 
@@ -108,7 +108,7 @@ def launch_fp8_block_matmul_experts(x_values: torch.Tensor, x_scales: torch.Tens
             x_values.data_ptr(), row_stride(x_values), x_scales.data_ptr(), *scale_strides(x_scales), m,
             None if rows is None else rows.data_ptr(), r, offsets.data_ptr(), weight.experts, weight.packed.data_ptr(),
             weight.scales.data_ptr(), weight.n, weight.k, out.data_ptr(), ROW_DTYPES[out_dtype], row_stride(out),
-            _native.stream_handle(stream)), "launch_fp8_block_matmul_experts")
+            _native.stream_handle(stream, dev)), "launch_fp8_block_matmul_experts")
     return out
 
 
@@ -139,7 +139,7 @@ def launch_iq3_s_fp8_matmul_experts(x_values: torch.Tensor, x_scales: torch.Tens
             x_values.data_ptr(), row_stride(x_values), x_scales.data_ptr(), row_stride(x_scales), m,
             None if rows is None else rows.data_ptr(), r, offsets.data_ptr(), weight.experts, weight.packed.data_ptr(),
             weight.packed.stride(0), weight.n, weight.blocks, out.data_ptr(), ROW_DTYPES[out_dtype], row_stride(out),
-            _native.stream_handle(stream)), "launch_iq3_s_fp8_matmul_experts")
+            _native.stream_handle(stream, dev)), "launch_iq3_s_fp8_matmul_experts")
     return out
 
 
@@ -171,5 +171,5 @@ def launch_combine_experts(y: torch.Tensor, slots: torch.Tensor, weights: torch.
         _native.check(_native.lib().mambo_combine_experts(
             y.data_ptr(), ROW_DTYPES[y.dtype], row_stride(y), y.shape[0], slots.data_ptr(), weights.data_ptr(), m,
             top_k, y.shape[1], out.data_ptr(), ROW_DTYPES[out_dtype], row_stride(out),
-            _native.stream_handle(stream)), "launch_combine_experts")
+            _native.stream_handle(stream, dev)), "launch_combine_experts")
     return out

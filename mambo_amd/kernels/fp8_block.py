@@ -39,7 +39,7 @@ def launch_quantize_fp8_block(x: torch.Tensor, *, stream=None, out: tuple[torch.
         if out is None:
             values = torch.empty((m, k), dtype=torch.uint8, device=dev)
             # a group's scales next to each other: the products copy those of 64 rows in one piece
-            scales = torch.empty((groups, m), dtype=torch.float32, device=dev).t()
+            scales = torch.empty_strided((m, groups), (1, m), dtype=torch.float32, device=dev)
             ldv, (lds, gss) = k, (1, m)
         else:
             values, scales = out
@@ -51,7 +51,7 @@ def launch_quantize_fp8_block(x: torch.Tensor, *, stream=None, out: tuple[torch.
             ldv, (lds, gss) = row_stride(values), scale_strides(scales)
         _native.check(_native.lib().mambo_quantize_fp8_block(
             x.data_ptr(), ROW_DTYPES[x.dtype], m, k, row_stride(x), values.data_ptr(), ldv, scales.data_ptr(), lds, gss,
-            _native.stream_handle(stream)), "launch_quantize_fp8_block")
+            _native.stream_handle(stream, dev)), "launch_quantize_fp8_block")
     return values, scales
 
 
@@ -95,7 +95,7 @@ def block_activations(x_values, x_scales, k: int, dev) -> tuple[torch.Tensor, to
         raise ValueError("x_scales must be float32 [M,ceil(K/128)]")
     if x_values.device != dev or x_scales.device != dev:
         raise ValueError("x_values and x_scales must be on the weight's device")
-    if not plain_rows(x_scales) and not plain_rows(x_scales.t()):
+    if x_scales.stride() != (1, m) and not plain_rows(x_scales) and not plain_rows(x_scales.t()):
         x_scales = x_scales.contiguous()
     return rows_in_place(x_values, 16), x_scales, m
 
@@ -132,5 +132,5 @@ def launch_fp8_block_matmul(x_values: torch.Tensor, x_scales: torch.Tensor, weig
         _native.check(_native.lib().mambo_fp8_block_matmul(
             x_values.data_ptr(), row_stride(x_values), x_scales.data_ptr(), *scale_strides(x_scales), m, packed.data_ptr(),
             weight.scales.data_ptr(), n, k, out.data_ptr(), ROW_DTYPES[out_dtype], row_stride(out),
-            _native.stream_handle(stream)), "launch_fp8_block_matmul")
+            _native.stream_handle(stream, dev)), "launch_fp8_block_matmul")
     return out
