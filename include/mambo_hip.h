@@ -312,7 +312,7 @@ int mambo_fp8_block_pack(const uint8_t *w, int64_t experts, int64_t n, int64_t k
  * shape fixes (bf16 outputs by the FP8 MFMAs, f32 ones by the bf16 MFMAs, which add more exactly at half
  * the rate). xv u8 [m, ldxv] E4M3, 16-byte aligned rows; xs f32, row i's of group g at xs + i * ldxs + g *
  * gsxs (rows or groups apart); packed from mambo_fp8_block_pack with one expert; ws f32 [ceil(n/128),
- * ceil(k/128)] contiguous; k % 16 == 0. m == 0: nothing to do. */
+ * ceil(k/128)] contiguous; k % 16 == 0, k <= 2^26. m == 0: nothing to do. */
 int mambo_fp8_block_matmul(const uint8_t *xv, int64_t ldxv, const float *xs, int64_t ldxs, int64_t gsxs,
                            int64_t m, const uint8_t *packed, const float *ws, int64_t n, int64_t k, void *out,
                            int out_dtype, int64_t ldo, mambo_stream_t stream);

@@ -23,7 +23,7 @@ def refused(lib, rc, text):
 def test_packed_bytes(lib):
     assert lib.mambo_fp8_block_packed_bytes(1, 32, 128) == 4096
     assert lib.mambo_fp8_block_packed_bytes(3, 33, 144) == 3 * 2 * 2 * 4096
-    for bad in ((0, 32, 128), (1, 0, 128), (1, 32, 0), (1025, 32, 128), (1, 2**31, 16), (-1, 32, 128)):
+    for bad in ((0, 32, 128), (1, 0, 128), (1, 32, 0), (1025, 32, 128), (1, 32, 2**26 + 16), (1, 2**31, 16), (-1, 32, 128)):
         assert lib.mambo_fp8_block_packed_bytes(*bad) == 0
 
 
@@ -43,6 +43,7 @@ def test_pack_refusals(lib):
     f = lib.mambo_fp8_block_pack
     refused(lib, f(16, 1, 8, 24, 192, 24, 16, None), "multiple of 16")
     refused(lib, f(16, 1025, 8, 32, 256, 32, 16, None), "E in [1, 1024]")
+    refused(lib, f(16, 1, 8, 2**26 + 16, 8 * (2**26 + 16), 2**26 + 16, 16, None), "up to 2^26")
     refused(lib, f(None, 1, 8, 32, 256, 32, 16, None), "null pointer")
     refused(lib, f(16, 1, 8, 32, 256, 32, 8, None), "16-byte aligned")
 
@@ -59,7 +60,7 @@ def test_product_refusals(lib):
         return lib.mambo_fp8_block_matmul(*args)
 
     for change, text in (({"dtype": 2}, "float32 or bfloat16"), ({"m": -1}, "negative"), ({"k": 40, "ldxv": 48}, "multiple of 16"),
-                         ({"n": 0}, "multiple of 16"), ({"ldxv": 16}, "must cover"), ({"ldxs": 0}, "must cover"), ({"gsxs": 0}, "must cover"),
+                         ({"n": 0}, "multiple of 16"), ({"k": 2**26 + 16, "ldxv": 2**26 + 16}, "up to 2^26"), ({"ldxv": 16}, "must cover"), ({"ldxs": 0}, "must cover"), ({"gsxs": 0}, "must cover"),
                          ({"ldo": 7}, "must cover"), ({"xv": None}, "null pointer"), ({"out": None}, "null pointer"),
                          ({"xv": 8}, "16-byte aligned"), ({"ldxv": 40}, "16-byte aligned"), ({"packed": 24}, "16-byte aligned"),
                          ({"xs": 18}, "aligned to their type"), ({"out": 18}, "aligned to their type")):
