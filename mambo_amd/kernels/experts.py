@@ -16,7 +16,8 @@ from typing import NamedTuple
 import torch
 
 from mambo_amd import _native
-from mambo_amd.kernels.fp8_block import ROW_DTYPES, block_activations, plain_rows, product_output, row_stride, rows_in_place, scale_strides
+from mambo_amd.kernels.fp8_block import (ROW_DTYPES, block_activations, plain_rows, product_output, row_stride,
+                                         rows_in_place)
 from mambo_amd.utils.fp8_block_weight import Fp8BlockWeight
 from mambo_amd.utils.iq3_s_weight import IQ3SExperts, IQ3_S_BLOCK_VALUES
 
@@ -101,11 +102,11 @@ def launch_fp8_block_matmul_experts(x_values: torch.Tensor, x_scales: torch.Tens
         raise TypeError("prepare FP8 weights with prepare_fp8_block_weight before launch")
     dev = weight.packed.device
     with _native.launch_on(dev, stream):
-        x_values, x_scales, m = block_activations(x_values, x_scales, weight.k, dev)
+        x_values, x_scales, strides, m = block_activations(x_values, x_scales, weight.k, dev)
         r = _plan_tensors(offsets, rows, m, weight.experts, dev)
         out = product_output(out, r, weight.n, out_dtype, dev)
         _native.check(_native.lib().mambo_fp8_block_matmul_experts(
-            x_values.data_ptr(), row_stride(x_values), x_scales.data_ptr(), *scale_strides(x_scales), m,
+            x_values.data_ptr(), row_stride(x_values), x_scales.data_ptr(), *strides, m,
             None if rows is None else rows.data_ptr(), r, offsets.data_ptr(), weight.experts, weight.packed.data_ptr(),
             weight.scales.data_ptr(), weight.n, weight.k, out.data_ptr(), ROW_DTYPES[out_dtype], row_stride(out),
             _native.stream_handle(stream, dev)), "launch_fp8_block_matmul_experts")

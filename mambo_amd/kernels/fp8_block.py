@@ -83,9 +83,9 @@ def rows_in_place(t: torch.Tensor, align: int) -> torch.Tensor:
     return torch.empty(t.shape, dtype=t.dtype, device=t.device).copy_(t)
 
 
-def block_activations(x_values, x_scales, k: int, dev) -> tuple[torch.Tensor, torch.Tensor, int]:
+def block_activations(x_values, x_scales, k: int, dev) -> tuple[torch.Tensor, torch.Tensor, tuple[int, int], int]:
     """Validate E4M3 rows [M,K] and scales [M,ceil(K/128)] on `dev`; return them in a form that the
-    kernels read in place, and M."""
+    kernels read in place, the scales' strides, and M."""
     if not isinstance(x_values, torch.Tensor) or x_values.ndim != 2 or x_values.dtype != torch.uint8 \
             or x_values.shape[1] != k:
         raise ValueError(f"x_values must be uint8 [M,{k}]")
@@ -95,9 +95,12 @@ def block_activations(x_values, x_scales, k: int, dev) -> tuple[torch.Tensor, to
         raise ValueError("x_scales must be float32 [M,ceil(K/128)]")
     if x_values.device != dev or x_scales.device != dev:
         raise ValueError("x_values and x_scales must be on the weight's device")
-    if x_scales.stride() != (1, m) and not plain_rows(x_scales) and not plain_rows(x_scales.t()):
-        x_scales = x_scales.contiguous()
-    return rows_in_place(x_values, 16), x_scales, m
+    strides = x_scales.stride()
+    if strides != (1, m):  # as the quantizer lays them out
+        if not plain_rows(x_scales) and not plain_rows(x_scales.t()):
+            x_scales = x_scales.contiguous()
+        strides = scale_strides(x_scales)
+    return rows_in_place(x_values, 16), x_scales, strides, m
 
 
 def product_output(out, rows: int, n: int, dtype, dev) -> torch.Tensor:
@@ -127,10 +130,10 @@ def launch_fp8_block_matmul(x_values: torch.Tensor, x_scales: torch.Tensor, weig
     packed, n, k = weight.packed, weight.n, weight.k
     dev = packed.device
     with _native.launch_on(dev, stream):
-        x_values, x_scales, m = block_activations(x_values, x_scales, k, dev)
+        x_values, x_scales, strides, m = block_activations(x_values, x_scales, k, dev)
         out = product_output(out, m, n, out_dtype, dev)
         _native.check(_native.lib().mambo_fp8_block_matmul(
-            x_values.data_ptr(), row_stride(x_values), x_scales.data_ptr(), *scale_strides(x_scales), m, packed.data_ptr(),
+            x_values.data_ptr(), row_stride(x_values), x_scales.data_ptr(), *strides, m, packed.data_ptr(),
             weight.scales.data_ptr(), n, k, out.data_ptr(), ROW_DTYPES[out_dtype], row_stride(out),
             _native.stream_handle(stream, dev)), "launch_fp8_block_matmul")
     return out

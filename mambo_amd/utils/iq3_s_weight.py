@@ -218,8 +218,10 @@ def prepare_iq3_s_experts(iq3_weights: torch.Tensor, *, stream=None) -> IQ3SExpe
     with _native.launch_on(dev, stream):
         packed = torch.empty((experts, packed_bytes(n, blocks)), dtype=torch.uint8, device=dev)
         se, sn, sb, sbyte = iq3_weights.stride()
-        for e in range(experts):
+        # weights of whole 16-row tiles whose rows follow each other are one tall weight: one launch for all
+        tall = n % 16 == 0 and se == n * sn
+        for e in range(1 if tall else experts):
             _native.check(_native.lib().mambo_iq3s_prepare(
-                iq3_weights.data_ptr() + e * se, n, blocks, sn, sb, sbyte, None, None, None, None, None,
+                iq3_weights.data_ptr() + e * se, n * experts if tall else n, blocks, sn, sb, sbyte, None, None, None, None, None,
                 packed.data_ptr() + e * packed.stride(0), _native.stream_handle(stream)), "prepare_iq3_s_experts")
     return IQ3SExperts(packed, experts, n, blocks)
