@@ -640,16 +640,18 @@ int mambo_wide_launch(const WidePlan &p, const uint8_t *xv, int64_t ldxv, const 
     return mambo_check_launch("iq3s_fp8_matmul (wide)");
 }
 
-// Rows grouped by expert: one round of the weights per tile of rows, K unsplit (no atomics), the shapes of one K group,
-// by the same times with the tiles that rows falling to the experts at random take (fp8_plan counts them alike).
+// Rows grouped by expert: one round of the weights per tile of rows, K unsplit (no atomics), by the same times with the
+// tiles that rows falling to the experts at random take (fp8_plan counts them alike), and several K groups while that is
+// one workgroup a CU (8 experts of 4096 x 14336, 16 rows each, 82 -> 67 us, 64 rows 115 -> 99; beyond, 64 rows of 64 experts,
+// 2048 x 4096, 110 -> 131).
 double mambo_wide_experts_plan(const ExpertRows &er, int64_t n, int64_t blocks, double tiles_of[2], WidePlan *plan)
 {
     const double mb = 4e-6 * (double)er.r * (double)n;
     double best = 0.0;
     for (const WideShape &w : kWideShapes) {
-        if (w.kg > 1)
-            continue;
         const int64_t wgs = cdiv(cdiv(n, 32), w.waves) * (int64_t)(tiles_of[w.mt == 4] + 0.5);
+        if (w.kg > 1 && wgs > kCUs)
+            continue;
         const double t = wide_time(w, wgs, blocks, 1, mb);
         if (best == 0.0 || t < best) {
             best = t;
@@ -659,15 +661,15 @@ double mambo_wide_experts_plan(const ExpertRows &er, int64_t n, int64_t blocks, 
     return best;
 }
 
-template <int MT, int W>
+template <int MT, int W, int KG>
 static void launch_wide_experts(dim3 grid, hipStream_t stream, const uint8_t *xv, int64_t ldxv, const uint8_t *xs, int64_t ldxs,
                                 const GroupArgs &ga, int blocks, bool bf16, const ExpertRows &er, int64_t expert_stride)
 {
     if (bf16)
-        MAMBO_LAUNCH((gemm_wide_kernel<MT, W, 1, 0, WideExperts<true>>), grid, dim3(W * 64), 0, stream, xv, ldxv, xs, ldxs,
+        MAMBO_LAUNCH((gemm_wide_kernel<MT, W, KG, 0, WideExperts<true>>), grid, dim3(W * KG * 64), 0, stream, xv, ldxv, xs, ldxs,
                      (int64_t)0, ga, blocks, blocks, 0, (WideExperts<true>{er, expert_stride}));
     else
-        MAMBO_LAUNCH((gemm_wide_kernel<MT, W, 1, 0, WideExperts<false>>), grid, dim3(W * 64), 0, stream, xv, ldxv, xs, ldxs,
+        MAMBO_LAUNCH((gemm_wide_kernel<MT, W, KG, 0, WideExperts<false>>), grid, dim3(W * KG * 64), 0, stream, xv, ldxv, xs, ldxs,
                      (int64_t)0, ga, blocks, blocks, 0, (WideExperts<false>{er, expert_stride}));
 }
 
@@ -682,11 +684,16 @@ int mambo_wide_experts_launch(const WidePlan &p, const uint8_t *xv, int64_t ldxv
     ga.n[0] = n;
     ga.ldo[0] = ldo;
     const dim3 grid((unsigned)cdiv(cdiv(n, 32), p.waves), (unsigned)expert_row_tiles(er.r, er.experts, 32 * p.mt));
-    if (p.mt == 2)
-        launch_wide_experts<2, 4>(grid, stream, xv, ldxv, xs, ldxs, ga, (int)blocks, bf16, er, expert_stride);
-    else if (p.waves == 4)
-        launch_wide_experts<4, 4>(grid, stream, xv, ldxv, xs, ldxs, ga, (int)blocks, bf16, er, expert_stride);
-    else
-        launch_wide_experts<4, 8>(grid, stream, xv, ldxv, xs, ldxs, ga, (int)blocks, bf16, er, expert_stride);
+    const auto is = [&](int mt, int waves, int kg) { return p.mt == mt && p.waves == waves && p.kg == kg; };
+#define MAMBO_WIDE_EXPERTS(MT, W, KG)                                                                              \
+    if (is(MT, W, KG))                                                                                             \
+    launch_wide_experts<MT, W, KG>(grid, stream, xv, ldxv, xs, ldxs, ga, (int)blocks, bf16, er, expert_stride)
+    MAMBO_WIDE_EXPERTS(2, 2, 4);
+    MAMBO_WIDE_EXPERTS(2, 4, 1);
+    MAMBO_WIDE_EXPERTS(2, 4, 2);
+    MAMBO_WIDE_EXPERTS(4, 4, 1);
+    MAMBO_WIDE_EXPERTS(4, 4, 2);
+    MAMBO_WIDE_EXPERTS(4, 8, 1);
+#undef MAMBO_WIDE_EXPERTS
     return mambo_check_launch("iq3s_fp8_matmul_experts");
 }

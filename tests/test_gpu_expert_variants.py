@@ -253,7 +253,9 @@ def test_join_and_router_far_apart(gpu):
 @pytest.mark.parametrize("r,experts,n,k", [
     (3, 4, 70, 2304), (6, 4, 9000, 2304), (150, 120, 1000, 2304),  # 4 tokens a tile: four waves, two, one
     (20, 4, 70, 2304), (60, 6, 6000, 2304), (200, 20, 4000, 2048),  # 16 tokens a tile: four, two, one
-    (300, 4, 2211, 1024),  # the 32 x 32 MFMAs
+    (300, 4, 2211, 1024),  # the 32 x 32 MFMAs, 64 x 128 tiles
+    (130, 8, 4090, 2048), (500, 8, 4090, 2304),  # of two K groups: 64 tokens, 128
+    (900, 2, 1500, 1280), (1100, 64, 600, 768), (1300, 3, 3000, 1024),
 ])
 def test_iq3s_kernels(gpu, r, experts, n, k, gather):
     """As test_gpu_experts.test_iq3s_experts, at sizes that each of the kernels takes; an expert may have
