@@ -369,10 +369,12 @@ __device__ __forceinline__ int slot_of(int row) { return (row ^ ((row >> 3) & 3)
 // More rows: a workgroup computes 32 MT tokens x 32 NB WN weight rows with KG groups of WN waves, each group taking a KG-th
 // of K; a wave owns 32 NB weight rows and all the tokens. A K group's token rows are copied straight into LDS, double
 // buffered, their scales beside them; the weights go to registers as they lie. Within a wave the MFMAs of one 32 x 32 tile
-// and the f32 scalings of the one before alternate, and the LDS reads of the next 32 tokens go between. Bound by the matrix
-// units where the launch fills the chip (128 x 256 tiles, 8192 x 14336 x 4096: 410 us, 2.35 PFLOP/s, 60 to 64% of the MFMA
-// cycles busy; a library product with one scale takes 325), else by a step's own chain of LDS reads, MFMAs, scalings and a
-// barrier, and by what a CU can fetch, about 33 GB/s (203 x 5003 x 2832 14 us; 64 x 4096 x 14336, on 128 CUs, 25).
+// and the f32 scalings of the one before alternate, and the LDS reads of the next 32 tokens go between; the next group's
+// weights are asked for as this one's last MFMAs have them, and a wave that multiplies goes before one that waits (2048 x 4096
+// x 14336 120.3 -> 118.1 us with both, 121.6 and 124.2 with either; 8192 x 14336 x 4096 417 -> 413). Bound by the matrix units
+// where the launch fills the chip (128 x 256 tiles, 8192 x 14336 x 4096: 413 us, 2.33 PFLOP/s, 60 to 64% of the MFMA cycles
+// busy; a library product with one scale takes 325), else by a step's own chain of LDS reads, MFMAs, scalings and a barrier,
+// and by what a CU can fetch, about 33 GB/s (203 x 5003 x 2832 12.6 us; 64 x 4096 x 14336, on 128 CUs, 25).
 template <int MT, int NB, int WN, int KG, bool kExperts, bool kBf16>
 __global__ __launch_bounds__(WN * KG * 64) __attribute__((amdgpu_waves_per_eu(2))) void fp8_tile_kernel(Fp8Args a)
 {
@@ -451,16 +453,15 @@ __global__ __launch_bounds__(WN * KG * 64) __attribute__((amdgpu_waves_per_eu(2)
         float wscale;
         uint32_t lane16 = 16 * lane;
         asm volatile("" : "+v"(lane16)); // or the compiler keeps a register for each of the four offsets below
-        auto load_w = [&](int g) {
+        auto load_w = [&](int nb, int g) {
             const int gc = min(g, G - 1);
 #pragma unroll
-            for (int nb = 0; nb < NB; ++nb)
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const auto v = __builtin_amdgcn_raw_buffer_load_b128(wp[nb], lane16 + 1024 * j, gc * kFp8Tile, 0);
-                    w[nb][j >> 1][j & 1] = uint4{v[0], v[1], v[2], v[3]};
-                }
-            wscale = KG == 1 || g < G ? ws[gc] : 0.0f;
+            for (int j = 0; j < 4; ++j) {
+                const auto v = __builtin_amdgcn_raw_buffer_load_b128(wp[nb], lane16 + 1024 * j, gc * kFp8Tile, 0);
+                w[nb][j >> 1][j & 1] = uint4{v[0], v[1], v[2], v[3]};
+            }
+            if (nb == NB - 1)
+                wscale = KG == 1 || g < G ? ws[gc] : 0.0f;
         };
         // chunk 4s + 2j + h of row r
         uint32_t slot[2][2];
@@ -468,7 +469,8 @@ __global__ __launch_bounds__(WN * KG * 64) __attribute__((amdgpu_waves_per_eu(2)
         for (int j = 0; j < 4; ++j)
             slot[j >> 1][j & 1] = kg * kRowBytes + 128u * col + 16u * ((2 * j + h) ^ slot_of(col));
 
-        auto multiply_group = [&](const uint8_t *rows, const float *scale) {
+        // the weights of group `next` are asked for as the last tiles are done with this group's
+        auto multiply_group = [&](const uint8_t *rows, const float *scale, int next) {
             v16f c[2];
             float f[2];
             uint4 x[2][2][2];
@@ -490,6 +492,10 @@ __global__ __launch_bounds__(WN * KG * 64) __attribute__((amdgpu_waves_per_eu(2)
                             acc[q / NB][q % NB][i] = __builtin_fmaf(c[q & 1][i], fq, acc[q / NB][q % NB][i]);
                     __builtin_amdgcn_sched_barrier(0);
                 };
+                if (p > MT * NB - NB) {
+                    load_w(p - (MT * NB - NB) - 1, next);
+                    __builtin_amdgcn_sched_barrier(0);
+                }
                 if (p < MT * NB) {
                     c[p & 1] = multiply<!kBf16>(w[nb][0], x[mt & 1][0], v16f{});
                     __builtin_amdgcn_sched_barrier(0);
@@ -509,7 +515,9 @@ __global__ __launch_bounds__(WN * KG * 64) __attribute__((amdgpu_waves_per_eu(2)
         constexpr int kVm = 0x0F70 | (4 * NB); // the copies are done, the weights behind them need not be
         stage(s_rows0, s_scale0, g0);
         __builtin_amdgcn_sched_barrier(0);
-        load_w(g0);
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb)
+            load_w(nb, g0);
         __builtin_amdgcn_sched_barrier(0);
         __builtin_amdgcn_s_waitcnt(kVm);
         __syncthreads();
@@ -517,10 +525,10 @@ __global__ __launch_bounds__(WN * KG * 64) __attribute__((amdgpu_waves_per_eu(2)
         for (int g = g0; g < end; g += 2) {
             stage(s_rows1, s_scale1, g + 1);
             __builtin_amdgcn_sched_barrier(0);
-            multiply_group(s_rows0, s_scale0);
+            __builtin_amdgcn_s_setprio(1);
+            multiply_group(s_rows0, s_scale0, g + 1);
             __builtin_amdgcn_sched_barrier(0);
-            load_w(g + 1);
-            __builtin_amdgcn_sched_barrier(0);
+            __builtin_amdgcn_s_setprio(0);
             __builtin_amdgcn_s_waitcnt(kVm);
             __syncthreads();
             __builtin_amdgcn_sched_barrier(0);
@@ -528,10 +536,10 @@ __global__ __launch_bounds__(WN * KG * 64) __attribute__((amdgpu_waves_per_eu(2)
                 break;
             stage(s_rows0, s_scale0, g + 2);
             __builtin_amdgcn_sched_barrier(0);
-            multiply_group(s_rows1, s_scale1);
+            __builtin_amdgcn_s_setprio(1);
+            multiply_group(s_rows1, s_scale1, g + 2);
             __builtin_amdgcn_sched_barrier(0);
-            load_w(g + 2);
-            __builtin_amdgcn_sched_barrier(0);
+            __builtin_amdgcn_s_setprio(0);
             __builtin_amdgcn_s_waitcnt(kVm);
             __syncthreads();
             __builtin_amdgcn_sched_barrier(0);
