@@ -94,3 +94,40 @@ def test_command(gpu, capsys):
                                   "--steps", "2", "--shared", "256", *extra]) == 0
         line = json.loads(capsys.readouterr().out)
         assert line["graph_equals_eager"] and line["graph_us"] > 0 and 0.01 < line["output_rms"] < 100
+
+
+def test_named_stream(gpu):
+    """Every operator on a stream that is not the current one, after work of that stream: what they
+    allocate and copy (strided rows, scales) belongs to it."""
+    from mambo_amd.kernels.experts import (launch_combine_experts, launch_fp8_block_matmul_experts,
+                                           launch_iq3_s_fp8_matmul_experts, launch_route_experts)
+    from mambo_amd.kernels.fp8_block import launch_quantize_fp8_block
+    from mambo_amd.kernels.quantize_fp8 import launch_quantize_fp8
+    from mambo_amd.utils.fp8_block_weight import prepare_fp8_block_weight
+    from mambo_amd.utils.iq3_s_weight import prepare_iq3_s_experts
+    rng = np.random.default_rng(21)
+    side = torch.cuda.Stream()
+    codes = torch.from_numpy(ref.random_codes(rng, (4, 512, 256))).to(gpu)
+    scales = torch.rand((4, 4, 2), device=gpu) * 1e-3
+    raws = torch.from_numpy(np.stack([make_synthetic_iq3_s(96, 512, seed=e) for e in range(4)])).to(gpu)
+
+    def layer(x, logits, stream):
+        with torch.cuda.stream(stream):  # the inputs are ready on the stream alone
+            x, logits = x * 2.0, logits * 2.0
+        s = None if stream == torch.cuda.current_stream() else stream
+        up, down = prepare_fp8_block_weight(codes, scales, stream=s), prepare_iq3_s_experts(raws, stream=s)
+        plan = launch_route_experts(logits, 2, stream=s)
+        values, row_scales = launch_quantize_fp8_block(x, stream=s)
+        h = launch_fp8_block_matmul_experts(values, row_scales, up, plan.offsets, rows=plan.rows, stream=s)
+        mx = launch_quantize_fp8(h, stream=s)
+        y = launch_iq3_s_fp8_matmul_experts(*mx, down, plan.offsets, stream=s)
+        return launch_combine_experts(y, plan.slots, plan.weights, stream=s)
+
+    for seed in range(3):
+        gen = torch.Generator(device=gpu).manual_seed(seed)
+        x, logits = torch.randn((90, 256), generator=gen, device=gpu), torch.randn((90, 4), generator=gen, device=gpu)
+        expected = layer(x, logits, torch.cuda.current_stream())
+        side.wait_stream(torch.cuda.current_stream())
+        out = layer(x, logits, side)
+        side.synchronize()
+        assert torch.equal(out, expected) and bool(out.any())
