@@ -666,7 +666,8 @@ double fp8_time(const Fp8Kernel &t, int64_t wgs, int64_t groups, double outputs,
 int64_t order_tiles(Fp8Args *a, int tokens, int64_t tiles, int64_t columns, double rows_of_expert)
 {
     const int64_t total = tiles * columns;
-    const bool grouped = a->er.offsets && a->er.experts > 1, reused = rows_of_expert > tokens;
+    const bool grouped = a->er.offsets && a->er.experts > 1;
+    const double reuse = rows_of_expert / tokens; // row tiles that read an expert's weight
     int64_t group = columns, deal = 1; // row tile by row tile, to the XCDs in turn
     if (!grouped) {
         // An eighth of all to each XCD, so that the row tiles that read a weight do it in one L2: 256 x 2880 x 5120 16.5 ->
@@ -674,12 +675,15 @@ int64_t order_tiles(Fp8Args *a, int tokens, int64_t tiles, int64_t columns, doub
         // row tiles a few columns at a time, which share the rows (8192 x 14336 x 4096 468 -> 444).
         group = tiles >= 8 ? 4 : 1;
         deal = cdiv(total, 8);
-    } else if (reused && total >= 768) {
+    } else if (total >= 768 && reuse >= (columns % 8 ? 2.0 / 3.0 : 4.0)) {
         // 32 neighbours at a time, for which row tiles there are is not known: an eighth at a time, the last XCD would have
-        // the tiles of no rows (65536 rows of 64 experts, 2048 x 4096: 601 us in turn, 553; 8192 of 32, 600 x 5120: 89, 62)
+        // the tiles of no rows. Where the columns are a multiple of eight, an XCD has columns of its own in turn too, and
+        // gains with many row tiles alone (65536 rows of 64 experts, 2048 x 4096 596 -> 569 us, 16384 188 -> 190, 4096 rows of
+        // 16, 4096 x 4096 74 -> 77); else 8192 of 32, 600 x 5120 89 -> 62, 16384 of 128, 1536 x 2048 129 -> 119, 12000 111 ->
+        // 100 (but 4096 of 32, 2880 x 2880 86 -> 97).
         group = 8;
         deal = 32;
-    } else if (reused && columns >= 8 && columns % 8) {
+    } else if (reuse > 1.0 && columns >= 8 && columns % 8) {
         group = 1; // every XCD has columns of its own
         deal = cdiv(total, 8);
     }
