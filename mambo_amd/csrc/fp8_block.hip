@@ -616,10 +616,11 @@ struct Fp8Kernel {
 };
 // Fitted to 355 products a dense table (1 to 8192 tokens, 300 to 57344 rows, K 272 to 28672, weights rotated past the caches)
 // and 174 by expert. The kernel that they pick takes 0.8% more than the fastest of the nine on average (f32 0.9%, by
-// expert, where they do not know how the rows fall, 3.3%). None of the nine is spare: without it the fastest of the others
-// takes 0.2 to 3% more on average and up to 1.11 to 1.63 times. Measured beside them: 128 x 128 tiles, 64 x 64 of eight K
-// groups, 64 x 128 and 64 x 64 of one and two (no gain of 0.5%); a second and a third buffer for the weights and the rows
-// (0 to 25% slower: a step is not bound by the latency of its loads).
+// expert, where they do not know how the rows fall, 3.3%; measured again, with 66 more by expert, 1.0%, 1.0% and 3.7%). None
+// of the nine is spare: without it the fastest of the others takes 0.2 to 3% more on average and up to 1.11 to 1.63 times.
+// Measured beside them: 128 x 128 tiles, 64 x 64 of eight K groups, 64 x 128 and 64 x 64 of one and two (no gain of 0.5%);
+// a second and a third buffer for the weights and the rows (0 to 25% slower: a step is not bound by the latency of its
+// loads).
 constexpr Fp8Kernel kFp8Kernels[3][9] = {
     // float32 outputs
     {{16, 16, 8, 2, 2.601, 0.338, {0.707, 1.432}, 9.221, 0.000},
