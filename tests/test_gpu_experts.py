@@ -136,6 +136,21 @@ def test_iq3s_experts(gpu, r, experts, unrouted, n, k, gather):
             assert np.linalg.norm(out[i] - expected[i]) <= tolerance * np.linalg.norm(expected[i]), i
 
 
+@pytest.mark.parametrize("n,k", [(32, 256), (33, 512), (16, 768), (130, 256)])
+def test_iq3s_experts_of_any_strides(gpu, n, k):
+    """Packed alike from contiguous weights, rows apart, experts apart, and one weight at a time."""
+    from mambo_amd.utils.iq3_s_weight import prepare_iq3_s_experts
+    raws = device(gpu, np.stack([make_synthetic_iq3_s(n, k, seed=50 + e) for e in range(5)]))[0]
+    expected = torch.cat([prepare_iq3_s_experts(raws[e:e + 1]).packed for e in range(5)])
+    apart = torch.zeros((5, n + 3, k // 256, 110), dtype=torch.uint8, device=gpu)
+    apart[:, :n] = raws
+    wide = torch.zeros((5, 2 * n, k // 256, 112), dtype=torch.uint8, device=gpu)
+    wide[:, ::2, :, 1:111] = raws
+    for source in (raws, apart[:, :n], wide[:, ::2, :, 1:111], raws.flip(0).flip(0), raws.transpose(0, 1).contiguous().transpose(0, 1)):
+        got = prepare_iq3_s_experts(source)
+        assert (got.experts, got.n, got.blocks) == (5, n, k // 256) and torch.equal(got.packed, expected)
+
+
 def test_experts_equal_the_projection(gpu):
     """One expert is the dense product (bit for bit where the rows take the same kernel)."""
     from mambo_amd.kernels.fp8_block import launch_fp8_block_matmul
