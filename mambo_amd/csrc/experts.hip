@@ -168,7 +168,7 @@ __global__ __launch_bounds__(kSortWaves * 64) void route_sort_kernel(const uint3
     auto load = [&](uint32_t(&id)[kSortLoads], int i, bool last) {
 #pragma unroll
         for (int j = 0; j < kSortLoads; ++j)
-            id[j] = !last || i + 64 * j + lane < hi ? ids[i + 64 * j + lane] : 0xFFFFFFFEu;
+            id[j] = !last || 64 * j + lane < hi - i ? ids[i + 64 * j + lane] : 0xFFFFFFFEu;
     };
     constexpr int kStep = 64 * kSortLoads;
     int less = 0, equal = 0;
@@ -182,7 +182,7 @@ __global__ __launch_bounds__(kSortWaves * 64) void route_sort_kernel(const uint3
         }
     };
     int i = lo;
-    for (; i + kStep <= hi; i += kStep)
+    for (; hi - i >= kStep; i += kStep) // (a sum would pass 2^31 in the last stretch of as many choices)
         tally(i, false);
     if (i < hi)
         tally(i, true);
@@ -219,7 +219,7 @@ __global__ __launch_bounds__(kSortWaves * 64) void route_sort_kernel(const uint3
             at += __popcll(here);
         }
     };
-    for (i = lo; i + kStep <= hi; i += kStep)
+    for (i = lo; hi - i >= kStep; i += kStep)
         place(i, false);
     if (i < hi)
         place(i, true);

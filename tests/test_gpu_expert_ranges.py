@@ -1,0 +1,93 @@
+"""The operators of a layer of experts over the ranges that they accept: long prompts, the last sizes
+before an index would not fit, and what lies beyond them."""
+
+from __future__ import annotations
+
+import numpy as np
+import pytest
+import torch
+
+import expert_reference as ref
+
+
+# ------------------------------------------------------------------------------ plain statements
+def chosen(logits: np.ndarray, top_k: int) -> np.ndarray:
+    """The ids of ref.route for many tokens: a stable sort of falling logits, -inf and NaN out."""
+    logits = np.where(np.isnan(logits), -np.inf, logits)
+    ids = np.argsort(-logits, axis=1, kind="stable")[:, :top_k].astype(np.int32)
+    return np.where(np.take_along_axis(logits, ids, 1) == -np.inf, np.int32(-1), ids)
+
+
+def plan_of(ids: np.ndarray, experts: int):
+    """ref.plan for many choices: a stable sort by expert, choices of none last."""
+    m, top_k = ids.shape
+    flat = np.where(ids < 0, experts, ids).ravel()
+    order = np.argsort(flat, kind="stable")
+    offsets = np.searchsorted(flat[order], np.arange(experts + 1)).astype(np.int32)
+    taken = flat[order] < experts
+    slots = np.empty(m * top_k, dtype=np.int32)
+    slots[order] = np.where(taken, np.arange(m * top_k), -1)
+    return offsets, np.where(taken, order // top_k, -1).astype(np.int32), slots.reshape(m, top_k)
+
+
+def some_logits(rng, m: int, experts: int, masked: float) -> np.ndarray:
+    """Logits on a coarse grid, so that many are equal, a share of them masked, some tokens wholly."""
+    logits = rng.integers(-6, 7, size=(m, experts)).astype(np.float32)
+    logits[rng.random((m, experts)) < masked] = -np.inf
+    if masked:
+        logits[rng.random(m) < 0.02] = -np.inf
+        logits[rng.random(m) < 0.02, 0] = np.nan
+    return logits
+
+
+def test_the_statements_for_many_choices_are_those_for_few():
+    rng = np.random.default_rng(0)
+    for m, experts, top_k, masked in ((7, 5, 2, 0.5), (40, 9, 9, 0.3), (1, 1, 1, 0.0), (30, 3, 1, 0.9)):
+        logits = some_logits(rng, m, experts, masked)
+        ids = chosen(logits, top_k)
+        assert np.array_equal(ids, ref.route(logits.astype(np.float64), top_k, True)[0])
+        for a, b in zip(plan_of(ids, experts), ref.plan(ids, experts)):
+            assert np.array_equal(a, b)
+
+
+# ------------------------------------------------------------------------------ router
+# more than 8192 choices, so that a wave's stretch of them passes the steps of 512 that no bound guards
+@pytest.mark.gpu
+@pytest.mark.parametrize("masked", [0.0, 0.4])
+@pytest.mark.parametrize("m,experts,top_k", [(2731, 9, 3), (8193, 2, 1), (4101, 64, 8), (8192, 256, 8), (1025, 70, 64),
+                                             (20011, 5, 5), (65537, 3, 1), (3001, 513, 10)])
+def test_route_of_many_choices(gpu, m, experts, top_k, masked):
+    from mambo_amd.kernels.experts import launch_route_experts
+    logits = some_logits(np.random.default_rng(m + experts), m, experts, masked)
+    ids = chosen(logits, top_k)
+    for dtype in (torch.float32, torch.bfloat16):  # the grid's values are the same in both
+        got = launch_route_experts(torch.from_numpy(logits).to(gpu).to(dtype), top_k)
+        assert np.array_equal(got.ids.cpu().numpy(), ids)
+        for name, expected in zip(("offsets", "rows", "slots"), plan_of(ids, experts)):
+            assert np.array_equal(getattr(got, name).cpu().numpy(), expected), name
+
+
+@pytest.mark.gpu
+def test_route_of_the_most_choices(gpu):
+    """2^31 - 64 choices: every token takes all of 64 experts, in an order of its own, so expert e has
+    the rows e m to (e + 1) m, a token each."""
+    from mambo_amd.kernels.experts import launch_route_experts
+    m, experts = 2**25 - 1, 64
+    logits = torch.empty((m, experts), dtype=torch.bfloat16, device=gpu)
+    expert = torch.arange(experts, dtype=torch.int32, device=gpu)
+    part = 1 << 20
+    tokens = [torch.arange(t, min(t + part, m), dtype=torch.int32, device=gpu) for t in range(0, m, part)]
+    for t in tokens:
+        logits[t[0]:t[0] + t.shape[0]] = ((expert[None] + t[:, None]) % experts).to(torch.bfloat16)
+    ids, weights, offsets, rows, slots = launch_route_experts(logits, experts)
+    assert offsets.tolist() == [e * m for e in range(experts + 1)]
+    rows = rows.view(experts, m)
+    for t in tokens:
+        at = slice(int(t[0]), int(t[0]) + t.shape[0])
+        # the j-th choice is the expert with the logit 63 - j
+        assert torch.equal(ids[at], (experts - 1 - expert[None] - t[:, None]) % experts)
+        assert torch.equal(slots[at], ids[at] * m + t[:, None])
+        assert bool((rows[:, at] == t[None]).all())
+        assert bool(((weights[at].sum(1) - 1.0).abs() < 64 * 2.0**-23).all())
+    del ids, weights, offsets, rows, slots, logits
+    torch.cuda.empty_cache()
