@@ -41,7 +41,7 @@ __device__ __forceinline__ bool find_row_tile(const ExpertRows &er, int tile, in
         int hi = e < er.experts ? er.offsets[min(e + 1, er.experts)] : r;
         lo = min(max(lo, 0), r);
         hi = min(max(hi, lo), r);
-        const int tiles = e <= er.experts ? (hi - lo + tile - 1) / tile : 0;
+        const int tiles = e <= er.experts ? (int)(((uint32_t)(hi - lo) + (uint32_t)tile - 1) / (uint32_t)tile) : 0;
         int incl = tiles;
 #pragma unroll
         for (int d = 1; d < 64; d <<= 1) {
@@ -71,6 +71,11 @@ __device__ __forceinline__ int64_t source_row(const ExpertRows &er, int64_t i)
     const int64_t s = er.rows[i];
     return s < 0 ? 0 : s >= er.m ? er.m - 1 : s;
 }
+
+// Threads of a grid's dimension that HIP launches, and whether `wgs` workgroups of `threads` are no more. (Of more it
+// launches what is left modulo 2^32, with no error: 3222784 workgroups of 20000000 x 256.)
+constexpr int64_t kMaxGridThreads = 0xFFFFFFFF;
+inline bool grid_takes(int64_t wgs, int64_t threads) { return wgs <= kMaxGridThreads / threads; }
 
 // Host checks that the grouped products share.
 inline int check_expert_rows(int64_t m, const int32_t *rows, int64_t r, const int32_t *offsets, int64_t experts)

@@ -433,7 +433,7 @@ extern "C" int mambo_combine_experts(const void *y, int y_dtype, int64_t ldy, in
                   "rows must be aligned to their type");
     const int threads = n <= (yb ? 512 : 256) ? 64 : 256;
     const int64_t columns = cdiv(n, (yb ? 8 : 4) * threads);
-    MAMBO_REQUIRE(columns <= 0x7FFFFFFF, MAMBO_ERR_VALUE, "rows too long");
+    MAMBO_REQUIRE(grid_takes(columns, threads), MAMBO_ERR_VALUE, "rows too long");
     const dim3 grid((unsigned)columns, (unsigned)(m < 65535 ? m : 65535));
     const bool in_vec = rows_take_vectors(y, ldy, y_dtype), out_vec = rows_take_vectors(out, ldo, out_dtype);
     hipStream_t s = (hipStream_t)stream;

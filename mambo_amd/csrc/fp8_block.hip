@@ -653,6 +653,7 @@ constexpr Fp8Kernel kFp8Kernels[3][9] = {
      {64, 256, 1, 2, 2.893, 0.000, {0.697, 1.118}, 0.775, 0.154},
      {128, 256, 1, 2, 4.436, 0.000, {1.007, 1.513}, 0.833, 0.139}}};
 constexpr int kFirstTile = 3; // those from here on address rows by 32-bit offsets
+constexpr int kThreads[9] = {512, 256, 256, 512, 512, 512, 512, 256, 256}; // of a workgroup
 constexpr int64_t kCUs = 256;
 
 double fp8_time(const Fp8Kernel &t, int64_t wgs, int64_t groups, double outputs, double weights)
@@ -710,7 +711,7 @@ int fp8_plan(Fp8Args *a, bool bf16, int64_t *wgs)
         if (!t.tokens)
             continue;
         const int64_t columns = cdiv(a->n, t.rows), most = er.offsets ? expert_row_tiles(er.r, er.experts, t.tokens) : cdiv(er.r, t.tokens);
-        if (most * columns > 0x3FFFFFFF) // with the order's rest, and the sums in place()
+        if (!grid_takes(most * columns + 255, kThreads[i])) // with what the order rounds up to; place() adds in 32 bits
             continue;
         const double tiles = grouped ? std::fmax(taken, r / t.tokens + 0.5 * taken) : (double)cdiv(er.r, t.tokens);
         const double us = fp8_time(t, (int64_t)std::ceil(tiles) * columns, a->groups, r * a->n, taken * a->n * a->k);
@@ -734,10 +735,12 @@ int launch_products(const Fp8Args &a, int which, int64_t wgs, hipStream_t stream
 {
 #define MAMBO_STREAM(I, H, W)                                                                                      \
     case I:                                                                                                        \
+        static_assert(kThreads[I] == W * 64);                                                                      \
         MAMBO_LAUNCH((fp8_stream_kernel<H, W, kExperts, kBf16>), dim3((unsigned)wgs), dim3(W * 64), 0, stream, a); \
         break
 #define MAMBO_TILE(I, MT, NB, WN, KG)                                                                              \
     case I:                                                                                                        \
+        static_assert(kThreads[I] == WN * KG * 64);                                                                \
         MAMBO_LAUNCH((fp8_tile_kernel<MT, NB, WN, KG, kExperts, kBf16>), dim3((unsigned)wgs), dim3(WN * KG * 64), 0,     \
                      stream, a);                                                                                   \
         break
@@ -855,7 +858,7 @@ extern "C" int mambo_fp8_block_pack(const uint8_t *w, int64_t experts, int64_t n
     MAMBO_REQUIRE(w && packed, MAMBO_ERR_VALUE, "null pointer");
     MAMBO_REQUIRE((uintptr_t)packed % 16 == 0, MAMBO_ERR_VALUE, "packed must be 16-byte aligned");
     const int64_t ntiles = cdiv(n, kTileN), groups = cdiv(k, kGroup), tiles = experts * ntiles * groups;
-    MAMBO_REQUIRE(tiles <= 0x7FFFFFFF, MAMBO_ERR_VALUE, "weights too large for one call");
+    MAMBO_REQUIRE(grid_takes(tiles, 256), MAMBO_ERR_VALUE, "weights too large for one call");
     const bool vec = (uintptr_t)w % 16 == 0 && stride_e % 16 == 0 && stride_n % 16 == 0;
     MAMBO_LAUNCH(fp8_block_pack_kernel, dim3((unsigned)tiles), dim3(256), 0, (hipStream_t)stream, w, n, k, stride_e,
                  stride_n, ntiles, groups, vec, packed);

@@ -183,9 +183,9 @@ extern "C" int mambo_iq3s_fp8_matmul_experts(const uint8_t *xv, int64_t ldxv, co
     auto tiles = [&](int t) { return std::fmax(taken, (double)r / t + 0.5 * taken); };
     // The 32 x 32 MFMA kernel from 14 rows of an expert on, where 16 tokens a tile fill the card four times: 64 experts of
     // 2048 x 4096 with 12 rows each take it 75.4 us (the 16-token kernel 72.5), with 16 76.1 (94.6), 4 experts of 1024 x
-    // 4096 with 64 rows 24.8 (16.1). It tells rows by 32-bit offsets.
-    if ((double)r > 14.0 * taken && tiles(16) * a.ntiles >= 1024.0 && (rows ? m : 256) * ldxv + 256 * blocks < ((int64_t)1 << 32) &&
-        (rows ? m : 256) * ldxs + 8 * blocks < ((int64_t)1 << 32) && expert_row_tiles(r, experts, 64) <= 65535) {
+    // 4096 with 64 rows 24.8 (16.1). It tells rows by 32-bit offsets, and a grid takes 2^29 weight rows of it.
+    if ((double)r > 14.0 * taken && tiles(16) * a.ntiles >= 1024.0 && n < (1 << 29) &&
+        (rows ? m : 256) * ldxv + 256 * blocks < ((int64_t)1 << 32) && (rows ? m : 256) * ldxs + 8 * blocks < ((int64_t)1 << 32) && expert_row_tiles(r, experts, 64) <= 65535) {
         double tiles_of[2] = {tiles(64), tiles(128)};
         WidePlan plan;
         mambo_wide_experts_plan(er, n, blocks, tiles_of, &plan);
@@ -200,7 +200,7 @@ extern "C" int mambo_iq3s_fp8_matmul_experts(const uint8_t *xv, int64_t ldxv, co
     const double expected = tiles(diag ? 4 : 16) * a.ntiles;
     const int waves = expected >= 2560.0 || blocks < 4 ? 1 : expected >= 640.0 || blocks < 8 ? 2 : 4;
     const int64_t wgs = expert_row_tiles(r, experts, diag ? 4 : 16) * a.ntiles;
-    MAMBO_REQUIRE(wgs <= 0x7FFFFFFF, MAMBO_ERR_VALUE, "too many rows and columns for one launch");
+    MAMBO_REQUIRE(grid_takes(wgs, 64 * waves), MAMBO_ERR_VALUE, "too many rows and columns for one launch");
 #define MAMBO_IQ3S(D, W, B)                                                                                            \
     if (diag == D && waves == W && bf16 == B)                                                                          \
     MAMBO_LAUNCH((iq3s_expert_stream_kernel<D, W, B>), dim3((unsigned)wgs), dim3(W * 64), 0, s, a)

@@ -91,3 +91,54 @@ def test_route_of_the_most_choices(gpu):
         assert bool(((weights[at].sum(1) - 1.0).abs() < 64 * 2.0**-23).all())
     del ids, weights, offsets, rows, slots, logits
     torch.cuda.empty_cache()
+
+
+# ------------------------------------------------------------------------------ launches that no grid holds
+GRID_THREADS = 2**32 - 1  # of a dimension
+THREADS = {(16, 16, 8): 512, (16, 32, 4): 256, (16, 64, 4): 256, (32, 64, 4): 512, (64, 64, 4): 512, (64, 128, 2): 512,
+           (64, 256, 2): 512, (64, 256, 1): 256, (128, 256, 1): 256}  # tokens, weight rows, K groups: of a workgroup
+
+
+def refusal(rc, text):
+    from mambo_amd import _native
+    assert rc == _native.MAMBO_ERR_VALUE and text in _native.lib().mambo_last_error().decode()
+
+
+@pytest.mark.parametrize("experts", [0, 1, 4, 1024])
+@pytest.mark.parametrize("bf16", [True, False])
+def test_products_are_planned_within_a_grid(experts, bf16):
+    """Whatever the sizes, the kernel that is chosen fits a grid, or none does and the call is refused."""
+    import ctypes
+    from mambo_amd import _native
+    lib, plan = _native.lib(), (ctypes.c_int32 * 5)()
+    kernels = [k for k in THREADS if bf16 or k[0] < 128]
+    taken = 0
+    for r in (1, 1000, 2**20 + 1, 2**25, 2**28, 2**30 + 77, 2**31 - 200, 2**31 - 1):
+        for n in (1, 300, 4096, 2**17, 2**24, 0x7FFFFF00):
+            def most(tokens):
+                return r // tokens + min(r, experts) + 1 if experts else -(-r // tokens)
+
+            near = 4 * (128 + r) < 2**32  # the scales of a tile within 32 bits; else the 16-token kernels alone
+            fits = [k for k in kernels if (near or k[0] == 16) and
+                    (most(k[0]) * -(-n // k[1]) + 255) * THREADS[k] <= GRID_THREADS]
+            rc = lib.mambo_fp8_block_plan(r, r, experts, n, 128, 128,
+                                          _native.DTYPE_BF16 if bf16 else _native.DTYPE_F32, plan)
+            if fits:
+                assert rc == 0 and tuple(plan[:3]) in fits, (r, n)
+                taken += 1
+            else:
+                refusal(rc, "too many rows and columns")
+    assert taken > 10
+
+
+def test_calls_that_no_grid_holds_are_refused():
+    """Before anything is launched, with the message written for it."""
+    from mambo_amd import _native
+    lib, r = _native.lib(), 2**31 - 1
+    refusal(lib.mambo_fp8_block_matmul(16, 16, 16, 1, r, r, 16, 16, 4096, 16, 16, 0, 4096, None), "too many rows and columns")
+    refusal(lib.mambo_fp8_block_matmul_experts(16, 16, 16, 1, 1, 1, 16, r, 16, 4, 16, 16, 1, 16, 16, 1, 1, None),
+            "too many rows and columns")
+    refusal(lib.mambo_iq3s_fp8_matmul_experts(16, 256, 16, 8, 1, 16, r, 16, 4, 16, 7040, 64, 1, 16, 0, 64, None),
+            "too many rows and columns")
+    refusal(lib.mambo_fp8_block_pack(16, 1, 0x7FFFFF00, 16, 0, 16, 16, None), "too large for one call")
+    refusal(lib.mambo_combine_experts(16, 1, 2**36, 4, 16, 16, 2, 2, 2**36, 16, 1, 2**36, None), "rows too long")
