@@ -25,11 +25,20 @@ void mambo_note_prior_error(hipError_t err)
         g_prior_error = err;
 }
 
+// A launch of this call was left out (mambo_note_oversized).
+static thread_local bool g_oversized = false;
+
+void mambo_note_oversized() { g_oversized = true; }
+
 int mambo_check_launch(const char *what)
 {
     const hipError_t prior = g_prior_error;
+    const bool oversized = g_oversized;
     g_prior_error = hipSuccess;
+    g_oversized = false;
     hipError_t err = hipGetLastError();
+    if (oversized)
+        return mambo_fail(MAMBO_ERR_VALUE, "%s: sizes too large for one launch (2^32 threads and more)", what);
     if (err != hipSuccess)
         return mambo_fail(MAMBO_ERR_RUNTIME, "%s: %s", what, hipGetErrorString(err));
     if (prior != hipSuccess) // the call succeeded; keep the earlier error readable

@@ -72,11 +72,6 @@ __device__ __forceinline__ int64_t source_row(const ExpertRows &er, int64_t i)
     return s < 0 ? 0 : s >= er.m ? er.m - 1 : s;
 }
 
-// Threads of a grid's dimension that HIP launches, and whether `wgs` workgroups of `threads` are no more. (Of more it
-// launches what is left modulo 2^32, with no error: 3222784 workgroups of 20000000 x 256.)
-constexpr int64_t kMaxGridThreads = 0xFFFFFFFF;
-inline bool grid_takes(int64_t wgs, int64_t threads) { return wgs <= kMaxGridThreads / threads; }
-
 // Host checks that the grouped products share.
 inline int check_expert_rows(int64_t m, const int32_t *rows, int64_t r, const int32_t *offsets, int64_t experts)
 {

@@ -15,14 +15,29 @@ int mambo_check_launch(const char *what);
 // reports it through mambo_last_error() (the call itself still succeeds).
 void mambo_note_prior_error(hipError_t err);
 
+// Records a launch that was left out because HIP would not have launched all of it;
+// mambo_check_launch then fails with MAMBO_ERR_VALUE.
+void mambo_note_oversized();
+
+// Threads of a grid's dimension that HIP launches, and whether `wgs` workgroups of
+// `threads` are no more. (Of more it launches what is left modulo 2^32, with no error:
+// 3222784 workgroups of 20000000 x 256.)
+constexpr int64_t kMaxGridThreads = 0xFFFFFFFF;
+inline bool grid_takes(int64_t wgs, int64_t threads) { return wgs <= kMaxGridThreads / threads; }
+
 // Launch with the calling thread's HIP error state taken first, so that the
 // mambo_check_launch after it reports this launch's own failure, not one that an
 // earlier, unrelated HIP call left behind; that earlier error stays readable through
-// mambo_last_error().
-#define MAMBO_LAUNCH(...)                                                                          \
+// mambo_last_error(). A grid that HIP would cut short is not launched.
+#define MAMBO_LAUNCH(kernel, grid, block, ...)                                                     \
     do {                                                                                           \
         mambo_note_prior_error(hipGetLastError());                                                 \
-        hipLaunchKernelGGL(__VA_ARGS__);                                                           \
+        const dim3 mambo_grid = (grid), mambo_block = (block);                                     \
+        if (grid_takes(mambo_grid.x, mambo_block.x) && grid_takes(mambo_grid.y, mambo_block.y) &&  \
+            grid_takes(mambo_grid.z, mambo_block.z))                                               \
+            hipLaunchKernelGGL(kernel, mambo_grid, mambo_block, __VA_ARGS__);                      \
+        else                                                                                       \
+            mambo_note_oversized();                                                                \
     } while (0)
 
 #define MAMBO_REQUIRE(cond, status, ...)                                                           \
