@@ -1,4 +1,5 @@
 // The router's plan and the join of the experts' rows.
+#include <algorithm>
 #include <type_traits>
 
 #include "experts.h"
@@ -363,6 +364,9 @@ struct Route {
     int32_t *offsets, *rows, *slots;
 };
 
+// Tokens of a launch: four a workgroup, as many as a grid takes.
+constexpr int64_t kChooseTokens = 4 * (kMaxGridThreads / 256);
+
 template <int V, bool kBf16>
 void launch_choose(const Route &a, bool few, hipStream_t s)
 {
@@ -370,8 +374,10 @@ void launch_choose(const Route &a, bool few, hipStream_t s)
         MAMBO_LAUNCH((route_few_kernel<V, kBf16>), dim3(1), dim3(1024), 0, s, a.logits, a.ld, (int)a.m, a.experts, a.top_k,
                      a.renormalize, a.ids, a.weights, a.offsets, a.rows, a.slots);
     else
-        MAMBO_LAUNCH((route_choose_kernel<V, kBf16>), dim3((unsigned)cdiv(a.m, 4)), dim3(256), 0, s, a.logits, a.ld, a.m,
-                     a.experts, a.top_k, a.renormalize, a.ids, a.weights);
+        for (int64_t t = 0; t < a.m; t += kChooseTokens)
+            MAMBO_LAUNCH((route_choose_kernel<V, kBf16>), dim3((unsigned)cdiv(std::min(kChooseTokens, a.m - t), 4)), dim3(256), 0,
+                         s, reinterpret_cast<const row_t<kBf16> *>(a.logits) + t * a.ld, a.ld, std::min(kChooseTokens, a.m - t),
+                         a.experts, a.top_k, a.renormalize, a.ids + t * a.top_k, a.weights + t * a.top_k);
 }
 
 } // namespace

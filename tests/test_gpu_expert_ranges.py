@@ -93,6 +93,23 @@ def test_route_of_the_most_choices(gpu):
     torch.cuda.empty_cache()
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_route_of_more_tokens_than_a_launch(gpu, dtype):
+    """2^26 + 5 tokens, one workgroup for four: token t takes expert (2 - t) mod 3."""
+    from mambo_amd.kernels.experts import launch_route_experts
+    m = 2**26 + 5
+    t = torch.arange(m, dtype=torch.int32, device=gpu)
+    logits = torch.stack([(t + e) % 3 for e in range(3)], dim=1).to(dtype)
+    ids, weights, offsets, rows, slots = launch_route_experts(logits, 1)
+    expected = (2 - t) % 3
+    counts = [int((expected == e).sum()) for e in range(3)]
+    starts = [0, counts[0], counts[0] + counts[1], m]
+    assert offsets.tolist() == starts and torch.equal(ids[:, 0], expected) and bool((weights == 1.0).all())
+    assert torch.equal(slots[:, 0], torch.tensor(starts[:3], dtype=torch.int32, device=gpu)[expected.long()] + t // 3)
+    assert torch.equal(rows, torch.cat([t[(2 - e) % 3::3] for e in range(3)]))
+
+
 # ------------------------------------------------------------------------------ launches that no grid holds
 GRID_THREADS = 2**32 - 1  # of a dimension
 THREADS = {(16, 16, 8): 512, (16, 32, 4): 256, (16, 64, 4): 256, (32, 64, 4): 512, (64, 64, 4): 512, (64, 128, 2): 512,
