@@ -224,7 +224,7 @@ def prepare_iq3_s_experts(iq3_weights: torch.Tensor, *, stream=None) -> IQ3SExpe
             iq3_weights = torch.nn.functional.pad(iq3_weights, (0, 0, 0, 0, 0, -n % 16)).contiguous()
         se, sn, sb, sbyte = iq3_weights.stride()
         n_tall = iq3_weights.shape[1]
-        tall = n_tall % 16 == 0 and se == n_tall * sn
+        tall = n_tall % 16 == 0 and se == n_tall * sn and n_tall * experts < 1 << 28  # what a launch takes
         for e in range(1 if tall else experts):
             _native.check(_native.lib().mambo_iq3s_prepare(
                 iq3_weights.data_ptr() + e * se, n_tall * experts if tall else n, blocks, sn, sb, sbyte, None, None, None, None, None,

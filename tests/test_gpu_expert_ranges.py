@@ -159,3 +159,19 @@ def test_calls_that_no_grid_holds_are_refused():
             "too many rows and columns")
     refusal(lib.mambo_fp8_block_pack(16, 1, 0x7FFFFF00, 16, 0, 16, 16, None), "too large for one call")
     refusal(lib.mambo_combine_experts(16, 1, 2**36, 4, 16, 16, 2, 2, 2**36, 16, 1, 2**36, None), "rows too long")
+
+
+@pytest.mark.gpu
+def test_iq3s_experts_of_more_rows_than_a_launch(gpu):
+    """17 experts of 2^24 rows follow each other: as one tall weight they would not fit a launch."""
+    from mambo_amd.utils.iq3_s_weight import prepare_iq3_s_experts
+    raws = torch.empty((17, 1 << 24, 1, 110), dtype=torch.uint8, device=gpu)
+    raws.view(-1)[:110 << 24].random_(0, 256)
+    for e in range(1, 17):
+        raws[e] = raws[0].roll(e, 0)
+    got = prepare_iq3_s_experts(raws)
+    assert (got.experts, got.n, got.blocks) == (17, 1 << 24, 1)
+    for e in (0, 1, 15, 16):
+        assert torch.equal(got.packed[e], prepare_iq3_s_experts(raws[e:e + 1]).packed[0]), e
+    del raws, got
+    torch.cuda.empty_cache()
