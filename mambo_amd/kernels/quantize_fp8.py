@@ -54,27 +54,26 @@ def launch_quantize_fp8(x: torch.Tensor, *, tile_m: int | None = None, tile_k_gr
         raise ValueError("activation must be float32 or bfloat16 [M,K] with K divisible by 32")
     if not x.is_cuda:
         raise ValueError("activation must be a GPU tensor")
-    if tile_m is None or tile_k_groups is None:
-        with _native.on_device(x.device):
+    with _native.launch_on(x.device, stream):
+        if tile_m is None or tile_k_groups is None:
             config = _activation_config(x.shape[0])
-        tile_m = config["tile_m"] if tile_m is None else tile_m
-        tile_k_groups = config["tile_k_groups"] if tile_k_groups is None else tile_k_groups
-    _power_of_two(tile_m, "tile_m")
-    _power_of_two(tile_k_groups, "tile_k_groups")
-    if x.stride(1) != 1:
-        x = x.contiguous()
-    m, k = x.shape
-    if out is None:
-        values = torch.empty((m, k), dtype=torch.uint8, device=x.device)
-        scales = torch.empty((m, k // 32), dtype=torch.uint8, device=x.device)
-    else:
-        values, scales = out
-        if values.shape != (m, k) or values.dtype != torch.uint8 or values.stride(1) != 1 \
-                or scales.shape != (m, k // 32) or scales.dtype != torch.uint8 or scales.stride(1) != 1:
-            raise ValueError("out must be (uint8 [M,K], uint8 [M,K/32]) with unit column stride")
-    dtype = _native.DTYPE_F32 if x.dtype == torch.float32 else _native.DTYPE_BF16
-    with _native.on_device(x.device):
+            tile_m = config["tile_m"] if tile_m is None else tile_m
+            tile_k_groups = config["tile_k_groups"] if tile_k_groups is None else tile_k_groups
+        _power_of_two(tile_m, "tile_m")
+        _power_of_two(tile_k_groups, "tile_k_groups")
+        if x.stride(1) != 1:
+            x = x.contiguous()
+        m, k = x.shape
+        if out is None:
+            values = torch.empty((m, k), dtype=torch.uint8, device=x.device)
+            scales = torch.empty((m, k // 32), dtype=torch.uint8, device=x.device)
+        else:
+            values, scales = out
+            if values.shape != (m, k) or values.dtype != torch.uint8 or values.stride(1) != 1 \
+                    or scales.shape != (m, k // 32) or scales.dtype != torch.uint8 or scales.stride(1) != 1:
+                raise ValueError("out must be (uint8 [M,K], uint8 [M,K/32]) with unit column stride")
+        dtype = _native.DTYPE_F32 if x.dtype == torch.float32 else _native.DTYPE_BF16
         _native.check(_native.lib().mambo_quantize_mxfp8(
             x.data_ptr(), dtype, m, k, x.stride(0), values.data_ptr(), values.stride(0),
-            scales.data_ptr(), scales.stride(0), _native.stream_handle(stream)), "launch_quantize_fp8")
+            scales.data_ptr(), scales.stride(0), _native.stream_handle(stream, x.device)), "launch_quantize_fp8")
     return values, scales
