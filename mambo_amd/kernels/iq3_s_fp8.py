@@ -21,6 +21,7 @@ weights uses scale d * (1 + 2 * scale_nibble).
 from __future__ import annotations
 
 import json
+from contextlib import nullcontext
 from dataclasses import dataclass, field
 from functools import lru_cache
 from pathlib import Path
@@ -130,9 +131,9 @@ def launch_dequant_iq3_s(iq3_weight: IQ3SFields, *, tile_n: int = 1, stream=None
         if not t.is_contiguous() or t.numel() == 0 and n_rows * blocks:
             raise ValueError(f"IQ3SFields.{name} must be a contiguous prepared field")
     dev = iq3_weight.d.device
-    values = torch.empty((n_rows, blocks * 256), dtype=torch.uint8, device=dev)
-    scales = torch.empty((n_rows, blocks * 8), dtype=torch.float32, device=dev)
-    with _native.on_device(dev):
+    with _native.launch_on(dev, stream):
+        values = torch.empty((n_rows, blocks * 256), dtype=torch.uint8, device=dev)
+        scales = torch.empty((n_rows, blocks * 8), dtype=torch.float32, device=dev)
         _native.check(_native.lib().mambo_iq3s_dequant(*(t.data_ptr() for t in fields), n_rows, blocks,
                                                        values.data_ptr(), scales.data_ptr(),
                                                        _native.stream_handle(stream)), "launch_dequant_iq3_s")
@@ -155,9 +156,10 @@ def default_config(m: int, arch: str = "gfx950") -> dict:
     return dict(BEST_CONFIGS[arch]["medium" if m < LARGE_TOKEN_THRESHOLD else "large"])
 
 
-def _prepare_activations(x_values, x_scales, k: int):
+def _prepare_activations(x_values, x_scales, k: int, stream):
     """Validate MXFP8 activations [M,K] + [M,K/32]; return them in a form the kernels
-    read in place (unit column stride, 16-byte aligned rows), copying only if needed."""
+    read in place (unit column stride, 16-byte aligned rows), copying only if needed, on
+    the launch's stream."""
     if not isinstance(x_values, torch.Tensor) or x_values.ndim != 2 or x_values.dtype != torch.uint8 \
             or x_values.shape[0] < 1 or x_values.shape[1] != k:
         raise ValueError("x_values must be uint8 [M,K]")
@@ -167,18 +169,19 @@ def _prepare_activations(x_values, x_scales, k: int):
         raise ValueError("x_scales must be uint8 [M,K/32]")
     if x_scales.device != x_values.device:
         raise ValueError("x_values and x_scales must be on the same device")
-    x_values = _aligned_rows(x_values, 16)
+    x_values = _aligned_rows(x_values, 16, stream)
     # the tiled kernel copies each token's 8 scale bytes of a block as two dwords
-    x_scales = _aligned_rows(x_scales, 8)
+    x_scales = _aligned_rows(x_scales, 8, stream)
     return x_values, x_scales, m
 
 
-def _aligned_rows(t: torch.Tensor, align: int) -> torch.Tensor:
+def _aligned_rows(t: torch.Tensor, align: int, stream=None) -> torch.Tensor:
     """`t` itself when its rows are unit-stride and start on `align`-byte boundaries,
     else a contiguous copy (rows of K and K/32 bytes are multiples of 16 and 8)."""
     if t.stride(1) == 1 and t.stride(0) % align == 0 and t.data_ptr() % align == 0:
         return t
-    return torch.empty(t.shape, dtype=t.dtype, device=t.device).copy_(t)
+    with nullcontext() if stream is None else _native.launch_on(t.device, stream):
+        return torch.empty(t.shape, dtype=t.dtype, device=t.device).copy_(t)
 
 
 def _output(out, m: int, n: int, dev) -> torch.Tensor:
@@ -202,9 +205,9 @@ def launch_iq3_s_fp8_matmul(x_values: torch.Tensor, x_scales: torch.Tensor, iq3_
     """
     n_rows, k_blocks = _weight_dimensions(iq3_weight)
     k = k_blocks * IQ3_S_BLOCK_VALUES
-    x_values, x_scales, m = _prepare_activations(x_values, x_scales, k)
+    x_values, x_scales, m = _prepare_activations(x_values, x_scales, k, stream)
     dev = x_values.device
-    with _native.on_device(dev):
+    with _native.launch_on(dev, stream):
         cfg = _native.GemmConfig.from_dict(config if config is not None else select_config(m, n_rows, k))
         packed = ensure_packed(iq3_weight, stream)
         out = _output(out, m, n_rows, dev)
@@ -234,12 +237,12 @@ def launch_iq3_s_fp8_matmul_grouped(x_values: torch.Tensor, x_scales: torch.Tens
     if any(b != k_blocks for _, b in dims):
         raise ValueError("grouped weights must share K")
     k = k_blocks * IQ3_S_BLOCK_VALUES
-    x_values, x_scales, m = _prepare_activations(x_values, x_scales, k)
+    x_values, x_scales, m = _prepare_activations(x_values, x_scales, k, stream)
     dev = x_values.device
     if outs is not None and len(outs) != len(weights):
         raise ValueError("outs must hold one output per weight")
     n_total = sum(n for n, _ in dims)
-    with _native.on_device(dev):
+    with _native.launch_on(dev, stream):
         cfg = _native.GemmConfig.from_dict(config if config is not None else select_config(m, n_total, k))
         result = [_output(None if outs is None else outs[i], m, n, dev) for i, (n, _) in enumerate(dims)]
         projections = (_native.Projection * len(weights))()
@@ -277,13 +280,13 @@ def launch_iq3_s_matmul_quantize(x: torch.Tensor, iq3_weights, *, stream=None, c
     dtypes = {torch.float32: _native.DTYPE_F32, torch.bfloat16: _native.DTYPE_BF16}
     if x.dtype not in dtypes:
         raise ValueError(f"x must be float32 or bfloat16, got {x.dtype}")
-    if x.stride(1) != 1:
-        x = x.contiguous()
     m, dev = int(x.shape[0]), x.device
     if outs is not None and len(outs) != len(weights):
         raise ValueError("outs must hold one output per weight")
     n_total = sum(n for n, _ in dims)
-    with _native.on_device(dev):
+    with _native.launch_on(dev, stream):
+        if x.stride(1) != 1:
+            x = x.contiguous()
         cfg = _native.GemmConfig.from_dict(config if config is not None else select_config(m, n_total, k))
         result = [_output(None if outs is None else outs[i], m, n, dev) for i, (n, _) in enumerate(dims)]
         projections = (_native.Projection * len(weights))()
@@ -367,20 +370,21 @@ def launch_iq3_s_fp8_matmul_chain(launches, *, stream=None, waves: int = 0, sync
             raise ValueError("every launch of a chain takes the same M tokens on the same device")
         desc = descs[i]
         if x.dtype == torch.uint8:
-            x, xs, _ = _prepare_activations(x, cl.x_scales, k)  # rows 16- and 8-byte aligned
+            x, xs, _ = _prepare_activations(x, cl.x_scales, k, stream)  # rows 16- and 8-byte aligned
             desc.x_dtype, desc.xs, desc.ldxs = _native.DTYPE_MXFP8, xs.data_ptr(), xs.stride(0)
         elif x.dtype in dtypes:
             if cl.x_scales is not None:
                 raise ValueError(f"launch {i}: x_scales belongs to MXFP8 (uint8) activations")
             esz = x.element_size()
             if x.stride(1) != 1 or x.data_ptr() % 16 or (x.stride(0) * esz) % 16:
-                x = x.contiguous() if x.data_ptr() % 16 == 0 else x.clone()
+                with _native.launch_on(dev, stream):
+                    x = x.contiguous() if x.data_ptr() % 16 == 0 else x.clone()
             desc.x_dtype, desc.xs, desc.ldxs = dtypes[x.dtype], None, 0
         else:
             raise ValueError(f"launch {i}: x must be uint8 (MXFP8), float32 or bfloat16, got {x.dtype}")
         if cl.outs is not None and len(cl.outs) != len(weights):
             raise ValueError(f"launch {i}: outs must hold one output per weight")
-        with _native.on_device(dev):
+        with _native.launch_on(dev, stream):
             outs = [_output(None if cl.outs is None else cl.outs[j], m, n, dev) for j, (n, _) in enumerate(dims)]
             for j, (w, (n, _)) in enumerate(zip(weights, dims)):
                 desc.proj[j] = _native.Projection(ensure_packed(w, stream).data_ptr(), n, outs[j].data_ptr(),
@@ -390,7 +394,7 @@ def launch_iq3_s_fp8_matmul_chain(launches, *, stream=None, waves: int = 0, sync
     cfg = _native.ChainConfig()
     cfg.waves, cfg.tiles_per_workgroup, cfg.timeout_us, cfg.wait_bias = waves, tiles_per_workgroup, timeout_us, \
         wait_bias
-    with _native.on_device(dev):
+    with _native.launch_on(dev, stream):
         if sync is None:
             sync = new_chain_sync(dev)
         if sync.dtype not in (torch.int32, torch.uint32) or sync.numel() < _native.CHAIN_SYNC_WORDS \
