@@ -350,6 +350,7 @@ def launch_iq3_s_fp8_matmul_chain(launches, *, stream=None, waves: int = 0, sync
     dtypes = {torch.float32: _native.DTYPE_F32, torch.bfloat16: _native.DTYPE_BF16}
     descs = (_native.ChainLaunch * len(launches))()
     results, m, dev = [], None, None
+    kept = []  # scales that were copied: until the launch
     for i, cl in enumerate(launches):
         if not isinstance(cl, ChainLaunch):
             raise TypeError("launches must be ChainLaunch objects")
@@ -371,6 +372,7 @@ def launch_iq3_s_fp8_matmul_chain(launches, *, stream=None, waves: int = 0, sync
         desc = descs[i]
         if x.dtype == torch.uint8:
             x, xs, _ = _prepare_activations(x, cl.x_scales, k, stream)  # rows 16- and 8-byte aligned
+            kept.append(xs)
             desc.x_dtype, desc.xs, desc.ldxs = _native.DTYPE_MXFP8, xs.data_ptr(), xs.stride(0)
         elif x.dtype in dtypes:
             if cl.x_scales is not None:
