@@ -54,6 +54,8 @@ class ExpertLayer:
     def __call__(self, x: torch.Tensor) -> torch.Tensor:
         """The layer's output [M, H] of bfloat16 rows x [M, H]."""
         dtype = torch.bfloat16
+        if x.shape[0] == 0:  # launch_quantize_fp8 takes one row and more
+            return torch.empty((0, self.down.n), dtype=dtype, device=x.device)
         plan = launch_route_experts(x @ self.router.t(), self.top_k, renormalize=self.renormalize)
         values, scales = launch_quantize_fp8_block(x)  # a token's row once, however many experts read it
         h = launch_fp8_block_matmul_experts(values, scales, self.gate_up, plan.offsets, rows=plan.rows, out_dtype=dtype)

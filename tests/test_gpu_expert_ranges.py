@@ -175,3 +175,15 @@ def test_iq3s_experts_of_more_rows_than_a_launch(gpu):
         assert torch.equal(got.packed[e], prepare_iq3_s_experts(raws[e:e + 1]).packed[0]), e
     del raws, got
     torch.cuda.empty_cache()
+
+
+# ------------------------------------------------------------------------------ the layer
+@pytest.mark.gpu
+@pytest.mark.parametrize("shared", [0, 256])
+@pytest.mark.parametrize("down", ["fp8", "iq3s"])
+def test_layer_of_no_tokens(gpu, down, shared):
+    from mambo_amd.utils.expert_layer import random_layer
+    layer = random_layer(512, 256, 4, 2, down=down, shared=shared)
+    out = layer(torch.empty((0, 512), dtype=torch.bfloat16, device=gpu))
+    assert out.shape == (0, 512) and out.dtype == torch.bfloat16 and out.device == gpu
+    assert layer(torch.ones((1, 512), dtype=torch.bfloat16, device=gpu)).shape == (1, 512)
