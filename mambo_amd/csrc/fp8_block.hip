@@ -9,12 +9,14 @@
 // tokens the B operand (its columns), so a lane's sums belong to one token and its scale is one
 // factor, xs * ws, of which ws is the same for the wave.
 //
-// An FP8 MFMA aligns the products of eight consecutive K and keeps 14 bits below the largest of them
-// (measured on gfx950: beside a product of 2^16 one of 2^3 counts and one of 2^2 does not, in the
-// 16 x 16 x 128 and 32 x 32 x 64 shapes and in the older 16 x 16 x 32 and 32 x 32 x 16 alike), an error of
-// up to 1.7e-4 of the sum of magnitudes, 5e-5 in the 2-norm over codes of all exponents. That is 2^-5 of
-// what rounding to bf16 takes, so bf16 outputs use it. f32 outputs are of f32 sums: the codes are widened
-// to bf16, exactly, and multiplied by the bf16 MFMAs, which add without that loss (2.5e-7 on the same
+// An FP8 MFMA adds the products of eight consecutive K as multiples of 2^-13 of 2^E and cuts what is below,
+// E being the largest sum of two codes' exponents among the eight (measured on gfx950: beside a product of 2^16
+// one of 2^3 counts and one of 2^2 does not, of either sign, in the 16 x 16 x 128 and 32 x 32 x 64 shapes and in
+// the older 16 x 16 x 32 and 32 x 32 x 16 alike; among other eights it does). At worst that leaves out seven
+// products of the eight, 7 x 2^-13 = 8.5e-4 of the largest (measured 7.5e-4 of the sum of magnitudes); over codes of
+// all exponents it is 5e-5 of the sums in the 2-norm, 2^-5 of what rounding them to bf16 takes, so bf16 outputs use
+// it. Where a row's terms cancel, what is cut does not shrink with the result. f32 outputs are of f32 sums: the codes
+// are widened to bf16, exactly, and multiplied by the bf16 MFMAs, which add without that loss (2.5e-7 on the same
 // data), at half the matrix rate.
 //
 // Layout of a weight (mambo_fp8_block_pack): tiles of 32 rows x 128 of K, 4096 bytes, ordered
