@@ -187,3 +187,65 @@ def test_layer_of_no_tokens(gpu, down, shared):
     out = layer(torch.empty((0, 512), dtype=torch.bfloat16, device=gpu))
     assert out.shape == (0, 512) and out.dtype == torch.bfloat16 and out.device == gpu
     assert layer(torch.ones((1, 512), dtype=torch.bfloat16, device=gpu)).shape == (1, 512)
+
+
+# ------------------------------------------------------------------------------ quantizer
+def encode(x: np.ndarray) -> np.ndarray:
+    """e4m3_encode_bruteforce for many values: between which two codes' middles a magnitude lies, the even
+    code on a middle."""
+    values = ref.VALUES[:127]
+    middles = (values[1:] + values[:-1]) / 2.0  # exact
+    a = np.abs(x.astype(np.float64))
+    code = np.searchsorted(middles, a, side="left")  # a middle: the lower code
+    on = code < 126
+    on[on] = middles[code[on]] == a[on]
+    code[on] += code[on] & 1
+    return (code | np.where(np.signbit(x), 0x80, 0)).astype(np.uint8)
+
+
+def quantized(x: np.ndarray):
+    """ref.quantize_block for many rows."""
+    (m, k), g = x.shape, -(-x.shape[1] // 128)
+    parts = np.pad(x, ((0, 0), (0, 128 * g - k))).reshape(m, g, 128)
+    amax = np.maximum(np.abs(parts).max(2, keepdims=True), np.float32(448.0 * 2.0**-100))
+    codes = encode((np.float32(0.875) * parts) / (amax * np.float32(2.0**-9)))
+    return codes.reshape(m, -1)[:, :k], amax[..., 0] / np.float32(448.0)
+
+
+def test_the_statement_for_many_rows_is_that_for_few():
+    rng = np.random.default_rng(5)
+    x = (rng.standard_normal((40, 300)) * np.exp2(rng.integers(-12, 12, size=(40, 300)))).astype(np.float32)
+    x[3], x[4] = 0.0, np.arange(300) * 448.0 / 299.0
+    x[5, :32] = np.concatenate([[448.0], np.arange(1, 32) * 0.5])  # middles among them
+    for a, b in zip(quantized(x), ref.quantize_block(x)):
+        assert a.dtype == b.dtype and np.array_equal(a, b)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("aligned", [True, False])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("m,k", [(4096, 128), (4097, 144), (5001, 16), (1367, 4112), (131073, 16)])
+def test_quantizer_of_many_rows(gpu, m, k, dtype, aligned):
+    """Sizes that take two rows at a time: an odd last row, a last group that is not whole, more pairs than
+    a grid's second dimension, rows that vectors do not reach."""
+    from mambo_amd.kernels.fp8_block import launch_quantize_fp8_block
+    assert m * -(-k // 2048) >= 4096  # rows times workgroups of a row
+    rng = np.random.default_rng(m + k)
+    x = rng.standard_normal((m, k)).astype(np.float32) * np.exp2(rng.integers(-20, 20, size=(m, 1))).astype(np.float32)
+    x[rng.random(m) < 0.05] = 0.0
+    x = torch.from_numpy(x).to(dtype)
+    expected = quantized(x.float().numpy())
+    rows = x.to(gpu)
+    if not aligned:
+        wide = torch.zeros((m, k + 5), dtype=dtype, device=gpu)
+        wide[:, 1:k + 1] = rows
+        rows = wide[:, 1:k + 1]
+    codes, scales = launch_quantize_fp8_block(rows)
+    assert np.array_equal(codes.cpu().numpy(), expected[0]) and np.array_equal(scales.cpu().numpy(), expected[1])
+    buffer = torch.full((m + 1, k + 19), 9, dtype=torch.uint8, device=gpu)
+    left = 16 if aligned else 3
+    by_row = torch.full((m + 1, scales.shape[1] + 2), 7.0, device=gpu)
+    launch_quantize_fp8_block(rows, out=(buffer[:m, left:left + k], by_row[:m, 1:-1]))
+    assert torch.equal(buffer[:m, left:left + k], codes) and torch.equal(by_row[:m, 1:-1], scales)
+    assert (buffer[m] == 9).all() and (buffer[:, :left] == 9).all() and (buffer[:, left + k:] == 9).all()
+    assert (by_row[m] == 7).all() and (by_row[:, 0] == 7).all() and (by_row[:, -1] == 7).all()
