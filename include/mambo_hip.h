@@ -342,6 +342,11 @@ int mambo_iq3s_fp8_matmul_experts(const uint8_t *xv, int64_t ldxv, const uint8_t
                                   const uint8_t *packed, int64_t expert_stride, int64_t n, int64_t blocks,
                                   void *out, int out_dtype, int64_t ldo, mambo_stream_t stream);
 
+/* How such a product is launched, on the host alone: plan[3] = tokens and weight rows that a workgroup works on at
+ * once, and the parts of K that its waves take. r rows of m (m != r: by rows). */
+int mambo_iq3s_experts_plan(int64_t m, int64_t r, int64_t experts, int64_t n, int64_t blocks, int64_t ldxv,
+                            int64_t ldxs, int32_t *plan);
+
 /* The router's plan: logits [m, ld] f32 or bf16 over `experts` <= MAMBO_MAX_EXPERTS; each token
  * takes its top_k (<= MAMBO_MAX_TOP_K) largest, ties to the lowest index, never one that is -inf or
  * NaN. ids i32 [m, top_k] in falling order, -1 where none was left; weights f32 [m, top_k]: the

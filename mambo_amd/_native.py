@@ -129,6 +129,7 @@ SIGNATURES = {
     "mambo_fp8_block_plan": (_i32, [_i64, _i64, _i64, _i64, _i64, _i64, _i32, _vp]),
     "mambo_iq3s_fp8_matmul_experts": (_i32, [_vp, _i64, _vp, _i64, _i64, _vp, _i64, _vp, _i64, _vp, _i64, _i64, _i64,
                                              _vp, _i32, _i64, _vp]),
+    "mambo_iq3s_experts_plan": (_i32, [_i64, _i64, _i64, _i64, _i64, _i64, _i64, _vp]),
     "mambo_route_experts": (_i32, [_vp, _i32, _i64, _i64, _i64, _i64, _i32, _vp, _vp, _vp, _vp, _vp, _vp]),
     "mambo_combine_experts": (_i32, [_vp, _i32, _i64, _i64, _vp, _vp, _i64, _i64, _i64, _vp, _i32, _i64, _vp]),
     "mambo_synth_iq3s": (_i32, [_u64, _i64, _i64, _i64, _vp, _vp]),

@@ -212,6 +212,7 @@ CONSTRAINTS: dict[str, list[dict]] = {
         _arr("packed", "uint8", ["experts", _PACKED], ["expert_stride", "1"], align=16),
         _arr("out", "float32|bfloat16", ["r", "n"], ["ldo", "1"], align=2, access="write"),
     ],
+    "mambo_iq3s_experts_plan": [_arr("plan", "int32", ["3"], align=4, memory="host", access="write")],
     "mambo_route_experts": [
         _arr("logits", "float32|bfloat16", ["m", "experts"], ["ld", "1"], align=2),
         _arr("ids", "int32", ["m", "top_k"], align=4, access="write"),

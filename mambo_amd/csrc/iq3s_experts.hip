@@ -147,20 +147,85 @@ __global__ __launch_bounds__(W * 64) __attribute__((amdgpu_waves_per_eu(2))) voi
     }
 }
 
+// The kernel of a product: the 32 x 32 MFMA kernel's plan, or the tokens of a tile and the waves that share K.
+struct Iq3sChoice {
+    bool wide;
+    WidePlan plan;
+    int tokens, waves;
+};
+
+Iq3sChoice iq3s_choose(const ExpertRows &er, int64_t n, int64_t blocks, int64_t ldxv, int64_t ldxs)
+{
+    const int64_t r = er.r, experts = er.experts, ntiles = (n + 31) / 32, apart = er.rows ? er.m : 256;
+    Iq3sChoice c = {};
+    // How the rows fall is not known here: experts with rows and tiles are counted for rows that fall at random.
+    const double taken = (double)experts * -std::expm1(-(double)r / (double)experts);
+    auto tiles = [&](int t) { return std::fmax(taken, (double)r / t + 0.5 * taken); };
+    // The 32 x 32 MFMA kernel from 14 rows of an expert on, where 16 tokens a tile fill the card four times: 64 experts of
+    // 2048 x 4096 with 12 rows each take it 75.4 us (the 16-token kernel 72.5), with 16 76.1 (94.6), 4 experts of 1024 x
+    // 4096 with 64 rows 24.8 (16.1). It tells rows by 32-bit offsets, and a grid takes 2^29 weight rows of it and 65535
+    // row tiles: past these the 16-token kernel is what is left, at a fraction of the rate (8 experts of 4096 x 14336, 4096
+    // rows, 1721 us and 487).
+    c.wide = (double)r > 14.0 * taken && tiles(16) * ntiles >= 1024.0 && n < (1 << 29) &&
+             apart * ldxv + 256 * blocks < ((int64_t)1 << 32) && apart * ldxs + 8 * blocks < ((int64_t)1 << 32) &&
+             expert_row_tiles(r, experts, 64) <= 65535;
+    if (c.wide) {
+        double tiles_of[2] = {tiles(64), tiles(128)};
+        mambo_wide_experts_plan(er, n, blocks, tiles_of, &c.plan);
+        return c;
+    }
+    // 4 tokens a tile up to 2.5 rows of an expert: 64 experts of 2048 x 4096 with 2.3 rows take 43.4 us (16 tokens a tile
+    // 47.6), with 4 62.5 (50.8).
+    c.tokens = (double)r <= 2.5 * taken ? 4 : 16;
+    // Waves that share a workgroup's K, two blocks each at least: one where workgroups fill the card, more where they do
+    // not (8 x 14336 x 4096, 4 tokens a tile, 3136 workgroups: 40.0 us with one, 42.1 with two, 43.6 with four; 2 experts,
+    // 896: 16.1, 14.5, 14.9; 2 of 4096 x 14336, 256: 34.8, 21.1, 14.7).
+    const double expected = tiles(c.tokens) * ntiles;
+    c.waves = expected >= 2560.0 || blocks < 4 ? 1 : expected >= 640.0 || blocks < 8 ? 2 : 4;
+    return c;
+}
+
+int check_iq3s_product(int64_t n, int64_t blocks, int out_dtype)
+{
+    MAMBO_REQUIRE(out_dtype == MAMBO_DTYPE_F32 || out_dtype == MAMBO_DTYPE_BF16, MAMBO_ERR_VALUE,
+                  "outputs must be float32 or bfloat16");
+    MAMBO_REQUIRE(n >= 1 && n <= 0x7FFFFF00 && blocks >= 1 && blocks <= 2000000, MAMBO_ERR_VALUE,
+                  "weights must be [N,K/256] blocks with N, K >= 1 (got %lld and %lld)", (long long)n, (long long)blocks);
+    return MAMBO_OK;
+}
+
 } // namespace
+
+extern "C" int mambo_iq3s_experts_plan(int64_t m, int64_t r, int64_t experts, int64_t n, int64_t blocks, int64_t ldxv,
+                                       int64_t ldxs, int32_t *plan)
+{
+    static const int32_t one = 0; // never read: that the rows are gathered, or by expert
+    const int32_t *rows = m != r ? &one : nullptr;
+    int rc = check_iq3s_product(n, blocks, MAMBO_DTYPE_F32);
+    if (rc == MAMBO_OK)
+        rc = check_expert_rows(m, rows, r, &one, experts);
+    if (rc != MAMBO_OK)
+        return rc;
+    MAMBO_REQUIRE(ldxv >= 256 * blocks && ldxs >= 8 * blocks && plan && r >= 1, MAMBO_ERR_VALUE, "a plan is of one row or more");
+    const Iq3sChoice c = iq3s_choose({&one, rows, r, m, (int)experts}, n, blocks, ldxv, ldxs);
+    MAMBO_REQUIRE(c.wide || grid_takes(expert_row_tiles(r, experts, c.tokens) * ((n + 31) / 32), 64 * c.waves), MAMBO_ERR_VALUE,
+                  "too many rows and columns for one launch");
+    plan[0] = c.wide ? 32 * c.plan.mt : c.tokens;
+    plan[1] = c.wide ? 32 * c.plan.waves : 32;
+    plan[2] = c.wide ? c.plan.kg : c.waves;
+    return MAMBO_OK;
+}
 
 extern "C" int mambo_iq3s_fp8_matmul_experts(const uint8_t *xv, int64_t ldxv, const uint8_t *xs, int64_t ldxs, int64_t m,
                                              const int32_t *rows, int64_t r, const int32_t *offsets, int64_t experts,
                                              const uint8_t *packed, int64_t expert_stride, int64_t n, int64_t blocks,
                                              void *out, int out_dtype, int64_t ldo, mambo_stream_t stream)
 {
-    const int rc = check_expert_rows(m, rows, r, offsets, experts);
+    int rc = check_expert_rows(m, rows, r, offsets, experts);
+    if (rc == MAMBO_OK)
+        rc = check_iq3s_product(n, blocks, out_dtype);
     if (rc != MAMBO_OK)
         return rc;
-    MAMBO_REQUIRE(out_dtype == MAMBO_DTYPE_F32 || out_dtype == MAMBO_DTYPE_BF16, MAMBO_ERR_VALUE,
-                  "outputs must be float32 or bfloat16");
-    MAMBO_REQUIRE(n >= 1 && n <= 0x7FFFFF00 && blocks >= 1 && blocks <= 2000000, MAMBO_ERR_VALUE,
-                  "weights must be [N,K/256] blocks with N, K >= 1 (got %lld and %lld)", (long long)n, (long long)blocks);
     MAMBO_REQUIRE(ldxv >= 256 * blocks && ldxs >= 8 * blocks && ldo >= n, MAMBO_ERR_VALUE,
                   "row strides must cover the rows");
     MAMBO_REQUIRE(expert_stride >= mambo_iq3s_packed_bytes(n, blocks) && expert_stride % 16 == 0, MAMBO_ERR_VALUE,
@@ -178,28 +243,12 @@ extern "C" int mambo_iq3s_fp8_matmul_experts(const uint8_t *xv, int64_t ldxv, co
     hipStream_t s = (hipStream_t)stream;
     const Iq3sArgs a = {xv, xs, ldxv, ldxs, er, packed, expert_stride, out, ldo, (int)n,
                         (int)blocks, (int)((n + 31) / 32), rows_take_vectors(out, ldo, out_dtype)};
-    // How the rows fall is not known here: experts with rows and tiles are counted for rows that fall at random.
-    const double taken = (double)experts * -std::expm1(-(double)r / (double)experts);
-    auto tiles = [&](int t) { return std::fmax(taken, (double)r / t + 0.5 * taken); };
-    // The 32 x 32 MFMA kernel from 14 rows of an expert on, where 16 tokens a tile fill the card four times: 64 experts of
-    // 2048 x 4096 with 12 rows each take it 75.4 us (the 16-token kernel 72.5), with 16 76.1 (94.6), 4 experts of 1024 x
-    // 4096 with 64 rows 24.8 (16.1). It tells rows by 32-bit offsets, and a grid takes 2^29 weight rows of it.
-    if ((double)r > 14.0 * taken && tiles(16) * a.ntiles >= 1024.0 && n < (1 << 29) &&
-        (rows ? m : 256) * ldxv + 256 * blocks < ((int64_t)1 << 32) && (rows ? m : 256) * ldxs + 8 * blocks < ((int64_t)1 << 32) && expert_row_tiles(r, experts, 64) <= 65535) {
-        double tiles_of[2] = {tiles(64), tiles(128)};
-        WidePlan plan;
-        mambo_wide_experts_plan(er, n, blocks, tiles_of, &plan);
-        return mambo_wide_experts_launch(plan, xv, ldxv, xs, ldxs, er, packed, expert_stride, n, blocks, out, bf16, ldo, s);
-    }
-    // 4 tokens a tile up to 2.5 rows of an expert: 64 experts of 2048 x 4096 with 2.3 rows take 43.4 us (16 tokens a tile
-    // 47.6), with 4 62.5 (50.8).
-    const bool diag = (double)r <= 2.5 * taken;
-    // Waves that share a workgroup's K, two blocks each at least: one where workgroups fill the card, more where they do
-    // not (8 x 14336 x 4096, 4 tokens a tile, 3136 workgroups: 40.0 us with one, 42.1 with two, 43.6 with four; 2 experts,
-    // 896: 16.1, 14.5, 14.9; 2 of 4096 x 14336, 256: 34.8, 21.1, 14.7).
-    const double expected = tiles(diag ? 4 : 16) * a.ntiles;
-    const int waves = expected >= 2560.0 || blocks < 4 ? 1 : expected >= 640.0 || blocks < 8 ? 2 : 4;
-    const int64_t wgs = expert_row_tiles(r, experts, diag ? 4 : 16) * a.ntiles;
+    const Iq3sChoice choice = iq3s_choose(er, n, blocks, ldxv, ldxs);
+    if (choice.wide)
+        return mambo_wide_experts_launch(choice.plan, xv, ldxv, xs, ldxs, er, packed, expert_stride, n, blocks, out, bf16, ldo, s);
+    const bool diag = choice.tokens == 4;
+    const int waves = choice.waves;
+    const int64_t wgs = expert_row_tiles(r, experts, choice.tokens) * a.ntiles;
     MAMBO_REQUIRE(grid_takes(wgs, 64 * waves), MAMBO_ERR_VALUE, "too many rows and columns for one launch");
 #define MAMBO_IQ3S(D, W, B)                                                                                            \
     if (diag == D && waves == W && bf16 == B)                                                                          \

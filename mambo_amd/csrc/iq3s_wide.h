@@ -22,10 +22,9 @@ bool mambo_wide_plan(int64_t m, const mambo_projection *proj, int count, int64_t
 int mambo_wide_launch(const WidePlan &plan, const uint8_t *xv, int64_t ldxv, const uint8_t *xs, int64_t ldxs, int64_t m,
                       const mambo_projection *proj, int count, int64_t blocks, hipStream_t stream);
 
-// Rows grouped by expert: the plan for the tiles of 64 and of 128 rows that are expected (tiles_of) and its time, and its
-// launch. The caller has checked the operands, that the offsets of all rows fit 32 bits where they are gathered, and that
+// Rows grouped by expert: the plan for the tiles of 64 and of 128 rows that are expected (tiles_of), and its launch. The caller has checked the operands, that the offsets of all rows fit 32 bits where they are gathered, and that
 // expert_row_tiles of 64 rows fit a grid's y.
-double mambo_wide_experts_plan(const ExpertRows &er, int64_t n, int64_t blocks, double tiles_of[2], WidePlan *plan);
+void mambo_wide_experts_plan(const ExpertRows &er, int64_t n, int64_t blocks, double tiles_of[2], WidePlan *plan);
 int mambo_wide_experts_launch(const WidePlan &plan, const uint8_t *xv, int64_t ldxv, const uint8_t *xs, int64_t ldxs,
                               const ExpertRows &er, const uint8_t *packed, int64_t expert_stride, int64_t n, int64_t blocks,
                               void *out, bool bf16, int64_t ldo, hipStream_t stream);

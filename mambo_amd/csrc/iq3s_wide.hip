@@ -644,7 +644,7 @@ int mambo_wide_launch(const WidePlan &p, const uint8_t *xv, int64_t ldxv, const 
 // tiles that rows falling to the experts at random take (fp8_plan counts them alike), and several K groups while that is
 // one workgroup a CU (8 experts of 4096 x 14336, 16 rows each, 82 -> 67 us, 64 rows 115 -> 99; beyond, 64 rows of 64 experts,
 // 2048 x 4096, 110 -> 131).
-double mambo_wide_experts_plan(const ExpertRows &er, int64_t n, int64_t blocks, double tiles_of[2], WidePlan *plan)
+void mambo_wide_experts_plan(const ExpertRows &er, int64_t n, int64_t blocks, double tiles_of[2], WidePlan *plan)
 {
     const double mb = 4e-6 * (double)er.r * (double)n;
     double best = 0.0;
@@ -658,7 +658,6 @@ double mambo_wide_experts_plan(const ExpertRows &er, int64_t n, int64_t blocks, 
             *plan = {w.mt, w.waves, w.kg, 1, (int)blocks, t};
         }
     }
-    return best;
 }
 
 template <int MT, int W, int KG>

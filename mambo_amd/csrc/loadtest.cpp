@@ -360,6 +360,7 @@ const std::vector<EntryDecl> &compiled_entries()
         MAMBO_ENTRY(mambo_fp8_block_plan, "m", "r", "experts", "n", "k", "ldxv", "out_dtype", "plan"),
         MAMBO_ENTRY(mambo_iq3s_fp8_matmul_experts, "xv", "ldxv", "xs", "ldxs", "m", "rows", "r", "offsets", "experts",
                     "packed", "expert_stride", "n", "blocks", "out", "out_dtype", "ldo", "stream"),
+        MAMBO_ENTRY(mambo_iq3s_experts_plan, "m", "r", "experts", "n", "blocks", "ldxv", "ldxs", "plan"),
         MAMBO_ENTRY(mambo_route_experts, "logits", "dtype", "ld", "m", "experts", "top_k", "renormalize", "ids",
                     "weights", "offsets", "rows", "slots", "stream"),
         MAMBO_ENTRY(mambo_combine_experts, "y", "y_dtype", "ldy", "r", "slots", "weights", "m", "top_k", "n", "out",
