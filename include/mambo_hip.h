@@ -288,12 +288,15 @@ int64_t mambo_gemm_config_enumerate(int64_t m, int64_t n, int64_t blocks, mambo_
  *   rows    i32[r]: the token of each row, ascending within an expert; -1 past offsets[experts]
  *   slots   i32[m, top_k]: the row of each choice; -1 where a token had none
  * A product holds what it reads of offsets and rows within [0, r] and [0, m), so that a plan with
- * other values gives wrong sums and no stray access. Rows past offsets[experts] come out as zeros. */
+ * other values gives wrong sums and no stray access. Rows past offsets[experts] come out as zeros.
+ * Sizes for which a launch would have 2^32 threads or more (HIP launches such a grid in part) are
+ * MAMBO_ERR_VALUE. Rows gathered out of 4 GiB and more, or so far apart that a tile spans it, and IQ3_S
+ * products of more than 65535 tiles of 64 rows, take kernels that read a weight once for 16 rows. */
 
 /* Block quantizer: x [m, k] f32 or bf16 (row stride ldx), k % 16 == 0, in groups of 128 along K (the
  * last may be shorter): f32 scales = max(amax / 448, 2^-100), row i's of group g at scales + i * lds +
- * g * gss, and values [m, ldv] = E4M3 of x / scale, computed as one division by amax and rounded
- * once to nearest even. A group that holds a NaN or an infinity gets the scale NaN and E4M3 NaN codes.
+ * g * gss, and values [m, ldv] = E4M3 of x / scale: 448 x / amax rounded to f32 (one division) and that
+ * to nearest even. A group that holds a NaN or an infinity gets the scale NaN and E4M3 NaN codes.
  * The products read scales of groups of rows (lds 1, gss >= m) faster than rows of groups (gss 1,
  * lds >= ceil(k/128)). m == 0: nothing to do. */
 int mambo_quantize_fp8_block(const void *x, int x_dtype, int64_t m, int64_t k, int64_t ldx, uint8_t *values,
@@ -311,7 +314,7 @@ int mambo_fp8_block_pack(const uint8_t *w, int64_t experts, int64_t n, int64_t k
  * xs[m, g] * ws[n / 128, g] * sum over the group of xv[m, k] * w[n, k], in f32, in an order that the
  * shape fixes (bf16 outputs by the FP8 MFMAs, which leave out up to 8.5e-4 of the largest of eight
  * consecutive products, f32 ones by the bf16 MFMAs, which add more exactly at half the rate). xv u8 [m, ldxv] E4M3, 16-byte aligned rows; xs f32, row i's of group g at xs + i * ldxs + g *
- * gsxs (rows or groups apart); packed from mambo_fp8_block_pack with one expert; ws f32 [ceil(n/128),
+ * gsxs (rows or groups apart; xs * ws is formed in f32 first, so it must not overflow); packed from mambo_fp8_block_pack with one expert; ws f32 [ceil(n/128),
  * ceil(k/128)] contiguous; k % 16 == 0, k <= 2^26. m == 0: nothing to do. */
 int mambo_fp8_block_matmul(const uint8_t *xv, int64_t ldxv, const float *xs, int64_t ldxs, int64_t gsxs,
                            int64_t m, const uint8_t *packed, const float *ws, int64_t n, int64_t k, void *out,

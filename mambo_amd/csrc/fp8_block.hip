@@ -375,8 +375,9 @@ __device__ __forceinline__ int slot_of(int row) { return (row ^ ((row >> 3) & 3)
 // weights are asked for as this one's last MFMAs have them, and a wave that multiplies goes before one that waits (2048 x 4096
 // x 14336 120.3 -> 118.1 us with both, 121.6 and 124.2 with either; 8192 x 14336 x 4096 417 -> 413). Bound by the matrix units
 // where the launch fills the chip (128 x 256 tiles, 8192 x 14336 x 4096: 413 us, 2.33 PFLOP/s, 60 to 64% of the MFMA cycles
-// busy; a library product with one scale takes 325), else by a step's own chain of LDS reads, MFMAs, scalings and a barrier,
-// and by what a CU can fetch, about 33 GB/s (203 x 5003 x 2832 12.6 us; 64 x 4096 x 14336, on 128 CUs, 25).
+// busy; a library product with one scale takes 325), else by a step's own chain of LDS reads, MFMAs, scalings and a barrier
+// (203 x 5003 x 2832 12.6 us; 64 x 4096 x 14336, on 128 CUs, 25: a CU fetches 43 and 55 GB/s there, and 53 where the launch
+// fills the chip).
 template <int MT, int NB, int WN, int KG, bool kExperts, bool kBf16>
 __global__ __launch_bounds__(WN * KG * 64) __attribute__((amdgpu_waves_per_eu(2))) void fp8_tile_kernel(Fp8Args a)
 {
@@ -617,7 +618,9 @@ struct Fp8Kernel {
     double launch, round, step[4], outputs, weights;
 };
 // Fitted to 355 products a dense table (1 to 8192 tokens, 300 to 57344 rows, K 272 to 28672, weights rotated past the caches)
-// and 174 by expert. The kernel that they pick takes 0.8% more than the fastest of the nine on average (f32 0.9%, by
+// and 174 by expert with bf16 outputs; float32 outputs by expert go by the dense table of theirs, and the kernel that it picks
+// takes 3% more than the fastest on average over 100 products (1 to 512 rows of each of 4 to 128 experts), most 58% (64 rows of
+// 8, 2880 x 2880). The kernel that they pick takes 0.8% more than the fastest of the nine on average (f32 0.9%, by
 // expert, where they do not know how the rows fall, 3.3%; measured again, with 66 more by expert, 1.0%, 1.0% and 3.7%). None
 // of the nine is spare: without it the fastest of the others takes 0.2 to 3% more on average and up to 1.11 to 1.63 times.
 // Measured beside them: 128 x 128 tiles, 64 x 64 of eight K groups, 64 x 128 and 64 x 64 of one and two (no gain of 0.5%);
@@ -681,7 +684,9 @@ int64_t order_tiles(Fp8Args *a, int tokens, int64_t tiles, int64_t columns, doub
         deal = cdiv(total, 8);
     } else if (total >= 768 && reuse >= (columns % 8 ? 2.0 / 3.0 : 4.0)) {
         // 32 neighbours at a time, for which row tiles there are is not known: an eighth at a time, the last XCD would have
-        // the tiles of no rows. Where the columns are a multiple of eight, an XCD has columns of its own in turn too, and
+        // the tiles of no rows. From 768 workgroups on, 24 deals, three an XCD: fewer fall too unevenly (48 rows of 16, 2880 x
+        // 2880, 348 workgroups, 30 -> 48 us; 96 of 8, 7000 x 4096, 588, 73 -> 83), though some would gain (192 of 32, 600 x 5120,
+        // 645, 80 -> 56). Where the columns are a multiple of eight, an XCD has columns of its own in turn too, and
         // gains with many row tiles alone (65536 rows of 64 experts, 2048 x 4096 596 -> 569 us, 16384 188 -> 190, 4096 rows of
         // 16, 4096 x 4096 74 -> 77); else 8192 of 32, 600 x 5120 89 -> 62, 16384 of 128, 1536 x 2048 129 -> 119, 12000 111 ->
         // 100 (but 4096 of 32, 2880 x 2880 86 -> 97).

@@ -23,7 +23,7 @@ def launch_quantize_fp8_block(x: torch.Tensor, *, stream=None, out: tuple[torch.
 
     ``x`` is float32 or bfloat16 [M,K] on the GPU, K a multiple of 16, M >= 0. A group of 128 along K
     (the last may be shorter) has the scale max(amax / 448, 2^-100) and the codes of x / scale,
-    rounded once to nearest even; a group that holds a NaN or an infinity becomes NaN. Row-strided
+    which is 448 x / amax in float32, rounded to nearest even; a group that holds a NaN or an infinity becomes NaN. Row-strided
     inputs are read in place. The scales are laid out group by group (strides (1, M)); ``out``
     optionally supplies codes with unit column stride and scales of either order.
     """

@@ -32,7 +32,8 @@ from mambo_amd.utils.iq3_s_weight import IQ3SExperts, prepare_iq3_s_experts
 
 
 def silu_mul(h: torch.Tensor) -> torch.Tensor:
-    """silu of the first half of each row times the second, in the rows' type."""
+    """silu of the first half of each row times the second, each rounded to the rows' type: of bfloat16
+    2^-8, beside the 2^-4 of the 8-bit codes that the next product makes of it."""
     gate, up = h.chunk(2, dim=1)
     return torch.nn.functional.silu(gate) * up
 
@@ -52,7 +53,9 @@ class ExpertLayer:
     renormalize: bool = True
 
     def __call__(self, x: torch.Tensor) -> torch.Tensor:
-        """The layer's output [M, H] of bfloat16 rows x [M, H]."""
+        """The layer's output [M, H] of bfloat16 rows x [M, H]. The joined rows and the shared MLP's are rounded to
+        bfloat16 each and then added (2^-8 of either; float32 ones would be read and written at twice
+        the bytes)."""
         dtype = torch.bfloat16
         if x.shape[0] == 0:  # launch_quantize_fp8 takes one row and more
             return torch.empty((0, self.down.n), dtype=dtype, device=x.device)
