@@ -249,3 +249,61 @@ def test_quantizer_of_many_rows(gpu, m, k, dtype, aligned):
     assert torch.equal(buffer[:m, left:left + k], codes) and torch.equal(by_row[:m, 1:-1], scales)
     assert (buffer[m] == 9).all() and (buffer[:, :left] == 9).all() and (buffer[:, left + k:] == 9).all()
     assert (by_row[m] == 7).all() and (by_row[:, 0] == 7).all() and (by_row[:, -1] == 7).all()
+
+
+# ------------------------------------------------------------------------------ many rows
+@pytest.mark.gpu
+@pytest.mark.parametrize("m,top_k,n", [(65536, 3, 5), (70001, 2, 520), (131073, 1, 64)])
+def test_combine_of_many_tokens(gpu, m, top_k, n):
+    """More tokens than a grid's second dimension; weights of powers of two and small integers: exact."""
+    from mambo_amd.kernels.experts import launch_combine_experts
+    gen = torch.Generator(device=gpu).manual_seed(m)
+    y = torch.randint(-64, 65, (m * top_k, n), generator=gen, device=gpu).to(torch.bfloat16)
+    slots = torch.randperm(m * top_k, generator=gen, device=gpu).to(torch.int32).view(m, top_k)
+    slots = slots.masked_fill(torch.rand((m, top_k), generator=gen, device=gpu) < 0.2, -1)
+    weights = torch.exp2(torch.randint(-2, 3, (m, top_k), generator=gen, device=gpu).float())
+    expected = torch.zeros((m, n), device=gpu)
+    for j in range(top_k):
+        some = slots[:, j] >= 0
+        expected[some] += weights[some, j, None] * y[slots[some, j].long()].float()
+    assert torch.equal(launch_combine_experts(y, slots, weights, out_dtype=torch.float32), expected)
+    assert torch.equal(launch_combine_experts(y, slots, weights), expected.to(torch.bfloat16))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("out_dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("weight", ["fp8", "iq3s"])
+def test_products_of_many_rows(gpu, weight, out_dtype):
+    """4.2 million rows of 700 tokens, more tiles of 64 than a grid's second dimension: each is the product of its token
+    with its expert, as those 700 rows give it alone."""
+    from mambo_amd.kernels.experts import launch_fp8_block_matmul_experts, launch_iq3_s_fp8_matmul_experts
+    from mambo_amd.kernels.quantize_fp8 import launch_quantize_fp8
+    from mambo_amd.utils.fp8_block_weight import prepare_fp8_block_weight
+    from mambo_amd.utils.iq3_s_weight import prepare_iq3_s_experts
+    rng = np.random.default_rng(3)
+    r, m, n, k, experts = 64 * 65535 + 77, 700, 70, 256, 3
+    offsets = torch.tensor([0, 1, r // 2, r - 1000], dtype=torch.int32, device=gpu)
+    rows = torch.from_numpy(rng.integers(0, m, size=r).astype(np.int32)).to(gpu)
+    if weight == "fp8":  # integers: the same in any order
+        call = launch_fp8_block_matmul_experts
+        values, wv = (torch.from_numpy(ref.integer_codes(rng, s)).to(gpu) for s in ((m, k), (experts, n, k)))
+        scales = torch.ones((m, 2), device=gpu)
+        w = prepare_fp8_block_weight(wv, torch.ones((experts, 1, 2), device=gpu))
+        tolerance = 0.0
+    else:  # float32 sums in another order: as test_gpu_experts.test_iq3s_experts
+        call = launch_iq3_s_fp8_matmul_experts
+        raw = rng.integers(0, 256, size=(experts, n, 1, 110), dtype=np.uint8)
+        raw[..., :2] = np.array([0.01], dtype=np.float16).view(np.uint8)
+        w = prepare_iq3_s_experts(torch.from_numpy(raw).to(gpu))
+        values, scales = launch_quantize_fp8(torch.randn((m, k), device=gpu))
+        tolerance = 1e-4 if out_dtype == torch.float32 else 2.0**-8
+    out = call(values, scales, w, offsets, rows=rows, out_dtype=out_dtype)
+    assert not bool(out[r - 1000:].any())
+    starts = offsets.tolist()
+    for e in range(experts):
+        alone = torch.zeros(experts + 1, dtype=torch.int32, device=gpu)
+        alone[e + 1:] = m
+        expected = call(values, scales, w, alone, out_dtype=out_dtype).float()
+        a, b = starts[e], starts[e + 1]
+        off = (out[a:b].float() - expected[rows[a:b].long()]).norm(dim=1)
+        assert bool((off <= tolerance * expected.norm(dim=1)[rows[a:b].long()]).all()), e
