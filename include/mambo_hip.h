@@ -367,6 +367,109 @@ int mambo_combine_experts(const void *y, int y_dtype, int64_t ldy, int64_t r, co
                           const float *weights, int64_t m, int64_t top_k, int64_t n, void *out, int out_dtype,
                           int64_t ldo, mambo_stream_t stream);
 
+/* ----------------------------------------------- rotary positions, paged 8-bit cache, attention
+ * No reference counterpart: what a layer does between its q/k/v and o projections. The cache holds
+ * keys and values as E4M3 codes in blocks of 32 tokens of one head, with a power of two for the
+ * keys and one for the values of each block. No call reads a size back. */
+#define MAMBO_KV_BLOCK 32
+#define MAMBO_KV_MAX_DIM 256
+#define MAMBO_ROTARY_MAX_DIM 1024
+
+/* Angles of rotary positions: pair i of a head turns by turns[i] / 2^64 of a turn a position. The
+ * first `size` (even) values of a head are rotated, in pairs (i, i + size/2), or (2i, 2i + 1) where
+ * interleaved != 0, and multiplied by magnitude; the others are copied. */
+typedef struct mambo_rotary_table {
+    const uint64_t *turns; /* u64[size / 2] */
+    int32_t size;
+    int32_t interleaved;
+    double magnitude;
+} mambo_rotary_table;
+
+/* The cache: codes u8 [pages, heads, page_size/32, 2 * 32 * D] (D: head_dim rounded up to 32; keys, then
+ * values, in a private order: mambo_amd/csrc/kv_cache.h) and scales u8 [pages, heads, page_size/32, 2]
+ * (E8M0 of the keys and of the values). head_dim is a multiple of 8 up to MAMBO_KV_MAX_DIM, page_size a
+ * power of two from 32 to 65536. codes is 16-byte aligned, scales 2-byte aligned. */
+typedef struct mambo_kv_cache {
+    uint8_t *codes;
+    uint8_t *scales;
+    int64_t pages;
+    int32_t heads;
+    int32_t head_dim;
+    int32_t page_size;
+    int32_t reserved;
+} mambo_kv_cache;
+
+/* The sequences of a call: sequence s has the rows [offsets[s], offsets[s+1]) of the call's `tokens`
+ * (offsets NULL: tokens / seqs rows each), the last of them at position lengths[s] - 1, and its page
+ * c (tokens [c * page_size, ...)) is tables[s * ldt + c], c < width. The kernels hold offsets within
+ * [0, tokens] and lengths within [0, width * page_size]; a page outside [0, pages) is none: nothing is
+ * stored there and its tokens are left out of attention. */
+typedef struct mambo_kv_batch {
+    const int32_t *tables;
+    int64_t ldt;
+    int64_t width;
+    const int32_t *lengths; /* i32[seqs], the call's own tokens included */
+    const int32_t *offsets; /* i32[seqs + 1] or NULL */
+    int64_t seqs;
+} mambo_kv_batch;
+
+/* out[t, h] = x[t, h] (f32 or bf16, strides ldt and ldh, `dim` values next to each other) rotated by
+ * positions[t], computed in f32 and rounded once to out's type. out may be x itself (same strides and
+ * type), and must not overlap it otherwise. dim <= MAMBO_ROTARY_MAX_DIM. tokens == 0: nothing to do. */
+int mambo_rotary(const void *x, int x_dtype, int64_t tokens, int64_t heads, int64_t dim, int64_t ldt, int64_t ldh,
+                 const int32_t *positions, const mambo_rotary_table *table, void *out, int out_dtype, int64_t ldot,
+                 int64_t ldoh, mambo_stream_t stream);
+
+/* Bytes of a cache's codes (its scales take 2 for each 2 * 32 * D of them); 0 where the sizes are refused. */
+int64_t mambo_kv_cache_bytes(int64_t pages, int64_t heads, int64_t head_dim, int64_t page_size);
+
+/* Rows that mambo_kv_append takes: f32 or bf16 (dtype), `tokens` of them, [tokens, heads, head_dim] with strides ld*t and
+ * ld*h in elements. q NULL: none; else q_heads heads of queries, rotated into q_out (bf16). */
+typedef struct mambo_kv_rows {
+    const void *k, *v, *q;
+    int64_t ldkt, ldkh, ldvt, ldvh, ldqt, ldqh;
+    void *q_out;
+    int64_t ldot, ldoh;
+    int64_t q_heads;
+    int32_t dtype;
+    int32_t reserved;
+} mambo_kv_rows;
+
+/* Stores the call's tokens in the cache, the keys rotated (table NULL: as they are) by positions[t] (NULL:
+ * by the position in the sequence). A block that is entered at its first token starts anew, one entered
+ * later keeps its older tokens: its exponent is the larger of the old and e = max(ceil(log2(amax / 448)),
+ * -100) of the new rows, and where it grows, the older codes are rounded again to it. A token with a key or value
+ * of a head that is not finite is held as NaN keys and zero values of that head and counts for no exponent. A row whose
+ * position in its sequence is negative is not stored (its queries are rotated). Sequences of a call
+ * must not share a block that one of them writes. */
+int mambo_kv_append(const mambo_kv_rows *rows, int64_t tokens, const mambo_kv_cache *cache, const mambo_kv_batch *batch,
+                    const mambo_rotary_table *table, const int32_t *positions, mambo_stream_t stream);
+
+/* The values that cached tokens stand for: k, v bf16 [n, heads, head_dim] contiguous, row i of position
+ * positions[i] of sequence sequences[i] (batch: tables and seqs; lengths and offsets are not read). Zeros
+ * where there is no such sequence or page. heads and dim are the cache's. */
+int mambo_kv_read(const mambo_kv_cache *cache, const mambo_kv_batch *batch, const int32_t *sequences,
+                  const int32_t *positions, int64_t n, int64_t heads, int64_t dim, void *k, void *v, mambo_stream_t stream);
+
+/* out[t, h] = sum_j p_j v_j over the cached tokens j < lengths[s] of the row's sequence s, p the softmax
+ * of scale * (q[t, h] . k_j), of the key/value head h / (q_heads / heads). causal != 0: j up to the row's own position
+ * only; window > 0 (causal only): no more than the last `window` of them. A row that sees no token
+ * becomes zeros with lse -inf. q and out bf16 [tokens, q_heads, dim] (dim: the cache's) (strides ld*t, ld*h), q's rows 16-byte
+ * aligned; lse f32 [tokens, q_heads] contiguous, the natural logarithm of the sum of exp(scores),
+ * or NULL. Sums are f32; the probabilities are rounded to bf16 for the product with the values.
+ * workspace: mambo_kv_attention_workspace bytes, 16-byte aligned, that no call running at the same time uses.
+ * Rows that no sequence has are not written. The results do not vary from run to run. */
+int64_t mambo_kv_attention_workspace(const mambo_kv_cache *cache, const mambo_kv_batch *batch, int64_t tokens, int64_t q_heads);
+int mambo_kv_attention(const void *q, int64_t tokens, int64_t q_heads, int64_t dim, int64_t ldqt, int64_t ldqh, const mambo_kv_cache *cache,
+                       const mambo_kv_batch *batch, float scale, int causal, int64_t window, void *out, int64_t ldot,
+                       int64_t ldoh, float *lse, void *workspace, int64_t workspace_bytes, mambo_stream_t stream);
+
+/* How such a call is launched, on the host alone: plan[4] = rows (queries x heads of a key/value head) up to
+ * which a sequence takes the kernel for few rows (0: it is not launched), its workgroups for each head,
+ * rows of a workgroup of the kernel for many (0: not launched) and the parts of its keys. */
+int mambo_kv_attention_plan(const mambo_kv_cache *cache, const mambo_kv_batch *batch, int64_t tokens, int64_t q_heads,
+                            int32_t *plan);
+
 /* Synthetic inputs for benchmarks and full-size checks (no reference counterpart; the
  * reference draws them with numpy/cupy RNGs, test_iq3_s_fp8.py:41-51). Counter-based:
  *   rnd(seed, stream, i) = splitmix64(splitmix64(seed*0xD1B54A32D192ED03 + stream) + i);

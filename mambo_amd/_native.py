@@ -89,8 +89,41 @@ class ChainConfig(ctypes.Structure):
                 ("wait_bias", ctypes.c_int32), ("reserved", ctypes.c_int32 * 3)]
 
 
+class RotaryTableArgs(ctypes.Structure):
+    """mirror of mambo_rotary_table"""
+
+    _fields_ = [("turns", ctypes.c_void_p), ("size", ctypes.c_int32), ("interleaved", ctypes.c_int32),
+                ("magnitude", ctypes.c_double)]
+
+
+class KVCacheArgs(ctypes.Structure):
+    """mirror of mambo_kv_cache"""
+
+    _fields_ = [("codes", ctypes.c_void_p), ("scales", ctypes.c_void_p), ("pages", ctypes.c_int64),
+                ("heads", ctypes.c_int32), ("head_dim", ctypes.c_int32), ("page_size", ctypes.c_int32),
+                ("reserved", ctypes.c_int32)]
+
+
+class KVBatchArgs(ctypes.Structure):
+    """mirror of mambo_kv_batch"""
+
+    _fields_ = [("tables", ctypes.c_void_p), ("ldt", ctypes.c_int64), ("width", ctypes.c_int64),
+                ("lengths", ctypes.c_void_p), ("offsets", ctypes.c_void_p), ("seqs", ctypes.c_int64)]
+
+
+class KVRowsArgs(ctypes.Structure):
+    """mirror of mambo_kv_rows"""
+
+    _fields_ = [("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("q", ctypes.c_void_p),
+                ("ldkt", ctypes.c_int64), ("ldkh", ctypes.c_int64), ("ldvt", ctypes.c_int64), ("ldvh", ctypes.c_int64),
+                ("ldqt", ctypes.c_int64), ("ldqh", ctypes.c_int64), ("q_out", ctypes.c_void_p),
+                ("ldot", ctypes.c_int64), ("ldoh", ctypes.c_int64), ("q_heads", ctypes.c_int64),
+                ("dtype", ctypes.c_int32), ("reserved", ctypes.c_int32)]
+
+
 # name -> (restype, argtypes); every symbol here is declared in include/mambo_hip.h.
 _vp, _i64, _i32, _u64 = ctypes.c_void_p, ctypes.c_int64, ctypes.c_int, ctypes.c_uint64
+_table, _cache, _batch = (ctypes.POINTER(t) for t in (RotaryTableArgs, KVCacheArgs, KVBatchArgs))
 SIGNATURES = {
     "mambo_last_error": (ctypes.c_char_p, []),
     "mambo_abi_version": (_i32, []),
@@ -132,6 +165,14 @@ SIGNATURES = {
     "mambo_iq3s_experts_plan": (_i32, [_i64, _i64, _i64, _i64, _i64, _i64, _i64, _vp]),
     "mambo_route_experts": (_i32, [_vp, _i32, _i64, _i64, _i64, _i64, _i32, _vp, _vp, _vp, _vp, _vp, _vp]),
     "mambo_combine_experts": (_i32, [_vp, _i32, _i64, _i64, _vp, _vp, _i64, _i64, _i64, _vp, _i32, _i64, _vp]),
+    "mambo_rotary": (_i32, [_vp, _i32, _i64, _i64, _i64, _i64, _i64, _vp, _table, _vp, _i32, _i64, _i64, _vp]),
+    "mambo_kv_cache_bytes": (_i64, [_i64, _i64, _i64, _i64]),
+    "mambo_kv_append": (_i32, [ctypes.POINTER(KVRowsArgs), _i64, _cache, _batch, _table, _vp, _vp]),
+    "mambo_kv_read": (_i32, [_cache, _batch, _vp, _vp, _i64, _i64, _i64, _vp, _vp, _vp]),
+    "mambo_kv_attention_workspace": (_i64, [_cache, _batch, _i64, _i64]),
+    "mambo_kv_attention": (_i32, [_vp, _i64, _i64, _i64, _i64, _i64, _cache, _batch, ctypes.c_float, _i32, _i64, _vp, _i64, _i64, _vp,
+                                  _vp, _i64, _vp]),
+    "mambo_kv_attention_plan": (_i32, [_cache, _batch, _i64, _i64, _vp]),
     "mambo_synth_iq3s": (_i32, [_u64, _i64, _i64, _i64, _vp, _vp]),
     "mambo_synth_bf16": (_i32, [_u64, _u64, ctypes.c_double, _i64, _i64, _vp, _vp]),
     "mambo_e4m3_convert": (_i32, [_vp, _i64, _vp, _vp, _vp]),

@@ -47,6 +47,8 @@ _SCALARS = {
     "float": "float32", "double": "float64", "mambo_gemm_config": "mambo_gemm_config",
     "mambo_projection": "mambo_projection", "mambo_stream_t": "hipStream_t",
     "mambo_chain_launch": "mambo_chain_launch", "mambo_chain_config": "mambo_chain_config",
+    "mambo_rotary_table": "mambo_rotary_table", "mambo_kv_cache": "mambo_kv_cache", "mambo_kv_batch": "mambo_kv_batch",
+    "mambo_kv_rows": "mambo_kv_rows",
 }
 
 
@@ -109,6 +111,10 @@ _FIELDS_IN = [
 
 def _fields_out(nullable: bool):
     return [dict(c, nullable=nullable, access="write") for c in _FIELDS_IN]
+
+
+_CACHE = _arr("cache", "mambo_kv_cache", ["1"], align=8, memory="host")
+_BATCH = _arr("batch", "mambo_kv_batch", ["1"], align=8, memory="host")
 
 
 # Every pointer parameter of every entry point: what the header's prose states.
@@ -227,6 +233,32 @@ CONSTRAINTS: dict[str, list[dict]] = {
         _arr("weights", "float32", ["m", "top_k"], align=4),
         _arr("out", "float32|bfloat16", ["m", "n"], ["ldo", "1"], align=2, access="write"),
     ],
+    "mambo_rotary": [
+        _arr("x", "float32|bfloat16", ["tokens", "heads", "dim"], ["ldt", "ldh", "1"], align=2),
+        _arr("positions", "int32", ["tokens"], align=4),
+        _arr("table", "mambo_rotary_table", ["1"], align=8, memory="host"),
+        _arr("out", "float32|bfloat16", ["tokens", "heads", "dim"], ["ldot", "ldoh", "1"], align=2, access="write"),
+    ],
+    "mambo_kv_cache_bytes": [],
+    "mambo_kv_append": [
+        _arr("rows", "mambo_kv_rows", ["1"], align=8, memory="host"), _CACHE, _BATCH,
+        _arr("table", "mambo_rotary_table", ["1"], align=8, memory="host", nullable=True),
+        _arr("positions", "int32", ["tokens"], align=4, nullable=True),
+    ],
+    "mambo_kv_read": [
+        _CACHE, _BATCH, _arr("sequences", "int32", ["n"], align=4), _arr("positions", "int32", ["n"], align=4),
+        _arr("k", "bfloat16", ["n", "heads", "dim"], align=16, access="write"),
+        _arr("v", "bfloat16", ["n", "heads", "dim"], align=16, access="write"),
+    ],
+    "mambo_kv_attention_workspace": [_CACHE, _BATCH],
+    "mambo_kv_attention": [
+        _arr("q", "bfloat16", ["tokens", "q_heads", "dim"], ["ldqt", "ldqh", "1"], align=16),
+        _CACHE, _BATCH,
+        _arr("out", "bfloat16", ["tokens", "q_heads", "dim"], ["ldot", "ldoh", "1"], align=2, access="write"),
+        _arr("lse", "float32", ["tokens", "q_heads"], align=4, nullable=True, access="write"),
+        _arr("workspace", "uint8", ["workspace_bytes"], align=16, access="readwrite"),
+    ],
+    "mambo_kv_attention_plan": [_CACHE, _BATCH, _arr("plan", "int32", ["4"], align=4, memory="host", access="write")],
     "mambo_synth_iq3s": [_arr("raw", "uint8", ["nrows", "blocks", "110"], access="write")],
     "mambo_synth_bf16": [_arr("out", "uint16", ["count"], align=2, access="write")],
     "mambo_e4m3_convert": [

@@ -1,0 +1,83 @@
+// Attention over the paged 8-bit cache: what its two kernels and the joins share.
+#pragma once
+#include "kv_cache.h"
+
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+
+struct Attention {
+    const __bf16 *q;
+    int64_t ldqt, ldqh;
+    KvCache cache;
+    KvBatch b;
+    int group; // query heads of a key/value head
+    float scale; // of the scores, times log2(e): softmax in powers of two
+    int causal, window;
+    __bf16 *out;
+    int64_t ldot, ldoh;
+    float *lse;
+    int few_rows; // sequences of up to so many rows (queries x group) are attend_rows' work, others attend_tiles'
+    int slots;    // attend_rows: workgroups of a head
+    int parts, tiles_each; // attend_tiles: parts of the keys; tiles of a sequence of a uniform batch
+    float *rows_o, *rows_ml; // partial sums, their largest scores and totals
+    int32_t *begins;         // first block of each sequence in the row kernel's order, and the total
+    float *tiles_o, *tiles_ml;
+};
+
+// A sequence's rows [first, first + n) and the blocks [lo, hi) of its keys that any of them sees.
+struct Sequence {
+    int first, n, len, lo, hi;
+};
+
+__device__ __forceinline__ Sequence sequence(const Attention &a, int s)
+{
+    Sequence q;
+    q.first = a.b.offset(s);
+    q.n = max(0, (a.b.offsets ? a.b.offset(s + 1) : q.first + a.b.each) - q.first);
+    q.len = a.b.length(s);
+    q.lo = a.window ? max(0, q.len - q.n + 1 - a.window) / kKvBlock : 0;
+    q.hi = (q.len + kKvBlock - 1) / kKvBlock;
+    return q;
+}
+
+// What row (query i of n) sees: keys in [from, to).
+__device__ __forceinline__ int sees_to(const Attention &a, const Sequence &q, int i)
+{
+    return a.causal ? q.len - q.n + i + 1 : q.len;
+}
+__device__ __forceinline__ int sees_from(const Attention &a, const Sequence &q, int i)
+{
+    return a.window ? q.len - q.n + i + 1 - a.window : 0;
+}
+
+// Eight E4M3 codes times a power of two as bf16, which holds them exactly (4 of its 8 bits).
+__device__ __forceinline__ bf16x8 widen(uint32_t lo, uint32_t hi, float scale)
+{
+    const bf16x2 a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, scale, false);
+    const bf16x2 b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, scale, true);
+    const bf16x2 c = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, scale, false);
+    const bf16x2 d = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, scale, true);
+    return bf16x8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
+}
+
+// 2^(byte - 127) of an E8M0 byte; the append makes bytes of 27 to 247.
+__device__ __forceinline__ float e8m0(uint32_t byte) { return __uint_as_float(byte << 23); }
+
+__device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
+
+// Codes past the first `left` (of eight) become zeros: what a page holds behind a sequence's last token is
+// anything, and a NaN there times a probability of zero would still be one.
+__device__ __forceinline__ uint2 keep_tokens(uint32_t lo, uint32_t hi, int left)
+{
+    const uint64_t mask = left >= 8 ? ~0ull : left <= 0 ? 0ull : (1ull << (8 * left)) - 1;
+    return make_uint2(lo & (uint32_t)mask, hi & (uint32_t)(mask >> 32));
+}
+
+// Most rows that attend_rows takes: 16 a tile, as many tiles as the registers and the LDS of its join hold.
+constexpr int max_row_tiles(int padded) { return padded <= 64 ? 4 : padded <= 128 ? 2 : 1; }
+constexpr int kTileRowsWg = 256; // rows of a workgroup of attend_tiles
+
+int launch_attend_rows(const Attention &a, int row_tiles, hipStream_t s);
+int launch_attend_tiles(const Attention &a, int64_t tiles, hipStream_t s);

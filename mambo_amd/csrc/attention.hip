@@ -1,0 +1,140 @@
+// Attention over the paged 8-bit cache: which kernels a call takes, its workspace, and the entry points.
+#include <algorithm>
+#include <math.h>
+
+#include "attention.h"
+
+namespace {
+
+int64_t cdiv(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+struct Plan {
+    int few_rows = 0, row_tiles = 0, slots = 0; // the kernel for few rows, 0: not launched
+    int64_t tiles = 0;                          // the kernel for many, tiles of a head; 0: not launched
+    int tiles_each = 1, parts = 1;
+    int64_t rows_entries = 0, tiles_entries = 0, bytes = 0;
+};
+
+constexpr int kCus = 256;
+
+int64_t aligned(int64_t bytes) { return (bytes + 15) & ~(int64_t)15; }
+
+Plan make_plan(const KvCache &c, const KvBatch &b, int group)
+{
+    Plan p;
+    const int padded = kv_padded(c.dim);
+    const int most = 16 * max_row_tiles(padded);
+    const int64_t rows = (int64_t)(b.offsets ? b.tokens : b.each) * group; // of one sequence, at most
+    const auto tiles_for = [](int64_t r) { return r <= 16 ? 1 : r <= 32 ? 2 : 4; };
+    if (rows <= most)
+        p.row_tiles = tiles_for(rows);
+    else if (b.offsets && group <= most) // prompts and single tokens in one call: each has its kernel
+        p.row_tiles = tiles_for(group);
+    if (p.row_tiles) {
+        p.few_rows = 16 * p.row_tiles;
+        // two workgroups a CU, fewer where there is no work for them
+        const int64_t blocks = (int64_t)b.seqs * (b.capacity / kKvBlock);
+        p.slots = (int)std::max<int64_t>(1, std::min<int64_t>(2 * kCus / c.heads, cdiv(blocks, 4)));
+        p.rows_entries = (int64_t)c.heads * p.slots * 2 * p.few_rows;
+    }
+    if (rows > most) {
+        p.tiles_each = (int)cdiv(rows, kTileRowsWg);
+        p.tiles = b.offsets ? (int64_t)b.tokens * group / kTileRowsWg + b.seqs : (int64_t)b.seqs * p.tiles_each;
+        // a workgroup a CU
+        p.parts = (int)std::max<int64_t>(1, std::min<int64_t>(kCus / (p.tiles * c.heads), cdiv(b.capacity, 512)));
+        if (p.parts > 1)
+            p.tiles_entries = (int64_t)p.parts * b.tokens * group * c.heads;
+    }
+    p.bytes = aligned(p.rows_entries * (padded + 2) * 4) + aligned(((int64_t)b.seqs + 1) * 4) +
+              aligned(p.tiles_entries * (padded + 2) * 4);
+    return p;
+}
+
+int check(const mambo_kv_cache *cache, const mambo_kv_batch *batch, int64_t tokens, int64_t q_heads, KvCache *c, KvBatch *b, Plan *p)
+{
+    if (const int rc = kv_check_cache(cache, c))
+        return rc;
+    if (const int rc = kv_check_batch(batch, tokens, cache, b))
+        return rc;
+    MAMBO_REQUIRE(q_heads >= c->heads && q_heads % c->heads == 0 && q_heads <= 65535, MAMBO_ERR_VALUE,
+                  "%lld query heads are no multiple of %d", (long long)q_heads, c->heads);
+    MAMBO_REQUIRE(tokens * q_heads <= 0x7FFFFFFF, MAMBO_ERR_VALUE, "tokens times query heads must be below 2^31 (got %lld)",
+                  (long long)tokens);
+    MAMBO_REQUIRE(batch->seqs * (int64_t)(b->capacity / kKvBlock) <= 0x7FFFFFFF, MAMBO_ERR_VALUE,
+                  "tables must hold below 2^36 tokens together");
+    *p = make_plan(*c, *b, (int)(q_heads / c->heads));
+    const int64_t rows = p->few_rows, heads = c->heads;
+    MAMBO_REQUIRE(grid_takes(batch->seqs * heads, 256) && rows <= 65535 && grid_takes(p->tiles * heads, 512) &&
+                      grid_takes(tokens * q_heads, 256),
+                  MAMBO_ERR_VALUE, "too many rows for one launch");
+    return MAMBO_OK;
+}
+
+} // namespace
+
+extern "C" int64_t mambo_kv_attention_workspace(const mambo_kv_cache *cache, const mambo_kv_batch *batch, int64_t tokens,
+                                                int64_t q_heads)
+{
+    KvCache c;
+    KvBatch b;
+    Plan p;
+    if (const int rc = check(cache, batch, tokens, q_heads, &c, &b, &p))
+        return rc;
+    return p.bytes;
+}
+
+extern "C" int mambo_kv_attention_plan(const mambo_kv_cache *cache, const mambo_kv_batch *batch, int64_t tokens,
+                                       int64_t q_heads, int32_t *plan)
+{
+    KvCache c;
+    KvBatch b;
+    Plan p;
+    if (const int rc = check(cache, batch, tokens, q_heads, &c, &b, &p))
+        return rc;
+    MAMBO_REQUIRE(plan != nullptr, MAMBO_ERR_VALUE, "null pointer");
+    plan[0] = p.few_rows;
+    plan[1] = p.slots;
+    plan[2] = p.tiles ? kTileRowsWg : 0;
+    plan[3] = p.parts;
+    return MAMBO_OK;
+}
+
+extern "C" int mambo_kv_attention(const void *q, int64_t tokens, int64_t q_heads, int64_t dim, int64_t ldqt, int64_t ldqh,
+                                  const mambo_kv_cache *cache,
+                                  const mambo_kv_batch *batch, float scale, int causal, int64_t window, void *out,
+                                  int64_t ldot, int64_t ldoh, float *lse, void *workspace, int64_t workspace_bytes,
+                                  mambo_stream_t stream)
+{
+    Attention a;
+    Plan p;
+    if (const int rc = check(cache, batch, tokens, q_heads, &a.cache, &a.b, &p))
+        return rc;
+    MAMBO_REQUIRE(dim == a.cache.dim, MAMBO_ERR_VALUE, "the cache has heads of %d (got %lld)", a.cache.dim, (long long)dim);
+    MAMBO_REQUIRE(scale > 0.0f && isfinite(scale), MAMBO_ERR_VALUE, "the scale of the scores must be positive and finite");
+    MAMBO_REQUIRE(window >= 0 && (window == 0 || causal), MAMBO_ERR_VALUE, "a window is positive, and of causal attention");
+    if (tokens == 0)
+        return MAMBO_OK;
+    MAMBO_REQUIRE(q && out, MAMBO_ERR_VALUE, "null pointer");
+    MAMBO_REQUIRE((uintptr_t)q % 16 == 0 && ldqt % 8 == 0 && ldqh % 8 == 0, MAMBO_ERR_VALUE, "queries must be 16-byte aligned");
+    MAMBO_REQUIRE((uintptr_t)out % 2 == 0 && (uintptr_t)lse % 4 == 0, MAMBO_ERR_VALUE, "outputs must be aligned to their type");
+    MAMBO_REQUIRE(workspace_bytes >= p.bytes && (workspace || p.bytes == 0), MAMBO_ERR_VALUE,
+                  "the workspace must hold %lld bytes (got %lld)", (long long)p.bytes, (long long)workspace_bytes);
+    MAMBO_REQUIRE((uintptr_t)workspace % 16 == 0, MAMBO_ERR_VALUE, "the workspace must be 16-byte aligned");
+    a.q = (const __bf16 *)q, a.ldqt = ldqt, a.ldqh = ldqh, a.group = (int)(q_heads / a.cache.heads);
+    a.scale = scale * kLog2e, a.causal = causal != 0;
+    a.window = (int)std::min<int64_t>(window, 0x3FFFFFFF);
+    a.out = (__bf16 *)out, a.ldot = ldot, a.ldoh = ldoh, a.lse = lse;
+    a.few_rows = p.few_rows, a.slots = p.slots, a.parts = p.parts, a.tiles_each = p.tiles_each;
+    const int padded = kv_padded(a.cache.dim);
+    char *at = (char *)workspace;
+    a.rows_o = (float *)at, a.rows_ml = a.rows_o + p.rows_entries * padded;
+    at += aligned(p.rows_entries * (padded + 2) * 4);
+    a.begins = (int32_t *)at;
+    at += aligned(((int64_t)a.b.seqs + 1) * 4);
+    a.tiles_o = (float *)at, a.tiles_ml = a.tiles_o + p.tiles_entries * padded;
+    hipStream_t s = (hipStream_t)stream;
+    if (p.tiles)
+        if (const int rc = launch_attend_tiles(a, p.tiles, s))
+            return rc;
+    return p.row_tiles ? launch_attend_rows(a, p.row_tiles, s) : MAMBO_OK;
+}

@@ -1,0 +1,440 @@
+// Attention of few rows (a token's heads, a short draft) over long caches: bound by the codes' bytes.
+//
+// The row kernel takes the blocks of 32 cached tokens of all its sequences, one after the other, in equal
+// shares, so that one long sequence among short ones keeps no workgroup longer than the others. A
+// workgroup's four waves take blocks in turn; a wave holds the scores of a block
+//     S^T = K Q^T  (16 x 16 x 32 MFMAs over two tiles of 16 tokens)
+// in such an order that lane 16 kk + i has query i's probabilities of the tokens 8 kk .. 8 kk + 7, the
+// operand that  O^T += V^T P^T  wants of it: nothing goes through LDS or other lanes but the largest
+// score. The running largest and total are f32; the codes are widened to bf16, which holds them exactly, and the
+// probabilities are rounded to bf16 (2^-9 of each, beside the outputs' own).
+#include "attention.h"
+
+namespace {
+
+// Largest of the four lanes that share a query: rows of 16 lanes, then halves of the wave, exchanged.
+__device__ __forceinline__ float across_max(float x)
+{
+    auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    x = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+    auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+__device__ __forceinline__ float across_sum(float x)
+{
+    auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    x = __uint_as_float(a[0]) + __uint_as_float(a[1]);
+    auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return __uint_as_float(b[0]) + __uint_as_float(b[1]);
+}
+
+// Blocks that a sequence has in the row kernel's order.
+__device__ __forceinline__ int row_blocks(const Attention &a, const Sequence &q)
+{
+    return q.n > 0 && q.n <= a.few_rows / a.group ? q.hi - q.lo : 0;
+}
+
+// The shares: workgroups that have any (at least four blocks each, one a wave), and where they begin.
+__device__ __forceinline__ int shares(const Attention &a, int total) { return max(1, min(a.slots, (total + 3) / 4)); }
+__device__ __forceinline__ int share_begin(int p, int total, int count) { return (int)((int64_t)p * total / count); }
+__device__ __forceinline__ int share_of(int block, int total, int count)
+{
+    return (int)((((int64_t)block + 1) * count + total - 1) / total) - 1;
+}
+
+// The sequences' blocks added up by every wave for itself, 256 sequences at a time, four a lane (about
+// 1 us up to 256; a table of them would be a launch of its own).
+struct Scan {
+    const Attention &a;
+    int w[4], before, through; // of this lane's sequences, and the blocks before them and through them
+    int s0;
+
+    __device__ Scan(const Attention &args) : a(args), s0(-1) {}
+    __device__ void strip(int from, int base)
+    {
+        s0 = from;
+        int sum = 0;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int s = from + 4 * lane_id() + j;
+            w[j] = 0;
+            if (s < a.b.seqs)
+                w[j] = row_blocks(a, sequence(a, s));
+            sum += w[j];
+        }
+        through = sum;
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) {
+            const int up = __shfl_up(through, d);
+            through += lane_id() >= d ? up : 0;
+        }
+        through += base;
+        before = through - sum;
+    }
+    __device__ int end() const { return __builtin_amdgcn_readlane(through, 63); }
+    // All blocks; where each sequence's begin, if asked for.
+    __device__ int total(int32_t *begins)
+    {
+        int base = 0;
+        for (int from = 0; from < a.b.seqs; from += 256) {
+            strip(from, base);
+            if (begins) {
+                int at = before;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const int s = from + 4 * lane_id() + j;
+                    if (s < a.b.seqs)
+                        begins[s] = at;
+                    at += w[j];
+                }
+            }
+            base = end();
+        }
+        if (begins && lane_id() == 0)
+            begins[a.b.seqs] = base;
+        return base;
+    }
+    // The sequence that has `block` (below the total), and its first block.
+    __device__ void find(int block, int *sequence, int *first)
+    {
+        if (a.b.seqs > 256 || s0 < 0) {
+            int base = 0;
+            for (int from = 0; from < a.b.seqs; from += 256) {
+                strip(from, base);
+                base = end();
+                if (base > block)
+                    break;
+            }
+        }
+        const uint64_t past = __ballot(through > block);
+        const int src = past ? __builtin_ctzll(past) : 63;
+        int s = s0 + 4 * lane_id(), at = before;
+#pragma unroll
+        for (int j = 0; j < 3; ++j)
+            if (at + w[j] <= block && s == s0 + 4 * lane_id() + j) {
+                at += w[j];
+                ++s;
+            }
+        *sequence = __builtin_amdgcn_readlane(s, src);
+        *first = __builtin_amdgcn_readlane(at, src);
+    }
+};
+
+// 16 RT rows by 32 DS values a head.
+template <int DS, int RT>
+__global__ __launch_bounds__(256, 2) void attend_rows_kernel(const Attention a)
+{
+    constexpr int DP = 32 * DS;
+    __shared__ float so[4][16 * RT][DP + 4];
+    __shared__ float sm[4][16 * RT], sl[4][16 * RT];
+    const int tid = (int)threadIdx.x, lane = lane_id(), kk = lane >> 4, col = lane & 15;
+    const int wave = __builtin_amdgcn_readfirstlane(tid / 64);
+    const int head = (int)(blockIdx.x % (unsigned)a.cache.heads), slot = (int)(blockIdx.x / (unsigned)a.cache.heads);
+    Scan scan(a);
+    const int total = scan.total(blockIdx.x == 0 && wave == 0 ? a.begins : nullptr);
+    const int count = shares(a, total);
+    if (slot >= count || total == 0)
+        return;
+    int at = share_begin(slot, total, count);
+    const int end = share_begin(slot + 1, total, count);
+    int s = 0, base = 0; // the sequence that `at` is in, and its first block in the order
+    scan.find(at, &s, &base);
+
+    while (at < end) {
+        const Sequence seq = sequence(a, s);
+        const int blocks = row_blocks(a, seq), rows = seq.n * a.group;
+        if (blocks == 0 || at >= base + blocks) { // sequences without blocks between
+            scan.find(at, &s, &base);
+            continue;
+        }
+        const int stop = min(end, base + blocks);
+        const int first_blk = seq.lo + at - base, last_blk = seq.lo + stop - base;
+
+        bf16x8 q[RT][DS];
+        int to[RT], from[RT];
+#pragma unroll
+        for (int r = 0; r < RT; ++r) {
+            const int row = 16 * r + col, i = row / a.group, h = head * a.group + row % a.group;
+            const bool some = row < rows;
+            to[r] = some ? sees_to(a, seq, i) : 0;
+            from[r] = some ? sees_from(a, seq, i) : 0;
+            const __bf16 *x = a.q + (int64_t)(seq.first + i) * a.ldqt + h * a.ldqh;
+#pragma unroll
+            for (int d = 0; d < DS; ++d) {
+                const int at_d = 32 * d + 8 * kk;
+                q[r][d] = bf16x8{};
+                if (some && at_d < a.cache.dim)
+                    q[r][d] = *reinterpret_cast<const bf16x8 *>(x + at_d);
+            }
+        }
+        // where no row's limits can be inside a block
+        const int all_to = sees_to(a, seq, 0), all_from = sees_from(a, seq, seq.n - 1);
+
+        v4f o[RT][2 * DS];
+        float m[RT], l[RT];
+#pragma unroll
+        for (int r = 0; r < RT; ++r) {
+            m[r] = -__builtin_inff();
+            l[r] = 0.0f;
+#pragma unroll
+            for (int d = 0; d < 2 * DS; ++d)
+                o[r][d] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+        }
+
+        struct Block {
+            uint4 k[DS], v[DS];
+            int scales; // -1: there is no such page
+        };
+        const auto page_of = [&](int blk) -> int {
+            return blk < last_blk ? a.b.page(s, blk >> a.cache.shift) : -1;
+        };
+        const auto load = [&](int blk, int page_any, Block &b) {
+            const int page = __builtin_amdgcn_readfirstlane(page_any);
+            b.scales = -1;
+            if (page < 0 || page >= a.cache.pages)
+                return;
+            const int64_t at_blk = a.cache.block(page, head, blk);
+            const uint4 *codes = reinterpret_cast<const uint4 *>(a.cache.codes + at_blk * (2 * kKvBlock * DP)) + lane;
+            b.scales = *reinterpret_cast<const uint16_t *>(a.cache.scales + 2 * at_blk);
+#pragma unroll
+            for (int d = 0; d < DS; ++d)
+                b.k[d] = codes[64 * d];
+#pragma unroll
+            for (int d = 0; d < DS; ++d)
+                b.v[d] = codes[64 * (DS + d)];
+        };
+        const auto take = [&](int blk, Block &b) {
+            const int scales = __builtin_amdgcn_readfirstlane(b.scales);
+            if (scales < 0)
+                return;
+            const float ks = e8m0(scales & 255), vs = e8m0(scales >> 8);
+            v4f x[RT][2];
+#pragma unroll
+            for (int r = 0; r < RT; ++r)
+                x[r][0] = x[r][1] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int d = 0; d < DS; ++d) {
+                const bf16x8 k0 = widen(b.k[d].x, b.k[d].y, ks), k1 = widen(b.k[d].z, b.k[d].w, ks);
+#pragma unroll
+                for (int r = 0; r < RT; ++r) {
+                    x[r][0] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k0, q[r][d], x[r][0], 0, 0, 0);
+                    x[r][1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k1, q[r][d], x[r][1], 0, 0, 0);
+                }
+            }
+            const int token = blk * kKvBlock + 8 * kk;
+            const bool edge = (blk + 1) * kKvBlock > all_to || blk * kKvBlock < all_from;
+            bf16x8 p[RT];
+#pragma unroll
+            for (int r = 0; r < RT; ++r) {
+                float y[8], top = -__builtin_inff();
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    y[j] = x[r][j >> 2][j & 3] * a.scale;
+                    if (edge)
+                        y[j] = token + j < to[r] && token + j >= from[r] ? y[j] : -__builtin_inff();
+                    top = fmaxf(top, y[j]);
+                }
+                top = across_max(top);
+                if (__any(top > m[r])) { // else nothing grows
+                    const float grown = fmaxf(m[r], top);
+                    const float by = m[r] == -__builtin_inff() ? 0.0f : exp2_fast(m[r] - grown);
+                    m[r] = grown;
+                    l[r] *= by;
+#pragma unroll
+                    for (int d = 0; d < 2 * DS; ++d)
+                        o[r][d] *= by;
+                }
+                const float less = m[r] == -__builtin_inff() ? 0.0f : m[r];
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    y[j] = exp2_fast(y[j] - less);
+                    l[r] += y[j];
+                    p[r][j] = (__bf16)y[j];
+                }
+            }
+            const int left = seq.len - token;
+            const bool tail = (blk + 1) * kKvBlock > seq.len;
+#pragma unroll
+            for (int d = 0; d < DS; ++d) {
+                uint2 v0 = make_uint2(b.v[d].x, b.v[d].y), v1 = make_uint2(b.v[d].z, b.v[d].w);
+                if (tail) {
+                    v0 = keep_tokens(v0.x, v0.y, left);
+                    v1 = keep_tokens(v1.x, v1.y, left);
+                }
+                const bf16x8 w0 = widen(v0.x, v0.y, vs), w1 = widen(v1.x, v1.y, vs);
+#pragma unroll
+                for (int r = 0; r < RT; ++r) {
+                    o[r][2 * d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w0, p[r], o[r][2 * d], 0, 0, 0);
+                    o[r][2 * d + 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w1, p[r], o[r][2 * d + 1], 0, 0, 0);
+                }
+            }
+        };
+
+        // a block is asked for while the one before it is worked on, its page one earlier
+        Block even, odd;
+        even.scales = odd.scales = -1;
+        int blk = first_blk + wave;
+        load(blk, page_of(blk), even);
+        int page = page_of(blk + 4);
+        while (blk < last_blk) {
+            load(blk + 4, page, odd);
+            page = page_of(blk + 8);
+            take(blk, even);
+            blk += 4;
+            if (blk >= last_blk)
+                break;
+            load(blk + 4, page, even);
+            page = page_of(blk + 8);
+            take(blk, odd);
+            blk += 4;
+        }
+
+#pragma unroll
+        for (int r = 0; r < RT; ++r) {
+            const float sum = across_sum(l[r]);
+            if (kk == 0) {
+                sm[wave][16 * r + col] = m[r];
+                sl[wave][16 * r + col] = sum;
+            }
+#pragma unroll
+            for (int d = 0; d < 2 * DS; ++d)
+                *reinterpret_cast<v4f *>(&so[wave][16 * r + col][16 * d + 4 * kk]) = o[r][d];
+        }
+        __syncthreads();
+        const bool whole = at == base && stop == base + blocks;
+        const int which = at == base ? 1 : 0; // a share ends with a sequence that goes on, or begins with one
+        const int64_t entry = ((int64_t)head * a.slots + slot) * 2 + which;
+        for (int item = tid; item < rows * (DP / 4); item += 256) {
+            const int row = item / (DP / 4), d = 4 * (item % (DP / 4));
+            float top = sm[0][row];
+#pragma unroll
+            for (int w = 1; w < 4; ++w)
+                top = fmaxf(top, sm[w][row]);
+            const float less = top == -__builtin_inff() ? 0.0f : top;
+            float sum = 0.0f;
+            v4f y = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int w = 0; w < 4; ++w) {
+                const float f = exp2_fast(sm[w][row] - less);
+                sum += f * sl[w][row];
+                y += f * *reinterpret_cast<const v4f *>(&so[w][row][d]);
+            }
+            if (whole) {
+                const int i = row / a.group, h = head * a.group + row % a.group;
+                const int64_t t = seq.first + i;
+                y *= sum == 0.0f ? 0.0f : 1.0f / sum;
+                if (d < a.cache.dim)
+                    store_row4<true>(a.out, t * a.ldot + h * a.ldoh + d, y, a.cache.dim - d, a.ldot % 4 == 0 && a.ldoh % 4 == 0 && (uintptr_t)a.out % 8 == 0);
+                if (a.lse && d == 0)
+                    a.lse[t * ((int64_t)a.group * a.cache.heads) + h] = sum == 0.0f ? -__builtin_inff() : (top + __log2f(sum)) * kLn2;
+            } else {
+                *reinterpret_cast<v4f *>(a.rows_o + (entry * (16 * RT) + row) * DP + d) = y;
+                if (d == 0)
+                    *reinterpret_cast<float2 *>(a.rows_ml + (entry * (16 * RT) + row) * 2) = make_float2(top, sum);
+            }
+        }
+        at = stop;
+        if (at < end) {
+            base += blocks;
+            ++s;
+            __syncthreads();
+        }
+    }
+}
+
+// The sum of a row's partial results, weighted by their largest scores; rows of sequences without keys become
+// zeros. A workgroup a row: DP / 4 threads side by side, the parts dealt to 256 / (DP / 4) such groups, which
+// are added in order.
+template <int DS>
+__global__ __launch_bounds__(256) void join_rows_kernel(const Attention a, int tile_rows)
+{
+    constexpr int DP = 32 * DS, kWide = DP / 4, kGroups = 256 / kWide;
+    __shared__ v4f so[kGroups][kWide];
+    __shared__ float sm[kGroups], sl[kGroups];
+    const int s = (int)(blockIdx.x / (unsigned)a.cache.heads), head = (int)(blockIdx.x % (unsigned)a.cache.heads);
+    const int row = (int)blockIdx.y, tid = (int)threadIdx.x, g = tid / kWide, d = 4 * (tid % kWide);
+    const Sequence seq = sequence(a, s);
+    if (seq.n <= 0 || seq.n > a.few_rows / a.group || row >= seq.n * a.group)
+        return;
+    const int blocks = seq.hi - seq.lo, total = a.begins[a.b.seqs], begin = a.begins[s];
+    const int i = row / a.group, h = head * a.group + row % a.group;
+    const int64_t t = seq.first + i;
+    int p0 = 0, p1 = -1;
+    if (blocks > 0) {
+        const int count = shares(a, total);
+        p0 = share_of(begin, total, count);
+        p1 = share_of(begin + blocks - 1, total, count);
+        if (p0 == p1)
+            return; // written by the one that had all of it
+    }
+    float m = -__builtin_inff(), l = 0.0f;
+    v4f o = {0.0f, 0.0f, 0.0f, 0.0f};
+    if (g < kGroups) {
+        for (int p = p0 + g; p <= p1; p += kGroups) {
+            const int64_t entry = ((int64_t)head * a.slots + p) * 2 + (p == p0);
+            const float2 ml = *reinterpret_cast<const float2 *>(a.rows_ml + (entry * tile_rows + row) * 2);
+            const v4f x = *reinterpret_cast<const v4f *>(a.rows_o + (entry * tile_rows + row) * DP + d);
+            const float top = fmaxf(m, ml.x), less = top == -__builtin_inff() ? 0.0f : top;
+            const float f = exp2_fast(m - less), e = exp2_fast(ml.x - less);
+            o = o * f + x * e;
+            l = l * f + ml.y * e;
+            m = top;
+        }
+        so[g][tid % kWide] = o;
+        if (tid % kWide == 0) {
+            sm[g] = m;
+            sl[g] = l;
+        }
+    }
+    __syncthreads();
+    if (g > 0)
+        return;
+    m = sm[0];
+#pragma unroll
+    for (int k = 1; k < kGroups; ++k)
+        m = fmaxf(m, sm[k]);
+    const float less = m == -__builtin_inff() ? 0.0f : m;
+    o = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+    l = 0.0f;
+#pragma unroll
+    for (int k = 0; k < kGroups; ++k) {
+        const float f = exp2_fast(sm[k] - less);
+        o += so[k][tid] * f;
+        l += sl[k] * f;
+    }
+    o *= l == 0.0f ? 0.0f : 1.0f / l;
+    if (d < a.cache.dim)
+        store_row4<true>(a.out, t * a.ldot + h * a.ldoh + d, o, a.cache.dim - d, a.ldot % 4 == 0 && a.ldoh % 4 == 0 && (uintptr_t)a.out % 8 == 0);
+    if (a.lse && d == 0)
+        a.lse[t * ((int64_t)a.group * a.cache.heads) + h] = l == 0.0f ? -__builtin_inff() : (m + __log2f(l)) * kLn2;
+}
+
+template <int DS, int RT>
+void launch_rows(const Attention &a, hipStream_t s)
+{
+    if constexpr (RT <= max_row_tiles(32 * DS)) {
+        MAMBO_LAUNCH((attend_rows_kernel<DS, RT>), dim3((unsigned)(a.slots * a.cache.heads)), dim3(256), 0, s, a);
+        const int rows = a.b.offsets ? a.few_rows : a.b.each * a.group;
+        MAMBO_LAUNCH((join_rows_kernel<DS>), dim3((unsigned)(a.b.seqs * a.cache.heads), (unsigned)rows), dim3(256), 0, s, a, 16 * RT);
+    }
+}
+
+} // namespace
+
+int launch_attend_rows(const Attention &a, int row_tiles, hipStream_t s)
+{
+    const int ds = kv_padded(a.cache.dim) / 32;
+#define MAMBO_ROWS(DS)                                                                                             \
+    if (ds == DS)                                                                                                  \
+    row_tiles == 1 ? launch_rows<DS, 1>(a, s) : row_tiles == 2 ? launch_rows<DS, 2>(a, s) : launch_rows<DS, 4>(a, s)
+    MAMBO_ROWS(1);
+    MAMBO_ROWS(2);
+    MAMBO_ROWS(3);
+    MAMBO_ROWS(4);
+    MAMBO_ROWS(5);
+    MAMBO_ROWS(6);
+    MAMBO_ROWS(7);
+    MAMBO_ROWS(8);
+#undef MAMBO_ROWS
+    return mambo_check_launch("kv_attention");
+}

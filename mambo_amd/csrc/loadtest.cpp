@@ -287,6 +287,10 @@ MAMBO_ABI_NAME(mambo_gemm_config, "mambo_gemm_config")
 MAMBO_ABI_NAME(mambo_projection, "mambo_projection")
 MAMBO_ABI_NAME(mambo_chain_launch, "mambo_chain_launch")
 MAMBO_ABI_NAME(mambo_chain_config, "mambo_chain_config")
+MAMBO_ABI_NAME(mambo_rotary_table, "mambo_rotary_table")
+MAMBO_ABI_NAME(mambo_kv_cache, "mambo_kv_cache")
+MAMBO_ABI_NAME(mambo_kv_batch, "mambo_kv_batch")
+MAMBO_ABI_NAME(mambo_kv_rows, "mambo_kv_rows")
 MAMBO_ABI_NAME(mambo_stream_t, "hipStream_t")
 #undef MAMBO_ABI_NAME
 template <class T> struct AbiName<T *> {
@@ -365,6 +369,15 @@ const std::vector<EntryDecl> &compiled_entries()
                     "weights", "offsets", "rows", "slots", "stream"),
         MAMBO_ENTRY(mambo_combine_experts, "y", "y_dtype", "ldy", "r", "slots", "weights", "m", "top_k", "n", "out",
                     "out_dtype", "ldo", "stream"),
+        MAMBO_ENTRY(mambo_rotary, "x", "x_dtype", "tokens", "heads", "dim", "ldt", "ldh", "positions", "table", "out",
+                    "out_dtype", "ldot", "ldoh", "stream"),
+        MAMBO_ENTRY(mambo_kv_cache_bytes, "pages", "heads", "head_dim", "page_size"),
+        MAMBO_ENTRY(mambo_kv_append, "rows", "tokens", "cache", "batch", "table", "positions", "stream"),
+        MAMBO_ENTRY(mambo_kv_read, "cache", "batch", "sequences", "positions", "n", "heads", "dim", "k", "v", "stream"),
+        MAMBO_ENTRY(mambo_kv_attention_workspace, "cache", "batch", "tokens", "q_heads"),
+        MAMBO_ENTRY(mambo_kv_attention, "q", "tokens", "q_heads", "dim", "ldqt", "ldqh", "cache", "batch", "scale", "causal", "window",
+                    "out", "ldot", "ldoh", "lse", "workspace", "workspace_bytes", "stream"),
+        MAMBO_ENTRY(mambo_kv_attention_plan, "cache", "batch", "tokens", "q_heads", "plan"),
         MAMBO_ENTRY(mambo_synth_iq3s, "seed", "blocks", "row0", "nrows", "raw", "stream"),
         MAMBO_ENTRY(mambo_synth_bf16, "seed", "outlier_seed", "outlier_frac", "i0", "count", "out", "stream"),
         MAMBO_ENTRY(mambo_e4m3_convert, "in", "n", "out_sw", "out_hw", "stream"),
@@ -439,7 +452,9 @@ struct Manifest {
 
 const std::set<std::string> kDtypes = {"uint8",  "uint16",  "uint32",           "int32",
                                        "float32", "char",   "float32|bfloat16", "mambo_gemm_config",
-                                       "mambo_projection", "mambo_chain_launch", "mambo_chain_config"};
+                                       "mambo_projection", "mambo_chain_launch", "mambo_chain_config",
+                                       "bfloat16", "mambo_rotary_table", "mambo_kv_cache", "mambo_kv_batch",
+                                       "mambo_kv_rows"};
 
 void validate_constraint(const Json &c, const std::map<std::string, std::string> &pointer_types)
 {

@@ -1,0 +1,63 @@
+"""Attention over the paged 8-bit cache on gfx950 (mambo_amd/csrc/attention_rows.hip for few rows of a sequence,
+attention_tiles.hip for many). The reference has no counterpart.
+
+    out[t, h] = sum_j p_j v_j,  p = softmax_j(scale * q[t, h] . k_j)   over the cached tokens j that the row sees
+
+Sequences are told as for launch_append_kv (mambo_amd.kernels.kv_cache).
+"""
+
+from __future__ import annotations
+
+import torch
+
+from mambo_amd import _native
+from mambo_amd.kernels.kv_cache import batch_args, check_cache
+from mambo_amd.kernels.rotary import check_heads, head_strides, heads_in_place, output_heads
+from mambo_amd.utils.kv_cache import KVCache
+
+
+def launch_attention_kv(q: torch.Tensor, cache: KVCache, tables: torch.Tensor, lengths: torch.Tensor, *,
+                        offsets: torch.Tensor | None = None, scale: float | None = None, causal: bool = True,
+                        window: int = 0, return_lse: bool = False, stream=None, out: torch.Tensor | None = None):
+    """Attention of bfloat16 queries ``q`` [T,Hq,D] over the cached keys and values of their sequences; query head h
+    reads key/value head h // (Hq / H). Returns bfloat16 [T,Hq,D], or (that, float32 [T,Hq]) with
+    ``return_lse``: the logarithm of the sum of the exponentials of a row's scores.
+
+    Row i of a sequence's n stands at position lengths[s] - n + i and sees the tokens up to itself (``causal``), no more
+    than the last ``window`` of them where that is not 0, or all of the sequence's. A row that sees none (a sequence of length
+    0, more rows than tokens, no page) becomes zeros, its lse -inf. ``scale`` defaults to D ** -0.5.
+
+    Scores, the running sum and the output are float32; the probabilities are rounded to bfloat16 (2^-9 of each) for the
+    product with the values, the result once to bfloat16. Results do not vary from run to run. Rows of no sequence are not written: they stay what they
+    were in ``out``, and are undefined without. T may be 0."""
+    cache = check_cache(cache)
+    dev, dim = cache.codes.device, cache.head_dim
+    check_heads(q, dim, dev, "q")
+    if q.dtype != torch.bfloat16:
+        raise ValueError("q must be bfloat16")
+    tokens, heads = q.shape[:2]
+    if heads % cache.heads:
+        raise ValueError(f"q must have a multiple of the cache's {cache.heads} heads, got {heads}")
+    scale = dim ** -0.5 if scale is None else float(scale)
+    window = int(window)
+    if window < 0 or (window and not causal):
+        raise ValueError("a window is positive, and of causal attention")
+    with _native.launch_on(dev, stream):
+        batch = batch_args(tables, lengths, offsets, tokens, dev)
+        q = heads_in_place(q)
+        strides = head_strides(q)
+        if q.data_ptr() % 16 or strides[0] % 8 or strides[1] % 8:
+            q = torch.empty(q.shape, dtype=q.dtype, device=dev).copy_(q)
+            strides = head_strides(q)
+        out = output_heads(out, q.shape, torch.bfloat16, dev)
+        lse = torch.empty((tokens, heads), dtype=torch.float32, device=dev) if return_lse else None
+        lib = _native.lib()
+        size = lib.mambo_kv_attention_workspace(cache.args, batch, tokens, heads)
+        if size < 0:
+            _native.check(size, "launch_attention_kv")
+        workspace = torch.empty(size, dtype=torch.uint8, device=dev)
+        _native.check(lib.mambo_kv_attention(
+            q.data_ptr(), tokens, heads, dim, *strides, cache.args, batch, scale, bool(causal), window, out.data_ptr(),
+            *head_strides(out), None if lse is None else lse.data_ptr(), workspace.data_ptr(), size,
+            _native.stream_handle(stream, dev)), "launch_attention_kv")
+    return (out, lse) if return_lse else out

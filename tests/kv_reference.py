@@ -1,0 +1,146 @@
+"""Plain statements, in 64 bits on the CPU, of rotary positions, the paged 8-bit cache and attention over
+it, and sequences to try them on. Written from the definitions; nothing of the package is used."""
+
+from __future__ import annotations
+
+import math
+
+import numpy as np
+import torch
+
+from conftest import e4m3_encode_bruteforce, e4m3_values
+
+VALUES = e4m3_values()
+BLOCK, LOWEST = 32, -100
+
+
+def rotate(x: np.ndarray, positions, frequencies, interleaved: bool, magnitude: float = 1.0) -> np.ndarray:
+    """x [T,H,D] rotated in float64."""
+    out = np.array(x, dtype=np.float64)
+    size = 2 * len(frequencies)
+    for t, p in enumerate(positions):
+        for i, f in enumerate(frequencies):
+            c, s = magnitude * math.cos(p * f), magnitude * math.sin(p * f)
+            i0, i1 = (2 * i, 2 * i + 1) if interleaved else (i, i + size // 2)
+            a, b = np.array(x[t, :, i0], dtype=np.float64), np.array(x[t, :, i1], dtype=np.float64)
+            out[t, :, i0], out[t, :, i1] = a * c - b * s, a * s + b * c
+    return out
+
+
+def rotation_bound(x: np.ndarray, size: int, interleaved: bool, magnitude: float = 1.0) -> np.ndarray:
+    """How far float32 rotations can be: the angle is off by 2^-24 of up to pi and by 2^-32 of a turn, the
+    sine and cosine by four units, their product with the magnitude, the two products and the sum by half a unit each."""
+    a = np.abs(np.array(x, dtype=np.float64))
+    out = np.zeros_like(a)
+    half = size // 2
+    pairs = [(2 * i, 2 * i + 1) if interleaved else (i, i + half) for i in range(half)]
+    for i, j in pairs:
+        out[..., i] = out[..., j] = magnitude * (a[..., i] + a[..., j]) * 12 * 2.0**-24
+    return out
+
+
+def exponent(amax: float) -> int:
+    """max(ceil(log2(amax / 448)), -100), exactly."""
+    if amax == 0.0:
+        return LOWEST
+    mant, exp = math.frexp(amax)
+    return max(LOWEST, exp - 9 if mant <= 0.875 else exp - 8)
+
+
+def nearest(x: np.ndarray, e: int) -> np.ndarray:
+    """E4M3(x 2^-e) 2^e."""
+    return (VALUES[e4m3_encode_bruteforce(np.ldexp(x, -e))] * 2.0**e).reshape(np.shape(x))
+
+
+class Model:
+    """What the cache holds of one sequence: values [L,H,D] and exponents of blocks, keys and values apart."""
+
+    def __init__(self, heads: int, dim: int):
+        self.heads, self.dim = heads, dim
+        self.k, self.v = np.zeros((0, heads, dim)), np.zeros((0, heads, dim))
+        self.e = {}  # (block, head, "k" or "v")
+
+    def append(self, k: np.ndarray, v: np.ndarray, start: int) -> None:
+        """Tokens start .. of rows k, v [n,H,D] (float64 of what the kernel is given, rotated); what was at or
+        behind start is overwritten or forgotten."""
+        n = k.shape[0]
+        for name, rows in (("k", k), ("v", v)):
+            old = getattr(self, name)[:start]
+            new = np.concatenate([old, np.zeros((n, self.heads, self.dim))])
+            for block in range(start // BLOCK, -(-(start + n) // BLOCK)):
+                lo, hi = max(start, block * BLOCK), min(start + n, (block + 1) * BLOCK)
+                for h in range(self.heads):
+                    part, mate = rows[lo - start:hi - start, h], (v if name == "k" else k)[lo - start:hi - start, h]
+                    bad = ~(np.isfinite(part).all(1) & np.isfinite(mate).all(1))
+                    e = exponent(float(np.abs(part[~bad]).max(initial=0.0)))
+                    if lo > block * BLOCK:
+                        before = self.e.get((block, h, name), LOWEST)
+                        if e > before:
+                            held = new[block * BLOCK:lo, h]
+                            new[block * BLOCK:lo, h] = np.where(np.isnan(held), held, nearest(np.nan_to_num(held), e))
+                        e = max(e, before)
+                    self.e[block, h, name] = e
+                    stored = nearest(np.where(bad[:, None], 0.0, part), e)
+                    if name == "k":
+                        stored[bad] = np.nan
+                    new[lo:hi, h] = stored
+            setattr(self, name, new)
+
+
+def attend(q: np.ndarray, k: np.ndarray, v: np.ndarray, group: int, scale: float, causal: bool, window: int, left_out=None):
+    """(out, lse, bound of out's error, bound of lse's) of a sequence's rows q [n,Hq,D] over its cached k, v [L,H,D].
+    ``left_out``: tokens that no page is for.
+
+    float32 scores of D products, each addition off by a unit of its last place (a matrix instruction may cut), and
+    scaled; exponentials off by a few units more; probabilities rounded to bfloat16 (half a step: 2^-8), sums in
+    float32, the result rounded to bfloat16."""
+    n, heads, dim = q.shape
+    length = k.shape[0]
+    out, lse = np.zeros(q.shape), np.full((n, heads), -np.inf)
+    bound, lse_bound = np.zeros(q.shape), np.zeros((n, heads))
+    token = np.arange(length)
+    unit = 2.0**-23
+    for i in range(n):
+        position = length - n + i
+        seen = token <= position if causal else token < length
+        if window:
+            seen = seen & (token > position - window)
+        if left_out is not None:
+            seen = seen & ~left_out
+        if not seen.any():
+            continue
+        for h in range(heads):
+            kk, vv = k[seen, h // group], v[seen, h // group]
+            s = scale * (kk @ q[i, h])
+            delta = (dim + 8) * unit * float((scale * (np.abs(kk) @ np.abs(q[i, h]))).max(initial=0.0)) + 8 * unit * float(np.abs(s).max())
+            top = s.max()
+            p = np.exp(s - top)
+            total = p.sum()
+            p /= total
+            out[i, h], lse[i, h] = p @ vv, top + math.log(total)
+            spread = p @ np.abs(vv)
+            sums = (len(s) + 64) * unit
+            bound[i, h] = spread * (2 * math.expm1(delta + 8 * unit) + 2.0**-8 + sums) + np.abs(out[i, h]) * 2.0**-8 + 1e-30
+            lse_bound[i, h] = 2 * delta + sums + 8 * unit * (1.0 + abs(lse[i, h]))
+    return out, lse, bound, lse_bound
+
+
+def tables_of(rng, lengths, page: int, *, spare: int = 2, extra: int = 1):
+    """(tables int32 [S,C], pages of the pool): every sequence's pages in any order, -1 behind them."""
+    counts = [-(-n // page) for n in lengths]
+    pages = sum(counts) + spare
+    order = rng.permutation(pages).astype(np.int32)
+    tables = np.full((len(lengths), max(counts) + extra), -1, dtype=np.int32)
+    at = 0
+    for s, c in enumerate(counts):
+        tables[s, :c] = order[at:at + c]
+        at += c
+    return tables, pages
+
+
+def offsets_of(counts) -> np.ndarray:
+    return np.concatenate([[0], np.cumsum(counts)]).astype(np.int32)
+
+
+def device(gpu, *arrays):
+    return [torch.from_numpy(np.ascontiguousarray(a)).to(gpu) for a in arrays]

@@ -1,0 +1,222 @@
+"""Attention over the paged 8-bit cache on the GPU against 64 bits, within what its roundings allow: single tokens,
+drafts, prompts and pieces of them, windows, empty sequences, pages that are missing."""
+
+from __future__ import annotations
+
+import math
+
+import numpy as np
+import pytest
+import torch
+
+import kv_reference as ref
+from test_gpu_kv_cache import new_cache, read_all, rows_of
+
+pytestmark = pytest.mark.gpu
+
+
+def attention():
+    from mambo_amd.kernels.attention import launch_attention_kv
+    return launch_attention_kv
+
+
+def filled(gpu, rng, lengths, heads, dim, page, extra=1):
+    """(cache, tables, keys and values that it holds by sequence)."""
+    from mambo_amd.kernels.kv_cache import launch_append_kv
+    host, pages = ref.tables_of(rng, lengths, page, extra=extra)
+    tables, cache = ref.device(gpu, host)[0], new_cache(pages, heads, dim, page)
+    n = sum(lengths)
+    k, v = rows_of(rng, n, heads, dim, torch.bfloat16).to(gpu), rows_of(rng, n, heads, dim, torch.bfloat16).to(gpu)
+    launch_append_kv(k, v, cache, tables, *ref.device(gpu, np.array(lengths, np.int32)),
+                     offsets=ref.device(gpu, ref.offsets_of(lengths))[0])
+    return cache, tables, *read_all(cache, tables, lengths)
+
+
+def check(out, lse, q, keys, values, counts, group, scale=None, causal=True, window=0, left_out=None):
+    cuts = ref.offsets_of(counts)
+    got, got_lse, q64 = out.double().cpu().numpy(), lse.double().cpu().numpy(), q.double().cpu().numpy()
+    scale = q.shape[2] ** -0.5 if scale is None else scale
+    for s in range(len(counts)):
+        part = slice(cuts[s], cuts[s + 1])
+        want, want_lse, bound, lse_bound = ref.attend(q64[part], keys[s], values[s], group, scale, causal, window,
+                                                      None if left_out is None else left_out[s])
+        off = np.abs(got[part] - want)
+        assert (off <= bound).all(), (s, float((off / np.maximum(bound, 1e-300)).max()))
+        some = np.isfinite(want_lse)
+        assert np.array_equal(some, np.isfinite(got_lse[part])) and (got_lse[part][~some] == -np.inf).all()
+        assert (np.abs(got_lse[part][some] - want_lse[some]) <= lse_bound[some]).all()
+
+
+# lengths, rows of each sequence, key/value heads, group, head size, page, window
+UNIFORM = [
+    ([1], 1, 1, 1, 8, 32, 0), ([31], 1, 2, 4, 64, 32, 0), ([32], 1, 1, 1, 32, 32, 0), ([33, 7], 1, 8, 4, 128, 64, 0),
+    ([1000], 1, 8, 4, 128, 64, 0), ([500, 0, 3, 129], 1, 2, 8, 128, 32, 0), ([70, 300], 1, 3, 7, 80, 128, 0),
+    ([200], 1, 2, 16, 96, 32, 0), ([200, 90], 1, 2, 32, 64, 32, 0), ([150], 1, 1, 5, 256, 64, 0), ([150], 1, 2, 3, 160, 64, 0),
+    ([90], 1, 1, 2, 192, 32, 0), ([90, 45], 1, 1, 2, 224, 32, 0), ([300, 290, 44], 5, 2, 6, 64, 32, 0), ([300, 280], 4, 2, 4, 128, 64, 0),
+    ([400, 30], 8, 1, 8, 40, 32, 0), ([3, 6], 6, 2, 2, 64, 32, 0), ([700, 650], 3, 2, 4, 64, 32, 100), ([64], 2, 1, 1, 64, 32, 1),
+    ([1000, 900], 1, 2, 4, 128, 256, 33), ([2000], 1, 1, 1, 64, 32, 0), ([5000, 1, 64, 3000], 1, 2, 4, 64, 128, 0),
+    # many rows of a sequence
+    ([40], 40, 2, 4, 64, 32, 0), ([300], 300, 1, 2, 128, 64, 0), ([100, 130], 33, 2, 3, 96, 32, 0), ([65], 65, 1, 1, 32, 32, 0),
+    ([260], 129, 2, 1, 80, 32, 0), ([200], 70, 1, 16, 256, 64, 0), ([150], 150, 1, 3, 160, 32, 0), ([90], 90, 1, 2, 192, 32, 0),
+    ([90], 90, 1, 2, 224, 32, 0), ([600], 200, 1, 2, 64, 32, 50), ([1500], 64, 1, 8, 64, 64, 0), ([1100, 20], 100, 1, 1, 128, 32, 0),
+    ([50, 0, 70], 60, 2, 4, 64, 32, 0), ([2000], 17, 1, 16, 128, 128, 0),
+]
+
+
+@pytest.mark.parametrize("lengths,n,heads,group,dim,page,window", UNIFORM)
+def test_uniform(gpu, lengths, n, heads, group, dim, page, window):
+    rng = np.random.default_rng(sum(lengths) + dim)
+    cache, tables, keys, values = filled(gpu, rng, lengths, heads, dim, page)
+    q = rows_of(rng, n * len(lengths), heads * group, dim, torch.bfloat16, 2.0).to(gpu)
+    out, lse = attention()(q, cache, tables, *ref.device(gpu, np.array(lengths, np.int32)), window=window, return_lse=True)
+    check(out, lse, q, keys, values, [n] * len(lengths), group, window=window)
+
+
+RAGGED = [
+    # lengths, rows
+    ([300, 77, 600, 1, 0, 33], [1, 77, 130, 1, 0, 20], 2, 4, 64, 32, 0),
+    ([300, 77, 600], [1, 1, 1], 2, 4, 128, 64, 0),
+    ([80, 200, 64, 90], [80, 3, 0, 90], 3, 5, 96, 32, 0),
+    ([500, 40], [400, 5], 1, 8, 128, 64, 64),
+    ([10, 500], [30, 260], 1, 2, 64, 32, 0),  # more rows than tokens
+    ([400], [300], 2, 1, 256, 128, 0),
+    ([129, 140], [40, 7], 1, 48, 64, 32, 0),
+    ([90, 120], [9, 100], 1, 24, 256, 32, 0),
+    ([0, 0], [3, 100], 1, 2, 64, 32, 0),
+    ([40] * 300, [1] * 299 + [20], 1, 2, 32, 32, 0),  # more sequences than a wave looks at in one go
+    ([33] * 130, [2] * 60 + [0] * 9 + [33] + [1] * 60, 1, 8, 64, 32, 0),
+]
+
+
+@pytest.mark.parametrize("lengths,counts,heads,group,dim,page,window", RAGGED)
+def test_ragged(gpu, lengths, counts, heads, group, dim, page, window):
+    rng = np.random.default_rng(sum(lengths) + dim)
+    cache, tables, keys, values = filled(gpu, rng, lengths, heads, dim, page)
+    n = sum(counts)
+    q = rows_of(rng, n + 5, heads * group, dim, torch.bfloat16, 2.0).to(gpu)
+    out = torch.full(q.shape, 7.0, dtype=torch.bfloat16, device=gpu)
+    got, lse = attention()(q, cache, tables, *ref.device(gpu, np.array(lengths, np.int32)), window=window, return_lse=True,
+                           offsets=ref.device(gpu, ref.offsets_of(counts))[0], out=out)
+    assert got is out and (out[n:] == 7.0).all()  # rows of no sequence
+    check(out, lse, q, keys, values, counts, group, window=window)
+
+
+@pytest.mark.parametrize("lengths,n,heads,group,dim", [([300, 41], 1, 2, 4, 64), ([300, 41], 6, 1, 8, 128), ([200, 90], 90, 2, 2, 64)])
+def test_all_of_the_sequence_is_seen_without_causal(gpu, lengths, n, heads, group, dim):
+    rng = np.random.default_rng(dim + n)
+    cache, tables, keys, values = filled(gpu, rng, lengths, heads, dim, 64)
+    q = rows_of(rng, n * len(lengths), heads * group, dim, torch.bfloat16).to(gpu)
+    out, lse = attention()(q, cache, tables, *ref.device(gpu, np.array(lengths, np.int32)), causal=False, scale=0.3, return_lse=True)
+    check(out, lse, q, keys, values, [n] * len(lengths), group, scale=0.3, causal=False)
+
+
+@pytest.mark.parametrize("n", [1, 60])
+def test_missing_pages_are_left_out(gpu, n):
+    rng = np.random.default_rng(n)
+    lengths, heads, group, dim, page = [500, 200], 2, 4, 64, 32
+    cache, tables, keys, values = filled(gpu, rng, lengths, heads, dim, page)
+    tables[0, 3], tables[0, 7], tables[1, :] = -1, 2**31 - 1, -5
+    gone = [np.zeros(x, dtype=bool) for x in lengths]
+    gone[0][96:128] = gone[0][224:256] = gone[1][:] = True
+    q = rows_of(rng, n * 2, heads * group, dim, torch.bfloat16).to(gpu)
+    out, lse = attention()(q, cache, tables, *ref.device(gpu, np.array(lengths, np.int32)), return_lse=True)
+    check(out, lse, q, keys, values, [n] * 2, group, left_out=gone)
+
+
+@pytest.mark.parametrize("n", [1, 3, 50, 300])
+def test_what_a_row_does_not_see_does_not_reach_it(gpu, n):
+    """NaN in keys and values: of tokens behind a row, before its window, and in the pages behind a sequence."""
+    from mambo_amd.kernels.kv_cache import launch_append_kv
+    rng = np.random.default_rng(n)
+    heads, group, dim, page, length = 1, 2, 64, 32, 330
+    cache = new_cache(12, heads, dim, page)  # NaN codes and scales everywhere
+    tables = torch.from_numpy(rng.permutation(12).astype(np.int32)[None]).to(gpu)
+    k, v = rows_of(rng, length, heads, dim, torch.float32), rows_of(rng, length, heads, dim, torch.float32)
+    bad = length - n + n // 2  # the middle row's own token
+    k[bad, 0, 5], v[20, 0, 3] = float("nan"), float("inf")
+    lengths = torch.tensor([length], dtype=torch.int32, device=gpu)
+    launch_append_kv(k.to(gpu), v.to(gpu), cache, tables, lengths)
+    q = rows_of(rng, n, heads * group, dim, torch.bfloat16).to(gpu)
+    out, lse = attention()(q, cache, tables, lengths, window=25, return_lse=True)
+    spoiled = np.array([bad <= p and bad > p - 25 or 20 <= p and 20 > p - 25 for p in range(length - n, length)])
+    nan = torch.isnan(out).all(2).all(1).cpu().numpy()
+    assert np.array_equal(nan, spoiled) and np.array_equal(torch.isnan(out).any(2).any(1).cpu().numpy(), spoiled)
+    assert np.array_equal(torch.isnan(lse).all(1).cpu().numpy(), spoiled)
+    got_k, got_v = read_all(cache, tables, [length])
+    keys, values = np.nan_to_num(got_k[0]), got_v[0]
+    want, _, bound, _ = ref.attend(q.double().cpu().numpy(), keys, values, group, dim ** -0.5, True, 25)
+    off = np.abs(out.double().cpu().numpy() - want)
+    assert (off[~spoiled] <= bound[~spoiled]).all()
+
+
+@pytest.mark.parametrize("n", [1, 100])
+def test_large_scores(gpu, n):
+    """Scores of hundreds, where one token takes everything, and rows of equal ones."""
+    rng = np.random.default_rng(9)
+    cache, tables, keys, values = filled(gpu, rng, [400], 2, 64, 32)
+    q = rows_of(rng, n, 4, 64, torch.bfloat16, 60.0).to(gpu)
+    q[0, 0] = 0.0
+    out, lse = attention()(q, cache, tables, *ref.device(gpu, np.array([400], np.int32)), return_lse=True)
+    check(out, lse, q, keys, values, [n], 2)
+
+
+def test_strides_alignment_and_repeats(gpu):
+    rng = np.random.default_rng(10)
+    lengths = [300, 45, 1]
+    cache, tables, keys, values = filled(gpu, rng, lengths, 2, 64, 32)
+    on = ref.device(gpu, np.array(lengths, np.int32))[0]
+    for n in (1, 70):
+        base = rows_of(rng, 3 * n, 10, 72, torch.bfloat16).to(gpu)
+        for q in (base[:, :4, :64], base[:, 1:5, 3:67], base[:, ::2, 8:72][:, :4], base[:, :4, :64].flip(2)):
+            whole = torch.full((3 * n, 6, 67), 7.0, dtype=torch.bfloat16, device=gpu)
+            out = whole[:, 1:5, 3:67]
+            first = attention()(q.contiguous(), cache, tables, on)
+            assert attention()(q, cache, tables, on, out=out) is out
+            assert torch.equal(out, first)
+            for _ in range(3):
+                assert torch.equal(attention()(q, cache, tables, on), first)
+            whole[:, 1:5, 3:67] = 7.0
+            assert (whole == 7.0).all()
+    assert attention()(q[:0], cache, tables, on).shape == (0, 4, 64)
+
+
+def test_arrays_of_any_values_stay_within_the_tensors(gpu):
+    rng = np.random.default_rng(11)
+    cache, tables, _, _ = filled(gpu, rng, [300, 45, 100], 2, 64, 32)
+    q = rows_of(rng, 90, 4, 64, torch.bfloat16).to(gpu)
+    for bad in ([-5, 70, 3], [2**31 - 1] * 3, [-2**31] * 3):
+        for cuts in (None, [0, 5, 3, 90], [-9, 4, 99, 2**31 - 1], [90, 10, 5, 0], [7, 7, 7, 7]):
+            attention()(q, cache, tables, torch.tensor(bad, dtype=torch.int32, device=gpu),
+                        offsets=None if cuts is None else torch.tensor(cuts, dtype=torch.int32, device=gpu))
+    torch.cuda.synchronize()
+
+
+def test_a_long_cache_is_split(gpu):
+    """Tens of thousands of tokens, in parts of many workgroups, against a product in float64 on the GPU."""
+    rng = np.random.default_rng(12)
+    for n, heads, group, dim, length in ((1, 2, 4, 64, 40011), (3, 1, 5, 128, 20000), (130, 1, 2, 64, 9000)):
+        cache, tables, keys, values = filled(gpu, rng, [length], heads, dim, 128)
+        q = rows_of(rng, n, heads * group, dim, torch.bfloat16, 2.0).to(gpu)
+        out, lse = attention()(q, cache, tables, *ref.device(gpu, np.array([length], np.int32)), return_lse=True)
+        check(out, lse, q, keys, values, [n], group)
+
+
+def test_offsets_past_32_bits(gpu):
+    """A pool of more than 4 GiB of codes, the sequence's pages at its end."""
+    from mambo_amd.kernels.kv_cache import launch_append_kv
+    from mambo_amd.utils.kv_cache import allocate_kv_cache
+    rng = np.random.default_rng(13)
+    heads, dim, page = 8, 128, 256
+    pages = (5 << 30) // (2 * heads * dim * page)
+    cache = allocate_kv_cache(pages, heads, dim, page_size=page)
+    tables = torch.tensor([[pages - 1, pages - 3]], dtype=torch.int32, device=gpu)
+    lengths = torch.tensor([300], dtype=torch.int32, device=gpu)
+    k, v = rows_of(rng, 300, heads, dim, torch.bfloat16), rows_of(rng, 300, heads, dim, torch.bfloat16)
+    launch_append_kv(k.to(gpu), v.to(gpu), cache, tables, lengths)
+    model = ref.Model(heads, dim)
+    model.append(k.double().numpy(), v.double().numpy(), 0)
+    for n in (1, 40):
+        q = rows_of(rng, n, heads * 2, dim, torch.bfloat16).to(gpu)
+        out, lse = attention()(q, cache, tables, lengths, return_lse=True)
+        check(out, lse, q, [model.k], [model.v], [n], 2)
+    assert not cache.codes[0].any() and math.isfinite(float(out.float().sum()))
