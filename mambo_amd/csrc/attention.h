@@ -67,6 +67,15 @@ __device__ __forceinline__ float e8m0(uint32_t byte) { return __uint_as_float(by
 
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
 
+// Zero, in a vector register: an address that it is part of is one of each lane to the compiler, which otherwise
+// brings a loaded value that all lanes share into a scalar register, and waits for it, right behind the load.
+__device__ __forceinline__ int vector_zero()
+{
+    int zero;
+    asm("v_mov_b32 %0, 0" : "=v"(zero));
+    return zero;
+}
+
 // Codes past the first `left` (of eight) become zeros: what a page holds behind a sequence's last token is
 // anything, and a NaN there times a probability of zero would still be one.
 __device__ __forceinline__ uint2 keep_tokens(uint32_t lo, uint32_t hi, int left)

@@ -64,7 +64,7 @@ int check(const mambo_kv_cache *cache, const mambo_kv_batch *batch, int64_t toke
                   "tables must hold below 2^36 tokens together");
     *p = make_plan(*c, *b, (int)(q_heads / c->heads));
     const int64_t rows = p->few_rows, heads = c->heads;
-    MAMBO_REQUIRE(grid_takes(batch->seqs * heads, 256) && rows <= 65535 && grid_takes(p->tiles * heads, 512) &&
+    MAMBO_REQUIRE(grid_takes(batch->seqs * heads, 256) && rows <= 65535 && grid_takes(p->tiles * heads, 2 * kTileRowsWg) &&
                       grid_takes(tokens * q_heads, 256),
                   MAMBO_ERR_VALUE, "too many rows for one launch");
     return MAMBO_OK;

@@ -191,7 +191,7 @@ __global__ __launch_bounds__(256, 2) void attend_rows_kernel(const Attention a)
         const auto load = [&](int blk, int page_any, Block &b) {
             const int page = __builtin_amdgcn_readfirstlane(page_any);
             b.scales = -1;
-            if (page < 0 || page >= a.cache.pages)
+            if ((uint32_t)page >= (uint32_t)a.cache.pages)
                 return;
             const int64_t at_blk = a.cache.block(page, head, blk);
             const uint4 *codes = reinterpret_cast<const uint4 *>(a.cache.codes + at_blk * (2 * kKvBlock * DP)) + lane;

@@ -25,6 +25,17 @@ __device__ __forceinline__ float halves_sum(float x)
     return __uint_as_float(b[0]) + __uint_as_float(b[1]);
 }
 
+// A word that every lane wants and no kernel writes while this one runs.
+__device__ __forceinline__ int scalar_load(const int32_t *p)
+{
+    return *(const __attribute__((address_space(4))) int32_t *)p;
+}
+
+// Nothing is moved across: between two of these stand one matrix instruction, the read of a later one's operand and
+// the vector instructions for which its 32 cycles leave time.
+#define MAMBO_FIXED_ORDER() __builtin_amdgcn_sched_barrier(0)
+constexpr int kAhead = 4; // operands read ahead
+
 // Tiles of the sequences before s: at least as many as their rows fill.
 __device__ __forceinline__ int64_t tiles_before(const Attention &a, int s)
 {
@@ -35,8 +46,7 @@ template <int DS>
 __global__ __launch_bounds__(kThreads, 2) void attend_tiles_kernel(const Attention a)
 {
     constexpr int DP = 32 * DS, kSteps = DP / 16;
-    constexpr int kPieces = kTileBlocks * DS * 64;               // 16-byte pieces of the keys of a tile, and of its values
-    constexpr int kEach = (kPieces + kThreads - 1) / kThreads;   // of a thread
+    constexpr int kUnits = kTileBlocks * DS, kEach = (kUnits + kWaves - 1) / kWaves; // staged by all waves, and by one
     // keys: [8 values of the head][64 rows of the first product]; values: [8 tokens][value of the head]
     __shared__ bf16x8 keys[2][DP / 8][32 * kTileBlocks];
     __shared__ bf16x8 values[2][4 * kTileBlocks][DP];
@@ -96,140 +106,232 @@ __global__ __launch_bounds__(kThreads, 2) void attend_tiles_kernel(const Attenti
 #pragma unroll
         for (int r = 0; r < 16; ++r)
             o[d][r] = 0.0f;
-    float m = -__builtin_inff(), l = 0.0f;
+    float m = -__builtin_inff(), l[2] = {0.0f, 0.0f};
 
-    uint4 kc[kEach], vc[kEach];
-    uint32_t sc[kEach]; // scales of the piece's block; bit 16: there is no such page
-    const auto load = [&](int blk0) {
+    const int zero = vector_zero();
+    const int32_t *table = a.b.tables + s * a.b.ldt;
+    // Staging: unit u of a tile is 32 values of the head of one of its blocks, a wave's 64 pieces of 16 bytes.
+    // Its blocks' pages are read a tile ahead of its codes, by scalar loads that nothing waits for in between.
+    struct Pages {
+        int of[kTileBlocks];
+    };
+    const auto pages_of = [&](int blk0) {
+        Pages p;
+#pragma unroll
+        for (int b = 0; b < kTileBlocks; ++b)
+            p.of[b] = scalar_load(table + (min(blk0 + b, hi - 1) >> a.cache.shift));
+        return p;
+    };
+    const auto has_page = [&](int blk, int page) { return blk < hi && (uint32_t)page < (uint32_t)a.cache.pages; };
+    // Loads and what is made of them have no branch between, whose end would wait for them: codes of a block that is
+    // not there are some other block's.
+    struct Codes {
+        uint4 c[kEach];
+        uint32_t scale[kEach]; // E8M0
+    };
+    const int in_page = (1 << a.cache.shift) - 1;
+    const auto load = [&](int blk0, const Pages &p, int of_values, Codes &x) {
 #pragma unroll
         for (int e = 0; e < kEach; ++e) {
-            const int piece = tid + kThreads * e, blk = blk0 + piece / (64 * DS);
-            kc[e] = vc[e] = make_uint4(0u, 0u, 0u, 0u);
-            sc[e] = 1u << 16;
-            if (piece >= kPieces || blk >= hi)
-                continue;
-            const int page = a.b.page(s, blk >> a.cache.shift);
-            if (page < 0 || page >= a.cache.pages)
-                continue;
+            const int u = min(wave + kWaves * e, kUnits - 1), b = u / DS, blk = blk0 + b;
+            const int any = b ? p.of[1] : p.of[0], page = has_page(blk, any) ? any : 0;
             const int64_t at = a.cache.block(page, head, blk);
-            const uint4 *codes = reinterpret_cast<const uint4 *>(a.cache.codes + at * (2 * kKvBlock * DP)) + piece % (64 * DS);
-            kc[e] = codes[0];
-            vc[e] = codes[64 * DS];
-            sc[e] = *reinterpret_cast<const uint16_t *>(a.cache.scales + 2 * at);
+            x.c[e] = reinterpret_cast<const uint4 *>(a.cache.codes + (at * 2 + of_values) * (kKvBlock * DP))[64 * (u % DS) + lane];
+            x.scale[e] = a.cache.scales[2 * at + of_values + zero];
         }
     };
-    // Piece (block b, 32 values ds, lane 16 kk + j) has, of the keys, tokens 8 (j / 4) + j % 4 and 4 more, which are
-    // rows 16 (j / 8) + 4 (j / 4 % 2) + j % 4 and 8 more of the first product.
-    const auto widen_tile = [&](int blk0, int buf) {
+    // Piece 16 kk + j has, of the keys, tokens 8 (j / 4) + j % 4 and 4 more, which are rows 16 (j / 8) + 4 (j / 4 % 2) +
+    // j % 4 and 8 more of the first product.
+    const int kk = lane >> 4, j16 = lane & 15, key_row = 16 * (j16 >> 3) + 4 * (j16 >> 2 & 1) + (j16 & 3);
+    const auto widen_keys = [&](Codes &x, int buf) {
 #pragma unroll
         for (int e = 0; e < kEach; ++e) {
-            const int piece = tid + kThreads * e;
-            if (kPieces % kThreads && piece >= kPieces)
+            const int u = wave + kWaves * e, b = u / DS, ds = u % DS;
+            asm volatile("" : "+v"(x.scale[e])); // not before
+            if (u >= kUnits)
                 continue;
-            const int b = piece / (64 * DS), ds = piece / 64 % DS, kk = piece >> 4 & 3, j = piece & 15;
-            const bool none = sc[e] >> 16;
-            const float ks = none ? 1.0f : e8m0(sc[e] & 255), vs = none ? 1.0f : e8m0(sc[e] >> 8);
-            const int at = 32 * b + 16 * (j >> 3) + 4 * (j >> 2 & 1) + (j & 3);
-            keys[buf][4 * ds + kk][at] = widen(kc[e].x, kc[e].y, ks);
-            keys[buf][4 * ds + kk][at + 8] = widen(kc[e].z, kc[e].w, ks);
-            uint2 v0 = make_uint2(vc[e].x, vc[e].y), v1 = make_uint2(vc[e].z, vc[e].w);
-            const int left = seq.len - (blk0 + b) * kKvBlock - 8 * kk;
-            if (left < 8) {
+            const float scale = e8m0(x.scale[e]);
+            keys[buf][4 * ds + kk][32 * b + key_row] = widen(x.c[e].x, x.c[e].y, scale);
+            keys[buf][4 * ds + kk][32 * b + key_row + 8] = widen(x.c[e].z, x.c[e].w, scale);
+        }
+    };
+    const auto widen_values = [&](Codes &x, int blk0, const Pages &p, int buf) {
+#pragma unroll
+        for (int e = 0; e < kEach; ++e) {
+            const int u = wave + kWaves * e, b = u / DS, ds = u % DS;
+            asm volatile("" : "+v"(x.scale[e]));
+            if (u >= kUnits)
+                continue;
+            uint2 v0 = make_uint2(x.c[e].x, x.c[e].y), v1 = make_uint2(x.c[e].z, x.c[e].w);
+            const bool there = has_page(blk0 + b, b ? p.of[1] : p.of[0]);
+            const float scale = there ? e8m0(x.scale[e]) : 1.0f; // a scale of anything would make NaN of zeros
+            if ((blk0 + b + 1) * kKvBlock > seq.len || !there) {
+                const int left = there ? seq.len - (blk0 + b) * kKvBlock - 8 * kk : 0;
                 v0 = keep_tokens(v0.x, v0.y, left);
                 v1 = keep_tokens(v1.x, v1.y, left);
             }
-            values[buf][4 * b + kk][32 * ds + j] = widen(v0.x, v0.y, vs);
-            values[buf][4 * b + kk][32 * ds + 16 + j] = widen(v1.x, v1.y, vs);
+            values[buf][4 * b + kk][32 * ds + j16] = widen(v0.x, v0.y, scale);
+            values[buf][4 * b + kk][32 * ds + 16 + j16] = widen(v1.x, v1.y, scale);
         }
     };
-    // Pages that a table does not have: their tokens are left out (bit b: block b of the tile).
-    const auto missing = [&](int blk0) {
-        uint32_t gone = 0;
+
+    struct Scores {
+        v16f x[kTileBlocks];
+    };
+    v16f zeros;
+#pragma unroll
+    for (int r = 0; r < 16; ++r)
+        zeros[r] = 0.0f;
+    const auto first_product = [&](Scores &sx, int buf) {
+#pragma unroll
+        for (int d = 0; d < kSteps; ++d)
+#pragma unroll
+            for (int b = 0; b < kTileBlocks; ++b)
+                sx.x[b] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(keys[buf][2 * d + half][32 * b + col], q[d], d ? sx.x[b] : zeros, 0, 0, 0);
+    };
+    // Whether any row of the wave sees any token of the tile.
+    const auto seen = [&](int blk0) { return blk0 * kKvBlock < any_to && (blk0 + kTileBlocks) * kKvBlock > any_from; };
+
+    // Leaves out what a row does not see and tokens without a page.
+    const auto mask = [&](int blk0, const Pages &pages, Scores &sx) {
+        const int token0 = blk0 * kKvBlock;
+        const uint32_t gone = (has_page(blk0, pages.of[0]) ? 0u : 1u) | (has_page(blk0 + 1, pages.of[1]) ? 0u : 2u);
+        if (token0 + 32 * kTileBlocks > all_to || token0 < all_from || gone) {
+            // score r of a block is of its token 16 (r / 8) + 8 half + r % 8
+#pragma unroll
+            for (int b = 0; b < kTileBlocks; ++b)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    const int token = token0 + 32 * b + 16 * (r >> 3) + 8 * half + (r & 7);
+                    if (!(token < to && token >= from) || (gone >> b & 1))
+                        sx.x[b][r] = -__builtin_inff();
+                }
+        }
+    };
+    const auto largest = [&](const Scores &sx) {
+        float top = -__builtin_inff();
 #pragma unroll
         for (int b = 0; b < kTileBlocks; ++b)
-            if (blk0 + b < hi) {
-                const int page = a.b.page(s, (blk0 + b) >> a.cache.shift);
-                gone |= (page < 0 || page >= a.cache.pages) ? 1u << b : 0u;
-            } else {
-                gone |= 1u << b;
-            }
-        return (uint32_t)__builtin_amdgcn_readfirstlane(gone);
+#pragma unroll
+            for (int r = 0; r < 16; ++r)
+                top = fmaxf(top, sx.x[b][r]);
+        return top;
     };
 
+    Pages p0, p1, p2;
+    Scores even, odd;
+    float top = -__builtin_inff(); // of the scores at hand, before the halves of a row are put together
     if (lo < hi) {
-        load(lo);
-        widen_tile(lo, 0);
+        Codes k0, v0, k1;
+        p0 = pages_of(lo), p1 = pages_of(lo + kTileBlocks), p2 = pages_of(lo + 2 * kTileBlocks);
+        load(lo, p0, false, k0);
+        load(lo, p0, true, v0);
+        load(lo + kTileBlocks, p1, false, k1);
+        widen_keys(k0, 0);
+        widen_values(v0, lo, p0, 0);
+        widen_keys(k1, 1);
+        __syncthreads();
+        if (seen(lo)) {
+            first_product(even, 0);
+            mask(lo, p0, even);
+            top = largest(even);
+        }
     }
-    __syncthreads();
-    for (int blk = lo, buf = 0; blk < hi; blk += kTileBlocks, buf ^= 1) {
-        const bool more = blk + kTileBlocks < hi;
-        if (more)
-            load(blk + kTileBlocks);
-        const int token0 = blk * kKvBlock;
-        if (token0 < any_to && token0 + 32 * kTileBlocks > any_from) { // of the wave's rows some see some
-            const uint32_t gone = missing(blk);
-            v16f sx[kTileBlocks];
-#pragma unroll
-            for (int b = 0; b < kTileBlocks; ++b)
-#pragma unroll
-                for (int r = 0; r < 16; ++r)
-                    sx[b][r] = 0.0f;
-#pragma unroll
-            for (int d = 0; d < kSteps; ++d)
-#pragma unroll
-                for (int b = 0; b < kTileBlocks; ++b)
-                    sx[b] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(keys[buf][2 * d + half][32 * b + col], q[d], sx[b], 0, 0, 0);
-            const bool edge = token0 + 32 * kTileBlocks > all_to || token0 < all_from || gone;
-            // score r of a block is of its token 16 (r / 8) + 8 half + r % 8
-            float top = -__builtin_inff();
-            if (edge) {
-#pragma unroll
-                for (int b = 0; b < kTileBlocks; ++b)
-#pragma unroll
-                    for (int r = 0; r < 16; ++r) {
-                        const int token = token0 + 32 * b + 16 * (r >> 3) + 8 * half + (r & 7);
-                        if (!(token < to && token >= from) || (gone >> b & 1))
-                            sx[b][r] = -__builtin_inff();
-                    }
-            }
-#pragma unroll
-            for (int b = 0; b < kTileBlocks; ++b)
-#pragma unroll
-                for (int r = 0; r < 16; ++r)
-                    top = fmaxf(top, sx[b][r]);
-            top = halves_max(top);
-            top *= a.scale;
-            if (__any(top > m)) {
+    // Tile at blk, whose scores are in `sx`: the next one's scores go into `next` by matrix instructions that the
+    // exponentials of this one run beside, and its largest are found beside the second product. Keys are staged a
+    // tile further ahead than values, so that of each two buffers and one barrier a tile do: what is written was
+    // last read before the barrier.
+    const auto step = [&](int blk, int buf, Scores &sx, Scores &next) {
+        __syncthreads();
+        const Pages p3 = pages_of(blk + 3 * kTileBlocks);
+        Codes kc, vc;
+        load(blk + 2 * kTileBlocks, p2, false, kc);
+        load(blk + kTileBlocks, p1, true, vc);
+        if (seen(blk)) {
+            top = halves_max(top) * a.scale;
+            // The running largest may lag by 2^8: probabilities up to there are as exact, and sums are far from
+            // overflow; most tiles then leave the sums as they are.
+            if (__any(top > m + 8.0f || m == -__builtin_inff())) {
                 const float grown = fmaxf(m, top);
                 const float by = m == -__builtin_inff() ? 0.0f : exp2_fast(m - grown);
                 m = grown;
-                l *= by;
+                l[0] *= by;
+                l[1] *= by;
 #pragma unroll
                 for (int d = 0; d < DS; ++d)
                     o[d] *= by;
             }
             const float less = m == -__builtin_inff() ? 0.0f : m;
-            bf16x8 p[2 * kTileBlocks];
+            bf16x8 p[2 * kTileBlocks], ahead[kAhead];
+            constexpr int kFirst = kTileBlocks * kSteps, kSecond = 2 * kTileBlocks * DS;
+            const auto key = [&](int n) { return keys[buf ^ 1][2 * (n / kTileBlocks) + half][32 * (n % kTileBlocks) + col]; };
+            const auto value = [&](int n) { return values[buf][2 * (n / DS) + half][32 * (n % DS) + col]; };
+            // Of the 32 probabilities of a lane 20 are worked out beside the first product, 12 beside the first half of
+            // the second (whose operands they are later), the next tile's largest beside the other half: about as much
+            // for the vector unit in all of them.
+            constexpr int kEarly = 10 * kTileBlocks, kLate = 6 * kTileBlocks;
+            const auto probability = [&](int i) {
+                const float y = exp2_fast(__builtin_fmaf(sx.x[i / 16][i % 16], a.scale, -less));
+                l[i & 1] += y;
+                p[i / 8][i % 8] = (__bf16)y;
+                if (i % 8 == 7 || i == kEarly - 1) // here, and not where it is used
+                    asm volatile("" : "+v"(p[i / 8]), "+v"(l[0]), "+v"(l[1]));
+            };
+            MAMBO_FIXED_ORDER();
 #pragma unroll
-            for (int b = 0; b < kTileBlocks; ++b)
+            for (int n = 0; n < kAhead; ++n)
+                ahead[n] = key(n);
 #pragma unroll
-                for (int r = 0; r < 16; ++r) {
-                    const float y = exp2_fast(__builtin_fmaf(sx[b][r], a.scale, -less));
-                    l += y;
-                    p[2 * b + (r >> 3)][r & 7] = (__bf16)y;
+            for (int n = 0; n < kFirst; ++n) {
+                MAMBO_FIXED_ORDER();
+                v16f &x = next.x[n % kTileBlocks];
+                x = __builtin_amdgcn_mfma_f32_32x32x16_bf16(ahead[n % kAhead], q[n / kTileBlocks], n < kTileBlocks ? zeros : x, 0, 0, 0);
+                if (n + kAhead < kFirst)
+                    ahead[n % kAhead] = key(n + kAhead);
+                else
+                    ahead[n % kAhead] = value(n + kAhead - kFirst);
+#pragma unroll
+                for (int i = n * kEarly / kFirst; i < (n + 1) * kEarly / kFirst; ++i)
+                    probability(i);
+            }
+            MAMBO_FIXED_ORDER();
+            mask(blk + kTileBlocks, p1, next);
+            top = -__builtin_inff();
+#pragma unroll
+            for (int n = 0; n < kSecond; ++n) {
+                MAMBO_FIXED_ORDER();
+                o[n % DS] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(ahead[(kFirst + n) % kAhead], p[n / DS], o[n % DS], 0, 0, 0);
+                if (n + kAhead < kSecond)
+                    ahead[(kFirst + n) % kAhead] = value(n + kAhead);
+                constexpr int kHalf = kSecond / 2;
+                if (n < kHalf) {
+#pragma unroll
+                    for (int i = n * kLate / kHalf; i < (n + 1) * kLate / kHalf; ++i)
+                        probability(kEarly + i);
+                } else {
+#pragma unroll
+                    for (int i = (n - kHalf) * 16 * kTileBlocks / kHalf; i < (n - kHalf + 1) * 16 * kTileBlocks / kHalf; ++i)
+                        top = fmaxf(top, next.x[i / 16][i % 16]);
                 }
-#pragma unroll
-            for (int k = 0; k < 2 * kTileBlocks; ++k)
-#pragma unroll
-                for (int d = 0; d < DS; ++d)
-                    o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(values[buf][2 * k + half][32 * d + col], p[k], o[d], 0, 0, 0);
+            }
+            MAMBO_FIXED_ORDER();
+        } else if (seen(blk + kTileBlocks)) {
+            first_product(next, buf ^ 1);
+            mask(blk + kTileBlocks, p1, next);
+            top = largest(next);
         }
-        if (more)
-            widen_tile(blk + kTileBlocks, buf ^ 1);
-        __syncthreads();
+        widen_keys(kc, buf);
+        widen_values(vc, blk + kTileBlocks, p1, buf ^ 1);
+        p0 = p1, p1 = p2, p2 = p3;
+    };
+    for (int blk = lo; blk < hi; blk += 2 * kTileBlocks) {
+        step(blk, 0, even, odd);
+        if (blk + kTileBlocks >= hi)
+            break;
+        step(blk + kTileBlocks, 1, odd, even);
     }
 
-    l = halves_sum(l);
+    const float sum = halves_sum(l[0] + l[1]);
     if (!some)
         return;
     const int64_t t = seq.first + i, q_heads = (int64_t)a.group * a.cache.heads;
@@ -242,10 +344,10 @@ __global__ __launch_bounds__(kThreads, 2) void attend_tiles_kernel(const Attenti
                 *reinterpret_cast<v4f *>(a.tiles_o + entry * DP + 32 * d + 2 * r + 4 * half) =
                     v4f{o[d][r], o[d][r + 1], o[d][r + 2], o[d][r + 3]};
         if (half == 0)
-            *reinterpret_cast<float2 *>(a.tiles_ml + entry * 2) = make_float2(m, l);
+            *reinterpret_cast<float2 *>(a.tiles_ml + entry * 2) = make_float2(m, sum);
         return;
     }
-    const float by = l == 0.0f ? 0.0f : 1.0f / l;
+    const float by = sum == 0.0f ? 0.0f : 1.0f / sum;
     const bool vec = a.ldot % 4 == 0 && a.ldoh % 4 == 0 && (uintptr_t)a.out % 8 == 0;
 #pragma unroll
     for (int d = 0; d < DS; ++d)
@@ -257,7 +359,7 @@ __global__ __launch_bounds__(kThreads, 2) void attend_tiles_kernel(const Attenti
                                  v4f{o[d][r] * by, o[d][r + 1] * by, o[d][r + 2] * by, o[d][r + 3] * by}, a.cache.dim - at, vec);
         }
     if (a.lse && half == 0)
-        a.lse[t * q_heads + h] = l == 0.0f ? -__builtin_inff() : (m + __log2f(l)) * kLn2;
+        a.lse[t * q_heads + h] = sum == 0.0f ? -__builtin_inff() : (m + __log2f(sum)) * kLn2;
 }
 
 // Rows whose keys were dealt to several workgroups: their sums weighted by the largest scores, in order.

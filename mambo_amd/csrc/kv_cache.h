@@ -28,8 +28,7 @@ __host__ __device__ constexpr int kv_value_byte(int token, int d)
 
 struct KvCache {
     uint8_t *codes, *scales;
-    int64_t pages;
-    int heads, dim, shift; // blocks of a page: 1 << shift
+    int pages, heads, dim, shift; // blocks of a page: 1 << shift
     // Index of a block, for 2 * 32 * padded bytes of codes and 2 of scales; page within [0, pages).
     __device__ int64_t block(int page, int head, int b) const
     {

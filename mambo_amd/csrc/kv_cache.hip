@@ -272,7 +272,7 @@ __global__ __launch_bounds__(256) void append_kernel(const Append a)
         rotate_queries(lo, hi - lo);
 
     const int page = a.b.page(s, blk >> a.cache.shift);
-    if (page < 0 || page >= a.cache.pages)
+    if ((uint32_t)page >= (uint32_t)a.cache.pages)
         return;
     const int64_t at = a.cache.block(page, head, blk);
     uint8_t *const keys = a.cache.codes + at * (2 * kKvBlock * padded), *const values = keys + kKvBlock * padded;
@@ -536,7 +536,7 @@ int kv_check_cache(const mambo_kv_cache *c, KvCache *out)
     MAMBO_REQUIRE(c->codes && c->scales, MAMBO_ERR_VALUE, "null pointer");
     MAMBO_REQUIRE((uintptr_t)c->codes % 16 == 0 && (uintptr_t)c->scales % 2 == 0, MAMBO_ERR_VALUE,
                   "codes must be 16-byte and scales 2-byte aligned");
-    *out = {c->codes, c->scales, c->pages, c->heads, c->head_dim, __builtin_ctz(c->page_size / kKvBlock)};
+    *out = {c->codes, c->scales, (int)c->pages, c->heads, c->head_dim, __builtin_ctz(c->page_size / kKvBlock)};
     return MAMBO_OK;
 }
 
