@@ -143,35 +143,27 @@ __global__ __launch_bounds__(kThreads, 2) void attend_tiles_kernel(const Attenti
     // Piece 16 kk + j has, of the keys, tokens 8 (j / 4) + j % 4 and 4 more, which are rows 16 (j / 8) + 4 (j / 4 % 2) +
     // j % 4 and 8 more of the first product.
     const int kk = lane >> 4, j16 = lane & 15, key_row = 16 * (j16 >> 3) + 4 * (j16 >> 2 & 1) + (j16 & 3);
-    const auto widen_keys = [&](Codes &x, int buf) {
-#pragma unroll
-        for (int e = 0; e < kEach; ++e) {
-            const int u = wave + kWaves * e, b = u / DS, ds = u % DS;
-            asm volatile("" : "+v"(x.scale[e])); // not before
-            if (u >= kUnits)
-                continue;
-            const float scale = e8m0(x.scale[e]);
-            keys[buf][4 * ds + kk][32 * b + key_row] = widen(x.c[e].x, x.c[e].y, scale);
-            keys[buf][4 * ds + kk][32 * b + key_row + 8] = widen(x.c[e].z, x.c[e].w, scale);
-        }
+    // Half h of piece e; a wave without a unit of its own does another's once more.
+    const auto widen_keys = [&](const Codes &x, int e, int h, int buf) {
+        const int u = min(wave + kWaves * e, kUnits - 1), b = u / DS, ds = u % DS;
+        keys[buf][4 * ds + kk][32 * b + key_row + 8 * h] = widen(h ? x.c[e].z : x.c[e].x, h ? x.c[e].w : x.c[e].y, e8m0(x.scale[e]));
     };
-    const auto widen_values = [&](Codes &x, int blk0, const Pages &p, int buf) {
+    const auto widen_values = [&](const Codes &x, int e, int h, int buf) {
+        const int u = min(wave + kWaves * e, kUnits - 1), b = u / DS, ds = u % DS;
+        values[buf][4 * b + kk][32 * ds + 16 * h + j16] = widen(h ? x.c[e].z : x.c[e].x, h ? x.c[e].w : x.c[e].y, e8m0(x.scale[e]));
+    };
+    // Values behind the sequence's last token, and of a block without a page, become zeros.
+    const auto trim_values = [&](Codes &x, int blk0, const Pages &p) {
 #pragma unroll
         for (int e = 0; e < kEach; ++e) {
-            const int u = wave + kWaves * e, b = u / DS, ds = u % DS;
-            asm volatile("" : "+v"(x.scale[e]));
-            if (u >= kUnits)
-                continue;
-            uint2 v0 = make_uint2(x.c[e].x, x.c[e].y), v1 = make_uint2(x.c[e].z, x.c[e].w);
+            const int u = min(wave + kWaves * e, kUnits - 1), b = u / DS;
             const bool there = has_page(blk0 + b, b ? p.of[1] : p.of[0]);
-            const float scale = there ? e8m0(x.scale[e]) : 1.0f; // a scale of anything would make NaN of zeros
             if ((blk0 + b + 1) * kKvBlock > seq.len || !there) {
                 const int left = there ? seq.len - (blk0 + b) * kKvBlock - 8 * kk : 0;
-                v0 = keep_tokens(v0.x, v0.y, left);
-                v1 = keep_tokens(v1.x, v1.y, left);
+                const uint2 v0 = keep_tokens(x.c[e].x, x.c[e].y, left), v1 = keep_tokens(x.c[e].z, x.c[e].w, left);
+                x.c[e] = make_uint4(v0.x, v0.y, v1.x, v1.y);
+                x.scale[e] = there ? x.scale[e] : 127u; // a scale of anything would make NaN of zeros
             }
-            values[buf][4 * b + kk][32 * ds + j16] = widen(v0.x, v0.y, scale);
-            values[buf][4 * b + kk][32 * ds + 16 + j16] = widen(v1.x, v1.y, scale);
         }
     };
 
@@ -219,17 +211,24 @@ __global__ __launch_bounds__(kThreads, 2) void attend_tiles_kernel(const Attenti
     };
 
     Pages p0, p1, p2;
+    Codes kc, vc; // keys two tiles ahead, values one
     Scores even, odd;
     float top = -__builtin_inff(); // of the scores at hand, before the halves of a row are put together
     if (lo < hi) {
-        Codes k0, v0, k1;
+        Codes k0, v0;
         p0 = pages_of(lo), p1 = pages_of(lo + kTileBlocks), p2 = pages_of(lo + 2 * kTileBlocks);
         load(lo, p0, false, k0);
         load(lo, p0, true, v0);
-        load(lo + kTileBlocks, p1, false, k1);
-        widen_keys(k0, 0);
-        widen_values(v0, lo, p0, 0);
-        widen_keys(k1, 1);
+        load(lo + kTileBlocks, p1, false, kc);
+        trim_values(v0, lo, p0);
+#pragma unroll
+        for (int i = 0; i < 2 * kEach; ++i) {
+            widen_keys(k0, i / 2, i % 2, 0);
+            widen_values(v0, i / 2, i % 2, 0);
+            widen_keys(kc, i / 2, i % 2, 1);
+        }
+        load(lo + 2 * kTileBlocks, p2, false, kc);
+        load(lo + kTileBlocks, p1, true, vc);
         __syncthreads();
         if (seen(lo)) {
             first_product(even, 0);
@@ -244,9 +243,13 @@ __global__ __launch_bounds__(kThreads, 2) void attend_tiles_kernel(const Attenti
     const auto step = [&](int blk, int buf, Scores &sx, Scores &next) {
         __syncthreads();
         const Pages p3 = pages_of(blk + 3 * kTileBlocks);
-        Codes kc, vc;
-        load(blk + 2 * kTileBlocks, p2, false, kc);
-        load(blk + kTileBlocks, p1, true, vc);
+        trim_values(vc, blk + kTileBlocks, p1);
+        const auto widen_part = [&](int i) { // of 4 kEach
+            if (i < 2 * kEach)
+                widen_keys(kc, i / 2, i % 2, buf);
+            else
+                widen_values(vc, i / 2 - kEach, i % 2, buf ^ 1);
+        };
         if (seen(blk)) {
             top = halves_max(top) * a.scale;
             // The running largest may lag by 2^8: probabilities up to there are as exact, and sums are far from
@@ -267,8 +270,8 @@ __global__ __launch_bounds__(kThreads, 2) void attend_tiles_kernel(const Attenti
             const auto key = [&](int n) { return keys[buf ^ 1][2 * (n / kTileBlocks) + half][32 * (n % kTileBlocks) + col]; };
             const auto value = [&](int n) { return values[buf][2 * (n / DS) + half][32 * (n % DS) + col]; };
             // Of the 32 probabilities of a lane 20 are worked out beside the first product, 12 beside the first half of
-            // the second (whose operands they are later), the next tile's largest beside the other half: about as much
-            // for the vector unit in all of them.
+            // the second (whose operands they are later), the next tile's largest and the widening of what was loaded for
+            // later ones beside the other half: about as much for the vector unit in all of them.
             constexpr int kEarly = 10 * kTileBlocks, kLate = 6 * kTileBlocks;
             const auto probability = [&](int i) {
                 const float y = exp2_fast(__builtin_fmaf(sx.x[i / 16][i % 16], a.scale, -less));
@@ -312,16 +315,24 @@ __global__ __launch_bounds__(kThreads, 2) void attend_tiles_kernel(const Attenti
 #pragma unroll
                     for (int i = (n - kHalf) * 16 * kTileBlocks / kHalf; i < (n - kHalf + 1) * 16 * kTileBlocks / kHalf; ++i)
                         top = fmaxf(top, next.x[i / 16][i % 16]);
+#pragma unroll
+                    for (int i = (n - kHalf) * 4 * kEach / kHalf; i < (n - kHalf + 1) * 4 * kEach / kHalf; ++i)
+                        widen_part(i);
                 }
             }
             MAMBO_FIXED_ORDER();
-        } else if (seen(blk + kTileBlocks)) {
-            first_product(next, buf ^ 1);
-            mask(blk + kTileBlocks, p1, next);
-            top = largest(next);
+        } else {
+            if (seen(blk + kTileBlocks)) {
+                first_product(next, buf ^ 1);
+                mask(blk + kTileBlocks, p1, next);
+                top = largest(next);
+            }
+#pragma unroll
+            for (int i = 0; i < 4 * kEach; ++i)
+                widen_part(i);
         }
-        widen_keys(kc, buf);
-        widen_values(vc, blk + kTileBlocks, p1, buf ^ 1);
+        load(blk + 3 * kTileBlocks, p3, false, kc);
+        load(blk + 2 * kTileBlocks, p2, true, vc);
         p0 = p1, p1 = p2, p2 = p3;
     };
     for (int blk = lo; blk < hi; blk += 2 * kTileBlocks) {
