@@ -114,6 +114,7 @@ __global__ __launch_bounds__(kThreads, 2) void attend_tiles_kernel(const Attenti
     // Its blocks' pages are read a tile ahead of its codes, by scalar loads that nothing waits for in between.
     struct Pages {
         int of[kTileBlocks];
+        uint32_t gone; // bit b: there is no page for block b
     };
     const auto pages_of = [&](int blk0) {
         Pages p;
@@ -122,22 +123,40 @@ __global__ __launch_bounds__(kThreads, 2) void attend_tiles_kernel(const Attenti
             p.of[b] = scalar_load(table + (min(blk0 + b, hi - 1) >> a.cache.shift));
         return p;
     };
-    const auto has_page = [&](int blk, int page) { return blk < hi && (uint32_t)page < (uint32_t)a.cache.pages; };
+    const auto checked = [&](int blk0, Pages p) {
+        p.gone = 0;
+#pragma unroll
+        for (int b = 0; b < kTileBlocks; ++b)
+            if (blk0 + b >= hi || (uint32_t)p.of[b] >= (uint32_t)a.cache.pages) {
+                p.of[b] = 0;
+                p.gone |= 1u << b;
+            }
+        return p;
+    };
     // Loads and what is made of them have no branch between, whose end would wait for them: codes of a block that is
     // not there are some other block's.
     struct Codes {
         uint4 c[kEach];
         uint32_t scale[kEach]; // E8M0
     };
-    const int in_page = (1 << a.cache.shift) - 1;
-    const auto load = [&](int blk0, const Pages &p, int of_values, Codes &x) {
+    struct Place {
+        int64_t at[kEach]; // of the unit's block, twice, and one more for its values
+    };
+    const auto place_of = [&](int blk0, const Pages &p, int of_values) {
+        Place x;
 #pragma unroll
         for (int e = 0; e < kEach; ++e) {
-            const int u = min(wave + kWaves * e, kUnits - 1), b = u / DS, blk = blk0 + b;
-            const int any = b ? p.of[1] : p.of[0], page = has_page(blk, any) ? any : 0;
-            const int64_t at = a.cache.block(page, head, blk);
-            x.c[e] = reinterpret_cast<const uint4 *>(a.cache.codes + (at * 2 + of_values) * (kKvBlock * DP))[64 * (u % DS) + lane];
-            x.scale[e] = a.cache.scales[2 * at + of_values + zero];
+            const int b = min(wave + kWaves * e, kUnits - 1) / DS;
+            x.at[e] = 2 * (int64_t)a.cache.block(b ? p.of[1] : p.of[0], head, blk0 + b) + of_values;
+        }
+        return x;
+    };
+    const auto load = [&](const Place &p, Codes &x) {
+#pragma unroll
+        for (int e = 0; e < kEach; ++e) {
+            const int ds = min(wave + kWaves * e, kUnits - 1) % DS;
+            x.c[e] = reinterpret_cast<const uint4 *>(a.cache.codes + p.at[e] * (kKvBlock * DP))[64 * ds + lane];
+            x.scale[e] = a.cache.scales[p.at[e] + zero];
         }
     };
     // Piece 16 kk + j has, of the keys, tokens 8 (j / 4) + j % 4 and 4 more, which are rows 16 (j / 8) + 4 (j / 4 % 2) +
@@ -157,7 +176,7 @@ __global__ __launch_bounds__(kThreads, 2) void attend_tiles_kernel(const Attenti
 #pragma unroll
         for (int e = 0; e < kEach; ++e) {
             const int u = min(wave + kWaves * e, kUnits - 1), b = u / DS;
-            const bool there = has_page(blk0 + b, b ? p.of[1] : p.of[0]);
+            const bool there = !(p.gone >> b & 1);
             if ((blk0 + b + 1) * kKvBlock > seq.len || !there) {
                 const int left = there ? seq.len - (blk0 + b) * kKvBlock - 8 * kk : 0;
                 const uint2 v0 = keep_tokens(x.c[e].x, x.c[e].y, left), v1 = keep_tokens(x.c[e].z, x.c[e].w, left);
@@ -187,15 +206,14 @@ __global__ __launch_bounds__(kThreads, 2) void attend_tiles_kernel(const Attenti
     // Leaves out what a row does not see and tokens without a page.
     const auto mask = [&](int blk0, const Pages &pages, Scores &sx) {
         const int token0 = blk0 * kKvBlock;
-        const uint32_t gone = (has_page(blk0, pages.of[0]) ? 0u : 1u) | (has_page(blk0 + 1, pages.of[1]) ? 0u : 2u);
-        if (token0 + 32 * kTileBlocks > all_to || token0 < all_from || gone) {
+        if (token0 + 32 * kTileBlocks > all_to || token0 < all_from || pages.gone) {
             // score r of a block is of its token 16 (r / 8) + 8 half + r % 8
 #pragma unroll
             for (int b = 0; b < kTileBlocks; ++b)
 #pragma unroll
                 for (int r = 0; r < 16; ++r) {
                     const int token = token0 + 32 * b + 16 * (r >> 3) + 8 * half + (r & 7);
-                    if (!(token < to && token >= from) || (gone >> b & 1))
+                    if (!(token < to && token >= from) || (pages.gone >> b & 1))
                         sx.x[b][r] = -__builtin_inff();
                 }
         }
@@ -210,16 +228,18 @@ __global__ __launch_bounds__(kThreads, 2) void attend_tiles_kernel(const Attenti
         return top;
     };
 
-    Pages p0, p1, p2;
+    Pages p1, p2; // of the next tile and the one after it
     Codes kc, vc; // keys two tiles ahead, values one
     Scores even, odd;
     float top = -__builtin_inff(); // of the scores at hand, before the halves of a row are put together
     if (lo < hi) {
         Codes k0, v0;
-        p0 = pages_of(lo), p1 = pages_of(lo + kTileBlocks), p2 = pages_of(lo + 2 * kTileBlocks);
-        load(lo, p0, false, k0);
-        load(lo, p0, true, v0);
-        load(lo + kTileBlocks, p1, false, kc);
+        Pages p0 = pages_of(lo);
+        p1 = pages_of(lo + kTileBlocks), p2 = pages_of(lo + 2 * kTileBlocks);
+        p0 = checked(lo, p0), p1 = checked(lo + kTileBlocks, p1), p2 = checked(lo + 2 * kTileBlocks, p2);
+        load(place_of(lo, p0, 0), k0);
+        load(place_of(lo, p0, 1), v0);
+        load(place_of(lo + kTileBlocks, p1, 0), kc);
         trim_values(v0, lo, p0);
 #pragma unroll
         for (int i = 0; i < 2 * kEach; ++i) {
@@ -227,8 +247,8 @@ __global__ __launch_bounds__(kThreads, 2) void attend_tiles_kernel(const Attenti
             widen_values(v0, i / 2, i % 2, 0);
             widen_keys(kc, i / 2, i % 2, 1);
         }
-        load(lo + 2 * kTileBlocks, p2, false, kc);
-        load(lo + kTileBlocks, p1, true, vc);
+        load(place_of(lo + 2 * kTileBlocks, p2, 0), kc);
+        load(place_of(lo + kTileBlocks, p1, 1), vc);
         __syncthreads();
         if (seen(lo)) {
             first_product(even, 0);
@@ -242,13 +262,19 @@ __global__ __launch_bounds__(kThreads, 2) void attend_tiles_kernel(const Attenti
     // last read before the barrier.
     const auto step = [&](int blk, int buf, Scores &sx, Scores &next) {
         __syncthreads();
-        const Pages p3 = pages_of(blk + 3 * kTileBlocks);
+        Pages p3 = pages_of(blk + 3 * kTileBlocks);
         trim_values(vc, blk + kTileBlocks, p1);
         const auto widen_part = [&](int i) { // of 4 kEach
             if (i < 2 * kEach)
                 widen_keys(kc, i / 2, i % 2, buf);
             else
                 widen_values(vc, i / 2 - kEach, i % 2, buf ^ 1);
+        };
+        Place next_keys, next_values;
+        const auto find_next = [&] {
+            p3 = checked(blk + 3 * kTileBlocks, p3);
+            next_keys = place_of(blk + 3 * kTileBlocks, p3, 0);
+            next_values = place_of(blk + 2 * kTileBlocks, p2, 1);
         };
         if (seen(blk)) {
             top = halves_max(top) * a.scale;
@@ -318,6 +344,8 @@ __global__ __launch_bounds__(kThreads, 2) void attend_tiles_kernel(const Attenti
 #pragma unroll
                     for (int i = (n - kHalf) * 4 * kEach / kHalf; i < (n - kHalf + 1) * 4 * kEach / kHalf; ++i)
                         widen_part(i);
+                    if (n == kSecond - 2)
+                        find_next();
                 }
             }
             MAMBO_FIXED_ORDER();
@@ -330,10 +358,11 @@ __global__ __launch_bounds__(kThreads, 2) void attend_tiles_kernel(const Attenti
 #pragma unroll
             for (int i = 0; i < 4 * kEach; ++i)
                 widen_part(i);
+            find_next();
         }
-        load(blk + 3 * kTileBlocks, p3, false, kc);
-        load(blk + 2 * kTileBlocks, p2, true, vc);
-        p0 = p1, p1 = p2, p2 = p3;
+        load(next_keys, kc);
+        load(next_values, vc);
+        p1 = p2, p2 = p3;
     };
     for (int blk = lo; blk < hi; blk += 2 * kTileBlocks) {
         step(blk, 0, even, odd);

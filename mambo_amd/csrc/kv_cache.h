@@ -29,10 +29,11 @@ __host__ __device__ constexpr int kv_value_byte(int token, int d)
 struct KvCache {
     uint8_t *codes, *scales;
     int pages, heads, dim, shift; // blocks of a page: 1 << shift
-    // Index of a block, for 2 * 32 * padded bytes of codes and 2 of scales; page within [0, pages).
-    __device__ int64_t block(int page, int head, int b) const
+    // Index of a block, for 2 * 32 * padded bytes of codes and 2 of scales; page within [0, pages). 32 bits: so many
+    // blocks are 4 TiB and more, and refused.
+    __device__ uint32_t block(int page, int head, int b) const
     {
-        return (((int64_t)page * heads + head) << shift) + (b & ((1 << shift) - 1));
+        return ((uint32_t)(page * heads + head) << shift) + (uint32_t)(b & ((1 << shift) - 1));
     }
 };
 

@@ -275,8 +275,8 @@ __global__ __launch_bounds__(256) void append_kernel(const Append a)
     if ((uint32_t)page >= (uint32_t)a.cache.pages)
         return;
     const int64_t at = a.cache.block(page, head, blk);
-    uint8_t *const keys = a.cache.codes + at * (2 * kKvBlock * padded), *const values = keys + kKvBlock * padded;
-    uint8_t *const scale = a.cache.scales + 2 * at;
+    uint8_t *const keys = a.cache.codes + (int64_t)at * (2 * kKvBlock * padded), *const values = keys + kKvBlock * padded;
+    uint8_t *const scale = a.cache.scales + 2 * (int64_t)at;
 
     const int chunks = padded / 8, base = blk * kKvBlock;
     float kx[P][8];
@@ -463,8 +463,8 @@ __global__ __launch_bounds__(256) void read_kernel(const KvCache cache, const Kv
         bf16x8 kv = {}, vv = {};
         if (page >= 0 && page < cache.pages) {
             const int64_t at = cache.block(page, head, blk);
-            const uint8_t *keys = cache.codes + at * (2 * kKvBlock * padded), *values = keys + kKvBlock * padded;
-            const int ke = (int)cache.scales[2 * at] - 127, ve = (int)cache.scales[2 * at + 1] - 127;
+            const uint8_t *keys = cache.codes + (int64_t)at * (2 * kKvBlock * padded), *values = keys + kKvBlock * padded;
+            const int ke = (int)cache.scales[2 * (int64_t)at] - 127, ve = (int)cache.scales[2 * (int64_t)at + 1] - 127;
             const uint2 w = *reinterpret_cast<const uint2 *>(keys + kv_key_byte(t, d));
             uint32_t c[8];
 #pragma unroll
@@ -533,6 +533,8 @@ int kv_check_cache(const mambo_kv_cache *c, KvCache *out)
                   MAMBO_ERR_VALUE, "page_size must be a power of two from 32 to 65536 (got %d)", (int)c->page_size);
     MAMBO_REQUIRE(c->heads >= 1 && c->heads <= 65535 && c->pages >= 1 && c->pages <= 0x7FFFFFFF, MAMBO_ERR_VALUE,
                   "a cache has 1 to 2^31 - 1 pages of 1 to 65535 heads (got %lld of %d)", (long long)c->pages, (int)c->heads);
+    MAMBO_REQUIRE(c->pages * c->heads * (c->page_size / kKvBlock) <= 0x7FFFFFFF, MAMBO_ERR_VALUE,
+                  "a cache has at most 2^31 - 1 blocks of 32 tokens and a head (got %lld pages)", (long long)c->pages);
     MAMBO_REQUIRE(c->codes && c->scales, MAMBO_ERR_VALUE, "null pointer");
     MAMBO_REQUIRE((uintptr_t)c->codes % 16 == 0 && (uintptr_t)c->scales % 2 == 0, MAMBO_ERR_VALUE,
                   "codes must be 16-byte and scales 2-byte aligned");
@@ -561,12 +563,9 @@ int kv_check_batch(const mambo_kv_batch *b, int64_t tokens, const mambo_kv_cache
 extern "C" int64_t mambo_kv_cache_bytes(int64_t pages, int64_t heads, int64_t head_dim, int64_t page_size)
 {
     if (pages < 1 || pages > 0x7FFFFFFF || heads < 1 || heads > 65535 || !kv_dim_ok(head_dim) || page_size < kKvBlock ||
-        page_size > 65536 || (page_size & (page_size - 1)))
+        page_size > 65536 || (page_size & (page_size - 1)) || pages * heads * (page_size / kKvBlock) > 0x7FFFFFFF)
         return 0;
-    int64_t bytes;
-    if (__builtin_mul_overflow(pages, heads * page_size * 2 * kv_padded((int)head_dim), &bytes))
-        return 0;
-    return bytes;
+    return pages * heads * page_size * 2 * kv_padded((int)head_dim);
 }
 
 extern "C" int mambo_rotary(const void *x, int x_dtype, int64_t tokens, int64_t heads, int64_t dim, int64_t ldt, int64_t ldh,
