@@ -86,7 +86,12 @@ __device__ __forceinline__ uint2 keep_tokens(uint32_t lo, uint32_t hi, int left)
 
 // Most rows that attend_rows takes: 16 a tile, as many tiles as the registers and the LDS of its join hold.
 constexpr int max_row_tiles(int padded) { return padded <= 64 ? 4 : padded <= 128 ? 2 : 1; }
-constexpr int kTileRowsWg = 256; // rows of a workgroup of attend_tiles
+
+// Waves of a workgroup of attend_tiles, each with 32 rows, by the head size in 32s. Eight, two a SIMD, while a wave's
+// registers are enough (D = 128: 8192 tokens of 32 heads 540 us, with four 580); from 192 on four with twice the
+// registers (4096 tokens of D = 256 408 us for 1507, of 192 330 for 331, of 160 295 for 236).
+constexpr int tile_waves(int ds) { return ds <= 5 ? 8 : 4; }
+constexpr int tile_rows(int ds) { return 32 * tile_waves(ds); }
 
 int launch_attend_rows(const Attention &a, int row_tiles, hipStream_t s);
 int launch_attend_tiles(const Attention &a, int64_t tiles, hipStream_t s);

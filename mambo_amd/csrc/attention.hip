@@ -38,8 +38,9 @@ Plan make_plan(const KvCache &c, const KvBatch &b, int group)
         p.rows_entries = (int64_t)c.heads * p.slots * 2 * p.few_rows;
     }
     if (rows > most) {
-        p.tiles_each = (int)cdiv(rows, kTileRowsWg);
-        p.tiles = b.offsets ? (int64_t)b.tokens * group / kTileRowsWg + b.seqs : (int64_t)b.seqs * p.tiles_each;
+        const int tile = tile_rows(padded / 32);
+        p.tiles_each = (int)cdiv(rows, tile);
+        p.tiles = b.offsets ? (int64_t)b.tokens * group / tile + b.seqs : (int64_t)b.seqs * p.tiles_each;
         // a workgroup a CU
         p.parts = (int)std::max<int64_t>(1, std::min<int64_t>(kCus / (p.tiles * c.heads), cdiv(b.capacity, 512)));
         if (p.parts > 1)
@@ -64,7 +65,7 @@ int check(const mambo_kv_cache *cache, const mambo_kv_batch *batch, int64_t toke
                   "tables must hold below 2^36 tokens together");
     *p = make_plan(*c, *b, (int)(q_heads / c->heads));
     const int64_t rows = p->few_rows, heads = c->heads;
-    MAMBO_REQUIRE(grid_takes(batch->seqs * heads, 256) && rows <= 65535 && grid_takes(p->tiles * heads, 2 * kTileRowsWg) &&
+    MAMBO_REQUIRE(grid_takes(batch->seqs * heads, 256) && rows <= 65535 && grid_takes(p->tiles * heads, 512) &&
                       grid_takes(tokens * q_heads, 256),
                   MAMBO_ERR_VALUE, "too many rows for one launch");
     return MAMBO_OK;
@@ -94,7 +95,7 @@ extern "C" int mambo_kv_attention_plan(const mambo_kv_cache *cache, const mambo_
     MAMBO_REQUIRE(plan != nullptr, MAMBO_ERR_VALUE, "null pointer");
     plan[0] = p.few_rows;
     plan[1] = p.slots;
-    plan[2] = p.tiles ? kTileRowsWg : 0;
+    plan[2] = p.tiles ? tile_rows(kv_padded(c.dim) / 32) : 0;
     plan[3] = p.parts;
     return MAMBO_OK;
 }

@@ -1,6 +1,6 @@
 // Attention of many rows (prompts, pieces of prompts): bound by the matrix units and the exponentials.
 //
-// A workgroup takes 256 rows (queries x heads of one key/value head, 32 a wave) and goes through their keys
+// A workgroup takes 256 rows (128 of large heads; queries x heads of one key/value head, 32 a wave) and goes through their keys
 // 64 at a time. The tile's codes are widened to bf16 once, on their way from registers into LDS, and every
 // wave reads them from there: S^T = K Q^T in 32 x 32 x 16 MFMAs, softmax in registers (a lane has one
 // query), O^T += V^T P^T. The key rows lie in LDS in such an order that the scores come out
@@ -10,8 +10,6 @@
 
 namespace {
 
-constexpr int kWaves = kTileRowsWg / 32;
-constexpr int kThreads = 64 * kWaves;
 constexpr int kTileBlocks = 2; // blocks of 32 tokens of a tile
 
 __device__ __forceinline__ float halves_max(float x)
@@ -37,14 +35,15 @@ __device__ __forceinline__ int scalar_load(const int32_t *p)
 constexpr int kAhead = 4; // operands read ahead
 
 // Tiles of the sequences before s: at least as many as their rows fill.
-__device__ __forceinline__ int64_t tiles_before(const Attention &a, int s)
+__device__ __forceinline__ int64_t tiles_before(const Attention &a, int tile_rows, int s)
 {
-    return (int64_t)a.b.offset(s) * a.group / kTileRowsWg + s;
+    return (int64_t)a.b.offset(s) * a.group / tile_rows + s;
 }
 
 template <int DS>
-__global__ __launch_bounds__(kThreads, 2) void attend_tiles_kernel(const Attention a)
+__global__ __launch_bounds__(64 * tile_waves(DS), tile_waves(DS) / 4) void attend_tiles_kernel(const Attention a)
 {
+    constexpr int kWaves = tile_waves(DS), kTileRows = 32 * kWaves;
     constexpr int DP = 32 * DS, kSteps = DP / 16;
     constexpr int kUnits = kTileBlocks * DS, kEach = (kUnits + kWaves - 1) / kWaves; // staged by all waves, and by one
     // keys: [8 values of the head][64 rows of the first product]; values: [8 tokens][value of the head]
@@ -59,20 +58,20 @@ __global__ __launch_bounds__(kThreads, 2) void attend_tiles_kernel(const Attenti
     const int tile = (int)(gridDim.x / (unsigned)a.cache.heads) - 1 - (int)(blockIdx.x / (unsigned)a.cache.heads);
     int s, part_tile;
     if (a.b.offsets) {
-        s = find_slot(a.b.seqs, tile, [&](int i) { return tiles_before(a, i); });
-        part_tile = tile - (int)tiles_before(a, s);
+        s = find_slot(a.b.seqs, tile, [&](int i) { return tiles_before(a, kTileRows, i); });
+        part_tile = tile - (int)tiles_before(a, kTileRows, s);
     } else {
         s = tile / a.tiles_each;
         part_tile = tile % a.tiles_each;
     }
     const Sequence seq = sequence(a, s);
-    const int64_t rows64 = (int64_t)seq.n * a.group, row0_64 = (int64_t)part_tile * kTileRowsWg;
+    const int64_t rows64 = (int64_t)seq.n * a.group, row0_64 = (int64_t)part_tile * kTileRows;
     if (part_tile < 0 || row0_64 >= rows64 || rows64 <= a.few_rows)
         return;
     const int rows = (int)rows64, row0 = (int)row0_64;
 
     // the tile's keys: what its first row sees of the window to what its last one sees
-    const int i0 = row0 / a.group, i1 = (min(row0 + kTileRowsWg, rows) - 1) / a.group;
+    const int i0 = row0 / a.group, i1 = (min(row0 + kTileRows, rows) - 1) / a.group;
     int lo = max(0, sees_from(a, seq, i0)) / kKvBlock, hi = (max(0, sees_to(a, seq, i1)) + kKvBlock - 1) / kKvBlock;
     if (a.parts > 1) { // an even share of them
         const int tiles = (hi - lo + kTileBlocks - 1) / kTileBlocks, part = (int)blockIdx.y;
@@ -449,7 +448,7 @@ __global__ __launch_bounds__(256) void join_tiles_kernel(const Attention a)
 template <int DS>
 void launch_tiles(const Attention &a, int64_t tiles, hipStream_t s)
 {
-    MAMBO_LAUNCH((attend_tiles_kernel<DS>), dim3((unsigned)(tiles * a.cache.heads), (unsigned)a.parts), dim3(kThreads), 0, s, a);
+    MAMBO_LAUNCH((attend_tiles_kernel<DS>), dim3((unsigned)(tiles * a.cache.heads), (unsigned)a.parts), dim3(64 * tile_waves(DS)), 0, s, a);
     if (a.parts > 1) {
         const int64_t rows = (int64_t)a.b.tokens * a.group * a.cache.heads, each = 256 / (8 * DS);
         MAMBO_LAUNCH((join_tiles_kernel<DS>), dim3((unsigned)((rows + each - 1) / each)), dim3(256), 0, s, a);
