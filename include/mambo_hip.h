@@ -459,16 +459,18 @@ int mambo_kv_read(const mambo_kv_cache *cache, const mambo_kv_batch *batch, cons
  * or NULL. Sums are f32; the probabilities are rounded to bf16 for the product with the values.
  * workspace: mambo_kv_attention_workspace bytes, 16-byte aligned, that no call running at the same time uses.
  * Rows that no sequence has are not written. The results do not vary from run to run. */
-int64_t mambo_kv_attention_workspace(const mambo_kv_cache *cache, const mambo_kv_batch *batch, int64_t tokens, int64_t q_heads);
+int64_t mambo_kv_attention_workspace(const mambo_kv_cache *cache, const mambo_kv_batch *batch, int64_t tokens, int64_t q_heads,
+                                     int64_t window);
 int mambo_kv_attention(const void *q, int64_t tokens, int64_t q_heads, int64_t dim, int64_t ldqt, int64_t ldqh, const mambo_kv_cache *cache,
                        const mambo_kv_batch *batch, float scale, int causal, int64_t window, void *out, int64_t ldot,
                        int64_t ldoh, float *lse, void *workspace, int64_t workspace_bytes, mambo_stream_t stream);
 
 /* How such a call is launched, on the host alone: plan[4] = rows (queries x heads of a key/value head) up to
- * which a sequence takes the kernel for few rows (0: it is not launched), its workgroups for each head,
+ * which a sequence takes the kernel for few rows (0: it is not launched), its workgroups for each head (0: one for each
+ * sequence, none of which has many keys),
  * rows of a workgroup of the kernel for many (0: not launched) and the parts of its keys. */
 int mambo_kv_attention_plan(const mambo_kv_cache *cache, const mambo_kv_batch *batch, int64_t tokens, int64_t q_heads,
-                            int32_t *plan);
+                            int64_t window, int32_t *plan);
 
 /* Synthetic inputs for benchmarks and full-size checks (no reference counterpart; the
  * reference draws them with numpy/cupy RNGs, test_iq3_s_fp8.py:41-51). Counter-based:

@@ -169,10 +169,10 @@ SIGNATURES = {
     "mambo_kv_cache_bytes": (_i64, [_i64, _i64, _i64, _i64]),
     "mambo_kv_append": (_i32, [ctypes.POINTER(KVRowsArgs), _i64, _cache, _batch, _table, _vp, _vp]),
     "mambo_kv_read": (_i32, [_cache, _batch, _vp, _vp, _i64, _i64, _i64, _vp, _vp, _vp]),
-    "mambo_kv_attention_workspace": (_i64, [_cache, _batch, _i64, _i64]),
+    "mambo_kv_attention_workspace": (_i64, [_cache, _batch, _i64, _i64, _i64]),
     "mambo_kv_attention": (_i32, [_vp, _i64, _i64, _i64, _i64, _i64, _cache, _batch, ctypes.c_float, _i32, _i64, _vp, _i64, _i64, _vp,
                                   _vp, _i64, _vp]),
-    "mambo_kv_attention_plan": (_i32, [_cache, _batch, _i64, _i64, _vp]),
+    "mambo_kv_attention_plan": (_i32, [_cache, _batch, _i64, _i64, _i64, _vp]),
     "mambo_synth_iq3s": (_i32, [_u64, _i64, _i64, _i64, _vp, _vp]),
     "mambo_synth_bf16": (_i32, [_u64, _u64, ctypes.c_double, _i64, _i64, _vp, _vp]),
     "mambo_e4m3_convert": (_i32, [_vp, _i64, _vp, _vp, _vp]),

@@ -19,7 +19,7 @@ struct Attention {
     int64_t ldot, ldoh;
     float *lse;
     int few_rows; // sequences of up to so many rows (queries x group) are attend_rows' work, others attend_tiles'
-    int slots;    // attend_rows: workgroups of a head
+    int slots;    // attend_rows: workgroups of a head; 0: attend_short takes its place
     int parts, tiles_each; // attend_tiles: parts of the keys; tiles of a sequence of a uniform batch
     float *rows_o, *rows_ml; // partial sums, their largest scores and totals
     int32_t *begins;         // first block of each sequence in the row kernel's order, and the total
@@ -74,6 +74,12 @@ __device__ __forceinline__ int vector_zero()
     int zero;
     asm("v_mov_b32 %0, 0" : "=v"(zero));
     return zero;
+}
+
+// A word that every lane wants and no kernel writes while this one runs.
+__device__ __forceinline__ int scalar_load(const int32_t *p)
+{
+    return *(const __attribute__((address_space(4))) int32_t *)p;
 }
 
 // Codes past the first `left` (of eight) become zeros: what a page holds behind a sequence's last token is

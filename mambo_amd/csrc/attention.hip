@@ -16,10 +16,14 @@ struct Plan {
 };
 
 constexpr int kCus = 256;
+// Keys of a sequence up to which one workgroup takes all of them. One user of 8 heads of 128, from a graph: 1000 tokens
+// 9.7 us for 8.6 by two launches, whose second costs the host 3 us more, 2000 14.5 for 8.9; 32 users (a workgroup a CU)
+// 1000 16.7 for 21.3, 2000 25.7 for 30.4.
+constexpr int64_t kShortTokens = 1280, kShortTokensOfMany = 2048;
 
 int64_t aligned(int64_t bytes) { return (bytes + 15) & ~(int64_t)15; }
 
-Plan make_plan(const KvCache &c, const KvBatch &b, int group)
+Plan make_plan(const KvCache &c, const KvBatch &b, int group, int64_t window)
 {
     Plan p;
     const int padded = kv_padded(c.dim);
@@ -32,10 +36,19 @@ Plan make_plan(const KvCache &c, const KvBatch &b, int group)
         p.row_tiles = tiles_for(group);
     if (p.row_tiles) {
         p.few_rows = 16 * p.row_tiles;
-        // two workgroups a CU, fewer where there is no work for them
-        const int64_t blocks = (int64_t)b.seqs * (b.capacity / kKvBlock);
-        p.slots = (int)std::max<int64_t>(1, std::min<int64_t>(2 * kCus / c.heads, cdiv(blocks, 4)));
-        p.rows_entries = (int64_t)c.heads * p.slots * 2 * p.few_rows;
+        // blocks of a sequence at most; few enough, and one workgroup takes all of them
+        const int64_t seen = window ? std::min<int64_t>(b.capacity, std::min<int64_t>(window, b.capacity) + p.few_rows / group + kKvBlock) : b.capacity;
+        if (seen > ((int64_t)b.seqs * c.heads >= kCus ? kShortTokensOfMany : kShortTokens)) {
+            // A workgroup a CU, fewer where there is no work for them: the blocks that its waves have on their way are enough
+            // (131149 tokens of 8 heads of 128 47.0 us, with two 49.6). Two of small heads (16 x 8000 of 64 28.7 us for 35.4),
+            // and where a workgroup comes to the ends of several sequences, at which the other goes on (64 sequences
+            // of up to 8192 109 us for 113, 32 of 4000 49.5 for 44.4).
+            const int64_t blocks = (int64_t)b.seqs * (b.capacity / kKvBlock);
+            const int size = padded / 32 * p.row_tiles;
+            const int per_cu = size <= 2 || (size <= 4 && (int64_t)b.seqs * c.heads >= 2 * kCus) ? 2 : 1;
+            p.slots = (int)std::max<int64_t>(1, std::min<int64_t>(per_cu * kCus / c.heads, cdiv(blocks, 4)));
+            p.rows_entries = (int64_t)c.heads * p.slots * 2 * p.few_rows;
+        }
     }
     if (rows > most) {
         const int tile = tile_rows(padded / 32);
@@ -46,12 +59,12 @@ Plan make_plan(const KvCache &c, const KvBatch &b, int group)
         if (p.parts > 1)
             p.tiles_entries = (int64_t)p.parts * b.tokens * group * c.heads;
     }
-    p.bytes = aligned(p.rows_entries * (padded + 2) * 4) + aligned(((int64_t)b.seqs + 1) * 4) +
+    p.bytes = aligned(p.rows_entries * (padded + 2) * 4) + aligned(p.slots ? ((int64_t)b.seqs + 1) * 4 : 0) +
               aligned(p.tiles_entries * (padded + 2) * 4);
     return p;
 }
 
-int check(const mambo_kv_cache *cache, const mambo_kv_batch *batch, int64_t tokens, int64_t q_heads, KvCache *c, KvBatch *b, Plan *p)
+int check(const mambo_kv_cache *cache, const mambo_kv_batch *batch, int64_t tokens, int64_t q_heads, int64_t window, KvCache *c, KvBatch *b, Plan *p)
 {
     if (const int rc = kv_check_cache(cache, c))
         return rc;
@@ -59,11 +72,12 @@ int check(const mambo_kv_cache *cache, const mambo_kv_batch *batch, int64_t toke
         return rc;
     MAMBO_REQUIRE(q_heads >= c->heads && q_heads % c->heads == 0 && q_heads <= 65535, MAMBO_ERR_VALUE,
                   "%lld query heads are no multiple of %d", (long long)q_heads, c->heads);
+    MAMBO_REQUIRE(window >= 0, MAMBO_ERR_VALUE, "a window is positive, and of causal attention");
     MAMBO_REQUIRE(tokens * q_heads <= 0x7FFFFFFF, MAMBO_ERR_VALUE, "tokens times query heads must be below 2^31 (got %lld)",
                   (long long)tokens);
     MAMBO_REQUIRE(batch->seqs * (int64_t)(b->capacity / kKvBlock) <= 0x7FFFFFFF, MAMBO_ERR_VALUE,
                   "tables must hold below 2^36 tokens together");
-    *p = make_plan(*c, *b, (int)(q_heads / c->heads));
+    *p = make_plan(*c, *b, (int)(q_heads / c->heads), window);
     const int64_t rows = p->few_rows, heads = c->heads;
     MAMBO_REQUIRE(grid_takes(batch->seqs * heads, 256) && rows <= 65535 && grid_takes(p->tiles * heads, 512) &&
                       grid_takes(tokens * q_heads, 256),
@@ -74,23 +88,23 @@ int check(const mambo_kv_cache *cache, const mambo_kv_batch *batch, int64_t toke
 } // namespace
 
 extern "C" int64_t mambo_kv_attention_workspace(const mambo_kv_cache *cache, const mambo_kv_batch *batch, int64_t tokens,
-                                                int64_t q_heads)
+                                                int64_t q_heads, int64_t window)
 {
     KvCache c;
     KvBatch b;
     Plan p;
-    if (const int rc = check(cache, batch, tokens, q_heads, &c, &b, &p))
+    if (const int rc = check(cache, batch, tokens, q_heads, window, &c, &b, &p))
         return rc;
     return p.bytes;
 }
 
 extern "C" int mambo_kv_attention_plan(const mambo_kv_cache *cache, const mambo_kv_batch *batch, int64_t tokens,
-                                       int64_t q_heads, int32_t *plan)
+                                       int64_t q_heads, int64_t window, int32_t *plan)
 {
     KvCache c;
     KvBatch b;
     Plan p;
-    if (const int rc = check(cache, batch, tokens, q_heads, &c, &b, &p))
+    if (const int rc = check(cache, batch, tokens, q_heads, window, &c, &b, &p))
         return rc;
     MAMBO_REQUIRE(plan != nullptr, MAMBO_ERR_VALUE, "null pointer");
     plan[0] = p.few_rows;
@@ -108,11 +122,11 @@ extern "C" int mambo_kv_attention(const void *q, int64_t tokens, int64_t q_heads
 {
     Attention a;
     Plan p;
-    if (const int rc = check(cache, batch, tokens, q_heads, &a.cache, &a.b, &p))
+    if (const int rc = check(cache, batch, tokens, q_heads, window, &a.cache, &a.b, &p))
         return rc;
     MAMBO_REQUIRE(dim == a.cache.dim, MAMBO_ERR_VALUE, "the cache has heads of %d (got %lld)", a.cache.dim, (long long)dim);
     MAMBO_REQUIRE(scale > 0.0f && isfinite(scale), MAMBO_ERR_VALUE, "the scale of the scores must be positive and finite");
-    MAMBO_REQUIRE(window >= 0 && (window == 0 || causal), MAMBO_ERR_VALUE, "a window is positive, and of causal attention");
+    MAMBO_REQUIRE(window == 0 || causal, MAMBO_ERR_VALUE, "a window is positive, and of causal attention");
     if (tokens == 0)
         return MAMBO_OK;
     MAMBO_REQUIRE(q && out, MAMBO_ERR_VALUE, "null pointer");
@@ -131,7 +145,7 @@ extern "C" int mambo_kv_attention(const void *q, int64_t tokens, int64_t q_heads
     a.rows_o = (float *)at, a.rows_ml = a.rows_o + p.rows_entries * padded;
     at += aligned(p.rows_entries * (padded + 2) * 4);
     a.begins = (int32_t *)at;
-    at += aligned(((int64_t)a.b.seqs + 1) * 4);
+    at += aligned(p.slots ? ((int64_t)a.b.seqs + 1) * 4 : 0);
     a.tiles_o = (float *)at, a.tiles_ml = a.tiles_o + p.tiles_entries * padded;
     hipStream_t s = (hipStream_t)stream;
     if (p.tiles)

@@ -120,35 +120,75 @@ struct Scan {
     }
 };
 
-// 16 RT rows by 32 DS values a head.
-template <int DS, int RT>
-__global__ __launch_bounds__(256, 2) void attend_rows_kernel(const Attention a)
-{
-    constexpr int DP = 32 * DS;
-    __shared__ float so[4][16 * RT][DP + 4];
-    __shared__ float sm[4][16 * RT], sl[4][16 * RT];
-    const int tid = (int)threadIdx.x, lane = lane_id(), kk = lane >> 4, col = lane & 15;
-    const int wave = __builtin_amdgcn_readfirstlane(tid / 64);
-    const int head = (int)(blockIdx.x % (unsigned)a.cache.heads), slot = (int)(blockIdx.x / (unsigned)a.cache.heads);
-    Scan scan(a);
-    const int total = scan.total(blockIdx.x == 0 && wave == 0 ? a.begins : nullptr);
-    const int count = shares(a, total);
-    if (slot >= count || total == 0)
-        return;
-    int at = share_begin(slot, total, count);
-    const int end = share_begin(slot + 1, total, count);
-    int s = 0, base = 0; // the sequence that `at` is in, and its first block in the order
-    scan.find(at, &s, &base);
+// A sequence's rows of a head over the blocks [first, last) of its keys.
+struct Stretch {
+    Sequence seq;
+    int s, first, last;
+};
 
-    while (at < end) {
-        const Sequence seq = sequence(a, s);
-        const int blocks = row_blocks(a, seq), rows = seq.n * a.group;
-        if (blocks == 0 || at >= base + blocks) { // sequences without blocks between
-            scan.find(at, &s, &base);
-            continue;
-        }
-        const int stop = min(end, base + blocks);
-        const int first_blk = seq.lo + at - base, last_blk = seq.lo + stop - base;
+// Such a stretch, whose blocks the workgroup's waves take in turn; what they found is left in LDS.
+template <int DS, int RT, int NW>
+struct Rows {
+    static constexpr int DP = 32 * DS;
+    struct Shared {
+        float o[4][16 * RT][DP + 4];
+        float m[4][16 * RT], l[4][16 * RT];
+    };
+    struct Block {
+        uint4 k[DS], v[DS];
+        uint32_t scales;
+        int page;
+    };
+    // Blocks that a wave holds, all but one of them on their way.
+    static constexpr int NB = NW == 8 && DS * RT <= 4 ? 3 : 2;
+
+    // Blocks of a stretch that are on their way to this wave.
+    struct Held {
+        Block b[NB];
+        int blk, next_page;
+    };
+
+    // Pages come by scalar loads, one block ahead of the codes; the last block's stands for those behind it, the first of
+    // the table for those of no blocks at all.
+    __device__ static int page_of(const Attention &a, const Stretch &st, int blk)
+    {
+        return scalar_load(a.b.tables + st.s * a.b.ldt + (max(min(blk, st.last - 1), 0) >> a.cache.shift));
+    }
+    __device__ static bool there(const Attention &a, int page) { return (uint32_t)page < (uint32_t)a.cache.pages; }
+
+    // No branch ends between a load and its use, where the compiler would wait for it.
+    __device__ static void load(const Attention &a, const Stretch &st, int head, int zero, int blk, int page, Block &b)
+    {
+        if (blk >= st.last)
+            return;
+        b.page = page;
+        const int64_t at = a.cache.block(there(a, page) ? page : 0, head, blk);
+        const uint4 *codes = reinterpret_cast<const uint4 *>(a.cache.codes + at * (2 * kKvBlock * DP)) + lane_id();
+        b.scales = *reinterpret_cast<const uint16_t *>(a.cache.scales + 2 * (at + zero));
+#pragma unroll
+        for (int d = 0; d < DS; ++d)
+            b.k[d] = codes[64 * d];
+#pragma unroll
+        for (int d = 0; d < DS; ++d)
+            b.v[d] = codes[64 * (DS + d)];
+    }
+
+    __device__ static void begin(const Attention &a, const Stretch &st, int head, int zero, Held &held)
+    {
+        held.blk = st.first + __builtin_amdgcn_readfirstlane((int)threadIdx.x / 64);
+#pragma unroll
+        for (int j = 0; j < NB - 1; ++j)
+            load(a, st, head, zero, held.blk + j * NW, page_of(a, st, held.blk + j * NW), held.b[j]);
+        held.next_page = page_of(a, st, held.blk + (NB - 1) * NW);
+    }
+
+    __device__ static void attend(const Attention &a, const Stretch &st, int head, Shared &sh)
+    {
+        const Sequence &seq = st.seq;
+        const int lane = lane_id(), kk = lane >> 4, col = lane & 15, zero = vector_zero();
+        const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x / 64), rows = seq.n * a.group;
+        Held held;
+        begin(a, st, head, zero, held);
 
         bf16x8 q[RT][DS];
         int to[RT], from[RT];
@@ -181,33 +221,10 @@ __global__ __launch_bounds__(256, 2) void attend_rows_kernel(const Attention a)
                 o[r][d] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
         }
 
-        struct Block {
-            uint4 k[DS], v[DS];
-            int scales; // -1: there is no such page
-        };
-        const auto page_of = [&](int blk) -> int {
-            return blk < last_blk ? a.b.page(s, blk >> a.cache.shift) : -1;
-        };
-        const auto load = [&](int blk, int page_any, Block &b) {
-            const int page = __builtin_amdgcn_readfirstlane(page_any);
-            b.scales = -1;
-            if ((uint32_t)page >= (uint32_t)a.cache.pages)
+        const auto take = [&](int blk, const Block &b) {
+            if (!there(a, b.page))
                 return;
-            const int64_t at_blk = a.cache.block(page, head, blk);
-            const uint4 *codes = reinterpret_cast<const uint4 *>(a.cache.codes + at_blk * (2 * kKvBlock * DP)) + lane;
-            b.scales = *reinterpret_cast<const uint16_t *>(a.cache.scales + 2 * at_blk);
-#pragma unroll
-            for (int d = 0; d < DS; ++d)
-                b.k[d] = codes[64 * d];
-#pragma unroll
-            for (int d = 0; d < DS; ++d)
-                b.v[d] = codes[64 * (DS + d)];
-        };
-        const auto take = [&](int blk, Block &b) {
-            const int scales = __builtin_amdgcn_readfirstlane(b.scales);
-            if (scales < 0)
-                return;
-            const float ks = e8m0(scales & 255), vs = e8m0(scales >> 8);
+            const float ks = e8m0(b.scales & 255), vs = e8m0(b.scales >> 8);
             v4f x[RT][2];
 #pragma unroll
             for (int r = 0; r < RT; ++r)
@@ -270,63 +287,126 @@ __global__ __launch_bounds__(256, 2) void attend_rows_kernel(const Attention a)
             }
         };
 
-        // a block is asked for while the one before it is worked on, its page one earlier
-        Block even, odd;
-        even.scales = odd.scales = -1;
-        int blk = first_blk + wave;
-        load(blk, page_of(blk), even);
-        int page = page_of(blk + 4);
-        while (blk < last_blk) {
-            load(blk + 4, page, odd);
-            page = page_of(blk + 8);
-            take(blk, even);
-            blk += 4;
-            if (blk >= last_blk)
-                break;
-            load(blk + 4, page, even);
-            page = page_of(blk + 8);
-            take(blk, odd);
-            blk += 4;
-        }
-
+        while (held.blk < st.last) {
 #pragma unroll
-        for (int r = 0; r < RT; ++r) {
-            const float sum = across_sum(l[r]);
-            if (kk == 0) {
-                sm[wave][16 * r + col] = m[r];
-                sl[wave][16 * r + col] = sum;
+            for (int j = 0; j < NB; ++j) {
+                if (held.blk < st.last) {
+                    load(a, st, head, zero, held.blk + (NB - 1) * NW, held.next_page, held.b[(j + NB - 1) % NB]);
+                    held.next_page = page_of(a, st, held.blk + NB * NW);
+                    take(held.blk, held.b[j]);
+                }
+                held.blk += NW;
             }
+        }
+        const auto leave = [&](int w) {
 #pragma unroll
-            for (int d = 0; d < 2 * DS; ++d)
-                *reinterpret_cast<v4f *>(&so[wave][16 * r + col][16 * d + 4 * kk]) = o[r][d];
+            for (int r = 0; r < RT; ++r) {
+                const float sum = across_sum(l[r]);
+                if (kk == 0) {
+                    sh.m[w][16 * r + col] = m[r];
+                    sh.l[w][16 * r + col] = sum;
+                }
+#pragma unroll
+                for (int d = 0; d < 2 * DS; ++d)
+                    *reinterpret_cast<v4f *>(&sh.o[w][16 * r + col][16 * d + 4 * kk]) = o[r][d];
+            }
+        };
+        if constexpr (NW == 8) { // the second four through the places of the first
+            if (wave >= 4)
+                leave(wave - 4);
+            __syncthreads();
+            if (wave < 4) {
+#pragma unroll
+                for (int r = 0; r < RT; ++r) {
+                    const float other = sh.m[wave][16 * r + col], top = fmaxf(m[r], other);
+                    const float less = top == -__builtin_inff() ? 0.0f : top;
+                    const float f = exp2_fast(m[r] - less), g = exp2_fast(other - less);
+                    // a quarter of the other total for each of the lanes that add theirs up
+                    l[r] = l[r] * f + 0.25f * sh.l[wave][16 * r + col] * g;
+                    m[r] = top;
+#pragma unroll
+                    for (int d = 0; d < 2 * DS; ++d)
+                        o[r][d] = o[r][d] * f + *reinterpret_cast<const v4f *>(&sh.o[wave][16 * r + col][16 * d + 4 * kk]) * g;
+                }
+                leave(wave);
+            }
+        } else {
+            leave(wave);
         }
         __syncthreads();
+    }
+
+    // Four values of a row over all waves; its largest score and total.
+    __device__ static v4f collect(const Shared &sh, int row, int d, float *top, float *sum)
+    {
+        *top = sh.m[0][row];
+#pragma unroll
+        for (int w = 1; w < 4; ++w)
+            *top = fmaxf(*top, sh.m[w][row]);
+        const float less = *top == -__builtin_inff() ? 0.0f : *top;
+        *sum = 0.0f;
+        v4f y = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+            const float f = exp2_fast(sh.m[w][row] - less);
+            *sum += f * sh.l[w][row];
+            y += f * *reinterpret_cast<const v4f *>(&sh.o[w][row][d]);
+        }
+        return y;
+    }
+};
+
+// A row's result: four values of it, and with the first of them its lse.
+__device__ __forceinline__ void store_row(const Attention &a, int64_t t, int h, int d, v4f o, float top, float sum)
+{
+    o *= sum == 0.0f ? 0.0f : 1.0f / sum;
+    if (d < a.cache.dim)
+        store_row4<true>(a.out, t * a.ldot + h * a.ldoh + d, o, a.cache.dim - d,
+                         a.ldot % 4 == 0 && a.ldoh % 4 == 0 && (uintptr_t)a.out % 8 == 0);
+    if (a.lse && d == 0)
+        a.lse[t * ((int64_t)a.group * a.cache.heads) + h] = sum == 0.0f ? -__builtin_inff() : (top + __log2f(sum)) * kLn2;
+}
+
+// Two waves a SIMD while a wave's registers are enough.
+constexpr int rows_occupancy(int ds, int rt) { return ds * rt <= 4 ? 2 : 1; }
+
+// 16 RT rows by 32 DS values a head, the blocks of all sequences in equal shares.
+template <int DS, int RT>
+__global__ __launch_bounds__(256, rows_occupancy(DS, RT)) void attend_rows_kernel(const Attention a)
+{
+    using R = Rows<DS, RT, 4>;
+    constexpr int DP = 32 * DS;
+    __shared__ typename R::Shared sh;
+    const int tid = (int)threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid / 64);
+    const int head = (int)(blockIdx.x % (unsigned)a.cache.heads), slot = (int)(blockIdx.x / (unsigned)a.cache.heads);
+    Scan scan(a);
+    const int total = scan.total(blockIdx.x == 0 && wave == 0 ? a.begins : nullptr);
+    const int count = shares(a, total);
+    if (slot >= count || total == 0)
+        return;
+    int at = share_begin(slot, total, count);
+    const int end = share_begin(slot + 1, total, count);
+    int s = 0, base = 0; // the sequence that `at` is in, and its first block in the order
+    scan.find(at, &s, &base);
+
+    while (at < end) {
+        const Sequence seq = sequence(a, s);
+        const int blocks = row_blocks(a, seq);
+        if (at >= base + blocks) { // sequences without blocks between
+            scan.find(at, &s, &base);
+            continue;
+        }
+        const int stop = min(end, base + blocks);
+        R::attend(a, {seq, s, seq.lo + at - base, seq.lo + stop - base}, head, sh);
         const bool whole = at == base && stop == base + blocks;
         const int which = at == base ? 1 : 0; // a share ends with a sequence that goes on, or begins with one
         const int64_t entry = ((int64_t)head * a.slots + slot) * 2 + which;
-        for (int item = tid; item < rows * (DP / 4); item += 256) {
+        for (int item = tid; item < seq.n * a.group * (DP / 4); item += 256) {
             const int row = item / (DP / 4), d = 4 * (item % (DP / 4));
-            float top = sm[0][row];
-#pragma unroll
-            for (int w = 1; w < 4; ++w)
-                top = fmaxf(top, sm[w][row]);
-            const float less = top == -__builtin_inff() ? 0.0f : top;
-            float sum = 0.0f;
-            v4f y = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-            for (int w = 0; w < 4; ++w) {
-                const float f = exp2_fast(sm[w][row] - less);
-                sum += f * sl[w][row];
-                y += f * *reinterpret_cast<const v4f *>(&so[w][row][d]);
-            }
+            float top, sum;
+            const v4f y = R::collect(sh, row, d, &top, &sum);
             if (whole) {
-                const int i = row / a.group, h = head * a.group + row % a.group;
-                const int64_t t = seq.first + i;
-                y *= sum == 0.0f ? 0.0f : 1.0f / sum;
-                if (d < a.cache.dim)
-                    store_row4<true>(a.out, t * a.ldot + h * a.ldoh + d, y, a.cache.dim - d, a.ldot % 4 == 0 && a.ldoh % 4 == 0 && (uintptr_t)a.out % 8 == 0);
-                if (a.lse && d == 0)
-                    a.lse[t * ((int64_t)a.group * a.cache.heads) + h] = sum == 0.0f ? -__builtin_inff() : (top + __log2f(sum)) * kLn2;
+                store_row(a, seq.first + row / a.group, head * a.group + row % a.group, d, y, top, sum);
             } else {
                 *reinterpret_cast<v4f *>(a.rows_o + (entry * (16 * RT) + row) * DP + d) = y;
                 if (d == 0)
@@ -339,6 +419,27 @@ __global__ __launch_bounds__(256, 2) void attend_rows_kernel(const Attention a)
             ++s;
             __syncthreads();
         }
+    }
+}
+
+// The same where no sequence has many blocks: one workgroup for all of a sequence and a head, nothing to join.
+template <int DS, int RT>
+__global__ __launch_bounds__(512, rows_occupancy(DS, RT)) void attend_short_kernel(const Attention a)
+{
+    using R = Rows<DS, RT, 8>;
+    constexpr int DP = 32 * DS;
+    __shared__ typename R::Shared sh;
+    const int head = (int)(blockIdx.x % (unsigned)a.cache.heads), s = (int)(blockIdx.x / (unsigned)a.cache.heads);
+    const Sequence seq = sequence(a, s);
+    const int rows = seq.n * a.group;
+    if (seq.n <= 0 || seq.n > a.few_rows / a.group)
+        return;
+    R::attend(a, {seq, s, seq.lo, seq.hi}, head, sh);
+    for (int item = (int)threadIdx.x; item < rows * (DP / 4); item += 512) {
+        const int row = item / (DP / 4), d = 4 * (item % (DP / 4));
+        float top, sum;
+        const v4f y = R::collect(sh, row, d, &top, &sum);
+        store_row(a, seq.first + row / a.group, head * a.group + row % a.group, d, y, top, sum);
     }
 }
 
@@ -370,15 +471,26 @@ __global__ __launch_bounds__(256) void join_rows_kernel(const Attention a, int t
     float m = -__builtin_inff(), l = 0.0f;
     v4f o = {0.0f, 0.0f, 0.0f, 0.0f};
     if (g < kGroups) {
-        for (int p = p0 + g; p <= p1; p += kGroups) {
-            const int64_t entry = ((int64_t)head * a.slots + p) * 2 + (p == p0);
-            const float2 ml = *reinterpret_cast<const float2 *>(a.rows_ml + (entry * tile_rows + row) * 2);
-            const v4f x = *reinterpret_cast<const v4f *>(a.rows_o + (entry * tile_rows + row) * DP + d);
-            const float top = fmaxf(m, ml.x), less = top == -__builtin_inff() ? 0.0f : top;
-            const float f = exp2_fast(m - less), e = exp2_fast(ml.x - less);
-            o = o * f + x * e;
-            l = l * f + ml.y * e;
-            m = top;
+        for (int p = p0 + g; p <= p1; p += 4 * kGroups) { // four at a time on their way
+            float2 ml[4];
+            v4f x[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const int part = min(p + k * kGroups, p1);
+                const int64_t entry = (((int64_t)head * a.slots + part) * 2 + (part == p0)) * tile_rows + row;
+                ml[k] = *reinterpret_cast<const float2 *>(a.rows_ml + entry * 2);
+                x[k] = *reinterpret_cast<const v4f *>(a.rows_o + entry * DP + d);
+            }
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                if (p + k * kGroups > p1)
+                    continue;
+                const float top = fmaxf(m, ml[k].x), less = top == -__builtin_inff() ? 0.0f : top;
+                const float f = exp2_fast(m - less), e = exp2_fast(ml[k].x - less);
+                o = o * f + x[k] * e;
+                l = l * f + ml[k].y * e;
+                m = top;
+            }
         }
         so[g][tid % kWide] = o;
         if (tid % kWide == 0) {
@@ -402,17 +514,17 @@ __global__ __launch_bounds__(256) void join_rows_kernel(const Attention a, int t
         o += so[k][tid] * f;
         l += sl[k] * f;
     }
-    o *= l == 0.0f ? 0.0f : 1.0f / l;
-    if (d < a.cache.dim)
-        store_row4<true>(a.out, t * a.ldot + h * a.ldoh + d, o, a.cache.dim - d, a.ldot % 4 == 0 && a.ldoh % 4 == 0 && (uintptr_t)a.out % 8 == 0);
-    if (a.lse && d == 0)
-        a.lse[t * ((int64_t)a.group * a.cache.heads) + h] = l == 0.0f ? -__builtin_inff() : (m + __log2f(l)) * kLn2;
+    store_row(a, t, h, d, o, m, l);
 }
 
 template <int DS, int RT>
 void launch_rows(const Attention &a, hipStream_t s)
 {
     if constexpr (RT <= max_row_tiles(32 * DS)) {
+        if (a.slots == 0) {
+            MAMBO_LAUNCH((attend_short_kernel<DS, RT>), dim3((unsigned)(a.b.seqs * a.cache.heads)), dim3(512), 0, s, a);
+            return;
+        }
         MAMBO_LAUNCH((attend_rows_kernel<DS, RT>), dim3((unsigned)(a.slots * a.cache.heads)), dim3(256), 0, s, a);
         const int rows = a.b.offsets ? a.few_rows : a.b.each * a.group;
         MAMBO_LAUNCH((join_rows_kernel<DS>), dim3((unsigned)(a.b.seqs * a.cache.heads), (unsigned)rows), dim3(256), 0, s, a, 16 * RT);

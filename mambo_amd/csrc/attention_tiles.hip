@@ -23,12 +23,6 @@ __device__ __forceinline__ float halves_sum(float x)
     return __uint_as_float(b[0]) + __uint_as_float(b[1]);
 }
 
-// A word that every lane wants and no kernel writes while this one runs.
-__device__ __forceinline__ int scalar_load(const int32_t *p)
-{
-    return *(const __attribute__((address_space(4))) int32_t *)p;
-}
-
 // Nothing is moved across: between two of these stand one matrix instruction, the read of a later one's operand and
 // the vector instructions for which its 32 cycles leave time.
 #define MAMBO_FIXED_ORDER() __builtin_amdgcn_sched_barrier(0)
@@ -409,24 +403,20 @@ __global__ __launch_bounds__(256) void join_tiles_kernel(const Attention a)
     const int64_t q_heads = (int64_t)a.group * a.cache.heads, all = a.b.tokens * q_heads;
     const int64_t entry = (int64_t)blockIdx.x * kRows + (int)threadIdx.x / kWide;
     const int d = 4 * ((int)threadIdx.x % kWide);
-    if ((int)threadIdx.x >= kRows * kWide || entry >= all)
-        return;
-    const int64_t t = entry / q_heads, h = entry % q_heads;
-    if (a.b.offsets) { // rows of sequences that this kernel has, and no others
-        if (t < a.b.offset(0) || t >= a.b.offset(a.b.seqs))
+    const int64_t t = min(entry, all - 1) / q_heads, h = min(entry, all - 1) % q_heads;
+    if (a.b.offsets) { // rows of sequences that attend_tiles has, and no others
+        // the last sequence that begins at or before the wave's first token, and from there on this thread's
+        int lo = find_slot(a.b.seqs, __builtin_amdgcn_readfirstlane((int)t), [&](int s) { return (int64_t)a.b.offset(s); });
+        while (lo + 1 < a.b.seqs && a.b.offset(lo + 1) <= t)
+            ++lo;
+        if (t < a.b.offset(lo))
             return;
-        int lo = 0, hi = a.b.seqs - 1; // the last sequence that begins at or before t
-        while (lo < hi) {
-            const int mid = (lo + hi + 1) / 2;
-            if (a.b.offset(mid) <= t)
-                lo = mid;
-            else
-                hi = mid - 1;
-        }
         const Sequence seq = sequence(a, lo);
         if (t >= seq.first + seq.n || (int64_t)seq.n * a.group <= a.few_rows)
             return;
     }
+    if ((int)threadIdx.x >= kRows * kWide || entry >= all)
+        return;
     float m = -__builtin_inff(), l = 0.0f;
     v4f o = {0.0f, 0.0f, 0.0f, 0.0f};
     for (int p = 0; p < a.parts; ++p) {

@@ -374,10 +374,10 @@ const std::vector<EntryDecl> &compiled_entries()
         MAMBO_ENTRY(mambo_kv_cache_bytes, "pages", "heads", "head_dim", "page_size"),
         MAMBO_ENTRY(mambo_kv_append, "rows", "tokens", "cache", "batch", "table", "positions", "stream"),
         MAMBO_ENTRY(mambo_kv_read, "cache", "batch", "sequences", "positions", "n", "heads", "dim", "k", "v", "stream"),
-        MAMBO_ENTRY(mambo_kv_attention_workspace, "cache", "batch", "tokens", "q_heads"),
+        MAMBO_ENTRY(mambo_kv_attention_workspace, "cache", "batch", "tokens", "q_heads", "window"),
         MAMBO_ENTRY(mambo_kv_attention, "q", "tokens", "q_heads", "dim", "ldqt", "ldqh", "cache", "batch", "scale", "causal", "window",
                     "out", "ldot", "ldoh", "lse", "workspace", "workspace_bytes", "stream"),
-        MAMBO_ENTRY(mambo_kv_attention_plan, "cache", "batch", "tokens", "q_heads", "plan"),
+        MAMBO_ENTRY(mambo_kv_attention_plan, "cache", "batch", "tokens", "q_heads", "window", "plan"),
         MAMBO_ENTRY(mambo_synth_iq3s, "seed", "blocks", "row0", "nrows", "raw", "stream"),
         MAMBO_ENTRY(mambo_synth_bf16, "seed", "outlier_seed", "outlier_frac", "i0", "count", "out", "stream"),
         MAMBO_ENTRY(mambo_e4m3_convert, "in", "n", "out_sw", "out_hw", "stream"),

@@ -8,12 +8,27 @@ Sequences are told as for launch_append_kv (mambo_amd.kernels.kv_cache).
 
 from __future__ import annotations
 
+from functools import lru_cache
+
 import torch
 
 from mambo_amd import _native
 from mambo_amd.kernels.kv_cache import batch_args, check_cache
 from mambo_amd.kernels.rotary import check_heads, head_strides, heads_in_place, output_heads
 from mambo_amd.utils.kv_cache import KVCache
+
+
+@lru_cache(maxsize=1024)
+def _workspace(pages: int, kv_heads: int, dim: int, page_size: int, seqs: int, width: int, ragged: bool, tokens: int, heads: int,
+               window: int) -> int:
+    """Bytes that a call of these sizes needs (asked once of each: a call of its own is a tenth of an eager launch)."""
+    unused = 256  # an address that is not looked at
+    cache = _native.KVCacheArgs(unused, unused, pages, kv_heads, dim, page_size, 0)
+    batch = _native.KVBatchArgs(unused, width, width, unused, unused if ragged else None, seqs)
+    size = _native.lib().mambo_kv_attention_workspace(cache, batch, tokens, heads, window)
+    if size < 0:
+        _native.check(size, "launch_attention_kv")
+    return size
 
 
 def launch_attention_kv(q: torch.Tensor, cache: KVCache, tables: torch.Tensor, lengths: torch.Tensor, *,
@@ -51,13 +66,11 @@ def launch_attention_kv(q: torch.Tensor, cache: KVCache, tables: torch.Tensor, l
             strides = head_strides(q)
         out = output_heads(out, q.shape, torch.bfloat16, dev)
         lse = torch.empty((tokens, heads), dtype=torch.float32, device=dev) if return_lse else None
-        lib = _native.lib()
-        size = lib.mambo_kv_attention_workspace(cache.args, batch, tokens, heads)
-        if size < 0:
-            _native.check(size, "launch_attention_kv")
-        workspace = torch.empty(size, dtype=torch.uint8, device=dev)
-        _native.check(lib.mambo_kv_attention(
+        size = _workspace(cache.pages, cache.heads, dim, cache.page_size, batch.seqs, batch.width, offsets is not None, tokens,
+                          heads, window)
+        workspace = torch.empty(size, dtype=torch.uint8, device=dev).data_ptr() if size else None
+        _native.check(_native.lib().mambo_kv_attention(
             q.data_ptr(), tokens, heads, dim, *strides, cache.args, batch, scale, bool(causal), window, out.data_ptr(),
-            *head_strides(out), None if lse is None else lse.data_ptr(), workspace.data_ptr(), size,
+            *head_strides(out), None if lse is None else lse.data_ptr(), workspace, size,
             _native.stream_handle(stream, dev)), "launch_attention_kv")
     return (out, lse) if return_lse else out
