@@ -54,8 +54,8 @@ Plan make_plan(const KvCache &c, const KvBatch &b, int group, int64_t window)
         const int tile = tile_rows(padded / 32);
         p.tiles_each = (int)cdiv(rows, tile);
         p.tiles = b.offsets ? (int64_t)b.tokens * group / tile + b.seqs : (int64_t)b.seqs * p.tiles_each;
-        // a workgroup a CU
-        p.parts = (int)std::max<int64_t>(1, std::min<int64_t>(kCus / (p.tiles * c.heads), cdiv(b.capacity, 512)));
+        // a workgroup a CU, two where sequences may differ: the longest then have more parts than the others
+        p.parts = (int)std::max<int64_t>(1, std::min<int64_t>((b.offsets ? 2 : 1) * kCus / (p.tiles * c.heads), cdiv(b.capacity, 512)));
         if (p.parts > 1)
             p.tiles_entries = (int64_t)p.parts * b.tokens * group * c.heads;
     }

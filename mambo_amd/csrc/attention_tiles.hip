@@ -34,6 +34,23 @@ __device__ __forceinline__ int64_t tiles_before(const Attention &a, int tile_row
     return (int64_t)a.b.offset(s) * a.group / tile_rows + s;
 }
 
+// The blocks [lo, hi) of keys of the rows from row0 on: what the first row sees of the window to what the last one sees.
+// They are dealt evenly to several workgroups where there are eight steps of the kernel and more for each.
+struct Keys {
+    int lo, hi, tiles, parts;
+    __device__ int begin(int part) const { return lo + kTileBlocks * (int)((int64_t)tiles * part / parts); }
+};
+__device__ __forceinline__ Keys tile_keys(const Attention &a, const Sequence &seq, int row0, int tile_rows)
+{
+    const int i0 = row0 / a.group, i1 = (min(row0 + tile_rows, seq.n * a.group) - 1) / a.group;
+    Keys k;
+    k.lo = max(0, sees_from(a, seq, i0)) / kKvBlock;
+    k.hi = (max(0, sees_to(a, seq, i1)) + kKvBlock - 1) / kKvBlock;
+    k.tiles = max(0, k.hi - k.lo + kTileBlocks - 1) / kTileBlocks;
+    k.parts = max(1, min(a.parts, k.tiles / 8));
+    return k;
+}
+
 template <int DS>
 __global__ __launch_bounds__(64 * tile_waves(DS), tile_waves(DS) / 4) void attend_tiles_kernel(const Attention a)
 {
@@ -64,15 +81,11 @@ __global__ __launch_bounds__(64 * tile_waves(DS), tile_waves(DS) / 4) void atten
         return;
     const int rows = (int)rows64, row0 = (int)row0_64;
 
-    // the tile's keys: what its first row sees of the window to what its last one sees
-    const int i0 = row0 / a.group, i1 = (min(row0 + kTileRows, rows) - 1) / a.group;
-    int lo = max(0, sees_from(a, seq, i0)) / kKvBlock, hi = (max(0, sees_to(a, seq, i1)) + kKvBlock - 1) / kKvBlock;
-    if (a.parts > 1) { // an even share of them
-        const int tiles = (hi - lo + kTileBlocks - 1) / kTileBlocks, part = (int)blockIdx.y;
-        const int begin = lo + kTileBlocks * (int)((int64_t)tiles * part / a.parts);
-        hi = min(hi, lo + kTileBlocks * (int)((int64_t)tiles * (part + 1) / a.parts));
-        lo = begin;
-    }
+    const Keys keys_of = tile_keys(a, seq, row0, kTileRows);
+    const int part = (int)blockIdx.y;
+    if (part >= keys_of.parts)
+        return;
+    const int lo = keys_of.begin(part), hi = min(keys_of.hi, keys_of.begin(part + 1));
 
     // this wave's rows: column col
     const int row = row0 + 32 * wave + col, i = row / a.group, h = head * a.group + row % a.group;
@@ -270,6 +283,14 @@ __global__ __launch_bounds__(64 * tile_waves(DS), tile_waves(DS) / 4) void atten
             next_values = place_of(blk + 2 * kTileBlocks, p2, 1);
         };
         if (seen(blk)) {
+            bf16x8 p[2 * kTileBlocks], ahead[kAhead];
+            constexpr int kFirst = kTileBlocks * kSteps, kSecond = 2 * kTileBlocks * DS;
+            const auto key = [&](int n) { return keys[buf ^ 1][2 * (n / kTileBlocks) + half][32 * (n % kTileBlocks) + col]; };
+            const auto value = [&](int n) { return values[buf][2 * (n / DS) + half][32 * (n % DS) + col]; };
+#pragma unroll
+            for (int n = 0; n < kAhead; ++n)
+                ahead[n] = key(n);
+            MAMBO_FIXED_ORDER();
             top = halves_max(top) * a.scale;
             // The running largest may lag by 2^8: probabilities up to there are as exact, and sums are far from
             // overflow; most tiles then leave the sums as they are.
@@ -284,10 +305,6 @@ __global__ __launch_bounds__(64 * tile_waves(DS), tile_waves(DS) / 4) void atten
                     o[d] *= by;
             }
             const float less = m == -__builtin_inff() ? 0.0f : m;
-            bf16x8 p[2 * kTileBlocks], ahead[kAhead];
-            constexpr int kFirst = kTileBlocks * kSteps, kSecond = 2 * kTileBlocks * DS;
-            const auto key = [&](int n) { return keys[buf ^ 1][2 * (n / kTileBlocks) + half][32 * (n % kTileBlocks) + col]; };
-            const auto value = [&](int n) { return values[buf][2 * (n / DS) + half][32 * (n % DS) + col]; };
             // Of the 32 probabilities of a lane 20 are worked out beside the first product, 12 beside the first half of
             // the second (whose operands they are later), the next tile's largest and the widening of what was loaded for
             // later ones beside the other half: about as much for the vector unit in all of them.
@@ -299,10 +316,6 @@ __global__ __launch_bounds__(64 * tile_waves(DS), tile_waves(DS) / 4) void atten
                 if (i % 8 == 7 || i == kEarly - 1) // here, and not where it is used
                     asm volatile("" : "+v"(p[i / 8]), "+v"(l[0]), "+v"(l[1]));
             };
-            MAMBO_FIXED_ORDER();
-#pragma unroll
-            for (int n = 0; n < kAhead; ++n)
-                ahead[n] = key(n);
 #pragma unroll
             for (int n = 0; n < kFirst; ++n) {
                 MAMBO_FIXED_ORDER();
@@ -368,7 +381,7 @@ __global__ __launch_bounds__(64 * tile_waves(DS), tile_waves(DS) / 4) void atten
     if (!some)
         return;
     const int64_t t = seq.first + i, q_heads = (int64_t)a.group * a.cache.heads;
-    if (a.parts > 1) {
+    if (keys_of.parts > 1) {
         const int64_t entry = ((int64_t)blockIdx.y * a.b.tokens + t) * q_heads + h;
 #pragma unroll
         for (int d = 0; d < DS; ++d)
@@ -404,22 +417,24 @@ __global__ __launch_bounds__(256) void join_tiles_kernel(const Attention a)
     const int64_t entry = (int64_t)blockIdx.x * kRows + (int)threadIdx.x / kWide;
     const int d = 4 * ((int)threadIdx.x % kWide);
     const int64_t t = min(entry, all - 1) / q_heads, h = min(entry, all - 1) % q_heads;
-    if (a.b.offsets) { // rows of sequences that attend_tiles has, and no others
+    int s = a.b.offsets ? 0 : (int)t / a.b.each;
+    if (a.b.offsets) {
         // the last sequence that begins at or before the wave's first token, and from there on this thread's
-        int lo = find_slot(a.b.seqs, __builtin_amdgcn_readfirstlane((int)t), [&](int s) { return (int64_t)a.b.offset(s); });
-        while (lo + 1 < a.b.seqs && a.b.offset(lo + 1) <= t)
-            ++lo;
-        if (t < a.b.offset(lo))
-            return;
-        const Sequence seq = sequence(a, lo);
-        if (t >= seq.first + seq.n || (int64_t)seq.n * a.group <= a.few_rows)
-            return;
+        s = find_slot(a.b.seqs, __builtin_amdgcn_readfirstlane((int)t), [&](int i) { return (int64_t)a.b.offset(i); });
+        while (s + 1 < a.b.seqs && a.b.offset(s + 1) <= t)
+            ++s;
     }
-    if ((int)threadIdx.x >= kRows * kWide || entry >= all)
-        return;
+    const Sequence seq = sequence(a, s);
+    if ((int)threadIdx.x >= kRows * kWide || entry >= all || t < seq.first || t >= seq.first + seq.n ||
+        (int64_t)seq.n * a.group <= a.few_rows)
+        return; // rows of sequences that attend_tiles has, and no others
+    const int row = ((int)t - seq.first) * a.group + (int)h % a.group;
+    const int parts = tile_keys(a, seq, row / tile_rows(DS) * tile_rows(DS), tile_rows(DS)).parts;
+    if (parts == 1)
+        return; // written by the one that had all of them
     float m = -__builtin_inff(), l = 0.0f;
     v4f o = {0.0f, 0.0f, 0.0f, 0.0f};
-    for (int p = 0; p < a.parts; ++p) {
+    for (int p = 0; p < parts; ++p) {
         const float2 ml = *reinterpret_cast<const float2 *>(a.tiles_ml + (p * all + entry) * 2);
         const v4f x = *reinterpret_cast<const v4f *>(a.tiles_o + (p * all + entry) * DP + d);
         const float top = fmaxf(m, ml.x), less = top == -__builtin_inff() ? 0.0f : top;
