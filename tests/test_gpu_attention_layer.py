@@ -1,0 +1,182 @@
+"""The operators between the projections together: the block of a layer against 64 bits, its command, HIP graphs that
+are replayed as sequences grow, named streams, several calls at once."""
+
+from __future__ import annotations
+
+import json
+
+import numpy as np
+import pytest
+import torch
+
+import kv_reference as ref
+from conftest import make_synthetic_iq3_s
+from oracle import oracle
+from test_gpu_kv_cache import new_cache, read_all, rows_of
+
+pytestmark = pytest.mark.gpu
+
+
+def prepared(gpu, n, k, seed):
+    from mambo_amd.utils.iq3_s_weight import prepare_iq3_s_fields
+    raw = make_synthetic_iq3_s(n, k, seed=seed)
+    return prepare_iq3_s_fields(torch.from_numpy(raw).to(gpu)), raw
+
+
+def test_block_against_64_bits(gpu):
+    """Prompts of two sequences, then two tokens each. The projections are the oracle's, on the rows that each was given;
+    between them stands the definition."""
+    from mambo_amd.utils.attention_layer import AttentionLayer
+    from mambo_amd.utils.kv_cache import allocate_kv_cache
+    from mambo_amd.utils.rotary_table import prepare_rotary_table, rotary_frequencies
+    heads, group, dim, width = 2, 2, 64, 256
+    q_heads = heads * group
+    (q, rq), (k, rk), (v, rv), (o, ro) = (prepared(gpu, n, kk, s) for s, (n, kk) in enumerate(
+        ((q_heads * dim, width), (heads * dim, width), (heads * dim, width), (width, q_heads * dim))))
+    layer = AttentionLayer(q, k, v, o, prepare_rotary_table(dim))
+    frequencies = rotary_frequencies(dim)[0]
+    rng = np.random.default_rng(0)
+    cache = allocate_kv_cache(6, heads, dim, page_size=32)
+    tables = torch.tensor([[5, 1, -1], [0, 3, 4]], dtype=torch.int32, device=gpu)
+    models = [ref.Model(heads, dim) for _ in range(2)]
+    lengths = np.zeros(2, dtype=np.int32)
+    for counts in ([33, 40], [1, 1], [2, 2]):
+        starts, n = lengths.copy(), sum(counts)
+        lengths += np.array(counts, dtype=np.int32)
+        x = torch.from_numpy(rng.standard_normal((n, width)).astype(np.float32)).to(torch.bfloat16)
+        out = layer(x.to(gpu), cache, tables, *ref.device(gpu, lengths), *ref.device(gpu, ref.offsets_of(counts)))
+        rows = oracle.quantize_mxfp8(x.float().numpy())
+        q64, k64, v64 = (oracle.iq3s_fp8_matmul(*rows, raw).astype(np.float64).reshape(n, -1, dim) for raw in (rq, rk, rv))
+        positions = np.concatenate([np.arange(s, s + c) for s, c in zip(starts, counts)])
+        q64, k64 = ref.rotate(q64, positions, frequencies, False), ref.rotate(k64, positions, frequencies, False)
+        cuts, a = ref.offsets_of(counts), np.zeros((n, q_heads, dim))
+        for s in range(2):
+            part = slice(cuts[s], cuts[s + 1])
+            models[s].append(k64[part], v64[part], int(starts[s]))
+            a[part] = ref.attend(q64[part], models[s].k, models[s].v, group, dim ** -0.5, True, 0)[0]
+        expected = oracle.iq3s_fp8_matmul(*oracle.quantize_mxfp8(a.reshape(n, -1).astype(np.float32)), ro).astype(np.float64)
+        got = out.double().cpu().numpy()
+        # Scores of a few hundred let single tokens win, so that a code that a projection's last bits move to its
+        # neighbour (2^-4 of a key) can change a row: all rows together, with the 2^-4 of the codes between.
+        assert np.linalg.norm(got - expected) <= 0.05 * np.linalg.norm(expected)
+
+
+def test_command(gpu, capsys):
+    from mambo_amd.utils import attention_layer
+    for extra in ([], ["--window", "20", "--page-size", "32"]):
+        assert attention_layer.main(["--users", "3", "--prompt", "45", "--steps", "5", *extra]) == 0
+        line = json.loads(capsys.readouterr().out)
+        assert line["graph_equals_eager"] and line["graph_us"] > 0 and line["output_rms"] > 0
+
+
+@pytest.mark.parametrize("ragged", [False, True])
+def test_two_graphs_with_their_own_caches(gpu, ragged):
+    """Two captured steps, replayed in turn and at once on two streams, between eager calls; lengths grow on the device."""
+    from mambo_amd.kernels.attention import launch_attention_kv
+    from mambo_amd.kernels.kv_cache import launch_append_kv
+    from mambo_amd.utils.rotary_table import prepare_rotary_table
+    rng = np.random.default_rng(1)
+    heads, group, dim, page, steps = 2, 4, 64, 32, 6
+    table = prepare_rotary_table(dim)
+    runs = []
+    for start in ([3000, 100], [40, 1500]):  # long enough to be split and joined
+        host, pages = ref.tables_of(rng, [n + steps * 2 for n in start], page)
+        tables, cache = ref.device(gpu, host)[0], new_cache(pages, heads, dim, page)
+        k, v = rows_of(rng, sum(start), heads, dim, torch.bfloat16).to(gpu), rows_of(rng, sum(start), heads, dim, torch.bfloat16).to(gpu)
+        lengths = ref.device(gpu, np.array(start, np.int32))[0]
+        launch_append_kv(k, v, cache, tables, lengths, offsets=ref.device(gpu, ref.offsets_of(start))[0])
+        new = [rows_of(rng, 2, h, dim, torch.float32).to(gpu) for h in (heads * group, heads, heads)]
+        offsets = ref.device(gpu, np.array([0, 1, 2], np.int32))[0] if ragged else None
+        runs.append((cache, tables, lengths, new, offsets))
+
+    def step(cache, tables, lengths, new, offsets):
+        lengths.add_(1)
+        q = launch_append_kv(new[1], new[2], cache, tables, lengths, offsets=offsets, rotary=table, q=new[0])
+        return launch_attention_kv(q, cache, tables, lengths, offsets=offsets, return_lse=True)
+
+    def copied(run):
+        from mambo_amd.utils.kv_cache import KVCache
+        cache, tables, lengths, new, offsets = run
+        return (KVCache(cache.codes.clone(), cache.scales.clone(), cache.heads, cache.head_dim, cache.page_size), tables,
+                lengths.clone(), new, offsets)
+
+    eager = [copied(r) for r in runs]
+    expected = [[tuple(t.clone() for t in step(*r)) for _ in range(steps)] for r in eager]
+    graphs, outs, streams = [], [], [torch.cuda.Stream(), torch.cuda.Stream()]
+    for run, stream in zip(runs, streams):
+        saved = run[2].clone()
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.stream(stream), torch.cuda.graph(graph, stream=stream):
+            outs.append(step(*run))
+        graphs.append(graph)
+        assert torch.equal(run[2], saved)
+    torch.cuda.synchronize()
+    for i in range(steps):
+        for graph, stream in zip(graphs, streams):
+            with torch.cuda.stream(stream):
+                graph.replay()
+        step(*copied(eager[0]))  # other work in between
+        torch.cuda.synchronize()
+        for got, want in zip(outs, expected):
+            assert torch.equal(got[0], want[i][0]) and torch.equal(got[1], want[i][1]), i
+
+
+def test_named_streams(gpu):
+    """Every operator on a stream that is not the current one, after work of that stream: what they allocate and copy
+    belongs to it, too."""
+    from mambo_amd.kernels.attention import launch_attention_kv
+    from mambo_amd.kernels.kv_cache import launch_append_kv, launch_read_kv
+    from mambo_amd.kernels.rotary import launch_rotary
+    from mambo_amd.utils.rotary_table import prepare_rotary_table
+    from test_gpu_named_streams import freed_blocks_of, made_on
+    rng = np.random.default_rng(2)
+    heads, group, dim, page, n = 2, 2, 64, 32, 200
+    table = prepare_rotary_table(dim)
+    lengths = torch.tensor([n], dtype=torch.int32, device=gpu)
+    tables = torch.arange(7, dtype=torch.int32, device=gpu)[None]
+    data = rows_of(rng, n, 8, 2 * dim, torch.float32).to(gpu)
+    at = ref.device(gpu, np.zeros(n, np.int32), np.arange(n, dtype=np.int32))
+    side = torch.cuda.Stream()
+
+    def run(x, stream, cache):
+        apart = x[..., ::2]  # values apart: copied first
+        q = launch_append_kv(apart[:, 4:6], apart[:, 6:], cache, tables, lengths, rotary=table, q=apart[:, :4], stream=stream)
+        turned = launch_rotary(apart, at[1], table, out_dtype=torch.bfloat16, stream=stream)
+        out, lse = launch_attention_kv(q, cache, tables, lengths, return_lse=True, stream=stream)
+        few = launch_attention_kv(turned[-1:, :4], cache, tables, lengths, stream=stream)
+        return [q, turned, out, lse, few, *launch_read_kv(cache, tables, *at, stream=stream)]
+
+    expected = run(data, None, new_cache(7, heads, dim, page))
+    for stream in (side, side.cuda_stream):
+        cache = new_cache(7, heads, dim, page)
+        late = made_on(side, data, torch.zeros_like(data))
+        freed_blocks_of([t.numel() * t.element_size() for t in expected])
+        got = run(late, stream, cache)
+        side.synchronize()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, expected))
+
+
+def test_calls_at_once_on_one_cache(gpu):
+    """Attention of several streams over one cache: nothing of the calls is shared."""
+    from mambo_amd.kernels.attention import launch_attention_kv
+    from mambo_amd.kernels.kv_cache import launch_append_kv
+    rng = np.random.default_rng(3)
+    heads, group, dim, page, lengths = 2, 4, 128, 64, [5000, 3000]
+    host, pages = ref.tables_of(rng, lengths, page)
+    tables, cache = ref.device(gpu, host)[0], new_cache(pages, heads, dim, page)
+    n = sum(lengths)
+    on = ref.device(gpu, np.array(lengths, np.int32))[0]
+    launch_append_kv(rows_of(rng, n, heads, dim, torch.bfloat16).to(gpu), rows_of(rng, n, heads, dim, torch.bfloat16).to(gpu), cache,
+                     tables, on, offsets=ref.device(gpu, ref.offsets_of(lengths))[0])
+    qs = [rows_of(rng, 2 * m, heads * group, dim, torch.bfloat16).to(gpu) for m in (1, 2, 90, 1)]
+    expected = [launch_attention_kv(q, cache, tables, on) for q in qs]
+    streams = [torch.cuda.Stream() for _ in qs]
+    torch.cuda.synchronize()
+    for _ in range(10):
+        got = [launch_attention_kv(q, cache, tables, on, stream=s) for q, s in zip(qs, streams)]
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, expected))
+    keys, _ = read_all(cache, tables, [1, 1])
+    assert all(np.isfinite(t).all() for t in keys)
