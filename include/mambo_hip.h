@@ -438,7 +438,7 @@ typedef struct mambo_kv_rows {
 /* Stores the call's tokens in the cache, the keys rotated (table NULL: as they are) by positions[t] (NULL:
  * by the position in the sequence). A block that is entered at its first token starts anew, one entered
  * later keeps its older tokens: its exponent is the larger of the old and e = max(ceil(log2(amax / 448)),
- * -100) of the new rows, and where it grows, the older codes are rounded again to it. A token with a key or value
+ * -100) of the new rows (values beyond 240 * 2^120 are held as that), and where it grows, the older codes are rounded again to it. A token with a key or value
  * of a head that is not finite is held as NaN keys and zero values of that head and counts for no exponent. A row whose
  * position in its sequence is negative is not stored (its queries are rotated). Sequences of a call
  * must not share a block that one of them writes. */

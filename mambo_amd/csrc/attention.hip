@@ -73,9 +73,9 @@ int check(const mambo_kv_cache *cache, const mambo_kv_batch *batch, int64_t toke
     MAMBO_REQUIRE(q_heads >= c->heads && q_heads % c->heads == 0 && q_heads <= 65535, MAMBO_ERR_VALUE,
                   "%lld query heads are no multiple of %d", (long long)q_heads, c->heads);
     MAMBO_REQUIRE(window >= 0, MAMBO_ERR_VALUE, "a window is positive, and of causal attention");
-    MAMBO_REQUIRE(tokens * q_heads <= 0x7FFFFFFF, MAMBO_ERR_VALUE, "tokens times query heads must be below 2^31 (got %lld)",
+    MAMBO_REQUIRE(tokens * q_heads <= 0x3FFFFFFF, MAMBO_ERR_VALUE, "tokens times query heads must be below 2^30 (got %lld)",
                   (long long)tokens);
-    MAMBO_REQUIRE(batch->seqs * (int64_t)(b->capacity / kKvBlock) <= 0x7FFFFFFF, MAMBO_ERR_VALUE,
+    MAMBO_REQUIRE(batch->seqs * (int64_t)(b->capacity / kKvBlock) <= 0x7FFFFFF0, MAMBO_ERR_VALUE,
                   "tables must hold below 2^36 tokens together");
     *p = make_plan(*c, *b, (int)(q_heads / c->heads), window);
     const int64_t rows = p->few_rows, heads = c->heads;
@@ -125,7 +125,7 @@ extern "C" int mambo_kv_attention(const void *q, int64_t tokens, int64_t q_heads
     if (const int rc = check(cache, batch, tokens, q_heads, window, &a.cache, &a.b, &p))
         return rc;
     MAMBO_REQUIRE(dim == a.cache.dim, MAMBO_ERR_VALUE, "the cache has heads of %d (got %lld)", a.cache.dim, (long long)dim);
-    MAMBO_REQUIRE(scale > 0.0f && isfinite(scale), MAMBO_ERR_VALUE, "the scale of the scores must be positive and finite");
+    MAMBO_REQUIRE(scale * kLog2e > 0.0f && isfinite(scale * kLog2e), MAMBO_ERR_VALUE, "the scale of the scores must be positive and finite");
     MAMBO_REQUIRE(window == 0 || causal, MAMBO_ERR_VALUE, "a window is positive, and of causal attention");
     if (tokens == 0)
         return MAMBO_OK;

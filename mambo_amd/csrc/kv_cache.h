@@ -15,6 +15,9 @@
 // which is what the product with the values wants of it.
 constexpr int kKvBlock = 32;
 constexpr int kKvLowest = -100; // lowest exponent: what an empty or all-zero block has
+// The largest float32 has the exponent 120, where the code after 240 would stand for 2^128.
+constexpr int kKvHighest = 120;
+constexpr float kKvMostThere = 240.0f;
 
 __host__ __device__ constexpr int kv_padded(int dim) { return (dim + 31) & ~31; }
 __host__ __device__ constexpr int kv_key_byte(int token, int d)

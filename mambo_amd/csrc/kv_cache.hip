@@ -390,6 +390,7 @@ __global__ __launch_bounds__(256) void append_kernel(const Append a)
     const int old_k = fresh ? kKvLowest : (int)scale[0] - 127, old_v = fresh ? kKvLowest : (int)scale[1] - 127;
     const uint2 amax = largest(ka, va, scratch); // its barrier: every wave has read the old exponents
     const int ke = max(old_k, kv_exponent(amax.x)), ve = max(old_v, kv_exponent(amax.y));
+    const float k_most = ke >= kKvHighest ? kKvMostThere : 448.0f, v_most = ve >= kKvHighest ? kKvMostThere : 448.0f;
     __syncthreads();
     if (!fresh && (ke > old_k || ve > old_v)) {
         for (int i = tid; i < 2 * 2 * padded; i += 256) {
@@ -413,7 +414,7 @@ __global__ __launch_bounds__(256) void append_kernel(const Append a)
             float y[8];
 #pragma unroll
             for (int e = 0; e < 8; ++e)
-                y[e] = __builtin_ldexpf(kx[i][e], -ke);
+                y[e] = fminf(fmaxf(__builtin_ldexpf(kx[i][e], -ke), -k_most), k_most);
             uint2 w = make_uint2(pack4<true>(y[0], y[1], y[2], y[3]), pack4<true>(y[4], y[5], y[6], y[7]));
             if (bad[t])
                 w = make_uint2(0x7F7F7F7Fu, 0x7F7F7F7Fu);
@@ -431,7 +432,7 @@ __global__ __launch_bounds__(256) void append_kernel(const Append a)
             float y[8];
 #pragma unroll
             for (int e = 0; e < 8; ++e)
-                y[e] = bad[8 * kk + e] ? 0.0f : __builtin_ldexpf(vx[i][e][c], -ve);
+                y[e] = bad[8 * kk + e] ? 0.0f : fminf(fmaxf(__builtin_ldexpf(vx[i][e][c], -ve), -v_most), v_most);
             const uint2 w = make_uint2(pack4<true>(y[0], y[1], y[2], y[3]), pack4<true>(y[4], y[5], y[6], y[7]));
             uint8_t *to = values + kv_value_byte(8 * kk, d + c);
             if (p >= lo && p + 8 <= hi) {

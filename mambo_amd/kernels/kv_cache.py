@@ -61,12 +61,13 @@ def launch_append_kv(k: torch.Tensor, v: torch.Tensor, cache: KVCache, tables: t
     A block of 32 tokens and a head gets the exponent e = max(ceil(log2(amax / 448)), -100) and the codes
     E4M3(x 2^-e), to nearest even. One that older tokens of the sequence are in keeps them: its exponent is the larger of the
     two, and where it grows the older codes are rounded again. A token's head with a key or value that is not finite is held
-    as NaN keys and zero values, so that what sees it becomes NaN and nothing else does.
+    as NaN keys and zero values, so that what sees it becomes NaN and nothing else does. Values beyond 240 * 2^120 (3.2e38) are
+    held as that.
 
     ``positions`` int32 [T] are the rotary positions, by default those in the sequence. Rows whose position in the
     sequence would be negative (more rows than ``lengths``), or that no page is for, are not stored; rows of no
     sequence are left alone, and so are their queries in ``out``. Sequences of a call may share pages that none of
-    them writes in this call. T may be 0."""
+    them writes in this call. ``out`` may be ``q`` itself (bfloat16). T may be 0."""
     cache = check_cache(cache)
     dev, dim = cache.codes.device, cache.head_dim
     check_heads(k, dim, dev, "k")

@@ -30,9 +30,19 @@ class KVCache:
     page_size: int
 
     def __post_init__(self):
+        pages, blocks = self.codes.shape[0], self.page_size // KV_BLOCK
+        size = _native.lib().mambo_kv_cache_bytes(pages, self.heads, self.head_dim, self.page_size)
+        shape = (pages, self.heads, blocks, size // max(1, pages * self.heads * blocks))
+        for t, want in ((self.codes, shape), (self.scales, (*shape[:3], 2))):
+            if size == 0 or tuple(t.shape) != want or t.dtype != torch.uint8 or not t.is_contiguous() \
+                    or t.device != self.codes.device:
+                raise ValueError(f"a cache of these sizes has contiguous uint8 tensors on one device, one of them {list(want)}")
         object.__setattr__(self, "args", _native.KVCacheArgs(
             self.codes.data_ptr(), self.scales.data_ptr(), self.codes.shape[0], self.heads, self.head_dim,
             self.page_size, 0))
+
+    def __reduce__(self):  # a copy's tensors are its own, and so are the addresses that it hands to the kernels
+        return KVCache, (self.codes, self.scales, self.heads, self.head_dim, self.page_size)
 
     @property
     def pages(self) -> int:

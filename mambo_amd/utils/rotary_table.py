@@ -45,8 +45,14 @@ class RotaryTable:
     magnitude: float
 
     def __post_init__(self):
+        if self.size < 2 or self.size % 2 or tuple(self.turns.shape) != (self.size // 2,) or self.turns.dtype != torch.int64 \
+                or not self.turns.is_contiguous():
+            raise ValueError(f"angles of {self.size} values are contiguous int64 [{self.size // 2}]")
         object.__setattr__(self, "args", _native.RotaryTableArgs(self.turns.data_ptr(), self.size, self.interleaved,
                                                                  self.magnitude))
+
+    def __reduce__(self):  # a copy's tensor is its own, and so is the address that it hands to the kernels
+        return RotaryTable, (self.turns, self.size, self.interleaved, self.magnitude)
 
 
 def rotary_frequencies(size: int, *, base: float = 10000.0, scaling: dict | None = None) -> tuple[list[float], float]:

@@ -48,7 +48,9 @@ def exponent(amax: float) -> int:
 
 
 def nearest(x: np.ndarray, e: int) -> np.ndarray:
-    """E4M3(x 2^-e) 2^e."""
+    """E4M3(x 2^-e) 2^e, no more than 240 * 2^120."""
+    if e >= 120:
+        x = np.clip(x, -240 * 2.0**120, 240 * 2.0**120)
     return (VALUES[e4m3_encode_bruteforce(np.ldexp(x, -e))] * 2.0**e).reshape(np.shape(x))
 
 

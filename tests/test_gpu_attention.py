@@ -220,3 +220,33 @@ def test_offsets_past_32_bits(gpu):
         out, lse = attention()(q, cache, tables, lengths, return_lse=True)
         check(out, lse, q, [model.k], [model.v], [n], 2)
     assert not cache.codes[0].any() and math.isfinite(float(out.float().sum()))
+
+
+def test_rows_before_the_first_sequence(gpu):
+    rng = np.random.default_rng(14)
+    for lengths, counts, skip in (([200, 90], [1, 2], 40), ([300, 100], [150, 60], 7), ([40, 2500], [1, 90], 300)):
+        cache, tables, keys, values = filled(gpu, rng, lengths, 2, 64, 32)
+        n = sum(counts)
+        q = rows_of(rng, n + skip, 8, 64, torch.bfloat16).to(gpu)
+        out = torch.full(q.shape, 7.0, dtype=torch.bfloat16, device=gpu)
+        out, lse = attention()(q, cache, tables, *ref.device(gpu, np.array(lengths, np.int32)), return_lse=True, out=out,
+                               offsets=ref.device(gpu, ref.offsets_of(counts) + skip)[0])
+        assert (out[:skip] == 7.0).all()
+        check(out[skip:], lse[skip:], q[skip:], keys, values, counts, 4)
+
+
+def test_refusals(gpu):
+    from mambo_amd.utils.kv_cache import allocate_kv_cache
+    cache = allocate_kv_cache(2, 2, 64, page_size=32)
+    tables, lengths = torch.zeros((2, 1), dtype=torch.int32, device=gpu), torch.ones(2, dtype=torch.int32, device=gpu)
+    q = torch.zeros((4, 4, 64), dtype=torch.bfloat16, device=gpu)
+    good = dict(q=q, cache=cache, tables=tables, lengths=lengths)
+    attention()(**good)
+    for change in ({"q": q.float()}, {"q": q[..., :32]}, {"q": q[:, :3]}, {"q": q[:3]}, {"q": q.cpu()}, {"scale": 0.0}, {"scale": float("nan")},
+                   {"scale": -1.0}, {"scale": 3.0e38}, {"window": -1}, {"window": 4, "causal": False}, {"tables": tables.long()},
+                   {"lengths": lengths[:1]}, {"offsets": lengths}, {"offsets": torch.zeros(3, device=gpu)}, {"out": q.float()},
+                   {"out": q[:2]}, {"out": q[:1].expand(4, 4, 64)}):
+        with pytest.raises(ValueError):
+            attention()(**(good | change))
+    with pytest.raises(TypeError):
+        attention()(**(good | {"cache": cache.codes}))

@@ -178,7 +178,8 @@ def test_extreme_values(gpu):
     k, v = torch.ones((6, heads, dim)), torch.ones((6, heads, dim))
     k[0, 0, 3], v[1, 1, 39], k[2, 0, 0], v[3, 0, 7] = nan, inf, -inf, nan
     k[2, 0, 1] = 1e30  # of a token that counts for nothing
-    k[4, 1], v[4, 1] = 3.0e38, -3.0e38
+    k[4, 1], v[4, 1] = 3.4e38, -3.4e38  # would round to 2^128
+    k[4, 1, 0], v[4, 1, 0] = 3.0e38, 3.18e38
     k[5, 0], v[5, 0] = 1e-38, 0.0
     cache = new_cache(2, heads, dim, 32)
     tables = torch.tensor([[1]], dtype=torch.int32, device=gpu)
@@ -263,3 +264,78 @@ def test_strided_rows(gpu):
         at = ref.device(gpu, np.zeros(n, np.int32), np.arange(n, dtype=np.int32))
         reads = [ops().launch_read_kv(cache, wide[:, :2], *at) for cache in caches]
         assert all(torch.equal(x, y) for r in reads[1:] for x, y in zip(reads[0], r))
+
+
+def test_rows_before_the_first_sequence_and_queries_in_place(gpu):
+    """Offsets that do not begin at 0; out that is q itself."""
+    from mambo_amd.kernels.rotary import launch_rotary
+    from mambo_amd.utils.rotary_table import prepare_rotary_table
+    rng = np.random.default_rng(8)
+    heads, dim, page = 2, 64, 32
+    table = prepare_rotary_table(dim)
+    for counts, skip in (([40, 3], 70), ([1, 1], 3), ([0, 100], 33)):
+        n = sum(counts) + skip
+        host, pages = ref.tables_of(rng, counts, page)
+        tables, cache = ref.device(gpu, host)[0], new_cache(pages, heads, dim, page)
+        k, v, q = (rows_of(rng, n, h, dim, torch.bfloat16).to(gpu) for h in (heads, heads, 4))
+        before, offsets = q.clone(), ref.offsets_of(counts) + skip
+        got = ops().launch_append_kv(k, v, cache, tables, *ref.device(gpu, np.array(counts, np.int32)), offsets=ref.device(gpu, offsets)[0],
+                                     rotary=table, q=q, out=q, positions=torch.zeros(n, dtype=torch.int32, device=gpu) + 9)
+        assert got is q and torch.equal(q[:skip], before[:skip])
+        nine = torch.full((n,), 9, dtype=torch.int32, device=gpu)
+        assert torch.equal(q[skip:], launch_rotary(before, nine, table)[skip:])
+        got_k, got_v = read_all(cache, tables, counts)
+        turned = launch_rotary(k.float(), nine, table).double().cpu().numpy()
+        for s, c in enumerate(counts):
+            model = ref.Model(heads, dim)
+            if c:
+                model.append(turned[offsets[s]:offsets[s + 1]], v[offsets[s]:offsets[s + 1]].double().cpu().numpy(), 0)
+            same(got_k[s], model.k)
+            same(got_v[s], model.v)
+
+
+def test_copies_of_a_cache_are_their_own(gpu):
+    import copy
+    import dataclasses
+    from mambo_amd.utils.rotary_table import prepare_rotary_table
+    rng = np.random.default_rng(9)
+    cache = new_cache(1, 1, 32, 32)
+    tables, lengths = torch.zeros((1, 1), dtype=torch.int32, device=gpu), torch.tensor([5], dtype=torch.int32, device=gpu)
+    other, table = copy.deepcopy(cache), copy.deepcopy(prepare_rotary_table(32))
+    assert other.args.codes == other.codes.data_ptr() != cache.codes.data_ptr() and table.args.turns == table.turns.data_ptr()
+    x = rows_of(rng, 5, 1, 32, torch.float32).to(gpu)
+    ops().launch_append_kv(x, x, other, tables, lengths, rotary=table)
+    assert (cache.codes == 0x7F).all() and not (other.codes == 0x7F).all()
+    for wrong in ({"page_size": 64}, {"heads": 2}, {"head_dim": 64}, {"codes": cache.codes[..., :-64]}, {"scales": cache.scales.float()},
+                  {"scales": cache.scales.cpu()}, {"head_dim": 20}):
+        with pytest.raises(ValueError):
+            dataclasses.replace(cache, **wrong)
+    with pytest.raises(ValueError):
+        dataclasses.replace(table, size=64)
+
+
+def test_refusals(gpu):
+    from mambo_amd.utils.rotary_table import prepare_rotary_table
+    cache, table = new_cache(2, 2, 64, 32), prepare_rotary_table(64)
+    tables, lengths = torch.zeros((2, 1), dtype=torch.int32, device=gpu), torch.ones(2, dtype=torch.int32, device=gpu)
+    k, q = torch.zeros((4, 2, 64), device=gpu), torch.zeros((4, 4, 64), device=gpu)
+    good = dict(k=k, v=k, cache=cache, tables=tables, lengths=lengths)
+    ops().launch_append_kv(**good)
+    for change in ({"k": k.half()}, {"k": k[..., :32]}, {"k": q}, {"v": k.bfloat16()}, {"v": k[:2]}, {"k": k.cpu()}, {"v": k.cpu()},
+                   {"tables": tables.long()}, {"tables": tables[0]}, {"tables": tables.cpu()}, {"tables": tables[:0]},
+                   {"tables": torch.zeros((2, 4), dtype=torch.int32, device=gpu)[:, ::2]}, {"lengths": lengths[:1]}, {"lengths": lengths.long()},
+                   {"offsets": lengths}, {"k": k[:3], "v": k[:3]}, {"q": q}, {"rotary": table, "q": q.bfloat16()}, {"rotary": table, "q": q[:, :3]},
+                   {"rotary": table, "q": q[:2]}, {"positions": torch.zeros(4, dtype=torch.int32, device=gpu)},
+                   {"rotary": table, "positions": lengths}, {"rotary": prepare_rotary_table(128)}, {"out": q.bfloat16()},
+                   {"rotary": table, "q": q, "out": q}, {"rotary": table, "q": q, "out": q.bfloat16()[:2]},
+                   {"rotary": table, "q": q, "out": torch.zeros((1, 4, 64), dtype=torch.bfloat16, device=gpu).expand(4, 4, 64)}):
+        with pytest.raises(ValueError):
+            ops().launch_append_kv(**(good | change))
+    for change in ({"cache": None}, {"rotary": "angles"}):
+        with pytest.raises(TypeError):
+            ops().launch_append_kv(**(good | change))
+    assert ops().launch_append_kv(**(good | {"k": k[:0], "v": k[:0]}), rotary=table, q=q[:0]).shape == (0, 4, 64)
+    for args in ((lengths.long(), lengths), (lengths, lengths[:1]), (lengths[None], lengths)):
+        with pytest.raises(ValueError):
+            ops().launch_read_kv(cache, tables, *args)
+    assert ops().launch_read_kv(cache, tables, lengths[:0], lengths[:0])[0].shape == (0, 2, 64)

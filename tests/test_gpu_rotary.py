@@ -110,3 +110,18 @@ def test_values_that_are_not_finite_stay_with_their_pair(gpu):
         got = rotary()(x, torch.tensor([5, 6], dtype=torch.int32, device=gpu), prepare_rotary_table(32, interleaved=interleaved))
         wrong = (~torch.isfinite(got)).nonzero().tolist()
         assert wrong == [[0, 0, i] for i in ((2, 3, 40) if interleaved else (3, 19, 40))] + [[1, 0, 47]]
+
+
+def test_refusals(gpu):
+    from mambo_amd.utils.rotary_table import prepare_rotary_table
+    x, at, table = torch.zeros((3, 2, 64), device=gpu), torch.zeros(3, dtype=torch.int32, device=gpu), prepare_rotary_table(64)
+    rotary()(x, at, table)
+    for args, more in (((x.half(), at, table), {}), ((x[0], at, table), {}), ((x.cpu(), at, table), {}), ((x, at.long(), table), {}),
+                       ((x, at[:2], table), {}), ((x, at.cpu(), table), {}), ((x, at, prepare_rotary_table(66)), {}),
+                       ((torch.zeros((3, 1, 1026), device=gpu), at, table), {}), ((x, at, table), {"out_dtype": torch.float16}),
+                       ((x, at, table), {"out": x.bfloat16()}), ((x, at, table), {"out": x[:2]}),
+                       ((x, at, table), {"out": x[:1].expand(3, 2, 64)}), ((x[:, :0], at, table), {})):
+        with pytest.raises(ValueError):
+            rotary()(*args, **more)
+    with pytest.raises(TypeError):
+        rotary()(x, at, None)

@@ -145,7 +145,7 @@ def test_attention_refusals(lib):
     assert call(tokens=0, q=None, out=None, ws=None) == 0
     big = batch(seqs=2**23, width=2**20, ldt=2**20)
     refused(lib, lib.mambo_kv_attention_workspace(cache(), big, 2**23, 4, 0), "2^36 tokens")
-    refused(lib, lib.mambo_kv_attention_workspace(cache(heads=2), batch(seqs=2**23), 2**23, 1024, 0), "below 2^31")
+    refused(lib, lib.mambo_kv_attention_workspace(cache(heads=2), batch(seqs=2**23), 2**23, 1024, 0), "below 2^30")
 
 
 def test_cache_bytes(lib):
