@@ -250,3 +250,83 @@ def test_refusals(gpu):
             attention()(**(good | change))
     with pytest.raises(TypeError):
         attention()(**(good | {"cache": cache.codes}))
+
+
+def plan_of(cache, tables, tokens, q_heads, ragged, window=0):
+    import ctypes
+    from mambo_amd import _native
+    out = (ctypes.c_int32 * 4)()
+    batch = _native.KVBatchArgs(256, tables.shape[1], tables.shape[1], 256, 256 if ragged else None, tables.shape[0])
+    _native.check(_native.lib().mambo_kv_attention_plan(cache.args, batch, tokens, q_heads, window, out))
+    return list(out)
+
+
+@pytest.mark.parametrize("split", [False, True])
+@pytest.mark.parametrize("dim", [24, 64, 88, 128, 160, 184, 224, 256])
+def test_every_kernel_for_few_rows(gpu, dim, split):
+    """16, 32 and 64 rows a sequence where the head's size allows it, by one workgroup and by shares that are joined
+    (tables wide enough for long sequences)."""
+    rng = np.random.default_rng(dim)
+    lengths = [300, 33, 0, 170]
+    cache, tables, keys, values = filled(gpu, rng, lengths, 1, dim, 32, extra=100 if split else 1)
+    for group in [11] + [27] * (dim <= 128) + [61] * (dim <= 64):
+        q = rows_of(rng, 4, group, dim, torch.bfloat16, 2.0).to(gpu)
+        plan = plan_of(cache, tables, 4, group, False)
+        assert plan[0] == (16 if group == 11 else 32 if group == 27 else 64) and (plan[1] > 0) == split and plan[2] == 0
+        out, lse = attention()(q, cache, tables, *ref.device(gpu, np.array(lengths, np.int32)), return_lse=True)
+        check(out, lse, q, keys, values, [1] * 4, group)
+
+
+@pytest.mark.parametrize("dim", [24, 64, 88, 128, 160, 184, 224, 256])
+def test_every_kernel_for_many_rows(gpu, dim):
+    """With the keys in one part and in several, of one sequence and of ragged ones, of odd numbers of blocks."""
+    rng = np.random.default_rng(dim + 1)
+    for lengths, counts, parts in (([1100], [70], 3), ([290], [90], 1), ([1090, 40, 300], [66, 40, 9], 3)):
+        cache, tables, keys, values = filled(gpu, rng, lengths, 1, dim, 32)
+        n, ragged = sum(counts), len(counts) > 1
+        q = rows_of(rng, n, 2, dim, torch.bfloat16, 2.0).to(gpu)
+        plan = plan_of(cache, tables, n, 2, ragged)
+        assert plan[2] == (256 if dim <= 160 else 128) and plan[3] == parts
+        out, lse = attention()(q, cache, tables, *ref.device(gpu, np.array(lengths, np.int32)), return_lse=True,
+                               offsets=ref.device(gpu, ref.offsets_of(counts))[0] if ragged else None)
+        check(out, lse, q, keys, values, counts, 2)
+
+
+@pytest.mark.parametrize("ragged", [False, True])
+def test_many_sequences_share_the_work(gpu, ragged):
+    """More sequences than a wave adds up at once, long, short and empty, some of them without rows."""
+    rng = np.random.default_rng(15)
+    lengths = [int(n) for n in rng.integers(0, 70, 700)]
+    lengths[5], lengths[300], lengths[699] = 3000, 1500, 900
+    lengths[310:600] = [0] * 290
+    counts = [int(c) for c in rng.integers(0, 3, 700)] if ragged else [1] * 700
+    counts[300] = 1
+    cache, tables, keys, values = filled(gpu, rng, lengths, 1, 32, 64)
+    n = sum(counts)
+    q = rows_of(rng, n, 4, 32, torch.bfloat16, 2.0).to(gpu)
+    assert plan_of(cache, tables, n, 4, ragged)[1] > 0
+    out, lse = attention()(q, cache, tables, *ref.device(gpu, np.array(lengths, np.int32)), return_lse=True,
+                           offsets=ref.device(gpu, ref.offsets_of(counts))[0] if ragged else None)
+    check(out, lse, q, keys, values, counts, 4)
+
+
+def test_probabilities_add_up_over_a_rising_sequence_of_scores(gpu):
+    """Every later key scores higher than all before it: the running largest grows at every step, by less and by more
+    than the lag that the kernel for many rows allows itself."""
+    from mambo_amd.kernels.kv_cache import launch_append_kv
+    rng = np.random.default_rng(16)
+    dim, page, length = 64, 64, 700
+    for rise in (0.02, 0.4):
+        for order in (1, -1):
+            cache = new_cache(11, 1, dim, page)
+            tables = torch.arange(11, dtype=torch.int32, device=gpu)[None]
+            k = torch.ones((length, 1, dim)) * (rise * torch.arange(length)[:, None, None] / 8.0)
+            k = k.flip(0) if order < 0 else k
+            v = rows_of(rng, length, 1, dim, torch.bfloat16)
+            lengths = torch.tensor([length], dtype=torch.int32, device=gpu)
+            launch_append_kv(k.bfloat16().to(gpu), v.to(gpu), cache, tables, lengths)
+            keys, values = read_all(cache, tables, [length])
+            for n in (1, 80):
+                q = torch.ones((n, 2, dim), dtype=torch.bfloat16, device=gpu)
+                out, lse = attention()(q, cache, tables, lengths, return_lse=True)
+                check(out, lse, q, keys, values, [n], 2)
