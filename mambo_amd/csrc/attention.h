@@ -99,5 +99,50 @@ constexpr int max_row_tiles(int padded) { return padded <= 64 ? 4 : padded <= 12
 constexpr int tile_waves(int ds) { return ds <= 5 ? 8 : 4; }
 constexpr int tile_rows(int ds) { return 32 * tile_waves(ds); }
 
+// Blocks that a sequence has in the row kernel's order.
+__device__ __forceinline__ int row_blocks(const Attention &a, const Sequence &q)
+{
+    return q.n > 0 && q.n <= a.few_rows / a.group ? q.hi - q.lo : 0;
+}
+
+// The shares: workgroups that have any (at least four blocks each, one a wave), and where they begin.
+__device__ __forceinline__ int shares(const Attention &a, int total) { return max(1, min(a.slots, (total + 3) / 4)); }
+__device__ __forceinline__ int share_begin(int p, int total, int count) { return (int)((int64_t)p * total / count); }
+__device__ __forceinline__ int share_of(int block, int total, int count)
+{
+    return (int)((((int64_t)block + 1) * count + total - 1) / total) - 1;
+}
+
+// A row's result: four values of it, and with the first of them its lse.
+__device__ __forceinline__ void store_row(const Attention &a, int64_t t, int h, int d, v4f o, float top, float sum)
+{
+    o *= sum == 0.0f ? 0.0f : 1.0f / sum;
+    if (d < a.cache.dim)
+        store_row4<true>(a.out, t * a.ldot + h * a.ldoh + d, o, a.cache.dim - d,
+                         a.ldot % 4 == 0 && a.ldoh % 4 == 0 && (uintptr_t)a.out % 8 == 0);
+    if (a.lse && d == 0)
+        a.lse[t * ((int64_t)a.group * a.cache.heads) + h] = sum == 0.0f ? -__builtin_inff() : (top + __log2f(sum)) * kLn2;
+}
+
+constexpr int kTileBlocks = 2; // blocks of 32 tokens of a tile
+
+// The blocks [lo, hi) of keys of the rows from row0 on: what the first row sees of the window to what the last one sees.
+// They are dealt evenly to several workgroups where there are five steps of the kernel and more for each.
+struct Keys {
+    int lo, hi, tiles, parts;
+    __device__ int begin(int part) const { return lo + kTileBlocks * (int)((int64_t)tiles * part / parts); }
+};
+__device__ __forceinline__ Keys tile_keys(const Attention &a, const Sequence &seq, int row0, int tile_rows)
+{
+    const int i0 = row0 / a.group, i1 = (min(row0 + tile_rows, seq.n * a.group) - 1) / a.group;
+    Keys k;
+    k.lo = max(0, sees_from(a, seq, i0)) / kKvBlock;
+    k.hi = (max(0, sees_to(a, seq, i1)) + kKvBlock - 1) / kKvBlock;
+    k.tiles = max(0, k.hi - k.lo + kTileBlocks - 1) / kTileBlocks;
+    k.parts = max(1, min(a.parts, k.tiles / 5));
+    return k;
+}
+
 int launch_attend_rows(const Attention &a, int row_tiles, hipStream_t s);
 int launch_attend_tiles(const Attention &a, int64_t tiles, hipStream_t s);
+int launch_attend_join(const Attention &a, int row_tiles, hipStream_t s);

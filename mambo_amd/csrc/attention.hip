@@ -78,9 +78,9 @@ int check(const mambo_kv_cache *cache, const mambo_kv_batch *batch, int64_t toke
     MAMBO_REQUIRE(batch->seqs * (int64_t)(b->capacity / kKvBlock) <= 0x7FFFFFF0, MAMBO_ERR_VALUE,
                   "tables must hold below 2^36 tokens together");
     *p = make_plan(*c, *b, (int)(q_heads / c->heads), window);
-    const int64_t rows = p->few_rows, heads = c->heads;
-    MAMBO_REQUIRE(grid_takes(batch->seqs * heads, 256) && rows <= 65535 && grid_takes(p->tiles * heads, 512) &&
-                      grid_takes(tokens * q_heads, 256),
+    const int64_t rows = p->slots ? p->few_rows : 0, heads = c->heads;
+    MAMBO_REQUIRE(grid_takes(batch->seqs * heads, 512) && grid_takes(p->tiles * heads, 512) &&
+                      grid_takes(tokens * q_heads + batch->seqs * heads * rows, 256),
                   MAMBO_ERR_VALUE, "too many rows for one launch");
     return MAMBO_OK;
 }
@@ -151,5 +151,8 @@ extern "C" int mambo_kv_attention(const void *q, int64_t tokens, int64_t q_heads
     if (p.tiles)
         if (const int rc = launch_attend_tiles(a, p.tiles, s))
             return rc;
-    return p.row_tiles ? launch_attend_rows(a, p.row_tiles, s) : MAMBO_OK;
+    if (p.row_tiles)
+        if (const int rc = launch_attend_rows(a, p.row_tiles, s))
+            return rc;
+    return p.slots || p.parts > 1 ? launch_attend_join(a, p.row_tiles, s) : MAMBO_OK;
 }

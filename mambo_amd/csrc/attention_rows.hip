@@ -28,20 +28,6 @@ __device__ __forceinline__ float across_sum(float x)
     return __uint_as_float(b[0]) + __uint_as_float(b[1]);
 }
 
-// Blocks that a sequence has in the row kernel's order.
-__device__ __forceinline__ int row_blocks(const Attention &a, const Sequence &q)
-{
-    return q.n > 0 && q.n <= a.few_rows / a.group ? q.hi - q.lo : 0;
-}
-
-// The shares: workgroups that have any (at least four blocks each, one a wave), and where they begin.
-__device__ __forceinline__ int shares(const Attention &a, int total) { return max(1, min(a.slots, (total + 3) / 4)); }
-__device__ __forceinline__ int share_begin(int p, int total, int count) { return (int)((int64_t)p * total / count); }
-__device__ __forceinline__ int share_of(int block, int total, int count)
-{
-    return (int)((((int64_t)block + 1) * count + total - 1) / total) - 1;
-}
-
 // The sequences' blocks added up by every wave for itself, 256 sequences at a time, four a lane (about
 // 1 us up to 256; a table of them would be a launch of its own).
 struct Scan {
@@ -356,17 +342,6 @@ struct Rows {
     }
 };
 
-// A row's result: four values of it, and with the first of them its lse.
-__device__ __forceinline__ void store_row(const Attention &a, int64_t t, int h, int d, v4f o, float top, float sum)
-{
-    o *= sum == 0.0f ? 0.0f : 1.0f / sum;
-    if (d < a.cache.dim)
-        store_row4<true>(a.out, t * a.ldot + h * a.ldoh + d, o, a.cache.dim - d,
-                         a.ldot % 4 == 0 && a.ldoh % 4 == 0 && (uintptr_t)a.out % 8 == 0);
-    if (a.lse && d == 0)
-        a.lse[t * ((int64_t)a.group * a.cache.heads) + h] = sum == 0.0f ? -__builtin_inff() : (top + __log2f(sum)) * kLn2;
-}
-
 // Two waves a SIMD while a wave's registers are enough.
 constexpr int rows_occupancy(int ds, int rt) { return ds * rt <= 4 ? 2 : 1; }
 
@@ -443,91 +418,14 @@ __global__ __launch_bounds__(512, rows_occupancy(DS, RT)) void attend_short_kern
     }
 }
 
-// The sum of a row's partial results, weighted by their largest scores; rows of sequences without keys become
-// zeros. A workgroup a row: DP / 4 threads side by side, the parts dealt to 256 / (DP / 4) such groups, which
-// are added in order.
-template <int DS>
-__global__ __launch_bounds__(256) void join_rows_kernel(const Attention a, int tile_rows)
-{
-    constexpr int DP = 32 * DS, kWide = DP / 4, kGroups = 256 / kWide;
-    __shared__ v4f so[kGroups][kWide];
-    __shared__ float sm[kGroups], sl[kGroups];
-    const int s = (int)(blockIdx.x / (unsigned)a.cache.heads), head = (int)(blockIdx.x % (unsigned)a.cache.heads);
-    const int row = (int)blockIdx.y, tid = (int)threadIdx.x, g = tid / kWide, d = 4 * (tid % kWide);
-    const Sequence seq = sequence(a, s);
-    if (seq.n <= 0 || seq.n > a.few_rows / a.group || row >= seq.n * a.group)
-        return;
-    const int blocks = seq.hi - seq.lo, total = a.begins[a.b.seqs], begin = a.begins[s];
-    const int i = row / a.group, h = head * a.group + row % a.group;
-    const int64_t t = seq.first + i;
-    int p0 = 0, p1 = -1;
-    if (blocks > 0) {
-        const int count = shares(a, total);
-        p0 = share_of(begin, total, count);
-        p1 = share_of(begin + blocks - 1, total, count);
-        if (p0 == p1)
-            return; // written by the one that had all of it
-    }
-    float m = -__builtin_inff(), l = 0.0f;
-    v4f o = {0.0f, 0.0f, 0.0f, 0.0f};
-    if (g < kGroups) {
-        for (int p = p0 + g; p <= p1; p += 4 * kGroups) { // four at a time on their way
-            float2 ml[4];
-            v4f x[4];
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                const int part = min(p + k * kGroups, p1);
-                const int64_t entry = (((int64_t)head * a.slots + part) * 2 + (part == p0)) * tile_rows + row;
-                ml[k] = *reinterpret_cast<const float2 *>(a.rows_ml + entry * 2);
-                x[k] = *reinterpret_cast<const v4f *>(a.rows_o + entry * DP + d);
-            }
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                if (p + k * kGroups > p1)
-                    continue;
-                const float top = fmaxf(m, ml[k].x), less = top == -__builtin_inff() ? 0.0f : top;
-                const float f = exp2_fast(m - less), e = exp2_fast(ml[k].x - less);
-                o = o * f + x[k] * e;
-                l = l * f + ml[k].y * e;
-                m = top;
-            }
-        }
-        so[g][tid % kWide] = o;
-        if (tid % kWide == 0) {
-            sm[g] = m;
-            sl[g] = l;
-        }
-    }
-    __syncthreads();
-    if (g > 0)
-        return;
-    m = sm[0];
-#pragma unroll
-    for (int k = 1; k < kGroups; ++k)
-        m = fmaxf(m, sm[k]);
-    const float less = m == -__builtin_inff() ? 0.0f : m;
-    o = v4f{0.0f, 0.0f, 0.0f, 0.0f};
-    l = 0.0f;
-#pragma unroll
-    for (int k = 0; k < kGroups; ++k) {
-        const float f = exp2_fast(sm[k] - less);
-        o += so[k][tid] * f;
-        l += sl[k] * f;
-    }
-    store_row(a, t, h, d, o, m, l);
-}
-
 template <int DS, int RT>
 void launch_rows(const Attention &a, hipStream_t s)
 {
     if constexpr (RT <= max_row_tiles(32 * DS)) {
-        if (a.slots == 0) {
+        if (a.slots == 0)
             MAMBO_LAUNCH((attend_short_kernel<DS, RT>), dim3((unsigned)(a.b.seqs * a.cache.heads)), dim3(512), 0, s, a);
-            return;
-        }
-        MAMBO_LAUNCH((attend_rows_kernel<DS, RT>), dim3((unsigned)(a.slots * a.cache.heads)), dim3(256), 0, s, a);
-        const int rows = a.b.offsets ? a.few_rows : a.b.each * a.group;
-        MAMBO_LAUNCH((join_rows_kernel<DS>), dim3((unsigned)(a.b.seqs * a.cache.heads), (unsigned)rows), dim3(256), 0, s, a, 16 * RT);
+        else
+            MAMBO_LAUNCH((attend_rows_kernel<DS, RT>), dim3((unsigned)(a.slots * a.cache.heads)), dim3(256), 0, s, a);
     }
 }
 

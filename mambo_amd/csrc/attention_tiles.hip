@@ -10,8 +10,6 @@
 
 namespace {
 
-constexpr int kTileBlocks = 2; // blocks of 32 tokens of a tile
-
 __device__ __forceinline__ float halves_max(float x)
 {
     auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
@@ -32,23 +30,6 @@ constexpr int kAhead = 4; // operands read ahead
 __device__ __forceinline__ int64_t tiles_before(const Attention &a, int tile_rows, int s)
 {
     return (int64_t)a.b.offset(s) * a.group / tile_rows + s;
-}
-
-// The blocks [lo, hi) of keys of the rows from row0 on: what the first row sees of the window to what the last one sees.
-// They are dealt evenly to several workgroups where there are eight steps of the kernel and more for each.
-struct Keys {
-    int lo, hi, tiles, parts;
-    __device__ int begin(int part) const { return lo + kTileBlocks * (int)((int64_t)tiles * part / parts); }
-};
-__device__ __forceinline__ Keys tile_keys(const Attention &a, const Sequence &seq, int row0, int tile_rows)
-{
-    const int i0 = row0 / a.group, i1 = (min(row0 + tile_rows, seq.n * a.group) - 1) / a.group;
-    Keys k;
-    k.lo = max(0, sees_from(a, seq, i0)) / kKvBlock;
-    k.hi = (max(0, sees_to(a, seq, i1)) + kKvBlock - 1) / kKvBlock;
-    k.tiles = max(0, k.hi - k.lo + kTileBlocks - 1) / kTileBlocks;
-    k.parts = max(1, min(a.parts, k.tiles / 8));
-    return k;
 }
 
 template <int DS>
@@ -408,56 +389,10 @@ __global__ __launch_bounds__(64 * tile_waves(DS), tile_waves(DS) / 4) void atten
         a.lse[t * q_heads + h] = sum == 0.0f ? -__builtin_inff() : (m + __log2f(sum)) * kLn2;
 }
 
-// Rows whose keys were dealt to several workgroups: their sums weighted by the largest scores, in order.
-template <int DS>
-__global__ __launch_bounds__(256) void join_tiles_kernel(const Attention a)
-{
-    constexpr int DP = 32 * DS, kWide = DP / 4, kRows = 256 / kWide;
-    const int64_t q_heads = (int64_t)a.group * a.cache.heads, all = a.b.tokens * q_heads;
-    const int64_t entry = (int64_t)blockIdx.x * kRows + (int)threadIdx.x / kWide;
-    const int d = 4 * ((int)threadIdx.x % kWide);
-    const int64_t t = min(entry, all - 1) / q_heads, h = min(entry, all - 1) % q_heads;
-    int s = a.b.offsets ? 0 : (int)t / a.b.each;
-    if (a.b.offsets) {
-        // the last sequence that begins at or before the wave's first token, and from there on this thread's
-        s = find_slot(a.b.seqs, __builtin_amdgcn_readfirstlane((int)t), [&](int i) { return (int64_t)a.b.offset(i); });
-        while (s + 1 < a.b.seqs && a.b.offset(s + 1) <= t)
-            ++s;
-    }
-    const Sequence seq = sequence(a, s);
-    if ((int)threadIdx.x >= kRows * kWide || entry >= all || t < seq.first || t >= seq.first + seq.n ||
-        (int64_t)seq.n * a.group <= a.few_rows)
-        return; // rows of sequences that attend_tiles has, and no others
-    const int row = ((int)t - seq.first) * a.group + (int)h % a.group;
-    const int parts = tile_keys(a, seq, row / tile_rows(DS) * tile_rows(DS), tile_rows(DS)).parts;
-    if (parts == 1)
-        return; // written by the one that had all of them
-    float m = -__builtin_inff(), l = 0.0f;
-    v4f o = {0.0f, 0.0f, 0.0f, 0.0f};
-    for (int p = 0; p < parts; ++p) {
-        const float2 ml = *reinterpret_cast<const float2 *>(a.tiles_ml + (p * all + entry) * 2);
-        const v4f x = *reinterpret_cast<const v4f *>(a.tiles_o + (p * all + entry) * DP + d);
-        const float top = fmaxf(m, ml.x), less = top == -__builtin_inff() ? 0.0f : top;
-        const float f = exp2_fast(m - less), e = exp2_fast(ml.x - less);
-        o = o * f + x * e;
-        l = l * f + ml.y * e;
-        m = top;
-    }
-    o *= l == 0.0f ? 0.0f : 1.0f / l;
-    if (d < a.cache.dim)
-        store_row4<true>(a.out, t * a.ldot + h * a.ldoh + d, o, a.cache.dim - d, a.ldot % 4 == 0 && a.ldoh % 4 == 0 && (uintptr_t)a.out % 8 == 0);
-    if (a.lse && d == 0)
-        a.lse[entry] = l == 0.0f ? -__builtin_inff() : (m + __log2f(l)) * kLn2;
-}
-
 template <int DS>
 void launch_tiles(const Attention &a, int64_t tiles, hipStream_t s)
 {
     MAMBO_LAUNCH((attend_tiles_kernel<DS>), dim3((unsigned)(tiles * a.cache.heads), (unsigned)a.parts), dim3(64 * tile_waves(DS)), 0, s, a);
-    if (a.parts > 1) {
-        const int64_t rows = (int64_t)a.b.tokens * a.group * a.cache.heads, each = 256 / (8 * DS);
-        MAMBO_LAUNCH((join_tiles_kernel<DS>), dim3((unsigned)((rows + each - 1) / each)), dim3(256), 0, s, a);
-    }
 }
 
 } // namespace

@@ -27,7 +27,8 @@ ARCH = "gfx950"
 
 SOURCES = ["api.hip", "quantize_mxfp8.hip", "iq3s_layout.hip", "iq3s_gemm.hip", "iq3s_wide.hip", "iq3s_chain.hip",
            "iq3s_experts.hip", "fp8_block.hip", "experts.hip", "kv_cache.hip",
-           "attention.hip", "attention_rows.hip", "attention_tiles.hip", "synth.hip"]
+           "attention.hip", "attention_rows.hip", "attention_tiles.hip", "attention_join.hip",
+           "synth.hip"]
 
 HIPCC_FLAGS = [
     f"--offload-arch={ARCH}",
