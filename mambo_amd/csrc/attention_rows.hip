@@ -7,7 +7,8 @@
 // in such an order that lane 16 kk + i has query i's probabilities of the tokens 8 kk .. 8 kk + 7, the
 // operand that  O^T += V^T P^T  wants of it: nothing goes through LDS or other lanes but the largest
 // score. The running largest and total are f32; the codes are widened to bf16, which holds them exactly, and the
-// probabilities are rounded to bf16 (2^-9 of each, beside the outputs' own).
+// probabilities are rounded to bf16 (2^-8 of each at most, beside the outputs' own).
+// One token at 131150 of 8 heads of 128: 43 us, 6.3 TB/s of codes; a large read reaches 6.4.
 #include "attention.h"
 
 namespace {

@@ -4,8 +4,10 @@
 // 64 at a time. The tile's codes are widened to bf16 once, on their way from registers into LDS, and every
 // wave reads them from there: S^T = K Q^T in 32 x 32 x 16 MFMAs, softmax in registers (a lane has one
 // query), O^T += V^T P^T. The key rows lie in LDS in such an order that the scores come out
-// of the first product as the operand of the second. Two buffers: the next tile's codes are asked for before
-// a tile is worked on and widened after it.
+// of the first product as the operand of the second. Two buffers of each: while a tile is worked on, the codes of the
+// keys two tiles ahead and of the values one ahead are widened into the places that its predecessor has left.
+// 8192 tokens of 32/8 heads of 128: 525 us, 1.05 PFLOP/s, 48% of the matrix units' cycles; a large library product of bf16
+// reaches 1.2 to 1.45.
 #include "attention.h"
 
 namespace {

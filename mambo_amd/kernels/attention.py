@@ -42,7 +42,7 @@ def launch_attention_kv(q: torch.Tensor, cache: KVCache, tables: torch.Tensor, l
     than the last ``window`` of them where that is not 0, or all of the sequence's. A row that sees none (a sequence of length
     0, more rows than tokens, no page) becomes zeros, its lse -inf. ``scale`` defaults to D ** -0.5.
 
-    Scores, the running sum and the output are float32; the probabilities are rounded to bfloat16 (2^-9 of each) for the
+    Scores, the running sum and the output are float32; the probabilities are rounded to bfloat16 (2^-8 of each at most) for the
     product with the values, the result once to bfloat16. Results do not vary from run to run. Rows of no sequence are not written: they stay what they
     were in ``out``, and are undefined without. ``out`` must not overlap ``q``. T may be 0."""
     cache = check_cache(cache)
