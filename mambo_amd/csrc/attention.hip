@@ -131,6 +131,7 @@ extern "C" int mambo_kv_attention(const void *q, int64_t tokens, int64_t q_heads
         return MAMBO_OK;
     MAMBO_REQUIRE(q && out, MAMBO_ERR_VALUE, "null pointer");
     MAMBO_REQUIRE((uintptr_t)q % 16 == 0 && ldqt % 8 == 0 && ldqh % 8 == 0, MAMBO_ERR_VALUE, "queries must be 16-byte aligned");
+    MAMBO_REQUIRE(ldot >= dim && ldoh >= dim, MAMBO_ERR_VALUE, "strides of the output must cover a head");
     MAMBO_REQUIRE((uintptr_t)out % 2 == 0 && (uintptr_t)lse % 4 == 0, MAMBO_ERR_VALUE, "outputs must be aligned to their type");
     MAMBO_REQUIRE(workspace_bytes >= p.bytes && (workspace || p.bytes == 0), MAMBO_ERR_VALUE,
                   "the workspace must hold %lld bytes (got %lld)", (long long)p.bytes, (long long)workspace_bytes);

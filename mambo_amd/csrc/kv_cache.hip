@@ -597,6 +597,7 @@ extern "C" int mambo_rotary(const void *x, int x_dtype, int64_t tokens, int64_t 
         return rc;
     if (const int rc = check_rows(out, out_dtype, "rotated rows"))
         return rc;
+    MAMBO_REQUIRE(ldot >= dim && ldoh >= dim, MAMBO_ERR_VALUE, "strides of the output must cover a head");
     a.x = x, a.out = out, a.ldt = ldt, a.ldh = ldh, a.ldot = ldot, a.ldoh = ldoh, a.positions = positions;
     a.tokens = tokens, a.heads = (int)heads, a.dim = (int)dim;
     // about a thousand workgroups, and eight tokens' angles at most
@@ -656,6 +657,7 @@ extern "C" int mambo_kv_append(const mambo_kv_rows *rows, int64_t tokens, const 
             return rc;
         if (const int rc = check_rows(rows->q_out, MAMBO_DTYPE_BF16, "rotated queries"))
             return rc;
+        MAMBO_REQUIRE(rows->ldot >= dim && rows->ldoh >= dim, MAMBO_ERR_VALUE, "strides of the output must cover a head");
         a.q = {rows->q, rows->ldqt, rows->ldqh};
         a.q_out = rows->q_out, a.ldot = rows->ldot, a.ldoh = rows->ldoh, a.q_heads = (int)rows->q_heads;
         // eight tokens each, unless there are no more

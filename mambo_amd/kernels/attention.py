@@ -14,7 +14,7 @@ import torch
 
 from mambo_amd import _native
 from mambo_amd.kernels.kv_cache import batch_args, check_cache
-from mambo_amd.kernels.rotary import check_heads, head_strides, heads_in_place, output_heads
+from mambo_amd.kernels.rotary import check_heads, heads_in_place, output_heads
 from mambo_amd.utils.kv_cache import KVCache
 
 
@@ -50,7 +50,8 @@ def launch_attention_kv(q: torch.Tensor, cache: KVCache, tables: torch.Tensor, l
     check_heads(q, dim, dev, "q")
     if q.dtype != torch.bfloat16:
         raise ValueError("q must be bfloat16")
-    tokens, heads = q.shape[:2]
+    shape = q.shape
+    tokens, heads, _ = shape
     if heads % cache.heads:
         raise ValueError(f"q must have a multiple of the cache's {cache.heads} heads, got {heads}")
     scale = dim ** -0.5 if scale is None else float(scale)
@@ -59,18 +60,16 @@ def launch_attention_kv(q: torch.Tensor, cache: KVCache, tables: torch.Tensor, l
         raise ValueError("a window is positive, and of causal attention")
     with _native.launch_on(dev, stream):
         batch = batch_args(tables, lengths, offsets, tokens, dev)
-        q = heads_in_place(q)
-        strides = head_strides(q)
-        if q.data_ptr() % 16 or strides[0] % 8 or strides[1] % 8:
-            q = torch.empty(q.shape, dtype=q.dtype, device=dev).copy_(q)
-            strides = head_strides(q)
-        out = output_heads(out, q.shape, torch.bfloat16, dev)
+        q, ldqt, ldqh = heads_in_place(q)
+        if q.data_ptr() % 16 or ldqt % 8 or ldqh % 8:
+            q, ldqt, ldqh = torch.empty(shape, dtype=q.dtype, device=dev).copy_(q), heads * dim, dim
+        out, ldot, ldoh = output_heads(out, shape, torch.bfloat16, dev)
         lse = torch.empty((tokens, heads), dtype=torch.float32, device=dev) if return_lse else None
         size = _workspace(cache.pages, cache.heads, dim, cache.page_size, batch.seqs, batch.width, offsets is not None, tokens,
                           heads, window)
         workspace = torch.empty(size, dtype=torch.uint8, device=dev).data_ptr() if size else None
         _native.check(_native.lib().mambo_kv_attention(
-            q.data_ptr(), tokens, heads, dim, *strides, cache.args, batch, scale, bool(causal), window, out.data_ptr(),
-            *head_strides(out), None if lse is None else lse.data_ptr(), workspace, size,
+            q.data_ptr(), tokens, heads, dim, ldqt, ldqh, cache.args, batch, scale, bool(causal), window, out.data_ptr(),
+            ldot, ldoh, None if lse is None else lse.data_ptr(), workspace, size,
             _native.stream_handle(stream, dev)), "launch_attention_kv")
     return (out, lse) if return_lse else out

@@ -18,7 +18,7 @@ import torch
 
 from mambo_amd import _native
 from mambo_amd.kernels.fp8_block import ROW_DTYPES
-from mambo_amd.kernels.rotary import check_heads, check_int32, head_strides, heads_in_place, output_heads
+from mambo_amd.kernels.rotary import check_heads, check_int32, heads_in_place, output_heads
 from mambo_amd.utils.kv_cache import KVCache
 from mambo_amd.utils.rotary_table import RotaryTable
 
@@ -29,25 +29,29 @@ def check_cache(cache) -> KVCache:
     return cache
 
 
-def check_tables(tables, dev) -> int:
-    if not isinstance(tables, torch.Tensor) or tables.ndim != 2 or tables.dtype != torch.int32 or tables.device != dev \
-            or tables.shape[0] < 1 or tables.shape[1] < 1 or (tables.shape[1] > 1 and tables.stride(1) != 1) \
-            or (tables.shape[0] > 1 and tables.stride(0) < tables.shape[1]):
-        raise ValueError("tables must be int32 [S,C] with unit column stride on the cache's device")
-    return tables.shape[0]
+def check_tables(tables, dev) -> tuple[int, int, int]:
+    """Sequences, columns and the stride of the rows of `tables`, checked."""
+    if isinstance(tables, torch.Tensor) and tables.ndim == 2 and tables.dtype == torch.int32 and tables.device == dev:
+        seqs, columns = tables.shape
+        if seqs and columns:
+            if tables.is_contiguous():
+                return seqs, columns, columns
+            row, value = tables.stride()
+            if (columns == 1 or value == 1) and (seqs == 1 or row >= columns):
+                return seqs, columns, row if seqs > 1 else columns
+    raise ValueError("tables must be int32 [S,C] with unit column stride on the cache's device")
 
 
 def batch_args(tables, lengths, offsets, tokens: int, dev) -> _native.KVBatchArgs:
     """The sequences of a call of `tokens` rows, checked."""
-    seqs = check_tables(tables, dev)
-    check_int32(lengths, (seqs,), dev, "lengths")
+    seqs, columns, row = check_tables(tables, dev)
+    check_int32(lengths, seqs, dev, "lengths")
     if offsets is not None:
-        check_int32(offsets, (seqs + 1,), dev, "offsets")
+        check_int32(offsets, seqs + 1, dev, "offsets")
+        offsets = offsets.data_ptr()
     elif tokens % seqs:
         raise ValueError(f"without offsets every sequence has as many rows: {tokens} rows of {seqs} sequences")
-    columns = tables.shape[1]
-    return _native.KVBatchArgs(tables.data_ptr(), tables.stride(0) if seqs > 1 else columns, columns, lengths.data_ptr(),
-                               None if offsets is None else offsets.data_ptr(), seqs)
+    return _native.KVBatchArgs(tables.data_ptr(), row, columns, lengths.data_ptr(), offsets, seqs)
 
 
 def launch_append_kv(k: torch.Tensor, v: torch.Tensor, cache: KVCache, tables: torch.Tensor, lengths: torch.Tensor, *,
@@ -85,7 +89,7 @@ def launch_append_kv(k: torch.Tensor, v: torch.Tensor, cache: KVCache, tables: t
     if positions is not None:
         if rotary is None:
             raise ValueError("positions are those of the rotation, and there is none")
-        check_int32(positions, (tokens,), dev, "positions")
+        check_int32(positions, tokens, dev, "positions")
     if q is not None:
         if rotary is None:
             raise ValueError("queries are taken to be rotated: they need angles")
@@ -96,16 +100,17 @@ def launch_append_kv(k: torch.Tensor, v: torch.Tensor, cache: KVCache, tables: t
         raise ValueError("out is for queries, and there are none")
     with _native.launch_on(dev, stream):
         batch = batch_args(tables, lengths, offsets, tokens, dev)
-        k, v = heads_in_place(k), heads_in_place(v)
-        rows = _native.KVRowsArgs(k.data_ptr(), v.data_ptr(), None, *head_strides(k), *head_strides(v))
-        rows.dtype = ROW_DTYPES[k.dtype]
-        if q is not None:
-            q = heads_in_place(q)
-            out = output_heads(out, q.shape, torch.bfloat16, dev)
-            rows.q, (rows.ldqt, rows.ldqh), rows.q_heads = q.data_ptr(), head_strides(q), q.shape[1]
-            rows.q_out, (rows.ldot, rows.ldoh) = out.data_ptr(), head_strides(out)
-            if tokens == 0:
-                rows.q = None
+        k, ldkt, ldkh = heads_in_place(k)
+        v, ldvt, ldvh = heads_in_place(v)
+        dtype = ROW_DTYPES[k.dtype]
+        if q is None:
+            rows = _native.KVRowsArgs(k.data_ptr(), v.data_ptr(), None, ldkt, ldkh, ldvt, ldvh, 0, 0, None, 0, 0, 0, dtype)
+        else:
+            shape = q.shape
+            q, ldqt, ldqh = heads_in_place(q)
+            out, ldot, ldoh = output_heads(out, shape, torch.bfloat16, dev)
+            rows = _native.KVRowsArgs(k.data_ptr(), v.data_ptr(), q.data_ptr() if tokens else None, ldkt, ldkh, ldvt, ldvh, ldqt, ldqh,
+                                      out.data_ptr(), ldot, ldoh, shape[1], dtype)
         _native.check(_native.lib().mambo_kv_append(
             rows, tokens, cache.args, batch, None if rotary is None else rotary.args,
             None if positions is None else positions.data_ptr(), _native.stream_handle(stream, dev)), "launch_append_kv")
@@ -120,15 +125,14 @@ def launch_read_kv(cache: KVCache, tables: torch.Tensor, sequences: torch.Tensor
     anything. For moving a prefix elsewhere and for looking at a cache."""
     cache = check_cache(cache)
     dev = cache.codes.device
-    seqs = check_tables(tables, dev)
+    seqs, columns, row = check_tables(tables, dev)
     if not isinstance(sequences, torch.Tensor) or sequences.ndim != 1:
         raise ValueError("sequences must be int32 [N]")
     n = sequences.shape[0]
-    check_int32(sequences, (n,), dev, "sequences")
-    check_int32(positions, (n,), dev, "positions")
-    columns = tables.shape[1]
+    check_int32(sequences, n, dev, "sequences")
+    check_int32(positions, n, dev, "positions")
     with _native.launch_on(dev, stream):
-        batch = _native.KVBatchArgs(tables.data_ptr(), tables.stride(0) if seqs > 1 else columns, columns, None, None, seqs)
+        batch = _native.KVBatchArgs(tables.data_ptr(), row, columns, None, None, seqs)
         k, v = torch.empty((2, n, cache.heads, cache.head_dim), dtype=torch.bfloat16, device=dev).unbind(0)
         _native.check(_native.lib().mambo_kv_read(
             cache.args, batch, sequences.data_ptr(), positions.data_ptr(), n, cache.heads, cache.head_dim, k.data_ptr(), v.data_ptr(),

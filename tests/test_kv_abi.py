@@ -108,7 +108,8 @@ def test_rotary_refusals(lib):
                          ({"table": table(size=3)}, "even number"), ({"table": table(size=0)}, "even number"),
                          ({"table": table(size=66)}, "even number"), ({"table": table(turns=260)}, "aligned to their type"),
                          ({"x": None}, "null pointer"), ({"positions": None}, "null pointer"), ({"out": None}, "null pointer"),
-                         ({"x": 258}, "aligned to their type"), ({"out": 257}, "aligned to their type")):
+                         ({"x": 258}, "aligned to their type"), ({"out": 257}, "aligned to their type"),
+                         ({"ldot": 63}, "cover a head"), ({"ldoh": 63}, "cover a head")):
         refused(lib, call(**change), text)
     assert call(tokens=0, x=None, positions=None, out=None) == 0
 
@@ -120,6 +121,7 @@ def test_append_refusals(lib):
                        (rows(v=257, dtype=1), None, "aligned to their type"), (rows(q=256, q_out=256, q_heads=2), None, "need a table"),
                        (rows(q=256, q_out=256, q_heads=3), table(), "no multiple"), (rows(q=256, q_out=256, q_heads=1), table(), "no multiple"),
                        (rows(q=256, q_heads=2), table(), "null pointer (rotated"), (rows(q=258, q_out=256, q_heads=2), table(), "aligned"),
+                       (rows(q=256, q_out=256, q_heads=2, ldot=128, ldoh=63), table(), "cover a head"),
                        (rows(), table(size=66), "even number"), (rows(), table(size=7), "even number")):
         refused(lib, f(r, 2, cache(), batch(), t, None, None), text)
     refused(lib, f(None, 2, cache(), batch(), None, None, None), "null pointer")
@@ -138,7 +140,7 @@ def test_attention_refusals(lib):
                          ({"scale": math.inf}, "positive and finite"), ({"scale": math.nan}, "positive and finite"),
                          ({"window": -1}, "a window"), ({"window": 5, "causal": 0}, "a window"), ({"q": None}, "null pointer"),
                          ({"out": None}, "null pointer"), ({"q": 264}, "16-byte"), ({"ldqt": 260}, "16-byte"), ({"ldqh": 68}, "16-byte"),
-                         ({"out": 257}, "aligned to their type"), ({"lse": 258}, "aligned to their type"),
+                         ({"out": 257}, "aligned to their type"), ({"lse": 258}, "aligned to their type"), ({"ldoh": 63}, "cover a head"), ({"ldot": 63}, "cover a head"),
                          ({"batch": batch(width=600, ldt=600), "size": 0}, "workspace must hold"),
                          ({"batch": batch(width=600, ldt=600), "ws": None}, "workspace must hold"), ({"ws": 264}, "16-byte")):
         refused(lib, call(**change), text)
