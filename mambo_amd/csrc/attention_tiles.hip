@@ -6,7 +6,7 @@
 // query), O^T += V^T P^T. The key rows lie in LDS in such an order that the scores come out
 // of the first product as the operand of the second. Two buffers of each: while a tile is worked on, the codes of the
 // keys two tiles ahead and of the values one ahead are widened into the places that its predecessor has left.
-// 8192 tokens of 32/8 heads of 128: 525 us, 1.05 PFLOP/s, 48% of the matrix units' cycles; a large library product of bf16
+// 8192 tokens of 32/8 heads of 128: 497 us, 1.11 PFLOP/s, half of the matrix units' cycles; a large library product of bf16
 // reaches 1.2 to 1.45.
 #include "attention.h"
 
@@ -41,8 +41,13 @@ __global__ __launch_bounds__(64 * tile_waves(DS), tile_waves(DS) / 4) void atten
     constexpr int DP = 32 * DS, kSteps = DP / 16;
     constexpr int kUnits = kTileBlocks * DS, kEach = (kUnits + kWaves - 1) / kWaves; // staged by all waves, and by one
     // keys: [8 values of the head][64 rows of the first product]; values: [8 tokens][value of the head]
-    __shared__ bf16x8 keys[2][DP / 8][32 * kTileBlocks];
-    __shared__ bf16x8 values[2][4 * kTileBlocks][DP];
+    struct Staged {
+        bf16x8 keys[2][DP / 8][32 * kTileBlocks];
+        bf16x8 values[2][4 * kTileBlocks][DP];
+    };
+    __shared__ Staged staged;
+    auto &keys = staged.keys;
+    auto &values = staged.values;
 
     const int tid = (int)threadIdx.x, lane = lane_id(), half = lane >> 5, col = lane & 31;
     const int wave = __builtin_amdgcn_readfirstlane(tid / 64);
@@ -361,10 +366,10 @@ __global__ __launch_bounds__(64 * tile_waves(DS), tile_waves(DS) / 4) void atten
     }
 
     const float sum = halves_sum(l[0] + l[1]);
-    if (!some)
-        return;
     const int64_t t = seq.first + i, q_heads = (int64_t)a.group * a.cache.heads;
     if (keys_of.parts > 1) {
+        if (!some)
+            return;
         const int64_t entry = ((int64_t)blockIdx.y * a.b.tokens + t) * q_heads + h;
 #pragma unroll
         for (int d = 0; d < DS; ++d)
@@ -377,6 +382,36 @@ __global__ __launch_bounds__(64 * tile_waves(DS), tile_waves(DS) / 4) void atten
         return;
     }
     const float by = sum == 0.0f ? 0.0f : 1.0f / sum;
+    if (a.lse && half == 0 && some)
+        a.lse[t * q_heads + h] = sum == 0.0f ? -__builtin_inff() : (m + __log2f(sum)) * kLn2;
+    const int64_t to_row = t * a.ldot + h * a.ldoh;
+    if ((uintptr_t)a.out % 16 == 0 && a.ldot % 8 == 0 && a.ldoh % 8 == 0) {
+        // A lane has four values here and there of its row: whole rows are written from LDS, each chunk of 8 values as many
+        // places on as its row's number, so that rows do not meet in a bank (8192 tokens 497 us for 529 with what a lane has
+        // written as it is, 16 prompts of 64 tokens 14 for 21).
+        constexpr int kChunks = DP / 8;
+        __syncthreads(); // all waves have read their last operands
+        __bf16 *const rows_of_wave = reinterpret_cast<__bf16 *>(&staged) + wave * (32 * DP);
+#pragma unroll
+        for (int d = 0; d < DS; ++d)
+#pragma unroll
+            for (int r = 0; r < 16; r += 4) {
+                const int chunk = (4 * d + r / 4 + col) % kChunks;
+                *reinterpret_cast<bf16x4 *>(rows_of_wave + col * DP + 8 * chunk + 4 * half) =
+                    __builtin_convertvector(v4f{o[d][r] * by, o[d][r + 1] * by, o[d][r + 2] * by, o[d][r + 3] * by}, bf16x4);
+            }
+        __builtin_amdgcn_wave_barrier();
+        for (int item = lane; item < 32 * kChunks; item += 64) {
+            const int r = item / kChunks, chunk = item % kChunks;
+            const int64_t to = ((int64_t)__shfl((int)(to_row >> 32), r) << 32) | (uint32_t)__shfl((int)to_row, r);
+            if (row0 + 32 * wave + r < rows && 8 * chunk < a.cache.dim)
+                *reinterpret_cast<uint4 *>(a.out + to + 8 * chunk) =
+                    *reinterpret_cast<const uint4 *>(rows_of_wave + r * DP + 8 * ((chunk + r) % kChunks));
+        }
+        return;
+    }
+    if (!some)
+        return;
     const bool vec = a.ldot % 4 == 0 && a.ldoh % 4 == 0 && (uintptr_t)a.out % 8 == 0;
 #pragma unroll
     for (int d = 0; d < DS; ++d)
@@ -384,11 +419,9 @@ __global__ __launch_bounds__(64 * tile_waves(DS), tile_waves(DS) / 4) void atten
         for (int r = 0; r < 16; r += 4) {
             const int at = 32 * d + 2 * r + 4 * half;
             if (at < a.cache.dim)
-                store_row4<true>(a.out, t * a.ldot + h * a.ldoh + at,
-                                 v4f{o[d][r] * by, o[d][r + 1] * by, o[d][r + 2] * by, o[d][r + 3] * by}, a.cache.dim - at, vec);
+                store_row4<true>(a.out, to_row + at, v4f{o[d][r] * by, o[d][r + 1] * by, o[d][r + 2] * by, o[d][r + 3] * by},
+                                 a.cache.dim - at, vec);
         }
-    if (a.lse && half == 0)
-        a.lse[t * q_heads + h] = sum == 0.0f ? -__builtin_inff() : (m + __log2f(sum)) * kLn2;
 }
 
 template <int DS>
