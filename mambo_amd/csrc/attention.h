@@ -94,9 +94,10 @@ __device__ __forceinline__ uint2 keep_tokens(uint32_t lo, uint32_t hi, int left)
 constexpr int max_row_tiles(int padded) { return padded <= 64 ? 4 : padded <= 128 ? 2 : 1; }
 
 // Waves of a workgroup of attend_tiles, each with 32 rows, by the head size in 32s. Eight, two a SIMD, while a wave's
-// registers are enough (D = 128: 8192 tokens of 32 heads 540 us, with four 580); from 192 on four with twice the
-// registers (4096 tokens of D = 256 408 us for 1507, of 192 330 for 331, of 160 295 for 236).
-constexpr int tile_waves(int ds) { return ds <= 5 ? 8 : 4; }
+// registers are enough, above that four with twice the registers. 4096 tokens of 32 heads with eight and with four: of 64 101 us
+// and 117, of 96 119 and 219, of 160 213 and 278, of 192 285 and 299, of 224 530 and 355, of 256 1968 and 417; 8192 tokens of
+// 128 498 and 814.
+constexpr int tile_waves(int ds) { return ds <= 6 ? 8 : 4; }
 constexpr int tile_rows(int ds) { return 32 * tile_waves(ds); }
 
 // Blocks that a sequence has in the row kernel's order.

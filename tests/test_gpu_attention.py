@@ -286,7 +286,7 @@ def test_every_kernel_for_many_rows(gpu, dim):
         n, ragged = sum(counts), len(counts) > 1
         q = rows_of(rng, n, 2, dim, torch.bfloat16, 2.0).to(gpu)
         plan = plan_of(cache, tables, n, 2, ragged)
-        assert plan[2] == (256 if dim <= 160 else 128) and plan[3] == parts
+        assert plan[2] == (256 if dim <= 192 else 128) and plan[3] == parts
         out, lse = attention()(q, cache, tables, *ref.device(gpu, np.array(lengths, np.int32)), return_lse=True,
                                offsets=ref.device(gpu, ref.offsets_of(counts))[0] if ragged else None)
         check(out, lse, q, keys, values, counts, 2)

@@ -173,7 +173,7 @@ def test_plans(lib):
     assert plan(2, 256, heads=128, seqs=2, width=64, ldt=64)[:2] == [16, 0]  # 2048 tokens of 256 workgroups
     assert plan(2, 256, heads=128, seqs=2, width=65, ldt=65)[:2] == [16, 4]
     assert plan(32, 8)[0] == 64 and plan(32, 8, dim=128)[2] == 256 and plan(32, 4, dim=128)[0] == 32
-    assert plan(34, 8)[:1] == [0] and plan(34, 8)[2] == 256 and plan(34, 8, dim=192)[2] == 128
+    assert plan(34, 8)[:1] == [0] and plan(34, 8)[2] == 256 and plan(34, 8, dim=192)[2] == 256 and plan(34, 8, dim=200)[2] == 128
     assert plan(40, 8, offsets=256) == [16, 0, 256, 1]
     assert plan(40, 96, offsets=256)[0] == 64 and plan(40, 160, offsets=256)[0] == 0
     assert plan(400, 8, width=2000, ldt=2000)[3] == 256 // (2 * 4 * 2) and plan(400, 8, offsets=256, width=2000, ldt=2000)[3] == 32
