@@ -438,8 +438,8 @@ typedef struct mambo_kv_rows {
 /* Stores the call's tokens in the cache, the keys rotated (table NULL: as they are) by positions[t] (NULL:
  * by the position in the sequence). A block that is entered at its first token starts anew, one entered
  * later keeps its older tokens: its exponent is the larger of the old and e = max(ceil(log2(amax / 448)),
- * -100) of the new rows (values beyond 240 * 2^120 are held as that), and where it grows, the older codes are rounded again to it. A token with a key or value
- * of a head that is not finite is held as NaN keys and zero values of that head and counts for no exponent. A row whose
+ * -100) of the new rows (values beyond 240 * 2^120 are held as that), and where it grows, the older codes are rounded
+ * again to it. A token with a key or value of a head that is not finite is held as NaN keys and zero values of that head and counts for no exponent. A row whose
  * position in its sequence is negative is not stored (its queries are rotated). Sequences of a call
  * must not share a block that one of them writes. */
 int mambo_kv_append(const mambo_kv_rows *rows, int64_t tokens, const mambo_kv_cache *cache, const mambo_kv_batch *batch,
@@ -461,14 +461,14 @@ int mambo_kv_read(const mambo_kv_cache *cache, const mambo_kv_batch *batch, cons
  * Rows that no sequence has are not written. The results do not vary from run to run. */
 int64_t mambo_kv_attention_workspace(const mambo_kv_cache *cache, const mambo_kv_batch *batch, int64_t tokens, int64_t q_heads,
                                      int64_t window);
-int mambo_kv_attention(const void *q, int64_t tokens, int64_t q_heads, int64_t dim, int64_t ldqt, int64_t ldqh, const mambo_kv_cache *cache,
-                       const mambo_kv_batch *batch, float scale, int causal, int64_t window, void *out, int64_t ldot,
-                       int64_t ldoh, float *lse, void *workspace, int64_t workspace_bytes, mambo_stream_t stream);
+int mambo_kv_attention(const void *q, int64_t tokens, int64_t q_heads, int64_t dim, int64_t ldqt, int64_t ldqh,
+                       const mambo_kv_cache *cache, const mambo_kv_batch *batch, float scale, int causal, int64_t window,
+                       void *out, int64_t ldot, int64_t ldoh, float *lse, void *workspace, int64_t workspace_bytes, mambo_stream_t stream);
 
 /* How such a call is launched, on the host alone: plan[4] = rows (queries x heads of a key/value head) up to
  * which a sequence takes the kernel for few rows (0: it is not launched), its workgroups for each head (0: one for each
- * sequence, none of which has many keys),
- * rows of a workgroup of the kernel for many (0: not launched) and the parts of its keys. */
+ * sequence, none of which has many keys), rows of a workgroup of the kernel for many (0: not launched) and the most
+ * parts that its keys are dealt to. */
 int mambo_kv_attention_plan(const mambo_kv_cache *cache, const mambo_kv_batch *batch, int64_t tokens, int64_t q_heads,
                             int64_t window, int32_t *plan);
 

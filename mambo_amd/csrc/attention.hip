@@ -37,7 +37,9 @@ Plan make_plan(const KvCache &c, const KvBatch &b, int group, int64_t window)
     if (p.row_tiles) {
         p.few_rows = 16 * p.row_tiles;
         // blocks of a sequence at most; few enough, and one workgroup takes all of them
-        const int64_t seen = window ? std::min<int64_t>(b.capacity, std::min<int64_t>(window, b.capacity) + p.few_rows / group + kKvBlock) : b.capacity;
+        int64_t seen = b.capacity;
+        if (window)
+            seen = std::min<int64_t>(seen, std::min(window, seen) + p.few_rows / group + kKvBlock);
         if (seen > ((int64_t)b.seqs * c.heads >= kCus ? kShortTokensOfMany : kShortTokens)) {
             // A workgroup a CU, fewer where there is no work for them: the blocks that its waves have on their way are enough
             // (131149 tokens of 8 heads of 128 47.0 us, with two 49.6). Two of small heads (16 x 8000 of 64 28.7 us for 35.4),
@@ -54,8 +56,10 @@ Plan make_plan(const KvCache &c, const KvBatch &b, int group, int64_t window)
         const int tile = tile_rows(padded / 32);
         p.tiles_each = (int)cdiv(rows, tile);
         p.tiles = b.offsets ? (int64_t)b.tokens * group / tile + b.seqs : (int64_t)b.seqs * p.tiles_each;
-        // a workgroup a CU, two where sequences may differ: the longest then have more parts than the others
-        p.parts = (int)std::max<int64_t>(1, std::min<int64_t>((b.offsets ? 2 : 1) * kCus / (p.tiles * c.heads), cdiv(b.capacity, 512)));
+        // A workgroup a CU, two of ragged sequences: the longest then have more parts than the others (pieces of six prompts 37 us
+        // for 41; of sequences with as many rows each, 4 of 16 rows behind 20000 tokens, 66 for 58).
+        const int64_t places = (b.offsets ? 2 : 1) * kCus / (p.tiles * c.heads);
+        p.parts = (int)std::max<int64_t>(1, std::min<int64_t>(places, cdiv(b.capacity, 512)));
         if (p.parts > 1)
             p.tiles_entries = (int64_t)p.parts * b.tokens * group * c.heads;
     }
@@ -64,7 +68,8 @@ Plan make_plan(const KvCache &c, const KvBatch &b, int group, int64_t window)
     return p;
 }
 
-int check(const mambo_kv_cache *cache, const mambo_kv_batch *batch, int64_t tokens, int64_t q_heads, int64_t window, KvCache *c, KvBatch *b, Plan *p)
+int check(const mambo_kv_cache *cache, const mambo_kv_batch *batch, int64_t tokens, int64_t q_heads, int64_t window,
+          KvCache *c, KvBatch *b, Plan *p)
 {
     if (const int rc = kv_check_cache(cache, c))
         return rc;
@@ -125,7 +130,8 @@ extern "C" int mambo_kv_attention(const void *q, int64_t tokens, int64_t q_heads
     if (const int rc = check(cache, batch, tokens, q_heads, window, &a.cache, &a.b, &p))
         return rc;
     MAMBO_REQUIRE(dim == a.cache.dim, MAMBO_ERR_VALUE, "the cache has heads of %d (got %lld)", a.cache.dim, (long long)dim);
-    MAMBO_REQUIRE(scale * kLog2e > 0.0f && isfinite(scale * kLog2e), MAMBO_ERR_VALUE, "the scale of the scores must be positive and finite");
+    MAMBO_REQUIRE(scale * kLog2e > 0.0f && isfinite(scale * kLog2e), MAMBO_ERR_VALUE,
+                  "the scale of the scores must be positive and finite");
     MAMBO_REQUIRE(window == 0 || causal, MAMBO_ERR_VALUE, "a window is positive, and of causal attention");
     if (tokens == 0)
         return MAMBO_OK;

@@ -112,11 +112,7 @@ __device__ void join_tiles(const Attention &a, int at)
         l = l * f + ml.y * e;
         m = top;
     }
-    o *= l == 0.0f ? 0.0f : 1.0f / l;
-    if (d < a.cache.dim)
-        store_row4<true>(a.out, t * a.ldot + h * a.ldoh + d, o, a.cache.dim - d, a.ldot % 4 == 0 && a.ldoh % 4 == 0 && (uintptr_t)a.out % 8 == 0);
-    if (a.lse && d == 0)
-        a.lse[entry] = l == 0.0f ? -__builtin_inff() : (m + __log2f(l)) * kLn2;
+    store_row(a, t, (int)h, d, o, m, l);
 }
 
 // Workgroups below `rows_from` join the rows of attend_tiles, the others those of attend_rows.

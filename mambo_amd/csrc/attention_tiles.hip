@@ -159,7 +159,8 @@ __global__ __launch_bounds__(64 * tile_waves(DS), tile_waves(DS) / 4) void atten
     // Half h of piece e; a wave without a unit of its own does another's once more.
     const auto widen_keys = [&](const Codes &x, int e, int h, int buf) {
         const int u = min(wave + kWaves * e, kUnits - 1), b = u / DS, ds = u % DS;
-        keys[buf][4 * ds + kk][32 * b + key_row + 8 * h] = widen(h ? x.c[e].z : x.c[e].x, h ? x.c[e].w : x.c[e].y, e8m0(x.scale[e]));
+        keys[buf][4 * ds + kk][32 * b + key_row + 8 * h] =
+            widen(h ? x.c[e].z : x.c[e].x, h ? x.c[e].w : x.c[e].y, e8m0(x.scale[e]));
     };
     const auto widen_values = [&](const Codes &x, int e, int h, int buf) {
         const int u = min(wave + kWaves * e, kUnits - 1), b = u / DS, ds = u % DS;
@@ -192,7 +193,8 @@ __global__ __launch_bounds__(64 * tile_waves(DS), tile_waves(DS) / 4) void atten
         for (int d = 0; d < kSteps; ++d)
 #pragma unroll
             for (int b = 0; b < kTileBlocks; ++b)
-                sx.x[b] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(keys[buf][2 * d + half][32 * b + col], q[d], d ? sx.x[b] : zeros, 0, 0, 0);
+                sx.x[b] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(keys[buf][2 * d + half][32 * b + col], q[d],
+                                                                  d ? sx.x[b] : zeros, 0, 0, 0);
     };
     // Whether any row of the wave sees any token of the tile.
     const auto seen = [&](int blk0) { return blk0 * kKvBlock < any_to && (blk0 + kTileBlocks) * kKvBlock > any_from; };
@@ -308,7 +310,8 @@ __global__ __launch_bounds__(64 * tile_waves(DS), tile_waves(DS) / 4) void atten
             for (int n = 0; n < kFirst; ++n) {
                 MAMBO_FIXED_ORDER();
                 v16f &x = next.x[n % kTileBlocks];
-                x = __builtin_amdgcn_mfma_f32_32x32x16_bf16(ahead[n % kAhead], q[n / kTileBlocks], n < kTileBlocks ? zeros : x, 0, 0, 0);
+                x = __builtin_amdgcn_mfma_f32_32x32x16_bf16(ahead[n % kAhead], q[n / kTileBlocks], n < kTileBlocks ? zeros : x,
+                                                            0, 0, 0);
                 if (n + kAhead < kFirst)
                     ahead[n % kAhead] = key(n + kAhead);
                 else
@@ -427,7 +430,8 @@ __global__ __launch_bounds__(64 * tile_waves(DS), tile_waves(DS) / 4) void atten
 template <int DS>
 void launch_tiles(const Attention &a, int64_t tiles, hipStream_t s)
 {
-    MAMBO_LAUNCH((attend_tiles_kernel<DS>), dim3((unsigned)(tiles * a.cache.heads), (unsigned)a.parts), dim3(64 * tile_waves(DS)), 0, s, a);
+    MAMBO_LAUNCH((attend_tiles_kernel<DS>), dim3((unsigned)(tiles * a.cache.heads), (unsigned)a.parts),
+                 dim3(64 * tile_waves(DS)), 0, s, a);
 }
 
 } // namespace

@@ -703,8 +703,8 @@ extern "C" int mambo_kv_read(const mambo_kv_cache *cache, const mambo_kv_batch *
     tables.offsets = nullptr;
     if (const int rc = kv_check_batch(&tables, 0, cache, &b))
         return rc;
-    MAMBO_REQUIRE(heads == c.heads && dim == c.dim, MAMBO_ERR_VALUE, "the cache has %d heads of %d (got %lld of %lld)", c.heads, c.dim,
-                  (long long)heads, (long long)dim);
+    MAMBO_REQUIRE(heads == c.heads && dim == c.dim, MAMBO_ERR_VALUE, "the cache has %d heads of %d (got %lld of %lld)",
+                  c.heads, c.dim, (long long)heads, (long long)dim);
     MAMBO_REQUIRE(n >= 0, MAMBO_ERR_VALUE, "a negative number of tokens");
     if (n == 0)
         return MAMBO_OK;

@@ -43,8 +43,8 @@ def launch_attention_kv(q: torch.Tensor, cache: KVCache, tables: torch.Tensor, l
     0, more rows than tokens, no page) becomes zeros, its lse -inf. ``scale`` defaults to D ** -0.5.
 
     Scores, the running sum and the output are float32; the probabilities are rounded to bfloat16 (2^-8 of each at most) for the
-    product with the values, the result once to bfloat16. Results do not vary from run to run. Rows of no sequence are not written: they stay what they
-    were in ``out``, and are undefined without. ``out`` must not overlap ``q``. T may be 0."""
+    product with the values, the result once to bfloat16. Results do not vary from run to run. Rows of no sequence are not
+    written: they stay what they were in ``out``, and are undefined without. ``out`` must not overlap ``q``. T may be 0."""
     cache = check_cache(cache)
     dev, dim = cache.codes.device, cache.head_dim
     check_heads(q, dim, dev, "q")

@@ -109,8 +109,8 @@ def launch_append_kv(k: torch.Tensor, v: torch.Tensor, cache: KVCache, tables: t
             shape = q.shape
             q, ldqt, ldqh = heads_in_place(q)
             out, ldot, ldoh = output_heads(out, shape, torch.bfloat16, dev)
-            rows = _native.KVRowsArgs(k.data_ptr(), v.data_ptr(), q.data_ptr() if tokens else None, ldkt, ldkh, ldvt, ldvh, ldqt, ldqh,
-                                      out.data_ptr(), ldot, ldoh, shape[1], dtype)
+            rows = _native.KVRowsArgs(k.data_ptr(), v.data_ptr(), q.data_ptr() if tokens else None, ldkt, ldkh, ldvt, ldvh,
+                                      ldqt, ldqh, out.data_ptr(), ldot, ldoh, shape[1], dtype)
         _native.check(_native.lib().mambo_kv_append(
             rows, tokens, cache.args, batch, None if rotary is None else rotary.args,
             None if positions is None else positions.data_ptr(), _native.stream_handle(stream, dev)), "launch_append_kv")
@@ -135,6 +135,6 @@ def launch_read_kv(cache: KVCache, tables: torch.Tensor, sequences: torch.Tensor
         batch = _native.KVBatchArgs(tables.data_ptr(), row, columns, None, None, seqs)
         k, v = torch.empty((2, n, cache.heads, cache.head_dim), dtype=torch.bfloat16, device=dev).unbind(0)
         _native.check(_native.lib().mambo_kv_read(
-            cache.args, batch, sequences.data_ptr(), positions.data_ptr(), n, cache.heads, cache.head_dim, k.data_ptr(), v.data_ptr(),
-            _native.stream_handle(stream, dev)), "launch_read_kv")
+            cache.args, batch, sequences.data_ptr(), positions.data_ptr(), n, cache.heads, cache.head_dim, k.data_ptr(),
+            v.data_ptr(), _native.stream_handle(stream, dev)), "launch_read_kv")
     return k, v

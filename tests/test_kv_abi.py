@@ -176,7 +176,8 @@ def test_plans(lib):
     assert plan(34, 8)[:1] == [0] and plan(34, 8)[2] == 256 and plan(34, 8, dim=192)[2] == 256 and plan(34, 8, dim=200)[2] == 128
     assert plan(40, 8, offsets=256) == [16, 0, 256, 1]
     assert plan(40, 96, offsets=256)[0] == 64 and plan(40, 160, offsets=256)[0] == 0
-    assert plan(400, 8, width=2000, ldt=2000)[3] == 256 // (2 * 4 * 2) and plan(400, 8, offsets=256, width=2000, ldt=2000)[3] == 32
+    assert plan(400, 8, width=2000, ldt=2000)[3] == 256 // (2 * 4 * 2)
+    assert plan(400, 8, seqs=1, width=2000, ldt=2000)[3] == 256 // (7 * 2) and plan(400, 8, offsets=256, width=2000, ldt=2000)[3] == 32
 
 
 def test_the_blocks_layout_is_a_permutation():
