@@ -90,8 +90,9 @@ __device__ __forceinline__ uint2 keep_tokens(uint32_t lo, uint32_t hi, int left)
     return make_uint2(lo & (uint32_t)mask, hi & (uint32_t)(mask >> 32));
 }
 
-// Most rows that attend_rows takes: 16 a tile, as many tiles as the registers and the LDS of its join hold.
-constexpr int max_row_tiles(int padded) { return padded <= 64 ? 4 : padded <= 128 ? 2 : 1; }
+// Most rows that attend_rows takes, in tiles of 16: more than that attend_tiles is faster at (4 x 64 rows of D = 128 behind 20000
+// tokens 57 us, with four tiles here 75; 4 x 32 of 192 behind 10000 52, here 37; of 256 73, here 53).
+constexpr int max_row_tiles(int padded) { return padded <= 64 ? 4 : 2; }
 
 // Waves of a workgroup of attend_tiles, each with 32 rows, by the head size in 32s. Eight, two a SIMD, while a wave's
 // registers are enough, above that four with twice the registers. 4096 tokens of 32 heads with eight and with four: of 64 101 us

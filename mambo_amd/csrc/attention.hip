@@ -40,13 +40,14 @@ Plan make_plan(const KvCache &c, const KvBatch &b, int group, int64_t window)
         int64_t seen = b.capacity;
         if (window)
             seen = std::min<int64_t>(seen, std::min(window, seen) + p.few_rows / group + kKvBlock);
-        if (seen > ((int64_t)b.seqs * c.heads >= kCus ? kShortTokensOfMany : kShortTokens)) {
+        // (whose eight waves have not the registers for two row tiles of large heads)
+        const int size = padded / 32 * p.row_tiles;
+        if (size > 9 || seen > ((int64_t)b.seqs * c.heads >= kCus ? kShortTokensOfMany : kShortTokens)) {
             // A workgroup a CU, fewer where there is no work for them: the blocks that its waves have on their way are enough
             // (131149 tokens of 8 heads of 128 47.0 us, with two 49.6). Two of small heads (16 x 8000 of 64 28.7 us for 35.4),
             // and where a workgroup comes to the ends of several sequences, at which the other goes on (64 sequences
             // of up to 8192 109 us for 113, 32 of 4000 49.5 for 44.4).
             const int64_t blocks = (int64_t)b.seqs * (b.capacity / kKvBlock);
-            const int size = padded / 32 * p.row_tiles;
             const int per_cu = size <= 2 || (size <= 4 && (int64_t)b.seqs * c.heads >= 2 * kCus) ? 2 : 1;
             p.slots = (int)std::max<int64_t>(1, std::min<int64_t>(per_cu * kCus / c.heads, cdiv(blocks, 4)));
             p.rows_entries = (int64_t)c.heads * p.slots * 2 * p.few_rows;

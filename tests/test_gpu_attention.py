@@ -83,6 +83,7 @@ RAGGED = [
     ([129, 140], [40, 7], 1, 48, 64, 32, 0),
     ([90, 120], [9, 100], 1, 24, 256, 32, 0),
     ([0, 0], [3, 100], 1, 2, 64, 32, 0),
+    ([129, 40, 1], [1, 30, 1], 1, 40, 128, 32, 0),  # more heads than the kernel for few rows takes
     ([40] * 300, [1] * 299 + [20], 1, 2, 32, 32, 0),  # more sequences than a wave looks at in one go
     ([33] * 130, [2] * 60 + [0] * 9 + [33] + [1] * 60, 1, 8, 64, 32, 0),
 ]
@@ -269,10 +270,10 @@ def test_every_kernel_for_few_rows(gpu, dim, split):
     rng = np.random.default_rng(dim)
     lengths = [300, 33, 0, 170]
     cache, tables, keys, values = filled(gpu, rng, lengths, 1, dim, 32, extra=100 if split else 1)
-    for group in [11] + [27] * (dim <= 128) + [61] * (dim <= 64):
+    for group in [11, 27] + [61] * (dim <= 64):
         q = rows_of(rng, 4, group, dim, torch.bfloat16, 2.0).to(gpu)
         plan = plan_of(cache, tables, 4, group, False)
-        assert plan[0] == (16 if group == 11 else 32 if group == 27 else 64) and (plan[1] > 0) == split and plan[2] == 0
+        assert plan[0] == (16 if group == 11 else 32 if group == 27 else 64) and (plan[1] > 0) == (split or (group == 27 and dim > 128)) and plan[2] == 0
         out, lse = attention()(q, cache, tables, *ref.device(gpu, np.array(lengths, np.int32)), return_lse=True)
         check(out, lse, q, keys, values, [1] * 4, group)
 
