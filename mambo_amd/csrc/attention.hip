@@ -20,6 +20,10 @@ constexpr int kCus = 256;
 // 9.7 us for 8.6 by two launches, whose second costs the host 3 us more, 2000 14.5 for 8.9; 32 users (a workgroup a CU)
 // 1000 16.7 for 21.3, 2000 25.7 for 30.4.
 constexpr int64_t kShortTokens = 1280, kShortTokensOfMany = 2048;
+// Sequences from which the kernel for many rows takes those of 33 to 64 rows that no single workgroup takes: the shares of the
+// other then end sequences too often. 36 rows of 8 heads of 64, by it and by the other: 32 x 2000 tokens 36.5 us for 52.3,
+// 8 x 4000 25.0 for 30.7, 4 x 8000 26.4 for 28.7, 2 x 16000 29.1 for 27.9, 30000 32.8 for 27.3.
+constexpr int kSeqsOfTiles = 4;
 
 int64_t aligned(int64_t bytes) { return (bytes + 15) & ~(int64_t)15; }
 
@@ -42,7 +46,10 @@ Plan make_plan(const KvCache &c, const KvBatch &b, int group, int64_t window)
             seen = std::min<int64_t>(seen, std::min(window, seen) + p.few_rows / group + kKvBlock);
         // (whose eight waves have not the registers for two row tiles of large heads)
         const int size = padded / 32 * p.row_tiles;
-        if (size > 9 || seen > ((int64_t)b.seqs * c.heads >= kCus ? kShortTokensOfMany : kShortTokens)) {
+        const bool short_ones = size <= 9 && seen <= ((int64_t)b.seqs * c.heads >= kCus ? kShortTokensOfMany : kShortTokens);
+        if (!short_ones && p.row_tiles > 2 && !b.offsets && b.seqs >= kSeqsOfTiles) {
+            p.row_tiles = p.few_rows = 0;
+        } else if (!short_ones) {
             // A workgroup a CU, fewer where there is no work for them: the blocks that its waves have on their way are enough
             // (131149 tokens of 8 heads of 128 47.0 us, with two 49.6). Two of small heads (16 x 8000 of 64 28.7 us for 35.4),
             // and where a workgroup comes to the ends of several sequences, at which the other goes on (64 sequences
@@ -53,7 +60,7 @@ Plan make_plan(const KvCache &c, const KvBatch &b, int group, int64_t window)
             p.rows_entries = (int64_t)c.heads * p.slots * 2 * p.few_rows;
         }
     }
-    if (rows > most) {
+    if (rows > most || !p.row_tiles) {
         const int tile = tile_rows(padded / 32);
         p.tiles_each = (int)cdiv(rows, tile);
         p.tiles = b.offsets ? (int64_t)b.tokens * group / tile + b.seqs : (int64_t)b.seqs * p.tiles_each;

@@ -270,12 +270,16 @@ def test_every_kernel_for_few_rows(gpu, dim, split):
     rng = np.random.default_rng(dim)
     lengths = [300, 33, 0, 170]
     cache, tables, keys, values = filled(gpu, rng, lengths, 1, dim, 32, extra=100 if split else 1)
-    for group in [11, 27] + [61] * (dim <= 64):
-        q = rows_of(rng, 4, group, dim, torch.bfloat16, 2.0).to(gpu)
-        plan = plan_of(cache, tables, 4, group, False)
-        assert plan[0] == (16 if group == 11 else 32 if group == 27 else 64) and (plan[1] > 0) == (split or (group == 27 and dim > 128)) and plan[2] == 0
-        out, lse = attention()(q, cache, tables, *ref.device(gpu, np.array(lengths, np.int32)), return_lse=True)
-        check(out, lse, q, keys, values, [1] * 4, group)
+    for group, seqs in [(11, 4), (27, 4)] + [(61, 3), (61, 4)] * (dim <= 64):
+        q = rows_of(rng, seqs, group, dim, torch.bfloat16, 2.0).to(gpu)
+        plan = plan_of(cache, tables[:seqs], seqs, group, False)
+        if split and (group, seqs) == (61, 4):  # from four sequences on
+            assert plan[:3] == [0, 0, 256]
+        else:
+            assert plan[0] == (16 if group == 11 else 32 if group == 27 else 64) and plan[2] == 0
+            assert (plan[1] > 0) == (split or (group == 27 and dim > 128))
+        out, lse = attention()(q, cache, tables[:seqs], *ref.device(gpu, np.array(lengths[:seqs], np.int32)), return_lse=True)
+        check(out, lse, q, keys[:seqs], values[:seqs], [1] * seqs, group)
 
 
 @pytest.mark.parametrize("dim", [24, 64, 88, 128, 160, 184, 224, 256])

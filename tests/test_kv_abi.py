@@ -174,6 +174,9 @@ def test_plans(lib):
     assert plan(2, 256, heads=128, seqs=2, width=65, ldt=65)[:2] == [16, 4]
     assert plan(32, 8)[0] == 64 and plan(32, 8, dim=128)[2] == 256 and plan(32, 4, dim=128)[0] == 32
     assert plan(34, 8)[:1] == [0] and plan(34, 8)[2] == 256 and plan(34, 8, dim=192)[2] == 256 and plan(34, 8, dim=200)[2] == 128
+    wide = {"width": 2000, "ldt": 2000}
+    assert plan(15 * 3, 8, seqs=3, **wide)[0] == 64 and plan(15 * 4, 8, seqs=4, **wide)[:3] == [0, 0, 256]
+    assert plan(8 * 4, 8, seqs=4, **wide)[0] == 32 and plan(15, 8, seqs=4, offsets=256, **wide)[0] == 64
     assert plan(40, 8, offsets=256) == [16, 0, 256, 1]
     assert plan(40, 96, offsets=256)[0] == 64 and plan(40, 160, offsets=256)[0] == 0
     assert plan(400, 8, width=2000, ldt=2000)[3] == 256 // (2 * 4 * 2)
