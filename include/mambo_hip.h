@@ -402,8 +402,8 @@ typedef struct mambo_kv_cache {
 /* The sequences of a call: sequence s has the rows [offsets[s], offsets[s+1]) of the call's `tokens`
  * (offsets NULL: tokens / seqs rows each), the last of them at position lengths[s] - 1, and its page
  * c (tokens [c * page_size, ...)) is tables[s * ldt + c], c < width. The kernels hold offsets within
- * [0, tokens] and lengths within [0, width * page_size]; a page outside [0, pages) is none: nothing is
- * stored there and its tokens are left out of attention. */
+ * [0, tokens] and take a length below 0 for 0. A page outside [0, pages), or past the table's width, is none:
+ * nothing is stored there and its tokens are left out of attention; rows keep their positions. */
 typedef struct mambo_kv_batch {
     const int32_t *tables;
     int64_t ldt;

@@ -26,9 +26,10 @@ struct Attention {
     float *tiles_o, *tiles_ml;
 };
 
-// A sequence's rows [first, first + n) and the blocks [lo, hi) of its keys that any of them sees.
+// A sequence's rows [first, first + n), the last at position end - 1, its cached tokens [0, len) and the blocks [lo, hi) of
+// them that any row sees (none: lo >= hi).
 struct Sequence {
-    int first, n, len, lo, hi;
+    int first, n, end, len, lo, hi;
 };
 
 __device__ __forceinline__ Sequence sequence(const Attention &a, int s)
@@ -36,8 +37,9 @@ __device__ __forceinline__ Sequence sequence(const Attention &a, int s)
     Sequence q;
     q.first = a.b.offset(s);
     q.n = max(0, (a.b.offsets ? a.b.offset(s + 1) : q.first + a.b.each) - q.first);
-    q.len = a.b.length(s);
-    q.lo = a.window ? max(0, q.len - q.n + 1 - a.window) / kKvBlock : 0;
+    q.end = a.b.length(s);
+    q.len = min(q.end, a.b.capacity);
+    q.lo = a.window ? max(0, q.end - q.n + 1 - a.window) / kKvBlock : 0;
     q.hi = (q.len + kKvBlock - 1) / kKvBlock;
     return q;
 }
@@ -45,11 +47,11 @@ __device__ __forceinline__ Sequence sequence(const Attention &a, int s)
 // What row (query i of n) sees: keys in [from, to).
 __device__ __forceinline__ int sees_to(const Attention &a, const Sequence &q, int i)
 {
-    return a.causal ? q.len - q.n + i + 1 : q.len;
+    return a.causal ? min(q.end - q.n + i + 1, q.len) : q.len;
 }
 __device__ __forceinline__ int sees_from(const Attention &a, const Sequence &q, int i)
 {
-    return a.window ? q.len - q.n + i + 1 - a.window : 0;
+    return a.window ? q.end - q.n + i + 1 - a.window : 0;
 }
 
 // Eight E4M3 codes times a power of two as bf16, which holds them exactly (4 of its 8 bits).
@@ -104,7 +106,7 @@ constexpr int tile_rows(int ds) { return 32 * tile_waves(ds); }
 // Blocks that a sequence has in the row kernel's order.
 __device__ __forceinline__ int row_blocks(const Attention &a, const Sequence &q)
 {
-    return q.n > 0 && q.n <= a.few_rows / a.group ? q.hi - q.lo : 0;
+    return q.n > 0 && q.n <= a.few_rows / a.group ? max(0, q.hi - q.lo) : 0;
 }
 
 // The shares: workgroups that have any (at least four blocks each, one a wave), and where they begin.

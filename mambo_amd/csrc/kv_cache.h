@@ -41,7 +41,8 @@ struct KvCache {
 };
 
 // The sequences of a call. Whatever the device's arrays hold, what is made of them stays in range:
-// rows within the call's tokens, lengths within the tables, pages (checked where they are read).
+// rows within the call's tokens, cached tokens within the tables, pages (checked where they are read).
+// Positions are those of the length that was given: past the table's end they are nobody's place.
 struct KvBatch {
     const int32_t *tables, *lengths, *offsets; // offsets NULL: `each` rows a sequence
     int64_t ldt;
@@ -51,7 +52,7 @@ struct KvBatch {
     {
         return offsets ? min(max(offsets[s], 0), tokens) : s * each;
     }
-    __device__ int length(int s) const { return min(max(lengths[s], 0), capacity); }
+    __device__ int length(int s) const { return max(lengths[s], 0); }
     __device__ int page(int s, int column) const { return tables[s * ldt + column]; }
 };
 

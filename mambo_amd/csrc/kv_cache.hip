@@ -228,10 +228,10 @@ __global__ __launch_bounds__(256) void append_kernel(const Append a)
     const int first = a.b.offset(s), n = (a.b.offsets ? a.b.offset(s + 1) : first + a.b.each) - first;
     const int len = a.b.length(s), start = len - n; // start: position of the first row
     const int from = max(start, 0), blk = from / kKvBlock + j;
-    // positions of this block, none where there are no rows that far
-    const int lo = max(from, blk * kKvBlock), hi = min(len, (blk + 1) * kKvBlock);
-    if (j < 0 || n <= 0 || j > n / kKvBlock + 1 || (j > 0 && lo >= hi))
+    if (j < 0 || n <= 0 || j > n / kKvBlock + 1 || (j > 0 && blk > (len - 1) / kKvBlock))
         return;
+    // positions of this block, none in the first where there are no rows that far
+    const int base = blk * kKvBlock, lo = max(from, base), hi = base + min(kKvBlock, len - base);
     const int half = a.table.size / 2;
     const int64_t row0 = (int64_t)first - start; // row of position p: row0 + p
 
@@ -246,8 +246,9 @@ __global__ __launch_bounds__(256) void append_kernel(const Append a)
         const int units = rotary_units<kVec>(dim, a.table.size, a.table.interleaved); // at most 256
         const int step = 256 / units, row_step = step % a.q_heads, token_step = step / a.q_heads;
         // this block's tokens, and with the first also those before the sequence's start, which are not stored
-        for (int p0 = (j == 0 ? start : lo) + part * each; p0 < hi; p0 += kKvBlock) {
-            const int count = min(each, hi - p0);
+        const int begin = j == 0 ? start : lo, rows = hi - begin;
+        for (int done = part * each; done < rows; done += kKvBlock) {
+            const int p0 = begin + done, count = min(each, rows - done);
             make_angles(p0, count);
             __syncthreads();
             int h = tid / units, t = h / a.q_heads;
@@ -267,7 +268,7 @@ __global__ __launch_bounds__(256) void append_kernel(const Append a)
         }
         return;
     }
-    if (lo >= hi)
+    if (lo >= hi || base >= a.b.capacity) // whole blocks: a table's pages are
         return;
     make_angles(lo, hi - lo);
     if (tid < kKvBlock)
@@ -281,7 +282,7 @@ __global__ __launch_bounds__(256) void append_kernel(const Append a)
     uint8_t *const keys = a.cache.codes + (int64_t)at * (2 * kKvBlock * padded), *const values = keys + kKvBlock * padded;
     uint8_t *const scale = a.cache.scales + 2 * (int64_t)at;
 
-    const int chunks = padded / 8, base = blk * kKvBlock;
+    const int chunks = padded / 8;
     float kx[P][8];
 #pragma unroll
     for (int i = 0; i < P; ++i) {

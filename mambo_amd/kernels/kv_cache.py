@@ -4,7 +4,8 @@ no counterpart.
 A call's sequences are told by ``tables`` int32 [S, C] (the page that holds a sequence's tokens
 [c * page_size, ...), any value outside the cache: none), ``lengths`` int32 [S] (cached tokens, the call's own
 included) and, unless every sequence has as many rows, ``offsets`` int32 [S + 1] (sequence s has the rows
-offsets[s] to offsets[s + 1], the last at position lengths[s] - 1). All of it stays on the device: nothing is
+offsets[s] to offsets[s + 1], the last at position lengths[s] - 1). A sequence may be longer than its row of the
+table: there is no page for what lies past it. All of it stays on the device: nothing is
 read back, so that a step can be recorded into a HIP graph and replayed with other lengths.
 
     cache = allocate_kv_cache(pages, kv_heads, head_dim)

@@ -335,3 +335,25 @@ def test_probabilities_add_up_over_a_rising_sequence_of_scores(gpu):
                 q = torch.ones((n, 2, dim), dtype=torch.bfloat16, device=gpu)
                 out, lse = attention()(q, cache, tables, lengths, return_lse=True)
                 check(out, lse, q, keys, values, [n], 2)
+
+
+@pytest.mark.parametrize("n,group,columns", [(1, 4, 3), (10, 4, 3), (90, 4, 3), (1, 4, 60), (10, 4, 60), (100, 2, 60)])
+@pytest.mark.parametrize("causal,window", [(True, 0), (True, 8), (True, 70), (False, 0)])
+def test_rows_past_a_table_keep_their_positions(gpu, n, group, columns, causal, window):
+    """Sequences that are longer than their tables: a row sees the cached tokens up to its own position and within its
+    window, which may be none. By every kernel."""
+    rng = np.random.default_rng(n + columns)
+    held, heads, dim = 32 * columns, 1, 64
+    cache, tables, keys, values = filled(gpu, rng, [held, held], heads, dim, 32, extra=0)
+    assert tables.shape == (2, columns)
+    q = rows_of(rng, 2 * n, heads * group, dim, torch.bfloat16, 2.0).to(gpu)
+    for past in ([1, 6], [n, 0], [n + 3, 75], [2**31 - 1 - held, 33]):
+        out, lse = attention()(q, cache, tables, *ref.device(gpu, np.array([held + p for p in past], np.int32)), causal=causal,
+                               window=window, return_lse=True)
+        for s, p in enumerate(past):
+            # far behind the table every row sees all of it, or nothing
+            p = min(p, held + 2 * n + window)
+            gone = np.arange(held + p) >= held
+            there = [np.concatenate([t[s], np.zeros((p, heads, dim))]) for t in (keys, values)]
+            part = slice(n * s, n * (s + 1))
+            check(out[part], lse[part], q[part], [there[0]], [there[1]], [n], group, causal=causal, window=window, left_out=[gone])

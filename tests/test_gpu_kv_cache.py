@@ -339,3 +339,65 @@ def test_refusals(gpu):
         with pytest.raises(ValueError):
             ops().launch_read_kv(cache, tables, *args)
     assert ops().launch_read_kv(cache, tables, lengths[:0], lengths[:0])[0].shape == (0, 2, 64)
+
+
+@pytest.mark.parametrize("ragged", [False, True])
+@pytest.mark.parametrize("start,n", [(64, 1), (96, 3), (40, 40), (0, 200), (63, 2), (70, 100), (5000, 1), (2**31 - 41, 40), (2**31 - 2, 1),
+                                     (-20, 300)])
+def test_tokens_past_a_table_are_dropped(gpu, start, n, ragged):
+    """A table of 64 tokens whose sequence grows past it: what is cached stays, rows within it are stored at their own
+    positions, the others nowhere, and queries turn by the positions that the lengths say."""
+    from mambo_amd.kernels.rotary import launch_rotary
+    from mambo_amd.utils.rotary_table import prepare_rotary_table
+    rng = np.random.default_rng(20)
+    heads, dim = 2, 64
+    cache, table = new_cache(4, heads, dim, 32), prepare_rotary_table(dim)
+    tables = torch.tensor([[3, 0]], dtype=torch.int32, device=gpu)
+    old_k, old_v = rows_of(rng, 64, heads, dim, torch.bfloat16), rows_of(rng, 64, heads, dim, torch.bfloat16)
+    ops().launch_append_kv(old_k.to(gpu), old_v.to(gpu), cache, tables, torch.tensor([64], dtype=torch.int32, device=gpu))
+    before = cache.codes.clone(), cache.scales.clone()
+    model = ref.Model(heads, dim)
+    model.append(old_k.double().numpy(), old_v.double().numpy(), 0)
+    k, v, q = (rows_of(rng, n, h, dim, torch.float32).to(gpu) for h in (heads, heads, 4))
+    positions = torch.arange(start, start + n, device=gpu).int()
+    got = ops().launch_append_kv(k, v, cache, tables, torch.tensor([start + n], dtype=torch.int32, device=gpu), rotary=table, q=q,
+                                 offsets=torch.tensor([0, n], dtype=torch.int32, device=gpu) if ragged else None)
+    assert torch.equal(got, launch_rotary(q, positions, table, out_dtype=torch.bfloat16))
+    stored = (positions >= 0) & (positions < 64)
+    if not stored.any():
+        assert torch.equal(cache.codes, before[0]) and torch.equal(cache.scales, before[1])
+        return
+    turned = launch_rotary(k, positions, table)[stored].double().cpu().numpy()
+    model.append(turned, v[stored].double().cpu().numpy(), max(start, 0))
+    got_k, got_v = read_all(cache, tables, [64])
+    same(got_k[0], model.k)
+    same(got_v[0], model.v)
+
+
+def test_a_captured_step_replayed_past_its_table(gpu):
+    rng = np.random.default_rng(21)
+    heads, dim = 1, 64
+    cache = new_cache(2, heads, dim, 32)
+    tables, lengths = torch.tensor([[1]], dtype=torch.int32, device=gpu), torch.tensor([29], dtype=torch.int32, device=gpu)
+    old = rows_of(rng, 29, heads, dim, torch.bfloat16).to(gpu)
+    ops().launch_append_kv(old, old, cache, tables, lengths)
+    new = rows_of(rng, 1, heads, dim, torch.bfloat16).to(gpu)
+    model = ref.Model(heads, dim)
+    model.append(old.double().cpu().numpy(), old.double().cpu().numpy(), 0)
+    graph, side = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side), torch.cuda.graph(graph, stream=side):
+        lengths.add_(1)
+        ops().launch_append_kv(new, new, cache, tables, lengths)
+    torch.cuda.synchronize()
+    for step in range(6):  # three tokens fit
+        new.copy_(rows_of(rng, 1, heads, dim, torch.bfloat16, 1.0 + step))
+        if step < 3:
+            model.append(new.double().cpu().numpy(), new.double().cpu().numpy(), 29 + step)
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        got_k, got_v = read_all(cache, tables, [len(model.k)])
+        same(got_k[0], model.k)
+        same(got_v[0], model.v)
+    assert int(lengths) == 35
