@@ -147,6 +147,14 @@ __device__ __forceinline__ Keys tile_keys(const Attention &a, const Sequence &se
     return k;
 }
 
+// What is joined: workgroups for rows of attend_tiles, each of join_tile_rows, then one for each of the row_count rows that a
+// sequence and a head can have in attend_rows.
+struct Join {
+    int64_t tiles = 0, rows = 0;
+    int row_count = 0;
+};
+constexpr int join_tile_rows(int ds) { return 256 / (8 * ds); }
+
 int launch_attend_rows(const Attention &a, int row_tiles, hipStream_t s);
 int launch_attend_tiles(const Attention &a, int64_t tiles, hipStream_t s);
-int launch_attend_join(const Attention &a, int row_tiles, hipStream_t s);
+int launch_attend_join(const Attention &a, int row_tiles, const Join &join, hipStream_t s);

@@ -13,6 +13,7 @@ struct Plan {
     int64_t tiles = 0;                          // the kernel for many, tiles of a head; 0: not launched
     int tiles_each = 1, parts = 1;
     int64_t rows_entries = 0, tiles_entries = 0, bytes = 0;
+    Join join;
 };
 
 constexpr int kCus = 256;
@@ -58,6 +59,8 @@ Plan make_plan(const KvCache &c, const KvBatch &b, int group, int64_t window)
             const int per_cu = size <= 2 || (size <= 4 && (int64_t)b.seqs * c.heads >= 2 * kCus) ? 2 : 1;
             p.slots = (int)std::max<int64_t>(1, std::min<int64_t>(per_cu * kCus / c.heads, cdiv(blocks, 4)));
             p.rows_entries = (int64_t)c.heads * p.slots * 2 * p.few_rows;
+            p.join.row_count = b.offsets ? p.few_rows : (int)rows;
+            p.join.rows = (int64_t)b.seqs * c.heads * p.join.row_count;
         }
     }
     if (rows > most || !p.row_tiles) {
@@ -68,8 +71,11 @@ Plan make_plan(const KvCache &c, const KvBatch &b, int group, int64_t window)
         // for 41; of sequences with as many rows each, 4 of 16 rows behind 20000 tokens, 66 for 58).
         const int64_t places = (b.offsets ? 2 : 1) * kCus / (p.tiles * c.heads);
         p.parts = (int)std::max<int64_t>(1, std::min<int64_t>(places, cdiv(b.capacity, 512)));
-        if (p.parts > 1)
-            p.tiles_entries = (int64_t)p.parts * b.tokens * group * c.heads;
+        if (p.parts > 1) {
+            const int64_t entries = (int64_t)b.tokens * group * c.heads;
+            p.tiles_entries = p.parts * entries;
+            p.join.tiles = cdiv(entries, join_tile_rows(padded / 32));
+        }
     }
     p.bytes = aligned(p.rows_entries * (padded + 2) * 4) + aligned(p.slots ? ((int64_t)b.seqs + 1) * 4 : 0) +
               aligned(p.tiles_entries * (padded + 2) * 4);
@@ -91,9 +97,9 @@ int check(const mambo_kv_cache *cache, const mambo_kv_batch *batch, int64_t toke
     MAMBO_REQUIRE(batch->seqs * (int64_t)(b->capacity / kKvBlock) <= 0x7FFFFFF0, MAMBO_ERR_VALUE,
                   "tables must hold below 2^36 tokens together");
     *p = make_plan(*c, *b, (int)(q_heads / c->heads), window);
-    const int64_t rows = p->slots ? p->few_rows : 0, heads = c->heads;
-    MAMBO_REQUIRE(grid_takes(batch->seqs * heads, 512) && grid_takes(p->tiles * heads, 512) &&
-                      grid_takes(tokens * q_heads + batch->seqs * heads * rows, 256),
+    const int64_t heads = c->heads;
+    MAMBO_REQUIRE((p->row_tiles == 0 || p->slots || grid_takes(batch->seqs * heads, 512)) && grid_takes(p->tiles * heads, 512) &&
+                      grid_takes(p->join.tiles + p->join.rows, 256),
                   MAMBO_ERR_VALUE, "too many rows for one launch");
     return MAMBO_OK;
 }
@@ -169,5 +175,5 @@ extern "C" int mambo_kv_attention(const void *q, int64_t tokens, int64_t q_heads
     if (p.row_tiles)
         if (const int rc = launch_attend_rows(a, p.row_tiles, s))
             return rc;
-    return p.slots || p.parts > 1 ? launch_attend_join(a, p.row_tiles, s) : MAMBO_OK;
+    return p.join.tiles + p.join.rows ? launch_attend_join(a, p.row_tiles, p.join, s) : MAMBO_OK;
 }

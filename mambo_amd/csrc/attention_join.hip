@@ -81,7 +81,7 @@ __device__ void join_rows(const Attention &a, int tile_rows, int row_count, int 
 template <int DS>
 __device__ void join_tiles(const Attention &a, int at)
 {
-    constexpr int DP = 32 * DS, kWide = DP / 4, kRows = 256 / kWide;
+    constexpr int DP = 32 * DS, kWide = DP / 4, kRows = join_tile_rows(DS);
     const int64_t q_heads = (int64_t)a.group * a.cache.heads, all = a.b.tokens * q_heads;
     const int64_t entry = (int64_t)at * kRows + (int)threadIdx.x / kWide;
     const int d = 4 * ((int)threadIdx.x % kWide);
@@ -127,28 +127,25 @@ __global__ __launch_bounds__(256) void attend_join_kernel(const Attention a, int
 }
 
 template <int DS>
-void launch_join(const Attention &a, int row_tiles, hipStream_t s)
+void launch_join(const Attention &a, int row_tiles, const Join &join, hipStream_t s)
 {
-    const int64_t entries = a.parts > 1 ? (int64_t)a.b.tokens * a.group * a.cache.heads : 0, each = 256 / (8 * DS);
-    const int64_t from = (entries + each - 1) / each;
-    const int row_count = a.b.offsets ? a.few_rows : a.b.each * a.group; // of a sequence, at most
-    const int64_t rows = a.slots ? (int64_t)a.b.seqs * a.cache.heads * row_count : 0;
-    MAMBO_LAUNCH((attend_join_kernel<DS>), dim3((unsigned)(from + rows)), dim3(256), 0, s, a, (int)from, 16 * row_tiles, row_count);
+    MAMBO_LAUNCH((attend_join_kernel<DS>), dim3((unsigned)(join.tiles + join.rows)), dim3(256), 0, s, a, (int)join.tiles,
+                 16 * row_tiles, join.row_count);
 }
 
 } // namespace
 
-int launch_attend_join(const Attention &a, int row_tiles, hipStream_t s)
+int launch_attend_join(const Attention &a, int row_tiles, const Join &join, hipStream_t s)
 {
     switch (kv_padded(a.cache.dim) / 32) {
-    case 1: launch_join<1>(a, row_tiles, s); break;
-    case 2: launch_join<2>(a, row_tiles, s); break;
-    case 3: launch_join<3>(a, row_tiles, s); break;
-    case 4: launch_join<4>(a, row_tiles, s); break;
-    case 5: launch_join<5>(a, row_tiles, s); break;
-    case 6: launch_join<6>(a, row_tiles, s); break;
-    case 7: launch_join<7>(a, row_tiles, s); break;
-    default: launch_join<8>(a, row_tiles, s); break;
+    case 1: launch_join<1>(a, row_tiles, join, s); break;
+    case 2: launch_join<2>(a, row_tiles, join, s); break;
+    case 3: launch_join<3>(a, row_tiles, join, s); break;
+    case 4: launch_join<4>(a, row_tiles, join, s); break;
+    case 5: launch_join<5>(a, row_tiles, join, s); break;
+    case 6: launch_join<6>(a, row_tiles, join, s); break;
+    case 7: launch_join<7>(a, row_tiles, join, s); break;
+    default: launch_join<8>(a, row_tiles, join, s); break;
     }
     return mambo_check_launch("kv_attention");
 }

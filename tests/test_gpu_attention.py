@@ -357,3 +357,20 @@ def test_rows_past_a_table_keep_their_positions(gpu, n, group, columns, causal, 
             there = [np.concatenate([t[s], np.zeros((p, heads, dim))]) for t in (keys, values)]
             part = slice(n * s, n * (s + 1))
             check(out[part], lse[part], q[part], [there[0]], [there[1]], [n], group, causal=causal, window=window, left_out=[gone])
+
+
+@pytest.mark.parametrize("n,group,seqs,few", [(1, 16, 2**20, 16), (64, 32, 2**13, 0), (1, 64, 2**18 + 5, 64)])
+def test_two_to_the_24_rows_and_more(gpu, n, group, seqs, few):
+    """The same sequences over and over: every repeat has the rows of the first, which are checked."""
+    rng = np.random.default_rng(30)
+    lengths, dim = [64, 40, 3, 0, 33, 1, 64, 50], 8
+    cache, tables, keys, values = filled(gpu, rng, lengths, 1, dim, 32)
+    times = -(-seqs // 8)
+    on = ref.device(gpu, np.array(lengths, np.int32))[0].repeat(times)[:seqs]
+    tables = tables.repeat(times, 1)[:seqs]
+    first = rows_of(rng, 8 * n, group, dim, torch.bfloat16, 2.0).to(gpu)
+    q = first.repeat(times, 1, 1)[:seqs * n]
+    assert q.shape[0] * group >= 2**24 and plan_of(cache, tables, seqs * n, group, False)[:2] == [few, 0]
+    out, lse = attention()(q, cache, tables, on, return_lse=True)
+    check(out[:8 * n], lse[:8 * n], first, keys, values, [n] * 8, group)
+    assert torch.equal(out, out[:8 * n].repeat(times, 1, 1)[:seqs * n]) and torch.equal(lse, lse[:8 * n].repeat(times, 1)[:seqs * n])

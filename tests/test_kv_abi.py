@@ -183,6 +183,23 @@ def test_plans(lib):
     assert plan(400, 8, seqs=1, width=2000, ldt=2000)[3] == 256 // (7 * 2) and plan(400, 8, offsets=256, width=2000, ldt=2000)[3] == 32
 
 
+def test_calls_of_two_to_the_24_rows_and_more(lib):
+    """What is launched decides, not the rows: of large calls nothing is joined."""
+    def size(tokens, q_heads, dim=128, heads=8, **b):
+        return lib.mambo_kv_attention_workspace(cache(head_dim=dim, heads=heads), batch(**b), tokens, q_heads, 0)
+
+    assert 2**17 * 128 == 2**18 * 64 == 2**19 * 32 == 2**24
+    for tokens, q_heads in ((2**17, 128), (2**18, 64), (2**19, 32), (2**23, 64), (2**24, 56)):
+        for more in ({"seqs": 1}, {"seqs": 2}, {"seqs": 1, "offsets": 256}, {"seqs": 1, "width": 2**20, "ldt": 2**20}):
+            assert size(tokens, q_heads, **more) == 0
+    assert size(2**20, 16, dim=8, heads=1, seqs=2**20) == 0        # single tokens, a workgroup each
+    assert size(2**20 - 1, 1023, dim=8, heads=1, seqs=2**20 - 1) == 0
+    assert size(2**20 - 1, 16, dim=8, heads=1, seqs=2**20 - 1, width=65, ldt=65) > 0  # joined, a workgroup for each of 2^24 - 16 rows
+    refused(lib, size(2**20, 16, dim=8, heads=1, seqs=2**20, width=65, ldt=65), "too many rows")
+    refused(lib, size(2**23, 8, seqs=2**23), "too many rows")      # 2^26 workgroups of 512
+    refused(lib, size(2**22, 1023, heads=1, dim=8, seqs=2), "below 2^30")
+
+
 def test_the_blocks_layout_is_a_permutation():
     """As mambo_amd/csrc/kv_cache.h states it, for every padded head size."""
     for dim in range(32, 257, 32):
