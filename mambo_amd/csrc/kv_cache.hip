@@ -563,7 +563,7 @@ int kv_check_batch(const mambo_kv_batch *b, int64_t tokens, const mambo_kv_cache
                   (long long)tokens);
     MAMBO_REQUIRE(b->offsets || tokens % b->seqs == 0, MAMBO_ERR_VALUE,
                   "without offsets every sequence has as many rows (got %lld of %lld)", (long long)tokens, (long long)b->seqs);
-    MAMBO_REQUIRE(b->width >= 1 && b->width * (int64_t)cache->page_size <= 0x3FFFFFFF && b->ldt >= b->width, MAMBO_ERR_VALUE,
+    MAMBO_REQUIRE(b->width >= 1 && b->width <= 0x3FFFFFFF / cache->page_size && b->ldt >= b->width, MAMBO_ERR_VALUE,
                   "tables must hold 1 to 2^30 - 1 tokens a sequence (got %lld pages, stride %lld)", (long long)b->width,
                   (long long)b->ldt);
     MAMBO_REQUIRE(b->tables && (b->lengths || tokens == 0), MAMBO_ERR_VALUE, "null pointer");

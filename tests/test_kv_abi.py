@@ -96,6 +96,13 @@ def test_read_refusals(lib):
     assert f(cache(), batch(lengths=None), None, None, 0, 2, 64, None, None, None) == 0
 
 
+@pytest.mark.parametrize("name", ["append", "attention", "plan", "workspace"])
+def test_sizes_whose_products_wrap(lib, name):
+    """Widths that 64 bits do not hold the tokens of, which wrap to nothing, to few and to a negative number of them."""
+    for page_size, width in ((65536, 2**48), (65536, 2**48 + 5), (32, 2**59 + 3), (32, 2**58), (65536, 2**63 - 1), (32, 2**62 + 1)):
+        refused(lib, calls(lib)[name](cache(page_size=page_size), batch(width=width, ldt=2**63 - 1)), "tables must hold")
+
+
 def test_rotary_refusals(lib):
     good = dict(x=256, xd=0, tokens=2, heads=2, dim=64, ldt=128, ldh=64, positions=256, table=table(), out=256, od=1, ldot=128, ldoh=64)
 
