@@ -711,7 +711,7 @@ extern "C" int mambo_kv_read(const mambo_kv_cache *cache, const mambo_kv_batch *
         return MAMBO_OK;
     MAMBO_REQUIRE(sequences && positions && k && v, MAMBO_ERR_VALUE, "null pointer");
     MAMBO_REQUIRE((uintptr_t)k % 16 == 0 && (uintptr_t)v % 16 == 0, MAMBO_ERR_VALUE, "keys and values must be 16-byte aligned");
-    MAMBO_REQUIRE(grid_takes(cdiv(n, 32), 256), MAMBO_ERR_VALUE, "too many rows for one launch");
+    MAMBO_REQUIRE(grid_takes(n / 32 + 1, 256), MAMBO_ERR_VALUE, "too many rows for one launch");
     MAMBO_LAUNCH(read_kernel, dim3((unsigned)cdiv(n, 32), (unsigned)c.heads), dim3(256),
                  (size_t)64 * 16 * (c.dim / 8 + 1), (hipStream_t)stream, c, b,
                  sequences, positions, n, (__bf16 *)k, (__bf16 *)v);

@@ -103,6 +103,12 @@ def test_sizes_whose_products_wrap(lib, name):
         refused(lib, calls(lib)[name](cache(page_size=page_size), batch(width=width, ldt=2**63 - 1)), "tables must hold")
 
 
+def test_rows_to_read_that_wrap(lib):
+    for n in (2**63 - 1, 2**63 - 31, 2**62):
+        refused(lib, lib.mambo_kv_read(cache(), batch(), 256, 256, n, 2, 64, 256, 256, None), "too many rows")
+    refused(lib, lib.mambo_kv_read(cache(page_size=65536), batch(width=2**48, ldt=2**48), 256, 256, 3, 2, 64, 256, 256, None), "tables must hold")
+
+
 def test_rotary_refusals(lib):
     good = dict(x=256, xd=0, tokens=2, heads=2, dim=64, ldt=128, ldh=64, positions=256, table=table(), out=256, od=1, ldot=128, ldoh=64)
 
