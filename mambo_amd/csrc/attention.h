@@ -96,6 +96,10 @@ __device__ __forceinline__ uint2 keep_tokens(uint32_t lo, uint32_t hi, int left)
 // tokens 57 us, with four tiles here 75; 4 x 32 of 192 behind 10000 52, here 37; of 256 73, here 53).
 constexpr int max_row_tiles(int padded) { return padded <= 64 ? 4 : 2; }
 
+// Whether attend_short takes so many tiles of heads of 32 ds: its eight waves have not the registers for two of heads above 128,
+// which always take the shares.
+constexpr bool short_fits(int ds, int row_tiles) { return ds * row_tiles <= 9; }
+
 // Waves of a workgroup of attend_tiles, each with 32 rows, by the head size in 32s. Eight, two a SIMD, while a wave's
 // registers are enough, above that four with twice the registers. 4096 tokens of 32 heads with eight and with four: of 64 101 us
 // and 117, of 96 119 and 219, of 160 213 and 278, of 192 285 and 299, of 224 530 and 355, of 256 1968 and 417; 8192 tokens of

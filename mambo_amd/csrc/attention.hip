@@ -45,9 +45,9 @@ Plan make_plan(const KvCache &c, const KvBatch &b, int group, int64_t window)
         int64_t seen = b.capacity;
         if (window)
             seen = std::min<int64_t>(seen, std::min(window, seen) + p.few_rows / group + kKvBlock);
-        // (whose eight waves have not the registers for two row tiles of large heads)
         const int size = padded / 32 * p.row_tiles;
-        const bool short_ones = size <= 9 && seen <= ((int64_t)b.seqs * c.heads >= kCus ? kShortTokensOfMany : kShortTokens);
+        const int64_t short_seen = (int64_t)b.seqs * c.heads >= kCus ? kShortTokensOfMany : kShortTokens;
+        const bool short_ones = short_fits(padded / 32, p.row_tiles) && seen <= short_seen;
         if (!short_ones && p.row_tiles > 2 && !b.offsets && b.seqs >= kSeqsOfTiles) {
             p.row_tiles = p.few_rows = 0;
         } else if (!short_ones) {

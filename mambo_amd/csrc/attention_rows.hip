@@ -423,10 +423,10 @@ template <int DS, int RT>
 void launch_rows(const Attention &a, hipStream_t s)
 {
     if constexpr (RT <= max_row_tiles(32 * DS)) {
-        if (a.slots == 0)
-            MAMBO_LAUNCH((attend_short_kernel<DS, RT>), dim3((unsigned)(a.b.seqs * a.cache.heads)), dim3(512), 0, s, a);
-        else
+        if (a.slots)
             MAMBO_LAUNCH((attend_rows_kernel<DS, RT>), dim3((unsigned)(a.slots * a.cache.heads)), dim3(256), 0, s, a);
+        else if constexpr (short_fits(DS, RT))
+            MAMBO_LAUNCH((attend_short_kernel<DS, RT>), dim3((unsigned)(a.b.seqs * a.cache.heads)), dim3(512), 0, s, a);
     }
 }
 

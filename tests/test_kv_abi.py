@@ -196,6 +196,29 @@ def test_plans(lib):
     assert plan(400, 8, seqs=1, width=2000, ldt=2000)[3] == 256 // (7 * 2) and plan(400, 8, offsets=256, width=2000, ldt=2000)[3] == 32
 
 
+def test_every_kernel_that_is_built_is_one_that_a_call_takes(lib):
+    """The kernels by head size (in 32s) and row tiles (of 16): their names in the library, and what the plans of calls of all
+    head sizes, rows and lengths come to."""
+    import re
+    from mambo_amd import _native
+    held = _native.LIB_PATH.read_bytes()
+    names = {(k.decode(), int(ds), int(rt or 0))
+             for k, ds, rt in re.findall(rb"attend_(short|rows|tiles)_kernelILi(\d+)E(?:Li(\d+)E)?E", held)}
+    taken = set()
+    for ds in range(1, 9):
+        for group in (1, 16, 17, 32, 33, 64, 65, 300):
+            for width in (5, 2000):
+                for ragged in (None, 256):
+                    out = (ctypes.c_int32 * 4)()
+                    assert lib.mambo_kv_attention_plan(cache(head_dim=32 * ds, heads=1), batch(width=width, ldt=width, offsets=ragged), 2,
+                                                       group, 0, out) == 0
+                    if out[0]:
+                        taken.add(("rows" if out[1] else "short", ds, out[0] // 16))
+                    if out[2]:
+                        taken.add(("tiles", ds, 0))
+    assert names == taken
+
+
 def test_calls_of_two_to_the_24_rows_and_more(lib):
     """What is launched decides, not the rows: of large calls nothing is joined."""
     def size(tokens, q_heads, dim=128, heads=8, **b):
