@@ -127,6 +127,58 @@ def attend(q: np.ndarray, k: np.ndarray, v: np.ndarray, group: int, scale: float
     return out, lse, bound, lse_bound
 
 
+# Keys and values by which every block of a long sequence shows in the results. Scores are 0 or, for two kinds of queries, 0 or 2
+# times ln 2 by the block, so that probabilities are 1 and 4 to each other, and a block's values are 1 in one column of each half
+# of the head and 0 elsewhere: sums are of small whole numbers, which float32 and the rounding to bfloat16 keep.
+def block_rows(rng, length: int, heads: int, dim: int):
+    """(keys, values) [L,H,D], exactly held by the cache."""
+    k = rng.uniform(-3.0, 3.0, (length, heads, dim)).astype(np.float32)
+    v = np.zeros((length, heads, dim), dtype=np.float32)
+    block, half = np.arange(length) // BLOCK, dim // 2
+    run = -(-(length // BLOCK + 1) // (dim - half))
+    for h in range(heads):
+        k[:, h, 0], k[:, h, 1] = 2 * ((5 * block + h) % 7 < 3), 2 * ((3 * block + h) % 5 < 2)
+        v[np.arange(length), h, (block + h) % half] = 1
+        v[np.arange(length), h, half + block // run] = 1
+    return k, v
+
+
+def block_queries(n: int, heads: int, dim: int) -> np.ndarray:
+    """Rows [n,Hq,D] for them, to be scaled by ln 2: of kind (row + head) % 3, 0 for scores of 0."""
+    q = np.zeros((n, heads, dim), dtype=np.float32)
+    kind = (np.arange(n)[:, None] + np.arange(heads)) % 3
+    q[..., 0], q[..., 1] = kind == 1, kind == 2
+    return q
+
+
+def block_attend(k: np.ndarray, v: np.ndarray, n: int, group: int, causal: bool, window: int):
+    """(out, lse, bound of out's error, bound of lse's) of such rows over such tokens.
+
+    Probabilities 1 are exact, their sums whole: what is left is the division and the product (half a unit each) and half a step of
+    bfloat16, and of lse the logarithm (a unit), its factor and the product. Those of 4 are off by the scale's and the exponential's
+    last bits, and the total by half a unit for each of up to a quarter of the tokens that a lane adds up."""
+    length, heads, dim = k.shape
+    out, lse = np.zeros((n, heads * group, dim)), np.full((n, heads * group), -np.inf)
+    bound, lse_bound = np.zeros(out.shape), np.zeros(lse.shape)
+    end = length - n + np.arange(n) + 1
+    to = np.clip(end, 0, length) if causal else np.full(n, length)
+    begin = np.clip(end - window, 0, to) if window else np.zeros(n, dtype=np.int64)
+    for h in range(heads):
+        for kind in range(3):
+            w = np.ones(length) if kind == 0 else 2.0 ** k[:, h, kind - 1].astype(np.float64)
+            weights = np.concatenate([[0.0], np.cumsum(w)])
+            sums = np.concatenate([np.zeros((1, dim)), np.cumsum(w[:, None] * v[:, h], axis=0)])
+            loose = 2.0**-22 if kind == 0 else 2.0**-20 + (length // 4 + 64) * 2.0**-24
+            for g in range(h * group, (h + 1) * group):
+                rows = np.flatnonzero(((np.arange(n) + g) % 3 == kind) & (to > begin))
+                total = (weights[to[rows]] - weights[begin[rows]])[:, None]
+                out[rows, g] = (sums[to[rows]] - sums[begin[rows]]) / total
+                lse[rows, g] = np.log(total[:, 0])
+                bound[rows, g] = out[rows, g] * (2.0**-8 + loose)
+                lse_bound[rows, g] = 2.0**-22 * (1 + lse[rows, g]) + (loose if kind else 0.0)
+    return out, lse, bound, lse_bound
+
+
 def tables_of(rng, lengths, page: int, *, spare: int = 2, extra: int = 1):
     """(tables int32 [S,C], pages of the pool): every sequence's pages in any order, -1 behind them."""
     counts = [-(-n // page) for n in lengths]

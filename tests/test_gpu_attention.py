@@ -374,3 +374,59 @@ def test_two_to_the_24_rows_and_more(gpu, n, group, seqs, few):
     out, lse = attention()(q, cache, tables, on, return_lse=True)
     check(out[:8 * n], lse[:8 * n], first, keys, values, [n] * 8, group)
     assert torch.equal(out, out[:8 * n].repeat(times, 1, 1)[:seqs * n]) and torch.equal(lse, lse[:8 * n].repeat(times, 1)[:seqs * n])
+
+
+# lengths, rows of each sequence, key/value heads, group, head size, page, tables in pages more than needed, causal, window,
+# the kernel for few rows (by shares, by one workgroup a sequence, or not launched), whether that for many has several parts
+BLOCKS = [
+    ([131149], [1], 1, 8, 128, 128, 1, True, 0, "shares", False),
+    ([40011], [1], 2, 6, 64, 128, 1, True, 0, "shares", False),
+    ([20000], [3], 1, 5, 128, 128, 1, True, 0, "shares", False),
+    ([20000, 5000, 9000], [1] * 3, 1, 4, 128, 32, 1, True, 4096, "shares", False),  # windows of many blocks
+    ([20000], [5], 2, 6, 64, 64, 1, True, 4100, "shares", False),
+    ([9000, 40, 0, 20000], [2, 16, 1, 5], 1, 2, 96, 32, 1, True, 4096, "shares", True),
+    ([9000, 6000], [1, 1], 3, 31, 256, 64, 1, True, 3000, "shares", False),
+    ([20000, 7000], [3, 3], 1, 4, 96, 32, 1, False, 0, "shares", False),  # all of the sequence, split
+    ([40011], [1], 1, 60, 40, 128, 1, False, 0, "shares", False),
+    ([5000, 9000], [2, 1], 2, 3, 128, 64, 1, False, 0, "shares", False),
+    ([5000] * 4, [4] * 4, 1, 12, 64, 32, 1, True, 2000, None, True),
+    ([9000], [130], 1, 2, 64, 128, 1, True, 0, None, True),
+    ([9000], [130], 1, 2, 64, 128, 1, True, 4096, None, True),
+    ([9000, 300, 7000], [100, 2, 90], 1, 3, 128, 32, 1, True, 3333, "shares", True),
+    ([9000], [130], 1, 2, 96, 128, 1, False, 0, None, True),
+    ([6000, 5000], [70, 70], 1, 4, 192, 64, 1, True, 2000, None, True),
+    ([6000, 70, 5000], [40, 70, 90], 1, 3, 256, 64, 1, True, 1500, "shares", True),
+    ([6000, 5000], [150, 30], 1, 2, 256, 64, 1, False, 0, "shares", True),
+    ([30001], [600], 2, 2, 64, 128, 1, True, 8000, None, True),
+    ([1200], [3], 1, 5, 64, 32, 1, True, 0, "one", False),  # by one workgroup
+    ([9000], [3], 1, 5, 64, 32, 1, True, 1000, "one", False),
+    ([1200, 30], [4, 4], 2, 4, 128, 32, 1, False, 0, "one", False),
+]
+
+
+@pytest.mark.parametrize("lengths,counts,heads,group,dim,page,extra,causal,window,few,several", BLOCKS)
+def test_every_block_of_a_long_cache_counts_once(gpu, lengths, counts, heads, group, dim, page, extra, causal, window, few, several):
+    """Long caches, windows of thousands and rows that see all of their sequence, by shares and by parts that are joined: the
+    comparison (kv_reference.block_rows) shows a block that is lost or counted twice, or whose values come with other keys."""
+    from mambo_amd.kernels.kv_cache import launch_append_kv
+    rng = np.random.default_rng(sum(lengths) + dim)
+    host, pages = ref.tables_of(rng, lengths, page, extra=extra)
+    tables, cache = ref.device(gpu, host)[0], new_cache(pages, heads, dim, page)
+    rows = [ref.block_rows(rng, n, heads, dim) for n in lengths]
+    k, v = (torch.from_numpy(np.concatenate([r[i] for r in rows])).bfloat16().to(gpu) for i in (0, 1))
+    on = ref.device(gpu, np.array(lengths, np.int32))[0]
+    launch_append_kv(k, v, cache, tables, on, offsets=ref.device(gpu, ref.offsets_of(lengths))[0])
+    ragged, n = len(set(counts)) > 1, sum(counts)
+    plan = plan_of(cache, tables, n, heads * group, ragged, window)
+    assert (few is None) == (plan[0] == 0) and (few == "shares") == (plan[1] > 0) and several == (plan[2] > 0 and plan[3] > 1), plan
+    q = torch.from_numpy(np.concatenate([ref.block_queries(c, heads * group, dim) for c in counts])).bfloat16().to(gpu)
+    out, lse = attention()(q, cache, tables, on, causal=causal, window=window, scale=math.log(2.0), return_lse=True,
+                           offsets=ref.device(gpu, ref.offsets_of(counts))[0] if ragged else None)
+    cuts = ref.offsets_of(counts)
+    for s, c in enumerate(counts):
+        part = slice(cuts[s], cuts[s + 1])
+        want, want_lse, bound, lse_bound = ref.block_attend(*rows[s], c, group, causal, window)
+        got, got_lse = out[part].double().cpu().numpy(), lse[part].double().cpu().numpy()
+        some = np.isfinite(want_lse)
+        assert (np.abs(got - want) <= bound).all(), s
+        assert np.array_equal(some, np.isfinite(got_lse)) and (np.abs(got_lse[some] - want_lse[some]) <= lse_bound[some]).all(), s

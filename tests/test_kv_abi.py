@@ -312,3 +312,27 @@ def test_the_models_agree_with_hand_counts():
     assert np.allclose(x, [[[0.0, 0.0, 1.0, -2.0, 5.0]]])
     out, lse, _, _ = ref.attend(np.zeros((2, 1, 8)), np.zeros((3, 1, 8)), np.arange(3.0)[:, None, None] * np.ones((3, 1, 8)), 1, 1.0, True, 2)
     assert np.allclose(out[:, 0, 0], [0.5, 1.5]) and np.allclose(lse, math.log(2))
+
+
+@pytest.mark.parametrize("length,dim", [(40011, 64), (9000, 64), (131149, 128), (20000, 128), (6000, 256)])
+def test_a_lost_or_repeated_block_shows(length, dim):
+    """Mistakes planted in the statement that long caches are compared with: every block left out moves the lse, and one left out
+    with another taken twice, or values of another block, move an output, by more than twice what the comparison allows."""
+    rng = np.random.default_rng(length)
+    k, v = ref.block_rows(rng, length, 1, dim)
+    block = np.arange(length) // ref.BLOCK
+    blocks = int(block[-1]) + 1
+    out, lse, bound, lse_bound = ref.block_attend(k, v, 1, 3, False, 0)  # rows of each kind
+    counts = np.bincount(block)
+    assert (lse[0, 0] - np.log(length - counts) > 2 * lse_bound[0, 0]).all()
+    sums = np.stack([np.bincount(block, v[:, 0, d]) for d in range(dim)], 1)  # [blocks, D]
+    for shift in (1, 2, 7, blocks // 2, blocks - 1):
+        moved = np.abs(np.roll(sums, shift, 0) - sums) / length  # block b for block b - shift
+        assert (moved > 2 * (bound[0, 0] + 2.0**-8 * moved)).any(1).all(), shift
+    first = np.arange(blocks) * ref.BLOCK
+    for kind in (1, 2):  # weights of a block that come with another one's values
+        w = 2.0 ** k[first, 0, kind - 1]
+        total = (w * counts).sum()
+        other = np.flatnonzero(w != np.roll(w, 1))
+        moved = np.abs((w - np.roll(w, 1))[other, None] * sums[other]) / total
+        assert len(other) > blocks // 4 and (moved > 2 * (bound[0, kind] + 2.0**-8 * moved)).any(1).all()
