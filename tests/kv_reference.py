@@ -127,6 +127,24 @@ def attend(q: np.ndarray, k: np.ndarray, v: np.ndarray, group: int, scale: float
     return out, lse, bound, lse_bound
 
 
+def turn_bound(x: np.ndarray, positions, frequencies, interleaved: bool, magnitude: float = 1.0) -> np.ndarray:
+    """How far a rotation in float32 by cosines and sines that are rounded once from 64 bits can be: half a unit of each, of the
+    one product that is rounded by itself and of the sum, counted at the values that they have; of the angle what 53 bits of the
+    frequency, here and there, leave at the position, and the ends of the two series (below 2^-36)."""
+    x = np.array(x, dtype=np.float64)
+    out = np.zeros_like(x)
+    half, p = 2.0**-24, np.array(positions, dtype=np.float64)
+    size = 2 * len(frequencies)
+    for i, f in enumerate(frequencies):
+        i0, i1 = (2 * i, 2 * i + 1) if interleaved else (i, i + size // 2)
+        c, s = (magnitude * t(p * f)[:, None] for t in (np.cos, np.sin))
+        a, b = x[:, :, i0], x[:, :, i1]
+        far = magnitude * (np.abs(a) + np.abs(b)) * (2.0**-36 + np.abs(p) * abs(f) * 2.0**-51)[:, None]
+        out[:, :, i0] = 1.001 * half * (np.abs(a * c) + 2 * np.abs(b * s) + np.abs(a * c - b * s)) + far
+        out[:, :, i1] = 1.001 * half * (np.abs(a * s) + 2 * np.abs(b * c) + np.abs(a * s + b * c)) + far
+    return out
+
+
 # Keys and values by which every block of a long sequence shows in the results. Scores are 0 or, for two kinds of queries, 0 or 2
 # times ln 2 by the block, so that probabilities are 1 and 4 to each other, and a block's values are 1 in one column of each half
 # of the head and 0 elsewhere: sums are of small whole numbers, which float32 and the rounding to bfloat16 keep.

@@ -401,3 +401,34 @@ def test_a_captured_step_replayed_past_its_table(gpu):
         same(got_k[0], model.k)
         same(got_v[0], model.v)
     assert int(lengths) == 35
+
+
+@pytest.mark.parametrize("dim,size,interleaved", [(64, 64, False), (64, 32, True), (128, 128, False), (80, 20, False), (72, 18, True), (256, 256, True)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_rotated_keys_are_rounded_as_the_exact_ones(gpu, dim, size, interleaved, dtype):
+    """A rotated key's code is that of the rotation in 64 bits, but where that lies as close to the border between two codes as the
+    rotation's last bits reach."""
+    from mambo_amd.utils.rotary_table import prepare_rotary_table, rotary_frequencies
+    rng = np.random.default_rng(dim + size)
+    heads, n = 2, 96
+    cache = new_cache(3, heads, dim, 32)
+    tables, lengths = torch.tensor([[2, 0, 1]], dtype=torch.int32, device=gpu), torch.tensor([n], dtype=torch.int32, device=gpu)
+    k = rows_of(rng, n, heads, dim, dtype)
+    positions = rng.integers(0, 50000, n).astype(np.int32)
+    ops().launch_append_kv(k.to(gpu), k.to(gpu), cache, tables, lengths, rotary=prepare_rotary_table(size, interleaved=interleaved),
+                           positions=ref.device(gpu, positions)[0])
+    frequencies = rotary_frequencies(size)[0]
+    turned = ref.rotate(k.double().numpy(), positions, frequencies, interleaved)
+    off = ref.turn_bound(k.double().numpy(), positions, frequencies, interleaved)
+    got = read_all(cache, tables, [n])[0][0]
+    settled = 0
+    for block in range(3):
+        part = slice(32 * block, 32 * block + 32)
+        for h in range(heads):
+            low, high = turned[part, h] - off[part, h], turned[part, h] + off[part, h]
+            e = ref.exponent(float(np.abs(turned[part, h]).max()))
+            assert e == ref.exponent(float(np.maximum(np.abs(low), np.abs(high)).max()))
+            low, high = ref.nearest(low, e), ref.nearest(high, e)
+            assert ((low <= got[part, h]) & (got[part, h] <= high)).all()
+            settled += int((low == high).sum())
+    assert settled >= 0.999 * turned.size

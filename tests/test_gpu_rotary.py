@@ -125,3 +125,20 @@ def test_refusals(gpu):
             rotary()(*args, **more)
     with pytest.raises(TypeError):
         rotary()(x, at, None)
+
+
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("tokens,heads,dim,size", SHAPES)
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_rotation_to_its_last_bits(gpu, tokens, heads, dim, size, interleaved, dtype):
+    """Cosines and sines are rounded once from 64 bits: angles of 32 bits, which the bound of test_rotation allows, are further off."""
+    from mambo_amd.utils.rotary_table import prepare_rotary_table, rotary_frequencies
+    rng = np.random.default_rng(dim + size + 1)
+    scaling = {"type": "yarn", "factor": 4.0, "original_length": 4096}
+    x = torch.from_numpy(rng.standard_normal((tokens, heads, dim)).astype(np.float32)).to(gpu).to(dtype)
+    positions = rng.integers(-1000, 100000, tokens).astype(np.int32)
+    frequencies, magnitude = rotary_frequencies(size, scaling=scaling)
+    got = rotary()(x, *ref.device(gpu, positions), prepare_rotary_table(size, scaling=scaling, interleaved=interleaved), out_dtype=torch.float32)
+    x64 = x.double().cpu().numpy()
+    off = np.abs(got.double().cpu().numpy() - ref.rotate(x64, positions, frequencies, interleaved, magnitude))
+    assert (off <= ref.turn_bound(x64, positions, frequencies, interleaved, magnitude)).all()

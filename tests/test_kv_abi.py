@@ -336,3 +336,25 @@ def test_a_lost_or_repeated_block_shows(length, dim):
         other = np.flatnonzero(w != np.roll(w, 1))
         moved = np.abs((w - np.roll(w, 1))[other, None] * sums[other]) / total
         assert len(other) > blocks // 4 and (moved > 2 * (bound[0, kind] + 2.0**-8 * moved)).any(1).all()
+
+
+@pytest.mark.parametrize("interleaved", [False, True])
+def test_angles_in_32_bits_are_told_apart(interleaved):
+    """The kernel's arithmetic stays within the bound of a rotation, the same with an angle of 32 bits does not."""
+    rng = np.random.default_rng(40)
+    f = [10000.0 ** (-2 * i / 64) for i in range(32)]
+    positions = rng.integers(0, 100000, 30)
+    x = rng.standard_normal((30, 4, 64)).astype(np.float32)
+    exact, bound = ref.rotate(x, positions, f, interleaved, 1.1), ref.turn_bound(x, positions, f, interleaved, 1.1)
+    off = []
+    for bits in (np.float64, np.float32):
+        got = np.array(x)
+        for i in range(32):
+            i0, i1 = (2 * i, 2 * i + 1) if interleaved else (i, i + 32)
+            angle = np.mod(positions * f[i] / (2 * math.pi) + 0.5, 1.0) * (2 * math.pi) - math.pi
+            c, s = (np.float32(1.1 * t(angle.astype(bits).astype(np.float64)))[:, None].astype(np.float64) for t in (np.cos, np.sin))
+            a, b = x[..., i0].astype(np.float64), x[..., i1].astype(np.float64)
+            got[..., i0] = np.float32(a * c - np.float32(b * s).astype(np.float64))
+            got[..., i1] = np.float32(a * s + np.float32(b * c).astype(np.float64))
+        off.append(np.abs(got.astype(np.float64) - exact) / bound)
+    assert off[0].max() <= 1.0 < 1.2 < off[1].max()
