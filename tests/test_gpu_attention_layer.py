@@ -180,3 +180,41 @@ def test_calls_at_once_on_one_cache(gpu):
         assert all(torch.equal(a, b) for a, b in zip(got, expected))
     keys, _ = read_all(cache, tables, [1, 1])
     assert all(np.isfinite(t).all() for t in keys)
+
+
+@pytest.mark.parametrize("window", [0, 40])
+def test_block_is_its_parts(gpu, window):
+    """The layer bit for bit out of the operators that it is said to call, each of which has its own tests: prompts, then tokens,
+    of uniform and of ragged sequences."""
+    from mambo_amd.kernels.attention import launch_attention_kv
+    from mambo_amd.kernels.iq3_s_fp8 import launch_iq3_s_fp8_matmul
+    from mambo_amd.kernels.kv_cache import launch_append_kv
+    from mambo_amd.kernels.quantize_fp8 import launch_quantize_fp8
+    from mambo_amd.kernels.rotary import launch_rotary
+    from mambo_amd.utils.attention_layer import AttentionLayer
+    from mambo_amd.utils.rotary_table import prepare_rotary_table
+    heads, group, dim, width = 2, 4, 64, 512
+    shapes = ((heads * group * dim, width), (heads * dim, width), (heads * dim, width), (width, heads * group * dim))
+    (q, _), (k, _), (v, _), (o, _) = (prepared(gpu, n, kk, s) for s, (n, kk) in enumerate(shapes))
+    table = prepare_rotary_table(dim)
+    layer = AttentionLayer(q, k, v, o, table, window)
+    rng = np.random.default_rng(5)
+    caches = [new_cache(6, heads, dim, 32) for _ in range(2)]
+    tables = torch.tensor([[5, 1, -1], [0, 3, 4]], dtype=torch.int32, device=gpu)
+    lengths = np.zeros(2, dtype=np.int32)
+    for counts, ragged in (([33, 40], True), ([2, 2], False), ([1, 1], True), ([1, 1], False)):
+        starts, n = lengths.copy(), sum(counts)
+        lengths += np.array(counts, dtype=np.int32)
+        x = rows_of(rng, n, 1, width, torch.bfloat16).view(n, width).to(gpu)
+        on = ref.device(gpu, lengths)[0]
+        offsets = ref.device(gpu, ref.offsets_of(counts))[0] if ragged else None
+        out = layer(x, caches[0], tables, on, offsets)
+        rows = launch_quantize_fp8(x)
+        q_rows, k_rows, v_rows = (launch_iq3_s_fp8_matmul(*rows, w).view(n, -1, dim) for w in (q, k, v))
+        positions = ref.device(gpu, np.concatenate([np.arange(s, s + c) for s, c in zip(starts, counts)]).astype(np.int32))[0]
+        launch_append_kv(k_rows, v_rows, caches[1], tables, on, offsets=offsets, rotary=table)
+        turned = launch_rotary(q_rows, positions, table, out_dtype=torch.bfloat16)
+        a = launch_attention_kv(turned, caches[1], tables, on, offsets=offsets, window=window)
+        expected = launch_iq3_s_fp8_matmul(*launch_quantize_fp8(a.view(n, -1)), o)
+        assert torch.equal(caches[0].codes, caches[1].codes) and torch.equal(caches[0].scales, caches[1].scales)
+        assert torch.equal(out, expected), counts
