@@ -430,3 +430,59 @@ def test_every_block_of_a_long_cache_counts_once(gpu, lengths, counts, heads, gr
         some = np.isfinite(want_lse)
         assert (np.abs(got - want) <= bound).all(), s
         assert np.array_equal(some, np.isfinite(got_lse)) and (np.abs(got_lse[some] - want_lse[some]) <= lse_bound[some]).all(), s
+
+
+class Guarded:
+    """A tensor in the middle of a larger one, whose ends must stay as they are."""
+
+    def __init__(self, gpu, shape, dtype, fill):
+        n = math.prod(shape)
+        self.margin = 1 << 16  # 128 KiB and more
+        self.whole = torch.full((n + 2 * self.margin,), fill, dtype=dtype, device=gpu)
+        self.ends = self.whole[:self.margin].clone()
+        self.inner = self.whole[self.margin:self.margin + n].view(shape)
+
+    def untouched(self):
+        bits = {1: torch.uint8, 2: torch.int16, 4: torch.int32}[self.whole.element_size()]
+        return all(torch.equal(part.view(bits), self.ends.view(bits)) for part in (self.whole[:self.margin], self.whole[-self.margin:]))
+
+
+HOSTILE_LENGTHS = ([-5, 70, 3], [2**31 - 1] * 3, [-2**31] * 3, [5000, 0, 2**31 - 40], [2**30, 3200, 31])
+HOSTILE_OFFSETS = (None, [0, 5, 3, 90], [-9, 4, 99, 2**31 - 1], [90, 10, 5, 0], [7, 7, 7, 7], [-2**31, 0, 2**31 - 1, 40], [0, 1, 2, 3])
+
+
+@pytest.mark.parametrize("columns,tokens,plan", [(4, 90, [16, 0, 256, 1]), (4, 3, [16, 0, 0, 1]), (100, 90, [16, 75, 256, 7]), (100, 3, [16, 75, 0, 1])])
+@pytest.mark.parametrize("causal,window", [(True, 0), (True, 1), (True, 40), (False, 0)])
+def test_arrays_of_any_values_write_nothing_elsewhere(gpu, columns, tokens, plan, causal, window):
+    """Lengths, offsets and pages of any values: what lies around the output, the lse and the workspace stays, and so do the cache and
+    the tables; rows that no sequence can have stay as well."""
+    from mambo_amd import _native
+    rng = np.random.default_rng(31)
+    lengths, heads, group, dim = [32 * columns, 45, 100], 2, 2, 64
+    cache, tables, _, _ = filled(gpu, rng, lengths, heads, dim, 32, extra=0)
+    tables = tables.clone()
+    tables[1, 1:], tables[2] = 2**31 - 1, torch.from_numpy(rng.integers(-2**31, 2**31, columns).astype(np.int32)).to(gpu)
+    before = [t.clone() for t in (cache.codes, cache.scales, tables)]
+    q = rows_of(rng, tokens, heads * group, dim, torch.bfloat16).to(gpu)
+    assert plan_of(cache, tables, tokens, heads * group, True, window) == [16, 0 if window else plan[1], *plan[2:]]
+    for bad in HOSTILE_LENGTHS:
+        on = torch.tensor(bad, dtype=torch.int64, device=gpu).int()
+        for cuts in HOSTILE_OFFSETS:
+            offsets = None if cuts is None else torch.tensor(cuts, dtype=torch.int64, device=gpu).int()
+            batch = _native.KVBatchArgs(tables.data_ptr(), columns, columns, on.data_ptr(), None if cuts is None else offsets.data_ptr(), 3)
+            size = _native.lib().mambo_kv_attention_workspace(cache.args, batch, tokens, heads * group, window)
+            out = Guarded(gpu, q.shape, torch.bfloat16, 7.0)
+            lse = Guarded(gpu, q.shape[:2], torch.float32, 7.0)
+            work = Guarded(gpu, (size,), torch.uint8, 77)
+            assert work.inner.data_ptr() % 16 == 0
+            _native.check(_native.lib().mambo_kv_attention(
+                q.data_ptr(), tokens, heads * group, dim, heads * group * dim, dim, cache.args, batch, 0.125, causal, window,
+                out.inner.data_ptr(), heads * group * dim, dim, lse.inner.data_ptr(), work.inner.data_ptr(), size,
+                _native.stream_handle(None)), "attention")
+            torch.cuda.synchronize()
+            assert out.untouched() and lse.untouched() and work.untouched(), (bad, cuts)
+            if cuts == [7, 7, 7, 7]:
+                assert (out.inner == 7.0).all() and (lse.inner == 7.0).all()
+            if cuts == [0, 1, 2, 3]:
+                assert (out.inner[3:] == 7.0).all() and (lse.inner[3:] == 7.0).all()
+    assert all(torch.equal(a, b) for a, b in zip(before, (cache.codes, cache.scales, tables)))

@@ -432,3 +432,42 @@ def test_rotated_keys_are_rounded_as_the_exact_ones(gpu, dim, size, interleaved,
             assert ((low <= got[part, h]) & (got[part, h] <= high)).all()
             settled += int((low == high).sum())
     assert settled >= 0.999 * turned.size
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_arrays_of_any_values_write_nothing_elsewhere(gpu, dtype):
+    """Lengths, offsets and pages of any values: what lies around the cache and the rotated queries stays, and so do pages that no
+    table names, queries of no sequence, and what is read."""
+    from mambo_amd.utils.kv_cache import KVCache
+    from mambo_amd.utils.rotary_table import prepare_rotary_table
+    from test_gpu_attention import HOSTILE_LENGTHS, HOSTILE_OFFSETS, Guarded
+    rng = np.random.default_rng(32)
+    heads, dim, pages, n = 2, 64, 8, 90
+    table = prepare_rotary_table(dim)
+    tables = torch.tensor([[4, 99, 1], [2, -7, 2**31 - 1], [2**31 - 1, -2**31, 6]], dtype=torch.int64, device=gpu).int()
+    k, v, q = (rows_of(rng, n, h, dim, dtype).to(gpu) for h in (heads, heads, 4))
+    given = [t.clone() for t in (tables, k, v, q)]
+    for bad in HOSTILE_LENGTHS:
+        on = torch.tensor(bad, dtype=torch.int64, device=gpu).int()
+        for cuts in HOSTILE_OFFSETS:
+            codes, scales = Guarded(gpu, (pages, heads, 1, 2 * 32 * dim), torch.uint8, 0x51), Guarded(gpu, (pages, heads, 1, 2), torch.uint8, 0x80)
+            out = Guarded(gpu, (n, 4, dim), torch.bfloat16, 7.0)
+            cache = KVCache(codes.inner, scales.inner, heads, dim, 32)
+            ops().launch_append_kv(k, v, cache, tables, on, offsets=None if cuts is None else torch.tensor(cuts, dtype=torch.int64, device=gpu).int(),
+                                   rotary=table, q=q, out=out.inner)
+            torch.cuda.synchronize()
+            assert codes.untouched() and scales.untouched() and out.untouched(), (bad, cuts)
+            assert (codes.inner[[0, 3, 5, 7]] == 0x51).all() and (scales.inner[[0, 3, 5, 7]] == 0x80).all(), (bad, cuts)
+            if cuts == [7, 7, 7, 7]:
+                assert (out.inner == 7.0).all() and (codes.inner == 0x51).all()
+            if cuts == [0, 1, 2, 3]:
+                assert (out.inner[3:] == 7.0).all()
+    at = torch.from_numpy(rng.integers(-2**31, 2**31, (2, 500))).int().to(gpu)
+    at[0, :400] %= 3
+    at[1, :300] %= 96
+    got = ops().launch_read_kv(cache, tables, at[0].contiguous(), at[1].contiguous())
+    there = (at[0] >= 0) & (at[0] < 3) & (at[1] >= 0) & (at[1] < 96)
+    named = torch.tensor([[1, 0, 1], [1, 0, 0], [0, 0, 1]], device=gpu).bool()
+    there &= named[at[0].clamp(0, 2).long(), (at[1].clamp(0, 95) // 32).long()]
+    assert there.sum() > 50 and not got[0][~there].any() and not got[1][~there].any() and got[0][there].any(2).all()
+    assert all(torch.equal(a, b) for a, b in zip(given, (tables, k, v, q)))
