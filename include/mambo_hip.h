@@ -403,7 +403,8 @@ typedef struct mambo_kv_cache {
  * (offsets NULL: tokens / seqs rows each), the last of them at position lengths[s] - 1, and its page
  * c (tokens [c * page_size, ...)) is tables[s * ldt + c], c < width. The kernels hold offsets within
  * [0, tokens] and take a length below 0 for 0. A page outside [0, pages), or past the table's width, is none:
- * nothing is stored there and its tokens are left out of attention; rows keep their positions. */
+ * nothing is stored there and its tokens are left out of attention; rows keep their positions. The arrays
+ * must not change while a call runs. */
 typedef struct mambo_kv_batch {
     const int32_t *tables;
     int64_t ldt;

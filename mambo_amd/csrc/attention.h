@@ -92,8 +92,8 @@ __device__ __forceinline__ uint2 keep_tokens(uint32_t lo, uint32_t hi, int left)
     return make_uint2(lo & (uint32_t)mask, hi & (uint32_t)(mask >> 32));
 }
 
-// Most rows that attend_rows takes, in tiles of 16: more than that attend_tiles is faster at (4 x 64 rows of D = 128 behind 20000
-// tokens 57 us, with four tiles here 75; 4 x 32 of 192 behind 10000 52, here 37; of 256 73, here 53).
+// Most rows that attend_rows takes, in tiles of 16: more than that attend_tiles is faster at (8 key/value heads: 4 x 64 rows of D = 128
+// behind 20000 tokens 57 us, with four tiles here 75; 4 x 32 of 192 behind 10000 52, here 37; of 256 73, here 53).
 constexpr int max_row_tiles(int padded) { return padded <= 64 ? 4 : 2; }
 
 // Whether attend_short takes so many tiles of heads of 32 ds: its eight waves have not the registers for two of heads above 128,

@@ -52,9 +52,9 @@ Plan make_plan(const KvCache &c, const KvBatch &b, int group, int64_t window)
             p.row_tiles = p.few_rows = 0;
         } else if (!short_ones) {
             // A workgroup a CU, fewer where there is no work for them: the blocks that its waves have on their way are enough
-            // (131149 tokens of 8 heads of 128 47.0 us, with two 49.6). Two of small heads (16 x 8000 of 64 28.7 us for 35.4),
-            // and where a workgroup comes to the ends of several sequences, at which the other goes on (64 sequences
-            // of up to 8192 109 us for 113, 32 of 4000 49.5 for 44.4).
+            // (131149 tokens of 8 heads of 128 47.0 us, with two 49.6). Two of small heads (16 x 8000 of 8 heads of 64 28.7 us
+            // for 35.4), and where a workgroup comes to the ends of several sequences, at which the other goes on (of 8 heads of
+            // 128 64 sequences of up to 8192 109 us for 113, 32 of 4000 49.5 for 44.4).
             const int64_t blocks = (int64_t)b.seqs * (b.capacity / kKvBlock);
             const int per_cu = size <= 2 || (size <= 4 && (int64_t)b.seqs * c.heads >= 2 * kCus) ? 2 : 1;
             p.slots = (int)std::max<int64_t>(1, std::min<int64_t>(per_cu * kCus / c.heads, cdiv(blocks, 4)));
@@ -68,7 +68,7 @@ Plan make_plan(const KvCache &c, const KvBatch &b, int group, int64_t window)
         p.tiles_each = (int)cdiv(rows, tile);
         p.tiles = b.offsets ? (int64_t)b.tokens * group / tile + b.seqs : (int64_t)b.seqs * p.tiles_each;
         // A workgroup a CU, two of ragged sequences: the longest then have more parts than the others (pieces of six prompts 37 us
-        // for 41; of sequences with as many rows each, 4 of 16 rows behind 20000 tokens, 66 for 58).
+        // for 41; of sequences with as many rows each, 4 of 16 tokens of 32/8 heads of 128 behind 20000, 66 for 58).
         const int64_t places = (b.offsets ? 2 : 1) * kCus / (p.tiles * c.heads);
         p.parts = (int)std::max<int64_t>(1, std::min<int64_t>(places, cdiv(b.capacity, 512)));
         if (p.parts > 1) {

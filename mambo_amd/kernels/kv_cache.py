@@ -6,7 +6,8 @@ A call's sequences are told by ``tables`` int32 [S, C] (the page that holds a se
 included) and, unless every sequence has as many rows, ``offsets`` int32 [S + 1] (sequence s has the rows
 offsets[s] to offsets[s + 1], the last at position lengths[s] - 1). A sequence may be longer than its row of the
 table: there is no page for what lies past it. All of it stays on the device: nothing is
-read back, so that a step can be recorded into a HIP graph and replayed with other lengths.
+read back, so that a step can be recorded into a HIP graph and replayed with other lengths; while a call
+runs they must not change.
 
     cache = allocate_kv_cache(pages, kv_heads, head_dim)
     q = launch_append_kv(k, v, cache, tables, lengths, rotary=table, q=q)
