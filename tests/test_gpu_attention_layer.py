@@ -218,3 +218,124 @@ def test_block_is_its_parts(gpu, window):
         expected = launch_iq3_s_fp8_matmul(*launch_quantize_fp8(a.view(n, -1)), o)
         assert torch.equal(caches[0].codes, caches[1].codes) and torch.equal(caches[0].scales, caches[1].scales)
         assert torch.equal(out, expected), counts
+
+
+def attended(cache, tables, lengths, q, **more):
+    from mambo_amd.kernels.attention import launch_attention_kv
+    return launch_attention_kv(q, cache, tables, lengths, return_lse=True, **more)
+
+
+def equal(a, b):
+    """Bit for bit: tokens that were never stored are NaN in these caches, and so is what sees them."""
+    return all(torch.equal(x.view(torch.int16), y.view(torch.int16)) for x, y in zip(a, b))
+
+
+@pytest.mark.parametrize("page", [32, 64])
+def test_a_prefix_shared_and_a_page_copied(gpu, page):
+    """Two sequences with the pages of one prefix, and the page that both go on in copied whole: as if each had its own."""
+    from mambo_amd.kernels.kv_cache import launch_append_kv
+    from mambo_amd.utils.rotary_table import prepare_rotary_table
+    rng = np.random.default_rng(6)
+    heads, group, dim, prefix = 2, 4, 64, 2 * page + 45 % page
+    table = prepare_rotary_table(dim)
+    cache, alone = new_cache(9, heads, dim, page), new_cache(9, heads, dim, page)
+    shared = torch.tensor([[4, 0, 7, 2], [4, 0, 5, 3]], dtype=torch.int32, device=gpu)
+    own = torch.tensor([[0, 1, 2, 3], [4, 5, 6, 7]], dtype=torch.int32, device=gpu)
+    old = [rows_of(rng, prefix, heads, dim, torch.bfloat16).to(gpu) for _ in range(2)]
+    at = ref.device(gpu, np.array([prefix], np.int32))[0]
+    launch_append_kv(*old, cache, shared[:1], at, rotary=table)
+    cache.codes[5], cache.scales[5] = cache.codes[7], cache.scales[7]
+    launch_append_kv(*(torch.cat([t, t]) for t in old), alone, own, at.repeat(2), rotary=table)
+    counts, lengths = np.array([1, 50]), at.repeat(2)
+    for _ in range(2):
+        n = int(counts.sum())
+        lengths = lengths + torch.from_numpy(counts).int().to(gpu)
+        offsets = ref.device(gpu, ref.offsets_of(counts))[0]
+        k, v, q = (rows_of(rng, n, h, dim, torch.bfloat16, 3.0).to(gpu) for h in (heads, heads, heads * group))
+        got = launch_append_kv(k, v, cache, shared, lengths, offsets=offsets, rotary=table, q=q)
+        want = launch_append_kv(k, v, alone, own, lengths, offsets=offsets, rotary=table, q=q)
+        assert torch.equal(got, want)
+        assert equal(attended(cache, shared, lengths, got, offsets=offsets), attended(alone, own, lengths, got, offsets=offsets))
+        counts = counts[::-1].copy() % 20
+
+
+@pytest.mark.parametrize("n,ragged", [(1, False), (1, True), (60, False), (60, True)])
+def test_replays_with_any_lengths(gpu, n, ragged):
+    """A call captured while its sequences are empty and replayed as they are long, short, past their tables and empty again, with
+    other queries and pages; eager calls and other work between."""
+    from mambo_amd.kernels.attention import launch_attention_kv
+    from test_gpu_attention import filled
+    rng = np.random.default_rng(7)
+    heads, group, dim, page, full = 2, 4, 64, 32, [4000, 2500, 64]
+    cache, tables, _, _ = filled(gpu, rng, full, heads, dim, page)
+    counts = [n, 2, 3 * n] if ragged else [n] * 3
+    offsets = ref.device(gpu, ref.offsets_of(counts))[0] if ragged else None
+    q = rows_of(rng, sum(counts), heads * group, dim, torch.bfloat16).to(gpu)
+    lengths, live = torch.zeros(3, dtype=torch.int32, device=gpu), tables.clone()
+    attended(cache, live, lengths, q, offsets=offsets)
+    graph, side = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side), torch.cuda.graph(graph, stream=side):
+        got = attended(cache, live, lengths, q, offsets=offsets)
+    torch.cuda.synchronize()
+    for step, values in enumerate((full, [0, 0, 0], [4000, 0, 1], [1, 2500, 64], [33, 64, 5], [4100, 2600, 70], [2**31 - 1, 3, 2000], full)):
+        lengths.copy_(torch.tensor(values, dtype=torch.int32))
+        q.copy_(rows_of(rng, sum(counts), heads * group, dim, torch.bfloat16))
+        live.copy_(tables if step % 2 else tables[[0, 1, 2]].roll(1, 1))
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert equal(got, attended(cache, live, lengths, q, offsets=offsets)), values
+    empty = launch_attention_kv(q[:0], cache, tables, lengths, return_lse=True)
+    assert empty[0].shape == (0, heads * group, dim) and empty[1].shape == (0, heads * group)
+
+
+@pytest.mark.parametrize("page", [1024, 65536])
+def test_large_pages(gpu, page):
+    from test_gpu_attention import check
+    from mambo_amd.kernels.kv_cache import launch_append_kv
+    rng = np.random.default_rng(8)
+    heads, group, dim, lengths = 2, 3, 40, [1500, 31]
+    cache = new_cache(4, heads, dim, page)
+    tables = torch.tensor([[2, 0], [3, -1]], dtype=torch.int32, device=gpu)
+    models = [ref.Model(heads, dim) for _ in lengths]
+    for start, end in (([0, 0], [1400, 30]), ([1400, 30], lengths)):
+        counts = [b - a for a, b in zip(start, end)]
+        k, v = (rows_of(rng, sum(counts), heads, dim, torch.bfloat16) for _ in range(2))
+        launch_append_kv(k.to(gpu), v.to(gpu), cache, tables, *ref.device(gpu, np.array(end, np.int32)),
+                         offsets=ref.device(gpu, ref.offsets_of(counts))[0])
+        cuts = ref.offsets_of(counts)
+        for s, model in enumerate(models):
+            model.append(k[cuts[s]:cuts[s + 1]].double().numpy(), v[cuts[s]:cuts[s + 1]].double().numpy(), start[s])
+    for n in (1, 90):
+        q = rows_of(rng, 2 * n, heads * group, dim, torch.bfloat16).to(gpu)
+        out, lse = attended(cache, tables, *ref.device(gpu, np.array(lengths, np.int32)), q)
+        check(out, lse, q, [m.k for m in models], [m.v for m in models], [n, n], group)
+
+
+def test_appends_at_once_to_one_cache(gpu):
+    """Sequences of one cache that grow on streams of their own."""
+    from mambo_amd.kernels.kv_cache import launch_append_kv
+    from mambo_amd.utils.rotary_table import prepare_rotary_table
+    rng = np.random.default_rng(9)
+    heads, dim, page, users = 2, 64, 32, 4
+    table = prepare_rotary_table(dim)
+    caches = [new_cache(4 * users, heads, dim, page) for _ in range(2)]
+    tables = torch.from_numpy(rng.permutation(4 * users).astype(np.int32).reshape(users, 4)).to(gpu)
+    streams = [torch.cuda.Stream() for _ in range(users)]
+    held = np.zeros(users, dtype=np.int32)
+    for step in range(6):
+        counts = [40, 1, 7, 1, 30, 2][step:] + [40, 1, 7, 1, 30, 2][:step]
+        data = [[rows_of(rng, c, h, dim, torch.float32).to(gpu) for h in (heads, heads, 4)] for c in counts[:users]]
+        held += np.array(counts[:users], dtype=np.int32)
+        lengths = ref.device(gpu, np.minimum(held, 128).astype(np.int32))[0]
+        outs = []
+        torch.cuda.synchronize()
+        for u, stream in enumerate(streams):
+            k, v, q = data[u]
+            outs.append(launch_append_kv(k, v, caches[0], tables[u:u + 1], lengths[u:u + 1], rotary=table, q=q, stream=stream))
+        torch.cuda.synchronize()
+        for u in range(users):
+            k, v, q = data[u]
+            assert torch.equal(outs[u], launch_append_kv(k, v, caches[1], tables[u:u + 1], lengths[u:u + 1], rotary=table, q=q))
+        assert torch.equal(caches[0].codes, caches[1].codes) and torch.equal(caches[0].scales, caches[1].scales)
