@@ -40,7 +40,7 @@ def launch_attention_kv(q: torch.Tensor, cache: KVCache, tables: torch.Tensor, l
 
     Row i of a sequence's n stands at position lengths[s] - n + i and sees the tokens up to itself (``causal``), no more
     than the last ``window`` of them where that is not 0, or all of the sequence's. A row that sees none (a sequence of length
-    0, more rows than tokens, no page) becomes zeros, its lse -inf. ``scale`` defaults to D ** -0.5.
+    0, more rows than tokens, no page) becomes zeros, its lse -inf. ``scale`` (positive) defaults to D ** -0.5.
 
     Scores, the running sum and the output are float32; the probabilities are rounded to bfloat16 (2^-8 of each at most) for the
     product with the values, the result once to bfloat16. Results do not vary from run to run. Rows of no sequence are not
